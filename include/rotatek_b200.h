@@ -30,7 +30,9 @@ typedef enum rtk_dtype {
   RTK_F32 = 0,
   RTK_BF16 = 1,
   RTK_F16 = 2,
-  RTK_U8 = 3
+  RTK_U8 = 3,
+  RTK_I32 = 4,   /* lengths and counts */
+  RTK_I64 = 5    /* token ids */
 } rtk_dtype;
 
 typedef enum rtk_status {
@@ -203,6 +205,96 @@ int rtk_spark_decode(const rtk_tensor *q_full, const rtk_tensor *k_full, const r
  * prefill.  A token whose kept count is not D_keep ORs RTK_DEVICE_BAD_INPUT
  * into *status (a device uint32; nullable). */
 int rtk_spark_pack(const rtk_tensor *keep_mask, const rtk_tensor *keep_idx_out, void *status, void *stream);
+
+/* ------------------------------------------------------------------------
+ * Many questions on shared prefixes
+ *
+ * A prefix is one prefilled image or video: its prompt at full width and its
+ * rotated, truncated visual span (what rtk_build_rotation leaves).  P prefixes
+ * serve B = P * N questions; question b belongs to prefix b / N and owns only
+ * its text: a cache [B, H_kv, C, D] of capacity C of which text_lens[b] rows
+ * are written.  Lengths live on the device, so that a captured step can be
+ * replayed while they grow.  No counterparts in the reference.
+ * ------------------------------------------------------------------------ */
+
+/* Bytes of workspace rtk_shared_decode needs for these shapes on `device`
+ * (16-byte aligned, no zeroing required, free again when the call's kernels
+ * have run). */
+size_t rtk_shared_decode_workspace_size(int64_t prefixes, int64_t batch, int64_t tokens, int64_t q_heads,
+                                        int64_t kv_heads, int64_t seq_full, int64_t seq_sparse, int64_t text_cap,
+                                        int32_t device);
+
+/* Attention of T new tokens per question (T = 1: ordinary decoding; more: drafts
+ * being checked) over its prefix and its own text in one softmax.
+ *   q          [B, T, H_q, D]             f32 | bf16 | f16, any strides
+ *   R_partial  [P, H_kv, D, D_keep], delta_mu [P, H_kv, D] (nullable),
+ *   k_full, v_full [P, H_kv, S_f, D], mask_full [P, S_f] u8 (nullable; 0 masks a token),
+ *   k_sparse [P, H_kv, S_v, D_keep], v_sparse [P, H_kv, S_v, D]
+ *                                         q's dtype, as in rtk_rotatek_decode
+ *   k_text, v_text [B, H_kv, C, D]        q's dtype, or u8 (e4m3) with
+ *   k_scale, v_scale [B, H_kv, C] f32     (both or neither; rtk_append_text)
+ *   text_lens  [B] i32                    rows written, the T new ones among them
+ *                                         (clamped to [0, C])
+ *   out        [B, T, H_q, D]             q's dtype, any strides
+ * Query t of question b sees all of its prefix and its text rows s <
+ * text_lens[b] - (T - 1 - t).  out = softmax([q.k_f ; q.R.k_s + q.delta_mu ;
+ * q.k_text] / sqrt(D)) . [v_f ; v_s ; v_text], 0 for a row that sees nothing.
+ * Rows of a cache past text_lens and masked prompt tokens may hold anything.
+ * `status` (device uint32, nullable) gets RTK_DEVICE_TIMEOUT if a bounded wait
+ * gives up.                                                                   */
+int rtk_shared_decode(const rtk_tensor *q, const rtk_tensor *R_partial, const rtk_tensor *delta_mu,
+                      const rtk_tensor *k_full, const rtk_tensor *v_full, const rtk_tensor *mask_full,
+                      const rtk_tensor *k_sparse, const rtk_tensor *v_sparse, const rtk_tensor *k_text,
+                      const rtk_tensor *v_text, const rtk_tensor *k_scale, const rtk_tensor *v_scale,
+                      const rtk_tensor *text_lens, int64_t num_kv_groups, const rtk_tensor *out, void *workspace,
+                      size_t workspace_bytes, void *status, void *stream);
+
+/* Write T new Keys and Values of each question into its text cache, at rows
+ * text_lens[b] .. text_lens[b] + counts[b] - 1 (counts nullable: T).  Rows that
+ * would lie past the capacity are dropped; text_lens itself is the caller's to
+ * advance (after every layer has been written).
+ *   k_new, v_new   [B, H_kv, T, D]  f32 | bf16 | f16, any strides
+ *   k_text, v_text [B, H_kv, C, D]  the same dtype (rows copied), or u8 with
+ *   k_scale, v_scale [B, H_kv, C] f32: x8 = e4m3(x / scale), scale = amax / 448 of
+ *                  the row (amax over finite values; 1 for a row of zeros), division
+ *                  and conversion rounded to nearest even; infinities become +-448,
+ *                  NaN stays NaN.  Any strides.
+ *   text_lens, counts [B] i32                                                  */
+int rtk_append_text(const rtk_tensor *k_new, const rtk_tensor *v_new, const rtk_tensor *text_lens,
+                    const rtk_tensor *counts, const rtk_tensor *k_text, const rtk_tensor *v_text,
+                    const rtk_tensor *k_scale, const rtk_tensor *v_scale, void *stream);
+
+/* An 8-bit text cache read back: out = round(e4m3 * scale) in the outputs' dtype
+ * for rows s < text_lens[b], 0 after them.
+ *   k_text, v_text [B, H_kv, C, D] u8, k_scale, v_scale [B, H_kv, C] f32,
+ *   k_out, v_out [B, H_kv, C, D] f32 | bf16 | f16; any strides                 */
+int rtk_read_text(const rtk_tensor *k_text, const rtk_tensor *v_text, const rtk_tensor *k_scale,
+                  const rtk_tensor *v_scale, const rtk_tensor *text_lens, const rtk_tensor *k_out,
+                  const rtk_tensor *v_out, void *stream);
+
+/* Bytes of workspace rtk_verify_drafts needs (16-byte aligned, no zeroing). */
+size_t rtk_verify_drafts_workspace_size(int64_t batch, int64_t drafts, int64_t vocab);
+
+/* Which drafted tokens the target model accepts, and the token after them.
+ *   target_logits [B, T + 1, V]  f32 | bf16 | f16; row j scores the token after draft j - 1
+ *   draft_tokens  [B, T] i64     at most 64 drafts
+ *   draft_logits  [B, T, V]      target's dtype, what the drafts were drawn from;
+ *                                nullable: proposals without probabilities
+ *   uniforms      [B, T] f32     in [0, 1)
+ *   noise         [B, V] f32     > 0, drawn from Exp(1)
+ *   temperature   [B] f32        of both models; <= 0 decodes greedily
+ *   draft_lens    [B] i32        drafts of each question (nullable: T)
+ *   tokens_out    [B, T + 1] i64 the accepted drafts, the next token, then -1
+ *   accepted_out  [B] i32        how many drafts were accepted
+ * Unit vocabulary strides.  Draft j is accepted while u_j q_j(x_j) < p_j(x_j)
+ * (greedy: x_j is the lowest argmax of row j); the next token is the lowest
+ * argmax_i of max(p_i - q_i, 0) / noise_i after a rejection (of p_i / noise_i
+ * after the last draft, or where the difference leaves nothing), which draws
+ * from that distribution normalised.  A drafted id outside [0, V) is rejected.  */
+int rtk_verify_drafts(const rtk_tensor *target_logits, const rtk_tensor *draft_tokens, const rtk_tensor *draft_logits,
+                      const rtk_tensor *uniforms, const rtk_tensor *noise, const rtk_tensor *temperature,
+                      const rtk_tensor *draft_lens, const rtk_tensor *tokens_out, const rtk_tensor *accepted_out,
+                      void *workspace, size_t workspace_bytes, void *stream);
 
 /* ------------------------------------------------------------------------
  * Prefill rotation builder (head_dim 128)

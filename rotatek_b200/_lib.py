@@ -20,7 +20,8 @@ LIB_PATH = os.path.join(_PKG, "librotatek_b200.so")
 RTK_OK, RTK_ERR_INVALID, RTK_ERR_UNSUPPORTED, RTK_ERR_WORKSPACE, RTK_ERR_CUDA = range(5)
 RTK_DEVICE_TIMEOUT = 1
 
-_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.uint8: 3}
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.uint8: 3,
+           torch.int32: 4, torch.int64: 5}
 
 
 class RtkTensor(ctypes.Structure):
@@ -46,6 +47,13 @@ SIGNATURES = {
     "rtk_full_channel_decode": (ctypes.c_int, [_P] * 3 + [ctypes.c_int64, _P, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "rtk_spark_decode": (ctypes.c_int, [_P] * 8 + [ctypes.c_int64, _P, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "rtk_spark_pack": (ctypes.c_int, [_P, _P, ctypes.c_void_p, ctypes.c_void_p]),
+    "rtk_shared_decode_workspace_size": (ctypes.c_size_t, [ctypes.c_int64] * 8 + [ctypes.c_int32]),
+    "rtk_shared_decode": (ctypes.c_int, [_P] * 13 + [ctypes.c_int64, _P, ctypes.c_void_p, ctypes.c_size_t,
+                                                     ctypes.c_void_p, ctypes.c_void_p]),
+    "rtk_append_text": (ctypes.c_int, [_P] * 8 + [ctypes.c_void_p]),
+    "rtk_read_text": (ctypes.c_int, [_P] * 7 + [ctypes.c_void_p]),
+    "rtk_verify_drafts_workspace_size": (ctypes.c_size_t, [ctypes.c_int64] * 3),
+    "rtk_verify_drafts": (ctypes.c_int, [_P] * 9 + [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "rtk_key_covariance": (ctypes.c_int, [_P, _P, _P, ctypes.c_void_p]),
     "rtk_rotate_keys": (ctypes.c_int, [_P, _P, _P, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "rtk_eigh_topk_workspace_size": (ctypes.c_size_t, [ctypes.c_int64]),
@@ -122,6 +130,21 @@ def require_cuda(*tensors):
             raise RuntimeError("rotatek_b200 runs on CUDA tensors only (no CPU fallback)")
 
 
+def require_one_device(*tensors) -> torch.device:
+    """The one CUDA device that the given tensors (None skipped) live on."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("rotatek_b200 runs on CUDA tensors only (no CPU fallback)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}: all must be on one device")
+    return dev
+
+
 # ------------------------------------------------------------------ workspace
 _ws_lock = threading.Lock()
 _workspaces = {}     # device index -> uint8 buffer
@@ -151,6 +174,16 @@ def workspace(device: torch.device, nbytes: int, counter_bytes: int) -> torch.Te
             buf[:counter_bytes].zero_()
         _zero_prefix[idx] = counter_bytes     # what follows is scratch after the call
         return buf
+
+
+def status_word(device: torch.device) -> int:
+    """Address of the device's status word (the head of its decode workspace), for
+    entry points that take it apart from their scratch; ``read_status`` reads it."""
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    buf = _workspaces.get(idx)
+    if buf is None:
+        buf = workspace(device, 256, 256)
+    return buf.data_ptr()
 
 
 def read_status(device: Optional[torch.device] = None) -> int:

@@ -306,5 +306,167 @@ def spark_decode(
     return out
 
 
+def rotatek_shared_decode(
+    q: torch.Tensor,                     # [B, T, H_q, D]
+    R_partial: torch.Tensor,             # [P, H_kv, D, D_keep]
+    delta_mu: Optional[torch.Tensor],    # [P, H_kv, D] or None
+    k_full: torch.Tensor,                # [P, H_kv, S_full, D]
+    v_full: torch.Tensor,                # [P, H_kv, S_full, D]
+    mask_full: Optional[torch.Tensor],   # [P, S_full] uint8 or None
+    k_sparse: torch.Tensor,              # [P, H_kv, S_sparse, D_keep]
+    v_sparse: torch.Tensor,              # [P, H_kv, S_sparse, D]
+    k_text: torch.Tensor,                # [B, H_kv, C, D], q's dtype or e4m3
+    v_text: torch.Tensor,                # [B, H_kv, C, D]
+    text_lens: torch.Tensor,             # [B] int32
+    num_kv_groups: int,
+    *,
+    k_scale: Optional[torch.Tensor] = None,   # [B, H_kv, C] float32: k_text / v_text are e4m3
+    v_scale: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,       # [B, T, H_q, D] to write into
+) -> torch.Tensor:
+    """Attention of T new tokens per question, for questions that share prefixes;
+    returns [B, T, H_q, D] in q's dtype.
+
+    P prefixes (an image's prompt and its rotated, truncated visual span: the
+    first eight arguments of ``rotatek_decode``, stored once) serve B = P * N
+    questions; question b reads prefix b // N and its own text cache, of which
+    ``text_lens[b]`` rows are written, the T new tokens' among them.  Query t
+    sees the prefix and text rows s < text_lens[b] - (T - 1 - t): T = 1 is an
+    ordinary decoding step, T > 1 checks drafted tokens (``verify_drafts``).
+    The visual logits use the rotated query and the q . delta_mu bias, prompt
+    and text logits the full query; all share one softmax.  A row that sees
+    nothing gives 0.  Text caches hold q's dtype, or e4m3 rows with one scale
+    each (``append_text``; uint8 or float8_e4m3fn tensors).  Inputs may be
+    strided views; rows past ``text_lens`` and masked prompt tokens may hold
+    anything.  bf16 / fp16 with D = 128, D_keep 16, 32 or 64 and 16-byte aligned
+    channel-contiguous rows run on the tensor cores, anything else (fp32, D up to
+    256) on a generic kernel.  No counterpart in the reference."""
+    if q.dim() != 4:
+        raise ValueError("q must be [B, T, H_q, D]")
+    if R_partial.dim() != 4:
+        raise ValueError("R_partial must be [P, H_kv, D, D_keep]")
+    if k_scale is not None:
+        k_text, v_text = _as_u8(k_text), _as_u8(v_text)
+    dev = _lib.require_one_device(q, R_partial, delta_mu, k_full, v_full, mask_full, k_sparse, v_sparse, k_text,
+                                  v_text, text_lens, k_scale, v_scale, out)
+    lib = _lib.load()
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    b, t, heads, _ = q.shape
+    key = ("sh", R_partial.shape[0], b, t, heads, R_partial.shape[1], k_full.shape[-2], k_sparse.shape[-2],
+           k_text.shape[-2], dev.index)
+    need = _ws_size_cache.get(key)
+    if need is None:
+        need = _ws_size_cache[key] = lib.rtk_shared_decode_workspace_size(*key[1:])
+    # scratch of this call alone, from the stream's own pool: calls on several
+    # streams do not share it
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    D = _lib.describe
+    _lib.check(lib.rtk_shared_decode(
+        D(q), D(R_partial), D(delta_mu), D(k_full), D(v_full), D(mask_full), D(k_sparse), D(v_sparse), D(k_text),
+        D(v_text), D(k_scale), D(v_scale), D(text_lens), num_kv_groups, D(out), ws.data_ptr(), need,
+        _lib.status_word(dev), _stream(dev)))
+    return out
+
+
+def append_text(
+    k_new: torch.Tensor,                      # [B, H_kv, T, D]
+    v_new: torch.Tensor,                      # [B, H_kv, T, D]
+    text_lens: torch.Tensor,                  # [B] int32
+    k_text: torch.Tensor,                     # [B, H_kv, C, D], written in place
+    v_text: torch.Tensor,
+    *,
+    k_scale: Optional[torch.Tensor] = None,   # [B, H_kv, C] float32, written in place
+    v_scale: Optional[torch.Tensor] = None,
+    counts: Optional[torch.Tensor] = None,    # [B] int32: new rows of each question
+) -> None:
+    """Write new Keys and Values into the questions' text caches, each at its own
+    length: rows text_lens[b] .. text_lens[b] + counts[b] - 1 (T without
+    ``counts``); rows past the capacity are dropped.  ``text_lens`` is not
+    advanced: it is shared by all layers, so the caller adds to it once per
+    step.
+
+    With scales the caches are e4m3 (uint8 or float8_e4m3fn tensors): each row
+    is stored as e4m3(x / scale) with its own scale = amax / 448 (1 for a row of
+    zeros), rounded to nearest even; infinities become +-448, NaN stays NaN.
+    Without scales the rows are copied.  Any strides; no host synchronisation."""
+    if k_new.dim() != 4:
+        raise ValueError("k_new must be [B, H_kv, T, D]")
+    if k_scale is not None:
+        k_text, v_text = _as_u8(k_text), _as_u8(v_text)
+    dev = _lib.require_one_device(k_new, v_new, text_lens, k_text, v_text, k_scale, v_scale, counts)
+    D = _lib.describe
+    _lib.check(_lib.load().rtk_append_text(D(k_new), D(v_new), D(text_lens), D(counts), D(k_text), D(v_text),
+                                           D(k_scale), D(v_scale), _stream(dev)))
+
+
+def read_text(
+    k_text: torch.Tensor,                     # [B, H_kv, C, D] e4m3
+    v_text: torch.Tensor,
+    text_lens: torch.Tensor,                  # [B] int32
+    *,
+    k_scale: torch.Tensor,                    # [B, H_kv, C] float32
+    v_scale: torch.Tensor,
+    dtype: torch.dtype = torch.bfloat16,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The Keys and Values an 8-bit text cache stands for: (k, v), each
+    [B, H_kv, C, D] in ``dtype`` (float32, bfloat16 or float16), e4m3 * scale
+    rounded once for rows s < text_lens[b] and 0 after them."""
+    if k_text.dim() != 4:
+        raise ValueError("k_text must be a uint8 (e4m3) [B, H_kv, C, D]")
+    k_text, v_text = _as_u8(k_text), _as_u8(v_text)
+    dev = _lib.require_one_device(k_text, v_text, text_lens, k_scale, v_scale)
+    k = torch.empty(k_text.shape, dtype=dtype, device=dev)
+    v = torch.empty(k_text.shape, dtype=dtype, device=dev)
+    D = _lib.describe
+    _lib.check(_lib.load().rtk_read_text(D(k_text), D(v_text), D(k_scale), D(v_scale), D(text_lens), D(k), D(v),
+                                         _stream(dev)))
+    return k, v
+
+
+def verify_drafts(
+    target_logits: torch.Tensor,              # [B, T + 1, V]
+    draft_tokens: torch.Tensor,               # [B, T] int64
+    draft_logits: Optional[torch.Tensor],     # [B, T, V] or None
+    uniforms: torch.Tensor,                   # [B, T] float32 in [0, 1)
+    noise: torch.Tensor,                      # [B, V] float32, Exp(1) draws
+    temperature: torch.Tensor,                # [B] float32, <= 0: greedy
+    *,
+    draft_lens: Optional[torch.Tensor] = None,   # [B] int32
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Which drafted tokens the target model accepts, and the token that follows:
+    returns (tokens [B, T + 1] int64 -- the accepted drafts, the next token, then
+    -1 -- and accepted [B] int32, the number of accepted drafts).
+
+    Row j of ``target_logits`` scores the token after draft j - 1.  With p_j and
+    q_j the two softmaxes at the question's temperature, draft x_j is accepted
+    when u_j q_j(x_j) < p_j(x_j) and every draft before it was; after the first
+    rejection the next token is drawn from max(p - q, 0) normalised, after the
+    last draft from p, in both cases as argmax_i weight_i / noise_i, an
+    exponential race (lowest index on ties).  The tokens so drawn are
+    distributed as the target model's own.  Without ``draft_logits`` the drafts
+    are proposals without probabilities (q_j is 1 at x_j).  A greedy question
+    accepts drafts that are the target's argmax and continues with the argmax.
+    fp32, bf16 or fp16 logits; no host synchronisation."""
+    if target_logits.dim() != 3:
+        raise ValueError("target_logits must be [B, T + 1, V]")
+    dev = _lib.require_one_device(target_logits, draft_tokens, draft_logits, uniforms, noise, temperature, draft_lens)
+    b, rows, vocab = target_logits.shape
+    lib = _lib.load()
+    tokens = torch.empty(b, rows, dtype=torch.int64, device=dev)
+    accepted = torch.empty(b, dtype=torch.int32, device=dev)
+    key = ("vd", b, rows - 1, vocab)
+    need = _ws_size_cache.get(key)
+    if need is None:
+        need = _ws_size_cache[key] = lib.rtk_verify_drafts_workspace_size(*key[1:])
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    D = _lib.describe
+    _lib.check(lib.rtk_verify_drafts(D(target_logits), D(draft_tokens), D(draft_logits), D(uniforms), D(noise),
+                                     D(temperature), D(draft_lens), D(tokens), D(accepted), ws.data_ptr(), need,
+                                     _stream(dev)))
+    return tokens, accepted
+
+
 __all__ = ["ROTATEK_KERNEL", "rotatek_decode", "full_channel_decode", "think_decode", "think_selection",
-           "quantize_visual_fp8", "rotatek_decode_fp8", "pack_spark_indices", "spark_decode"]
+           "quantize_visual_fp8", "rotatek_decode_fp8", "pack_spark_indices", "spark_decode",
+           "rotatek_shared_decode", "append_text", "read_text", "verify_drafts"]

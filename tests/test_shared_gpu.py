@@ -1,0 +1,494 @@
+"""Shared-prefix attention, text caches and draft verification on a B200 against
+their float64 definitions (oracle/shared.py).
+
+Attention tolerance, for an output o with A = sum w |v| over its softmax weights:
+  16-bit  u |o| + (2 u + 2^-11) A, u = half a unit in the last place (2^-9 bf16,
+          2^-12 fp16): the output's rounding; each weight rounded to 16 bits once in
+          the numerator (u) and once in the normaliser (u); and logits off by up to
+          2^-12 (fp32 sums of 128 products and the rotated query in two 16-bit parts),
+          which moves a weight by 2^-12 in each
+  fp32    2^-22 |o| + 2^-14 A: logits of size up to about 50 from fp32 sums of up to 256
+          products (256 * 2^-24 * 50 / 16 < 2^-15), twice
+Quantisation and reading back are exact.  Verification is exact wherever no
+decision of the question is closer than 1e-4 (relative) to going the other way.
+"""
+import math
+
+import pytest
+import torch
+
+from oracle import shared as osh
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+HALF_ULP = {torch.bfloat16: 2.0 ** -9, torch.float16: 2.0 ** -12}
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _library():
+    from rotatek_b200 import _lib
+    _lib.load()
+    yield
+    assert _lib.read_status() == 0
+
+
+def make(P, N, T, hq, hk, sv, sf, cap, dk, dtype=torch.bfloat16, fp8=False, mask=None, bias=True, lens=None, D=128,
+         seed=0, std=1.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    B = P * N
+
+    def n(*s, scale=1.0):
+        return (torch.randn(*s, generator=g, device=DEV) * scale).to(dtype)
+
+    R = torch.linalg.qr(torch.randn(P, hk, D, dk, generator=g, device=DEV))[0].to(dtype)
+    spread = torch.exp(-torch.arange(dk, device=DEV) / 10.0)
+    spread = torch.sqrt(D * spread / spread.sum())
+    a = dict(q=n(B, T, hq, D, scale=std), R_partial=R, delta_mu=n(P, hk, D, scale=0.3) if bias else None,
+             k_full=n(P, hk, sf, D), v_full=n(P, hk, sf, D), mask_full=None,
+             k_sparse=(torch.randn(P, hk, sv, dk, generator=g, device=DEV) * spread).to(dtype),
+             v_sparse=n(P, hk, sv, D), k_text=n(B, hk, cap, D), v_text=n(B, hk, cap, D), num_kv_groups=hq // hk)
+    if mask is not None:
+        a["mask_full"] = (torch.rand(P, sf, generator=g, device=DEV) < mask).to(torch.uint8)
+    if lens is None:
+        lens = [cap - (i * max(1, cap // 3)) % (cap + 1) for i in range(B)]
+    a["text_lens"] = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    if fp8:
+        for side in ("k", "v"):
+            val, scale = osh.quantize_rows(a[f"{side}_text"])
+            a[f"{side}_text"] = val.float().to(torch.float8_e4m3fn).to(DEV).view(torch.uint8)
+            a[f"{side}_scale"] = scale.to(DEV)
+    return a
+
+
+def check(a, **kw):
+    from rotatek_b200.kernels import rotatek_shared_decode
+    got = rotatek_shared_decode(**a, **kw)
+    torch.cuda.synchronize()
+    compare(got, a)
+    return got
+
+
+def compare(got, a):
+    want, mag = osh.shared_decode(**a)
+    got64 = got.cpu().double()
+    if a["q"].dtype == torch.float32:
+        tol = 2.0 ** -22 * want.abs() + 2.0 ** -14 * mag
+    else:
+        u = HALF_ULP[a["q"].dtype]
+        tol = u * want.abs() + (2 * u + 2.0 ** -11) * mag
+        if a["q"].dtype == torch.float16:
+            tol = tol + 2.0 ** -25          # half a step of the subnormals
+    bad = (got64 - want).abs() > tol
+    assert torch.isfinite(got64).all()
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()}, worst {((got64 - want).abs() / tol.clamp_min(1e-30)).max():.2f}"
+
+
+SHAPES = [
+    # P, N, T, H_q, H_kv, S_v, S_f, C, D_keep
+    (1, 2, 1, 28, 4, 1000, 64, 64, 32),
+    (1, 1, 1, 4, 4, 1, 1, 1, 16),
+    (1, 1, 1, 8, 2, 127, 63, 65, 64),
+    (1, 3, 2, 8, 2, 129, 65, 33, 32),
+    (2, 3, 5, 28, 4, 700, 100, 130, 32),
+    (1, 40, 1, 14, 2, 300, 31, 17, 64),         # 280 rows of a head: three row tiles
+    (3, 2, 8, 16, 2, 257, 5, 200, 16),
+    (1, 2, 3, 32, 2, 140, 70, 96, 32),          # 16 query heads per KV head, 48 rows of a question
+    (1, 1, 16, 24, 2, 90, 10, 70, 32),          # 192 rows of one question
+    (2, 5, 1, 4, 4, 513, 0, 40, 32),            # no prompt
+    (2, 2, 2, 8, 4, 0, 77, 50, 32),             # no visual span
+    (1, 4, 2, 8, 2, 200, 20, 0, 32),            # no text
+    (1, 2, 4, 8, 2, 0, 0, 90, 32),              # text alone
+]
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("dtype,fp8", [(torch.bfloat16, False), (torch.float16, False), (torch.bfloat16, True),
+                                       (torch.float16, True)])
+def test_decode_shapes(shape, dtype, fp8):
+    check(make(*shape, dtype=dtype, fp8=fp8, seed=sum(shape)))
+
+
+@pytest.mark.parametrize("shape,D", [((1, 2, 2, 8, 2, 50, 20, 30, 32), 128), ((2, 2, 3, 6, 2, 33, 9, 12, 24), 64),
+                                     ((1, 3, 1, 4, 4, 40, 7, 9, 5), 40), ((1, 1, 2, 4, 2, 20, 4, 6, 200), 256)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_decode_any_width_and_type(shape, D, dtype, fp8):
+    check(make(*shape, dtype=dtype, D=D, fp8=fp8, seed=D, mask=0.7))
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("T", [1, 4])
+def test_decode_lengths(T, fp8):
+    """Every kind of length: none, fewer than the queries, one, tile edges, the
+    capacity, past it and negative (both clamped)."""
+    lens = [0, 1, 2, 3, 4, 15, 16, 17, 31, 32, 33, 63, 64, 65, 95, 96, 99, 100, 250, -3]
+    check(make(1, len(lens), T, 8, 2, 150, 40, 100, 32, fp8=fp8, lens=lens, seed=5))
+
+
+@pytest.mark.parametrize("mask", [0.0, 0.05, 0.8, 1.0])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_decode_prompt_mask(mask, dtype):
+    check(make(2, 3, 2, 8, 2, 100, 333, 20, 32, dtype=dtype, mask=mask, seed=7))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_decode_rows_that_see_nothing_are_zero(dtype, fp8):
+    """All prompt tokens masked, no visual span, and a length below the drafts'."""
+    a = make(1, 4, 3, 8, 2, 0, 50, 20, 32, dtype=dtype, fp8=fp8, mask=0.0, lens=[0, 1, 2, 3])
+    got = check(a)
+    for b, n in enumerate([0, 1, 2, 3]):
+        for t in range(3):
+            assert (got[b, t] == 0).all().item() == (n - (2 - t) <= 0)
+    none = make(1, 2, 1, 4, 2, 0, 0, 0, 16, dtype=dtype)
+    assert (check(none) == 0).all()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_decode_ignores_what_is_not_seen(bad, dtype, fp8):
+    """Masked prompt tokens and text rows past the length hold NaN / infinity in
+    Keys, Values and scales: outputs are those without them, to the bit."""
+    a = make(2, 3, 2, 8, 2, 140, 200, 80, 32, dtype=dtype, fp8=fp8, mask=0.7, lens=[0, 3, 17, 64, 79, 80], seed=9)
+    from rotatek_b200.kernels import rotatek_shared_decode
+    clean = rotatek_shared_decode(**a)
+    hidden = (a["mask_full"] == 0)[:, None, :, None]
+    past = (torch.arange(80, device=DEV) >= a["text_lens"][:, None])[:, None, :, None]
+    for name in ("k_full", "v_full"):
+        a[name] = torch.where(hidden, torch.tensor(bad, device=DEV, dtype=dtype), a[name])
+    for name in ("k_text", "v_text"):
+        fill = torch.tensor(0x7F, device=DEV, dtype=torch.uint8) if fp8 else torch.tensor(bad, device=DEV, dtype=dtype)
+        a[name] = torch.where(past, fill, a[name])
+    if fp8:
+        for name in ("k_scale", "v_scale"):
+            a[name] = torch.where(past[..., 0], torch.tensor(bad, device=DEV), a[name])
+    dirty = check(a)
+    assert torch.equal(clean, dirty)
+
+
+def test_decode_extreme_logits():
+    """Logits of hundreds, of both signs: one token takes all the weight."""
+    for dtype in (torch.bfloat16, torch.float16):
+        a = make(1, 2, 2, 8, 2, 300, 70, 90, 32, dtype=dtype, std=1.0, seed=3)
+        a["q"] = a["q"] * 16
+        a["k_full"] = a["k_full"] * 4
+        from rotatek_b200.kernels import rotatek_shared_decode
+        got = rotatek_shared_decode(**a).cpu().double()
+        want, mag = osh.shared_decode(**a)
+        # logits reach ~700 with 2^-16 relative error from the rotated query's two parts:
+        # weights move by up to 2 * 700 * 2^-16 log2(e)
+        tol = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -5) * mag
+        assert ((got - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_decode_text_scales_of_any_size(fp8):
+    """Value rows whose sizes differ by 2^40 within a question (and rows of zeros)."""
+    a = make(1, 2, 2, 8, 2, 64, 10, 150, 32, dtype=torch.bfloat16, lens=[150, 131], seed=11)
+    size = torch.exp2(torch.randint(-30, 11, (2, 2, 150, 1), device=DEV).float())
+    size[:, :, 7] = 0
+    a["v_text"] = (a["v_text"].float() * size).to(torch.bfloat16)
+    if fp8:
+        for side in ("k", "v"):
+            val, scale = osh.quantize_rows(a[f"{side}_text"])
+            a[f"{side}_text"] = val.float().to(torch.float8_e4m3fn).to(DEV).view(torch.uint8)
+            a[f"{side}_scale"] = scale.to(DEV)
+    check(a)
+
+
+def test_decode_strided_and_unaligned_views():
+    a = make(2, 2, 3, 8, 2, 150, 60, 40, 32, seed=13)
+    qkv = torch.randn(4, 3, 12, 128, device=DEV).to(torch.bfloat16)
+    check({**a, "q": qkv[:, :, :8]})                                        # fused projection slice
+    wide = torch.randn(4, 3, 8, 130, device=DEV).to(torch.bfloat16)
+    check({**a, "q": wide[..., 1:129]})                                     # 2-byte aligned queries
+    cache = torch.randn(2, 2, 300, 128, device=DEV).to(torch.bfloat16)
+    check({**a, "v_sparse": cache[:, :, 60:210], "v_full": cache[:, :, :60]})
+    bshd = torch.randn(4, 40, 2, 128, device=DEV).to(torch.bfloat16)
+    check({**a, "k_text": bshd.transpose(1, 2)})                            # tokens before heads
+    odd = torch.randn(4, 2, 40, 129, device=DEV).to(torch.bfloat16)
+    check({**a, "v_text": odd[..., 1:]})                                    # rows no 16-byte copy can take
+    oddk = torch.randn(2, 2, 150, 33, device=DEV).to(torch.bfloat16)
+    check({**a, "k_sparse": oddk[..., :32]})
+    one = a["k_full"][:1].expand(2, -1, -1, -1)                             # both prefixes are one tensor
+    check({**a, "k_full": one})
+    lens = torch.tensor([40, 0, 9, 0, 33, 0, 2, 0], dtype=torch.int32, device=DEV)
+    check({**a, "text_lens": lens[::2]})
+    mask = (torch.rand(60, 2, device=DEV) < 0.6).to(torch.uint8)
+    check({**a, "mask_full": mask.t()})
+
+
+def test_decode_into_a_given_tensor():
+    a = make(1, 3, 2, 8, 2, 100, 30, 20, 32, seed=15)
+    from rotatek_b200.kernels import rotatek_shared_decode
+    buf = torch.zeros(3, 8, 2, 128, device=DEV, dtype=torch.bfloat16)
+    got = check(a, out=buf.transpose(1, 2))
+    assert got.data_ptr() == buf.data_ptr()
+    odd = torch.zeros(3, 2, 8, 131, device=DEV, dtype=torch.bfloat16)
+    compare(rotatek_shared_decode(**a, out=odd[..., 1:129]), a)
+    assert (odd[..., 0] == 0).all() and (odd[..., 129:] == 0).all()
+
+
+def test_decode_is_the_same_each_time_and_on_other_streams():
+    from rotatek_b200.kernels import rotatek_shared_decode
+    a = make(2, 9, 2, 28, 4, 2000, 100, 150, 32, fp8=True, seed=17)
+    b = make(1, 5, 1, 28, 4, 1500, 64, 90, 32, seed=18)
+    first, other = rotatek_shared_decode(**a), rotatek_shared_decode(**b)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = []
+    for i in range(10):
+        for s, args in zip(streams, (a, b)):
+            with torch.cuda.stream(s):
+                outs.append(rotatek_shared_decode(**args))
+    torch.cuda.synchronize()
+    for i in range(0, 20, 2):
+        assert torch.equal(outs[i], first) and torch.equal(outs[i + 1], other)
+
+
+def test_decode_captured_and_replayed_while_lengths_grow():
+    from rotatek_b200.kernels import rotatek_shared_decode
+    a = make(1, 4, 1, 8, 2, 500, 30, 64, 32, fp8=True, lens=[1, 2, 3, 4], seed=19)
+    rotatek_shared_decode(**a)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = rotatek_shared_decode(**a)
+    for step in (0, 1, 30, 60):
+        a["text_lens"].copy_(torch.tensor([1, 2, 3, 4]) + step)
+        g.replay()
+        torch.cuda.synchronize()
+        compare(out, a)
+
+
+def test_decode_equals_the_decode_of_each_question_alone():
+    """A question's attention does not depend on who shares its prefix, and is the
+    framework's rotatek_decode of its own copy of everything."""
+    from rotatek_b200.kernels import rotatek_decode, rotatek_shared_decode
+    a = make(1, 3, 1, 28, 4, 600, 40, 24, 32, lens=[24, 10, 1], seed=21)
+    got = rotatek_shared_decode(**a)
+    for b, n in enumerate([24, 10, 1]):
+        ref, _, _ = rotatek_decode(
+            a["q"][b:b + 1, 0], a["R_partial"], a["delta_mu"],
+            torch.cat([a["k_full"], a["k_text"][b:b + 1, :, :n]], 2),
+            torch.cat([a["v_full"], a["v_text"][b:b + 1, :, :n]], 2), None, a["k_sparse"], a["v_sparse"], 7)
+        # each is within its tolerance of the same float64 value
+        assert (got[b:b + 1].float() - ref.float()).abs().max() < 2.0 ** -6
+
+
+# ------------------------------------------------------------------ text caches
+def filled_caches(B, H, C, D, dtype, fp8, seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    if not fp8:
+        return [torch.randn(B, H, C, D, generator=g, device=DEV).to(dtype) for _ in range(2)], [None, None]
+    return ([torch.randint(0, 120, (B, H, C, D), generator=g, device=DEV, dtype=torch.uint8) for _ in range(2)],
+            [torch.rand(B, H, C, generator=g, device=DEV) for _ in range(2)])
+
+
+@pytest.mark.parametrize("B,H,T,C,D", [(1, 1, 1, 1, 128), (3, 4, 1, 50, 128), (2, 8, 77, 200, 128), (5, 3, 7, 9, 128),
+                                       (2, 2, 5, 16, 64), (2, 3, 4, 8, 33), (40, 8, 33, 64, 128)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("fp8", [True, False])
+def test_append(B, H, T, C, D, dtype, fp8):
+    """Written rows are exact, all others keep their bits; rows past the capacity
+    are dropped, counts bound each question's rows."""
+    from rotatek_b200.kernels import append_text
+    g = torch.Generator(device=DEV).manual_seed(B * T + D)
+    kv = torch.randn(B, T, 2 * H, D, generator=g, device=DEV).mul_(
+        torch.exp2(torch.randint(-12, 9, (B, T, 2 * H, 1), generator=g, device=DEV).float())).to(dtype)
+    kv[0, 0, 0] = 0
+    new = [kv[:, :, :H].transpose(1, 2), kv[:, :, H:].transpose(1, 2)]
+    for counted in (False, True):
+        caches, scales = filled_caches(B, H, C, D, dtype, fp8, 3)
+        lens = [(7 * i) % (C + 2) - 1 if B > 1 else 0 for i in range(B)]
+        counts = [(i * 3) % (T + 1) for i in range(B)] if counted else [T] * B
+        want = [c.clone() for c in caches]
+        want_s = [None if s is None else s.clone() for s in scales]
+        quant = [osh.quantize_rows(n) for n in new]
+        for i in range(B):
+            for t in range(counts[i]):
+                at = lens[i] + t
+                if 0 <= at < C:
+                    for side in range(2):
+                        if fp8:
+                            want[side][i, :, at] = quant[side][0][i, :, t].float().to(torch.float8_e4m3fn).view(
+                                torch.uint8).to(DEV)
+                            want_s[side][i, :, at] = quant[side][1][i, :, t].to(DEV)
+                        else:
+                            want[side][i, :, at] = new[side][i, :, t]
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+        append_text(new[0], new[1], i32(lens), caches[0], caches[1], k_scale=scales[0], v_scale=scales[1],
+                    counts=i32(counts) if counted else None)
+        for side in range(2):
+            assert torch.equal(caches[side], want[side])
+            if fp8:
+                assert torch.equal(scales[side], want_s[side])
+
+
+def test_append_special_values():
+    """Rows of zeros, subnormals, values at the rounding ties, infinities and NaN."""
+    from rotatek_b200.kernels import append_text
+    x = torch.zeros(1, 1, 8, 128, device=DEV, dtype=torch.float32)
+    x[0, 0, 1] = 1e-41
+    x[0, 0, 2, :5] = torch.tensor([448.0, 17.0, 19.0, 2.0 ** -10, -(2.0 ** -9) * 1.5])
+    x[0, 0, 3, :3] = torch.tensor([math.inf, 3.0, -1.0])
+    x[0, 0, 4, :3] = torch.tensor([math.nan, 3.0, -1.0])
+    x[0, 0, 5] = -math.inf
+    x[0, 0, 6] = torch.linspace(-3.3e38, 3.3e38, 128)
+    x[0, 0, 7] = 2.0 ** -120 * torch.linspace(-1, 1, 128)
+    for dtype in (torch.float32, torch.bfloat16):
+        y = x.to(dtype)
+        caches, scales = filled_caches(1, 1, 8, 128, dtype, True, 1)
+        append_text(y, y, torch.zeros(1, dtype=torch.int32, device=DEV), *caches, k_scale=scales[0], v_scale=scales[1])
+        val, scale = osh.quantize_rows(y)
+        got = osh.e4m3_values(caches[0].cpu())
+        assert torch.equal(scales[0].cpu(), scale)
+        assert torch.equal(torch.isnan(got), torch.isnan(val))
+        assert torch.equal(torch.nan_to_num(got, nan=0.0), torch.nan_to_num(val, nan=0.0))
+
+
+@pytest.mark.parametrize("B,H,C,D", [(1, 1, 1, 128), (3, 4, 50, 128), (2, 8, 333, 128), (2, 3, 20, 64), (2, 2, 9, 33)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_read(B, H, C, D, dtype):
+    from rotatek_b200.kernels import read_text
+    caches, scales = filled_caches(B, H, C, D, dtype, True, 5)
+    lens = torch.tensor([(C - 5 * i) if i % 3 < 2 else 0 for i in range(B)], dtype=torch.int32, device=DEV)
+    past = (torch.arange(C, device=DEV) >= lens[:, None])[:, None]
+    for s in scales:
+        s.masked_fill_(past, math.nan)             # never read
+    got = read_text(*caches, lens, k_scale=scales[0], v_scale=scales[1], dtype=dtype)
+    for out, cache, scale in zip(got, caches, scales):
+        want = torch.where(past[..., None], 0.0, cache.view(torch.float8_e4m3fn).float() * scale[..., None]).to(dtype)
+        assert torch.equal(out, want)
+
+
+def test_append_then_read_strided():
+    """Caches with tokens before heads, and as views of one buffer."""
+    from rotatek_b200.kernels import append_text, read_text
+    g = torch.Generator(device=DEV).manual_seed(2)
+    both = torch.zeros(3, 40, 2, 4, 128, device=DEV, dtype=torch.uint8)
+    k8, v8 = both[:, :, 0].transpose(1, 2), both[:, :, 1].transpose(1, 2)
+    sc = torch.zeros(3, 4, 2, 40, device=DEV)
+    new = torch.randn(3, 4, 11, 128, generator=g, device=DEV).to(torch.bfloat16)
+    lens = torch.tensor([0, 5, 29], dtype=torch.int32, device=DEV)
+    append_text(new, new * 2, lens, k8, v8, k_scale=sc[:, :, 0], v_scale=sc[:, :, 1])
+    k, v = read_text(k8, v8, lens + 11, k_scale=sc[:, :, 0], v_scale=sc[:, :, 1], dtype=torch.float32)
+    val, scale = osh.quantize_rows(new)
+    for i, n in enumerate([0, 5, 29]):
+        want = (val[i].float() * scale[i][..., None]).to(DEV)
+        assert torch.equal(k[i, :, n:n + 11], want)
+        assert torch.equal(v[i, :, n:n + 11], want * 2)
+        assert (k[i, :, :n] == 0).all() and (k[i, :, n + 11:] == 0).all()
+
+
+# ------------------------------------------------------------------ verification
+def make_verify(B, T, V, dtype, logits, seed, spread=2.5, near=0.7):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    target = torch.randn(B, T + 1, V, generator=g, device=DEV) * spread
+    draft = target[:, :T] + near * torch.randn(B, T, V, generator=g, device=DEV)
+    temperature = 0.5 + torch.rand(B, generator=g, device=DEV)
+    temperature[::3] = 0.0
+    soft = torch.softmax(draft / temperature.clamp_min(0.2)[:, None, None], -1)
+    drafts = torch.where(temperature[:, None] > 0, torch.multinomial(soft.view(-1, V), 1, generator=g).view(B, T)
+                         if T else torch.zeros(B, 0, dtype=torch.int64, device=DEV), draft.argmax(-1))
+    lens = torch.tensor([(T - i) % (T + 1) for i in range(B)], dtype=torch.int32, device=DEV)
+    return dict(target_logits=target.to(dtype), draft_tokens=drafts, draft_logits=draft.to(dtype) if logits else None,
+                uniforms=torch.rand(B, T, generator=g, device=DEV),
+                noise=torch.empty(B, V, device=DEV).exponential_(generator=g).clamp_min_(1e-9),
+                temperature=temperature, draft_lens=lens)
+
+
+def check_verify(a):
+    from rotatek_b200.kernels import verify_drafts
+    tokens, accepted = verify_drafts(**a)
+    want_t, want_a, margin = osh.verify(a["target_logits"], a["draft_tokens"], a["draft_logits"], a["uniforms"],
+                                        a["noise"], a["temperature"], a.get("draft_lens"))
+    sure = margin > 1e-4
+    assert sure.float().mean() > 0.9
+    assert torch.equal(tokens.cpu()[sure], want_t[sure]) and torch.equal(accepted.cpu()[sure], want_a[sure])
+    return tokens, accepted
+
+
+@pytest.mark.parametrize("B,T,V", [(1, 1, 7), (2, 0, 100), (7, 3, 1000), (33, 5, 4097), (4, 8, 32000), (3, 64, 513),
+                                   (2, 2, 131071), (5, 4, 8192), (3, 2, 1)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("logits", [True, False])
+def test_verify(B, T, V, dtype, logits):
+    check_verify(make_verify(B, T, V, dtype, logits, seed=B + T + V))
+
+
+def test_verify_without_lengths_and_strided():
+    a = make_verify(6, 4, 3001, torch.bfloat16, True, 1)
+    del a["draft_lens"]
+    check_verify(a)
+    wide = torch.randn(6, 5, 3100, device=DEV).to(torch.bfloat16)
+    wide[:, :, 50:3051] = a["target_logits"]
+    check_verify({**a, "target_logits": wide[:, :, 50:3051], "uniforms": a["uniforms"].t().contiguous().t()})
+
+
+def test_verify_masked_and_tied_logits():
+    """-inf logits (tokens that may not follow), whole rows of them, equal logits."""
+    from rotatek_b200.kernels import verify_drafts
+    a = make_verify(9, 3, 700, torch.float16, True, 4)
+    ban = torch.rand(9, 4, 700, device=DEV) < 0.9
+    a["target_logits"] = a["target_logits"].masked_fill(ban, -math.inf)
+    check_verify(a)
+    a["target_logits"] = torch.zeros_like(a["target_logits"])            # ties: the lowest index
+    a["temperature"] = torch.zeros_like(a["temperature"])
+    tokens, accepted = check_verify(a)
+    assert set(tokens[torch.arange(9), accepted.long()].tolist()) == {0}
+    a["noise"] = torch.ones_like(a["noise"])
+    a["temperature"] = torch.ones_like(a["temperature"])
+    a["draft_lens"] = torch.zeros_like(a["draft_lens"])
+    tokens, accepted = verify_drafts(**a)                                 # a race with equal runners
+    assert (tokens[:, 0] == 0).all() and (tokens[:, 1:] == -1).all() and (accepted == 0).all()
+    a["target_logits"] = torch.full_like(a["target_logits"], -math.inf)   # nothing may follow
+    tokens, accepted = verify_drafts(**a)
+    assert (tokens[:, 0] == 0).all() and (accepted == 0).all()
+
+
+def test_verify_equal_models_accept_all_and_bad_ids_are_rejected():
+    from rotatek_b200.kernels import verify_drafts
+    a = make_verify(8, 4, 2000, torch.float32, True, 6)
+    a["draft_logits"] = a["target_logits"][:, :4].contiguous()
+    a["temperature"] = torch.full_like(a["temperature"], 0.8)
+    del a["draft_lens"]
+    _, accepted = verify_drafts(**a)
+    assert (accepted == 4).all()
+    # rejected where nothing is left of the difference: the target's own race
+    a["draft_tokens"][:, 1] = -1
+    a["draft_tokens"][1, 1] = 2000
+    tokens, accepted = verify_drafts(**a)
+    assert (accepted == 1).all()
+    p = torch.softmax(a["target_logits"][:, 1].double() / 0.8, -1) / a["noise"].double()
+    assert torch.equal(tokens[:, 1], p.argmax(-1)) and (tokens[:, 2:] == -1).all()
+
+
+def test_verify_draws_the_targets_distribution():
+    """Over many questions the first token follows p, whatever the draft model is:
+    each of 6 tokens within 5 standard deviations."""
+    from rotatek_b200.kernels import verify_drafts
+    B, V = 60000, 6
+    g = torch.Generator(device=DEV).manual_seed(8)
+    tl, dl = torch.randn(V, generator=g, device=DEV), torch.randn(V, generator=g, device=DEV)
+    drafts = torch.multinomial(torch.softmax(dl, 0), B, replacement=True, generator=g)[:, None]
+    tokens, accepted = verify_drafts(
+        torch.stack([tl, tl]).expand(B, 2, V), drafts, dl.expand(B, 1, V), torch.rand(B, 1, generator=g, device=DEV),
+        torch.empty(B, V, device=DEV).exponential_(generator=g), torch.ones(B, device=DEV))
+    p = torch.softmax(tl.double(), 0).cpu()
+    freq = torch.bincount(tokens[:, 0].cpu(), minlength=V).double() / B
+    assert ((freq - p).abs() < 5 * torch.sqrt(p * (1 - p) / B)).all()
+    assert 0.05 < accepted.float().mean() < 0.999
+
+
+def test_verify_captured():
+    from rotatek_b200.kernels import verify_drafts
+    a = make_verify(4, 3, 5000, torch.bfloat16, True, 10)
+    want = verify_drafts(**a)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = verify_drafts(**a)
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
