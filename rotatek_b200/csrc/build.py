@@ -21,7 +21,7 @@ PKG = os.path.dirname(CSRC)
 REPO = os.path.dirname(PKG)
 LIB_NAME = "librotatek_b200.so"
 SOURCES = ["capi.cu", "decode_tc.cu", "decode_simt.cu", "decode_static.cu", "quant_fp8.cu", "spark_pack.cu", "cov_tc.cu", "kproj_tc.cu", "eigen.cu",
-           "rotate.cu", "selftest.cu", "capi_shared.cu", "shared_simt.cu", "text_cache.cu", "verify.cu"]
+           "rotate.cu", "selftest.cu", "capi_shared.cu", "shared_simt.cu", "shared_prefix.cu", "shared_text.cu", "shared_merge.cu", "text_cache.cu", "verify.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -259,6 +259,17 @@ size_t decode_counter_bytes(int64_t batch, int64_t q_heads) { return counter_end
 
 // Record `msg` as this thread's rtk_last_error() and return `code`.
 int report_error(int code, const char *msg) { return fail(code, "%s", msg); }
+
+int device_sms(int device) { return sm_count(device); }
+
+// A 4-D tensor map over a 16-bit [B, H, S, D] tensor with boxes of box_rows x
+// box_inner, swizzled over the box's row; false where TMA cannot describe it.
+bool encode_rows_map(CUtensorMap *map, const rtk_tensor *t, int box_inner, int box_rows) {
+  View4 v;
+  if (!as4(t, v)) return false;
+  return encode_map(map, v, t->dtype == RTK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                    box_inner, box_rows, swizzle_for_row_bytes(box_inner * 2));
+}
 }  // namespace rtk
 
 namespace {

@@ -16,6 +16,10 @@
 #include "decode.h"
 #include "shared.h"
 
+namespace rtk {
+bool encode_rows_map(CUtensorMap *map, const rtk_tensor *t, int box_inner, int box_rows);   // capi.cu
+}
+
 namespace {
 
 int fail(int code, const char *fmt, ...) {
@@ -62,6 +66,44 @@ bool present(const rtk_tensor *t) {
 
 constexpr int64_t kMaxInt = (1ll << 31) - 1;
 
+// Rows (the last dimension) that 16-byte accesses can take: unit stride, an aligned
+// address and strides of whole 16 bytes wherever a dimension has more than one entry.
+bool rows16(const rtk_tensor *t, int esize) {
+  const int n = t->ndim;
+  if (t->shape[n - 1] > 1 && t->stride[n - 1] != 1) return false;
+  if (reinterpret_cast<uintptr_t>(t->data) % 16 != 0) return false;
+  for (int i = 0; i + 1 < n; ++i)
+    if (t->shape[i] > 1 && (t->stride[i] * esize) % 16 != 0) return false;
+  return true;
+}
+
+// ---- workspace of the tensor-core path: a status word for callers that give none,
+// the prefix partials, the text's
+struct SharedSpace {
+  size_t prefix_ml, prefix_acc, text_ml, text_acc, bytes;
+};
+
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+SharedSpace shared_space(const rtk::PrefixSplit &sp, int64_t batch, int64_t kv_heads, int64_t rows, int64_t chunks) {
+  SharedSpace w;
+  const size_t slots = (size_t)sp.slots() * 128, text = (size_t)(batch * kv_heads * chunks * rows);
+  w.prefix_ml = 256;
+  w.prefix_acc = up256(w.prefix_ml + slots * 8);
+  w.text_ml = up256(w.prefix_acc + slots * 512);
+  w.text_acc = up256(w.text_ml + text * 8);
+  w.bytes = up256(w.text_acc + text * 512);
+  return w;
+}
+
+int64_t text_chunks(int64_t cap) { return (cap + rtk::kTextChunk - 1) / rtk::kTextChunk; }
+
+int current_device() {
+  int d = 0;
+  cudaGetDevice(&d);
+  return d;
+}
+
 }  // namespace
 
 extern "C" {
@@ -69,9 +111,11 @@ extern "C" {
 size_t rtk_shared_decode_workspace_size(int64_t prefixes, int64_t batch, int64_t tokens, int64_t q_heads,
                                         int64_t kv_heads, int64_t seq_full, int64_t seq_sparse, int64_t text_cap,
                                         int32_t device) {
-  (void)prefixes; (void)batch; (void)tokens; (void)q_heads; (void)kv_heads; (void)seq_full; (void)seq_sparse;
-  (void)text_cap; (void)device;
-  return 256;
+  if (prefixes < 1 || kv_heads < 1 || batch < 0 || tokens < 0) return 0;
+  const int64_t groups = q_heads / kv_heads;
+  const rtk::PrefixSplit sp =
+      rtk::prefix_split(prefixes, batch / prefixes, tokens, groups, kv_heads, seq_full, seq_sparse, rtk::device_sms(device));
+  return shared_space(sp, batch, kv_heads, tokens * groups, text_chunks(text_cap)).bytes;
 }
 
 int rtk_shared_decode(const rtk_tensor *q, const rtk_tensor *R_partial, const rtk_tensor *delta_mu,
@@ -147,9 +191,66 @@ int rtk_shared_decode(const rtk_tensor *q, const rtk_tensor *R_partial, const rt
   p.lens = static_cast<const int *>(text_lens->data); p.lens_s = text_lens->stride[0];
   p.out = out->data;
   for (int i = 0; i < 4; ++i) p.o_s[i] = out->stride[i];
-  (void)workspace; (void)workspace_bytes; (void)status;
-  const cudaError_t e = rtk::launch_shared_simt(p, static_cast<cudaStream_t>(stream));
-  if (e != cudaSuccess) return cuda_fail(e, "shared decode launch");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+
+  // ---- tensor-core path
+  bool tc = (q->dtype == RTK_BF16 || q->dtype == RTK_F16) && D == 128 && rows16(q, 2) && (C == 0 || (rows16(k_text, fp8 ? 1 : 2) && rows16(v_text, fp8 ? 1 : 2)));
+  if (Sv > 0)
+    tc = tc && (DK == 16 || DK == 32 || DK == 64) && rows16(R_partial, 2) && (delta_mu == nullptr || delta_mu->stride[2] == 1);
+  rtk::PrefixMaps maps;
+  std::memset(&maps, 0, sizeof(maps));
+  if (tc && Sf > 0) tc = rtk::encode_rows_map(&maps.kf, k_full, 64, 64) && rtk::encode_rows_map(&maps.vf, v_full, 64, 64);
+  if (tc && Sv > 0)
+    tc = rtk::encode_rows_map(&maps.ks, k_sparse, (int)DK, 128) && rtk::encode_rows_map(&maps.vs, v_sparse, 64, 128);
+  if (!tc) {
+    const cudaError_t e = rtk::launch_shared_simt(p, st);
+    if (e != cudaSuccess) return cuda_fail(e, "shared decode (generic kernel) launch");
+    return RTK_OK;
+  }
+  const int device = current_device();
+  const rtk::PrefixSplit sp =
+      rtk::prefix_split(P, B / P, T, num_kv_groups, Hkv, Sf, Sv, rtk::device_sms(device));
+  const int64_t rows = T * num_kv_groups, chunks = text_chunks(C);
+  if ((int64_t)sp.rows != B / P * rows || (int64_t)P * Hkv * sp.row_tiles > kMaxInt / 256 || chunks > 65535 ||
+      rows > 65535 * 16 || B * Hkv > kMaxInt)
+    return fail(RTK_ERR_UNSUPPORTED, "too many query rows or text tokens");
+  const SharedSpace w = shared_space(sp, B, Hkv, rows, chunks);
+  if (workspace == nullptr || workspace_bytes < w.bytes)
+    return fail(RTK_ERR_WORKSPACE, "workspace has %zu bytes, needs %zu", workspace == nullptr ? (size_t)0 : workspace_bytes,
+                w.bytes);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return fail(RTK_ERR_INVALID, "workspace must be 16-byte aligned");
+  unsigned char *ws = static_cast<unsigned char *>(workspace);
+  if (Sv == 0) p.head_dim_keep = 16;               // no visual block uses it
+  cudaError_t e = cudaSuccess;
+  rtk::MergeParams mp;
+  std::memset(&mp, 0, sizeof(mp));
+  mp.s = p;
+  mp.split = sp;
+  mp.has_prefix = Sf + Sv > 0;
+  mp.has_text = C > 0;
+  mp.text_rows = (int)rows; mp.text_chunks = (int)chunks;
+  float *pml = reinterpret_cast<float *>(ws + w.prefix_ml), *pacc = reinterpret_cast<float *>(ws + w.prefix_acc);
+  float *tml = reinterpret_cast<float *>(ws + w.text_ml), *tacc = reinterpret_cast<float *>(ws + w.text_acc);
+  mp.prefix_ml = pml; mp.prefix_acc = pacc; mp.text_ml = tml; mp.text_acc = tacc;
+  if (mp.has_prefix) {
+    rtk::PrefixParams pp;
+    pp.s = p;
+    pp.split = sp;
+    pp.ml = pml; pp.acc = pacc;
+    pp.status = static_cast<unsigned int *>(status != nullptr ? status : workspace);
+    e = rtk::launch_shared_prefix(maps, pp, st);
+    if (e != cudaSuccess) return cuda_fail(e, "shared decode (prefix kernel) launch");
+  }
+  if (mp.has_text) {
+    rtk::TextParams tp;
+    tp.s = p;
+    tp.rows = (int)rows; tp.chunks = (int)chunks;
+    tp.ml = tml; tp.acc = tacc;
+    e = rtk::launch_shared_text(tp, st);
+    if (e != cudaSuccess) return cuda_fail(e, "shared decode (text kernel) launch");
+  }
+  e = rtk::launch_shared_merge(mp, st);
+  if (e != cudaSuccess) return cuda_fail(e, "shared decode (merge kernel) launch");
   return RTK_OK;
 }
 

@@ -37,6 +37,96 @@ struct SharedParams {
 // Generic kernel (shared_simt.cu): any dtype, any strides, head_dim <= 256.
 cudaError_t launch_shared_simt(const SharedParams &p, cudaStream_t stream);
 
+// ---- tensor-core path: bf16 / fp16, D = 128, D_keep 16 / 32 / 64, rows that TMA
+// and 16-byte copies can take.  Three kernels: the prefix (shared_prefix.cu), the
+// questions' text (shared_text.cu), and the join of their partial results
+// (shared_merge.cu).  A partial result of a query row is (m, l, O[128]): the base-2
+// maximum it is relative to, sum 2^(x - m) and sum 2^(x - m) v.
+
+// How the prefix work is cut.  A unit is 128 query rows of one (prefix, KV head):
+// rows (n, t, g) of its N questions, T tokens and G heads.  Its tokens come in
+// blocks, 64 prompt tokens (weight 1) or 128 visual tokens (weight 2) each; the
+// list of all units' blocks is cut into `grid` ranges of equal weight, one per CTA.
+struct PrefixSplit {
+  int rows;                  // N T G query rows of a (prefix, KV head)
+  int row_tiles;             // ceil(rows / 128)
+  int units;                 // P H_kv row_tiles
+  int blocks_full, blocks_vis, unit_weight;   // unit_weight counts kUnitStart too
+  long long total;           // units * unit_weight
+  int grid;
+
+  static constexpr int kUnitStart = 2;        // weight of starting a unit (its queries)
+
+  __host__ __device__ int blocks() const { return blocks_full + blocks_vis; }
+  // weight at which block j of a unit starts
+  __host__ __device__ int block_start(int j) const {
+    return kUnitStart + (j < blocks_full ? j : blocks_full + 2 * (j - blocks_full));
+  }
+  // first block of a unit that starts at weight >= w
+  __host__ __device__ int block_from(int w) const {
+    w -= kUnitStart;
+    if (w <= 0) return 0;
+    if (w <= blocks_full) return w;
+    const int j = blocks_full + (w - blocks_full + 1) / 2;
+    return j < blocks() ? j : blocks();
+  }
+  __host__ __device__ long long range_begin(int c) const { return (long long)c * total / grid; }
+  // the CTA whose range holds weight w
+  __host__ __device__ int owner(long long w) const { return (int)(((w + 1) * grid - 1) / total); }
+  // CTAs that hold blocks of unit u.  Ranges are at least 2 long and block starts
+  // at most 2 apart, so every CTA from the first to the last holds one.
+  __host__ __device__ int first_cta(int u) const { return owner((long long)u * unit_weight + kUnitStart); }
+  __host__ __device__ int last_cta(int u) const {
+    return owner((long long)u * unit_weight + block_start(blocks() - 1));
+  }
+  // (unit, CTA) pairs lie on a staircase, so u + c numbers them without collision
+  __host__ __device__ int slots() const { return units + grid; }
+};
+
+inline PrefixSplit prefix_split(long long prefixes, long long questions, long long tokens, long long groups,
+                                long long kv_heads, long long seq_full, long long seq_sparse, int sms) {
+  PrefixSplit s;
+  s.rows = (int)(questions * tokens * groups);
+  s.row_tiles = (s.rows + 127) / 128;
+  s.units = (int)(prefixes * kv_heads * s.row_tiles);
+  s.blocks_full = (int)((seq_full + 63) / 64);
+  s.blocks_vis = (int)((seq_sparse + 127) / 128);
+  s.unit_weight = PrefixSplit::kUnitStart + s.blocks_full + 2 * s.blocks_vis;
+  s.total = (long long)s.units * s.unit_weight;
+  s.grid = (int)(s.total / 2 < sms ? (s.total / 2 > 0 ? s.total / 2 : 1) : sms);
+  return s;
+}
+
+struct PrefixMaps {
+  CUtensorMap kf, vf, ks, vs;   // 64-token boxes of the prompt, 128-token boxes of the visual span
+};
+
+struct PrefixParams {
+  SharedParams s;
+  PrefixSplit split;
+  float *ml, *acc;              // per slot: [128][2] and [128][128]
+  unsigned int *status;
+};
+cudaError_t launch_shared_prefix(const PrefixMaps &maps, const PrefixParams &p, cudaStream_t stream);
+
+// Text: CTAs per (question, KV head, chunk of kTextChunk tokens, 16 or 32 query rows).
+constexpr int kTextChunk = 256;
+struct TextParams {
+  SharedParams s;
+  int rows, chunks;             // T G query rows, ceil(cap / kTextChunk)
+  float *ml, *acc;              // per (question, KV head, chunk): [rows][2] and [rows][128]
+};
+cudaError_t launch_shared_text(const TextParams &p, cudaStream_t stream);
+
+struct MergeParams {
+  SharedParams s;
+  PrefixSplit split;
+  int has_prefix, has_text;
+  int text_rows, text_chunks;
+  const float *prefix_ml, *prefix_acc, *text_ml, *text_acc;
+};
+cudaError_t launch_shared_merge(const MergeParams &p, cudaStream_t stream);
+
 // New Keys and Values written into text caches at their lengths (text_cache.cu).
 struct AppendParams {
   int dtype;                              // rtk_dtype of the new rows
@@ -74,6 +164,9 @@ struct VerifyParams {
   int *accepted;                          // [B] contiguous
   void *workspace;
 };
+// SMs of a device (capi.cu)
+int device_sms(int device);
+
 size_t verify_workspace_bytes(long long batch, long long drafts, long long vocab);
 cudaError_t launch_verify(const VerifyParams &p, int sms, cudaStream_t stream);
 

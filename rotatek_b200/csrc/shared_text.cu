@@ -1,0 +1,412 @@
+// Shared-prefix attention, the text part: each question's T tokens and G heads of a
+// KV head (rows = T G, few) over that question's own text cache.
+//
+// A question's text belongs to it alone, so its Keys and Values are read once for a
+// handful of rows: the bound is HBM, and the work is cut so that bytes stay in
+// flight.  A CTA takes (question, KV head, 256 tokens, up to 16 kRT query rows); its
+// four warps take every fourth block of tokens through cp.async rings of their own
+// (no CTA-wide barrier in the loop), keep (m, l, O) in registers, and meet once at the
+// end.  Per block a warp runs m16n8k16 MMAs: S = Q . K^T with the query rows as M, and
+// O += P . V with P straight out of S's registers.
+//
+// 16-bit text: blocks of 16 tokens.  P is rounded to 16 bits, l sums P as rounded.
+// 8-bit text: blocks of 32 tokens, the e4m3 bytes converted in registers to f16
+// (exact).  ldmatrix of Key bytes gives lane (g, j) bytes 4j .. 4j+3 of token g: the
+// MMA's k index runs over a 16-channel group in the order 0 1 4 5 8 9 12 13 2 3 6 7 10 11
+// 14 15, and the queries are stored in that order.  ldmatrix.trans of Value bytes
+// pairs two tokens' bytes of channels (2g, 2g+1): one byte permute separates them into
+// B fragments of an "even" and an "odd" n-tile.  Queries go in as f16 scaled by a
+// power of two per row (bf16 has more range, f16 more bits: exact but for what lies
+// 2^-24 below the row's largest).  A token's Key scale multiplies its logit; its Value
+// scale multiplies its weight relative to the largest Value scale met so far (`vref`),
+// so weights stay within f16 whatever the scales are.
+//
+// Tokens past the length are zero-filled on the way in (cp.async reads nothing there).
+#include <type_traits>
+
+#include "common.cuh"
+#include "shared.h"
+
+namespace rtk {
+namespace {
+
+constexpr int kWarps = 4;
+
+template <bool FP8, int kRT>
+struct TextSmem {
+  static constexpr int kTok = FP8 ? 32 : 16;               // tokens of a block
+  static constexpr int kRow = FP8 ? 128 : 256;             // bytes of a token's Key (or Value)
+  static constexpr int kStage = 2 * kTok * kRow;           // 8 KB
+  static constexpr int kStages = 3;
+  static constexpr int kQ = 0;                             // 16 kRT rows of 256 bytes
+  static constexpr int kRing = kQ + kRT * 4096;
+  static constexpr int kBytes = kRing + kWarps * kStages * kStage;
+  // after the loop: O [4][16 kRT][128] and (m, l) [4][16 kRT], over the ring
+  static constexpr int kMerge = kWarps * kRT * 16 * (128 + 2) * 4;
+  static_assert(kMerge <= kWarps * kStages * kStage, "merge area");
+};
+
+// 16-byte chunk c of row r, rows of kRow bytes: chunks XORed with the row spread the
+// eight rows of an ldmatrix over the banks
+template <int kRow>
+__device__ __forceinline__ uint32_t at(int r, int c) {
+  return (uint32_t)(r * kRow + ((c ^ (r & 7)) << 4));
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  mma_16816<__half>(d, a, b0, b1);
+}
+
+__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint16_t v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
+  return r;
+}
+
+template <typename T, bool FP8, int kRT>
+__global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextParams p) {
+  using L = TextSmem<FP8, kRT>;
+  using M = typename std::conditional<FP8, __half, T>::type;   // MMA operand type
+  extern __shared__ __align__(128) unsigned char smem[];
+  const SharedParams &a = p.s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, j4 = lane & 3;
+  const int chunk = blockIdx.y, bh = blockIdx.x, row0 = blockIdx.z * 16 * kRT;
+  const int b = bh / a.kv_heads, h = bh % a.kv_heads;
+  const int len = min(max(a.lens[b * a.lens_s], 0), a.cap);
+  const int t0 = chunk * kTextChunk;
+  if (t0 >= len) return;
+  const int t1 = min(len, t0 + kTextChunk);
+  const int blocks = (t1 - t0 + L::kTok - 1) / L::kTok;
+
+  // this warp's ring
+  unsigned char *ring = smem + L::kRing + warp * L::kStages * L::kStage;
+  const unsigned char *kbase = static_cast<const unsigned char *>(a.kt.data);
+  const unsigned char *vbase = static_cast<const unsigned char *>(a.vt.data);
+  constexpr int kEsize = FP8 ? 1 : 2;
+  kbase += (b * a.kt.s[0] + h * a.kt.s[1]) * kEsize;
+  vbase += (b * a.vt.s[0] + h * a.vt.s[1]) * kEsize;
+  const long long ks = a.kt.s[2] * kEsize, vs = a.vt.s[2] * kEsize;
+  auto fetch = [&](int blk, int stage) {
+    unsigned char *dst = ring + stage * L::kStage;
+    constexpr int kChunks = L::kRow / 16;
+    const int first = t0 + blk * L::kTok;
+#pragma unroll
+    for (int e = 0; e < L::kTok * kChunks / 32; ++e) {
+      const int i = e * 32 + lane, r = i / kChunks, c = i % kChunks;
+      const int tok = first + r;
+      const bool in = tok < t1;
+      cp_async_16_zfill(dst + at<L::kRow>(r, c), kbase + (in ? tok * ks + c * 16 : 0), in ? 16 : 0);
+      cp_async_16_zfill(dst + L::kTok * L::kRow + at<L::kRow>(r, c), vbase + (in ? tok * vs + c * 16 : 0), in ? 16 : 0);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < L::kStages - 1; ++i) {
+    if (warp + kWarps * i < blocks) fetch(warp + kWarps * i, i);
+    cp_async_commit();
+  }
+
+  // queries: 16 kRT rows x 128 channels; per-row factor of the logits
+  __shared__ float qscale_s[16 * kRT];
+  for (int e = warp; e < 16 * kRT; e += kWarps) {
+    const int r = row0 + e;
+    uint2 v = make_uint2(0, 0);                      // channels 4 lane .. 4 lane + 3
+    if (r < p.rows) {
+      const int t = r / a.groups, gh = r % a.groups;
+      v = __ldg(reinterpret_cast<const uint2 *>(static_cast<const T *>(a.q.data) + b * a.q.s[0] + t * a.q.s[1] +
+                                                (h * a.groups + gh) * a.q.s[2] + lane * 4));
+    }
+    float f = a.scale_log2;
+    if constexpr (FP8) {
+      float x[4];
+      unpack2<T>(v.x, x[0], x[1]);
+      unpack2<T>(v.y, x[2], x[3]);
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        float mx = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        // 2^e with mx / 2^e in [1, 2): the exponent bits of mx (0 and subnormals: 2^-126)
+        const uint32_t ex = min(max(__float_as_uint(mx) >> 23, 1u), 253u);
+        const float inv = __uint_as_float((254u - ex) << 23);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] *= inv;
+        f *= __uint_as_float(ex << 23);
+      }
+      // channels 4 jj .. 4 jj + 3 of a 16-channel group go to positions 2 jj, 2 jj + 1 and
+      // 2 jj + 8, 2 jj + 9 (lane = 4 * group + jj)
+      const int grp = lane >> 2, jj = lane & 3;
+      const uint32_t q0 = smem_u32(smem + L::kQ);
+      const uint32_t w0 = pack2<__half>(x[0], x[1]), w1 = pack2<__half>(x[2], x[3]);
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(q0 + at<256>(e, 2 * grp) + jj * 4), "r"(w0) : "memory");
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(q0 + at<256>(e, 2 * grp + 1) + jj * 4), "r"(w1) : "memory");
+    } else {
+      *reinterpret_cast<uint2 *>(smem + L::kQ + at<256>(e, lane >> 1) + (lane & 1) * 8) = v;
+    }
+    if (lane == 0) qscale_s[e] = f;
+  }
+  __syncthreads();
+
+  // per query row of this lane (g and g + 8 of each row tile): tokens it sees, logit factor
+  int limit[kRT][2];
+  float qf[kRT][2];
+#pragma unroll
+  for (int rt = 0; rt < kRT; ++rt)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int e = rt * 16 + g + 8 * i, r = row0 + e;
+      limit[rt][i] = r < p.rows ? len - (a.tokens - 1 - r / a.groups) : 0;
+      qf[rt][i] = qscale_s[e];
+    }
+  const int all_see = len - (a.tokens - 1);          // every row sees tokens below this
+
+  float m[kRT][2], l[kRT][2], acc[kRT][16][4];
+  float vref = 0.f;
+#pragma unroll
+  for (int rt = 0; rt < kRT; ++rt) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      m[rt][i] = -INFINITY;
+      l[rt][i] = 0.f;
+    }
+#pragma unroll
+    for (int n = 0; n < 16; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[rt][n][i] = 0.f;
+  }
+  const uint32_t q_addr = smem_u32(smem + L::kQ);
+  const float *ksc = FP8 ? static_cast<const float *>(a.ksc.data) + b * a.ksc.s[0] + h * a.ksc.s[1] : nullptr;
+  const float *vsc = FP8 ? static_cast<const float *>(a.vsc.data) + b * a.vsc.s[0] + h * a.vsc.s[1] : nullptr;
+
+  int stage = 0;
+  for (int blk = warp; blk < blocks; blk += kWarps) {
+    const int first = t0 + blk * L::kTok;
+    constexpr int kNT = L::kTok / 8;                 // n-tiles of 8 tokens
+    float kscale[kNT][2], vscale[kNT][2];
+    if constexpr (FP8) {
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int tok = first + n * 8 + 2 * j4 + i;
+          kscale[n][i] = tok < t1 ? __ldg(ksc + tok * a.ksc.s[2]) : 0.f;
+          vscale[n][i] = tok < t1 ? __ldg(vsc + tok * a.vsc.s[2]) : 0.f;
+        }
+    }
+    {
+      const int next = blk + kWarps * (L::kStages - 1);
+      int st2 = stage + L::kStages - 1;
+      if (st2 >= L::kStages) st2 -= L::kStages;
+      if (next < blocks) fetch(next, st2);
+      cp_async_commit();
+    }
+    cp_async_wait_group<L::kStages - 1>();
+    __syncwarp();
+    const uint32_t k_addr = smem_u32(ring + stage * L::kStage), v_addr = k_addr + L::kTok * L::kRow;
+
+    if constexpr (FP8) {
+      // the largest Value scale of the block, over the warp
+      float top = 0.f;
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) top = fmaxf(top, fmaxf(vscale[n][0], vscale[n][1]));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      if (top > vref) {                              // the same in every lane
+        const float f = vref / top;
+        vref = top;
+#pragma unroll
+        for (int rt = 0; rt < kRT; ++rt)
+#pragma unroll
+          for (int n = 0; n < 16; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[rt][n][i] *= f;
+      }
+      const float inv = vref > 0.f ? 1.f / vref : 0.f;
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) {
+        vscale[n][0] *= inv;
+        vscale[n][1] *= inv;
+      }
+    }
+#pragma unroll
+    for (int rt = 0; rt < kRT; ++rt) {
+      float s[kNT][4];
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {                  // 16 channels
+        uint32_t qa[4];
+        ldmatrix_x4(q_addr + at<256>(rt * 16 + (lane & 15), 2 * k + (lane >> 4)), qa[0], qa[1], qa[2], qa[3]);
+        if constexpr (FP8) {
+          // four n-tiles of 8 tokens, the 16-byte chunk k of each
+          uint32_t r[4];
+          ldmatrix_x4(k_addr + at<128>(lane, k), r[0], r[1], r[2], r[3]);
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+            mma_f16(s[n], qa, e4m3x2_f16x2((uint16_t)(r[n] & 0xffffu)), e4m3x2_f16x2((uint16_t)(r[n] >> 16)));
+        } else {
+          // two n-tiles, the chunks 2k and 2k + 1
+          uint32_t r[4];
+          ldmatrix_x4(k_addr + at<256>((lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)), r[0], r[1], r[2], r[3]);
+          mma_16816<T>(s[0], qa, r[0], r[1]);
+          mma_16816<T>(s[1], qa, r[2], r[3]);
+        }
+      }
+      // logits in base 2; unseen tokens weigh nothing
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float x = s[n][i] * qf[rt][i >> 1];
+          if constexpr (FP8) x *= kscale[n][i & 1];
+          if (first + L::kTok > all_see && first + n * 8 + 2 * j4 + (i & 1) >= limit[rt][i >> 1]) x = -INFINITY;
+          s[n][i] = x;
+          mx[i >> 1] = fmaxf(mx[i >> 1], x);
+        }
+      float base[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+        const float m2 = fmaxf(m[rt][i], mx[i]);
+        base[i] = m2 > -INFINITY ? m2 : 0.f;
+        const float f = fast_exp2(m[rt][i] - base[i]);         // nothing yet: 2^-inf = 0
+        m[rt][i] = m2;
+        l[rt][i] *= f;
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          acc[rt][n][2 * i] *= f;
+          acc[rt][n][2 * i + 1] *= f;
+        }
+      }
+      uint32_t pa[kNT][2];                           // weights of rows g, g + 8
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float w0 = fast_exp2(s[n][2 * i] - base[i]), w1 = fast_exp2(s[n][2 * i + 1] - base[i]);
+          if constexpr (FP8) {
+            l[rt][i] += w0 + w1;
+            w0 *= vscale[n][0];
+            w1 *= vscale[n][1];
+            pa[n][i] = pack2<M>(w0, w1);
+          } else {
+            pa[n][i] = pack2<M>(w0, w1);
+            unpack2<M>(pa[n][i], w0, w1);
+            l[rt][i] += w0 + w1;
+          }
+        }
+#pragma unroll
+      for (int kk = 0; kk < kNT / 2; ++kk) {         // 16 tokens
+        const uint32_t pf[4] = {pa[2 * kk][0], pa[2 * kk][1], pa[2 * kk + 1][0], pa[2 * kk + 1][1]};
+        if constexpr (FP8) {
+#pragma unroll
+          for (int c = 0; c < 8; c += 2) {           // two 16-byte chunks of channels
+            uint32_t r[4];
+            ldmatrix_x4_trans(v_addr + at<128>(kk * 16 + (lane & 15), c + (lane >> 4)), r[0], r[1], r[2], r[3]);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const uint32_t lo = __byte_perm(r[2 * q], 0, 0x3120), hi = __byte_perm(r[2 * q + 1], 0, 0x3120);
+              mma_f16(acc[rt][2 * (c + q)], pf, e4m3x2_f16x2((uint16_t)(lo & 0xffffu)),
+                      e4m3x2_f16x2((uint16_t)(hi & 0xffffu)));
+              mma_f16(acc[rt][2 * (c + q) + 1], pf, e4m3x2_f16x2((uint16_t)(lo >> 16)),
+                      e4m3x2_f16x2((uint16_t)(hi >> 16)));
+            }
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 16; c += 2) {          // two chunks of 8 channels
+            uint32_t r[4];
+            ldmatrix_x4_trans(v_addr + at<256>(kk * 16 + (lane & 15), c + (lane >> 4)), r[0], r[1], r[2], r[3]);
+            mma_16816<T>(acc[rt][c], pf, r[0], r[1]);
+            mma_16816<T>(acc[rt][c + 1], pf, r[2], r[3]);
+          }
+        }
+      }
+    }
+    __syncwarp();
+    if (++stage == L::kStages) stage = 0;
+  }
+  cp_async_wait_all();
+  __syncthreads();                                   // every warp is done with its ring
+
+  // join the warps, in warp order
+  float *o_s = reinterpret_cast<float *>(smem + L::kRing);
+  float2 *ml_s = reinterpret_cast<float2 *>(o_s + kWarps * kRT * 16 * 128);
+  const float scale_o = FP8 ? vref : 1.f;
+#pragma unroll
+  for (int rt = 0; rt < kRT; ++rt)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float ll = l[rt][i];
+      ll += __shfl_xor_sync(0xffffffffu, ll, 1);
+      ll += __shfl_xor_sync(0xffffffffu, ll, 2);
+      const int e = rt * 16 + g + 8 * i;
+      if (j4 == 0) ml_s[warp * kRT * 16 + e] = make_float2(m[rt][i], ll);
+      float *row = o_s + (warp * kRT * 16 + e) * 128;
+      if constexpr (FP8) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          *reinterpret_cast<float4 *>(row + 16 * c + 4 * j4) =
+              make_float4(acc[rt][2 * c][2 * i] * scale_o, acc[rt][2 * c + 1][2 * i] * scale_o,
+                          acc[rt][2 * c][2 * i + 1] * scale_o, acc[rt][2 * c + 1][2 * i + 1] * scale_o);
+      } else {
+#pragma unroll
+        for (int n = 0; n < 16; ++n)
+          *reinterpret_cast<float2 *>(row + 8 * n + 2 * j4) = make_float2(acc[rt][n][2 * i], acc[rt][n][2 * i + 1]);
+      }
+    }
+  __syncthreads();
+  const long long slot = ((long long)bh * p.chunks + chunk) * p.rows;
+  for (int e = warp; e < 16 * kRT; e += kWarps) {
+    const int r = row0 + e;
+    if (r >= p.rows) break;
+    float mm = -INFINITY, ll = 0.f;
+    float2 st[kWarps];
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      st[w] = ml_s[w * kRT * 16 + e];
+      mm = fmaxf(mm, st[w].x);
+    }
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (!(st[w].x > -INFINITY)) continue;
+      const float f = fast_exp2(st[w].x - mm);
+      ll = fmaf(st[w].y, f, ll);
+      const float4 v = *reinterpret_cast<const float4 *>(o_s + (w * kRT * 16 + e) * 128 + lane * 4);
+      o.x = fmaf(v.x, f, o.x);
+      o.y = fmaf(v.y, f, o.y);
+      o.z = fmaf(v.z, f, o.z);
+      o.w = fmaf(v.w, f, o.w);
+    }
+    *reinterpret_cast<float4 *>(p.acc + (slot + r) * 128 + lane * 4) = o;
+    if (lane == 0) reinterpret_cast<float2 *>(p.ml)[slot + r] = make_float2(mm, ll);
+  }
+}
+
+template <typename T, bool FP8, int kRT>
+cudaError_t launch(const TextParams &p, cudaStream_t stream) {
+  const int smem = TextSmem<FP8, kRT>::kBytes;
+  cudaError_t e = cudaFuncSetAttribute(shared_text_kernel<T, FP8, kRT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  const dim3 grid(p.s.prefixes * p.s.questions * p.s.kv_heads, p.chunks, (p.rows + 16 * kRT - 1) / (16 * kRT));
+  shared_text_kernel<T, FP8, kRT><<<grid, kWarps * 32, smem, stream>>>(p);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_t(const TextParams &p, cudaStream_t stream) {
+  if (p.s.text_fp8) return launch<T, true, 1>(p, stream);
+  return launch<T, false, 1>(p, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_shared_text(const TextParams &p, cudaStream_t stream) {
+  return p.s.dtype == 1 ? launch_t<__nv_bfloat16>(p, stream) : launch_t<__half>(p, stream);
+}
+
+}  // namespace rtk
