@@ -196,7 +196,7 @@ int rtk_shared_decode(const rtk_tensor *q, const rtk_tensor *R_partial, const rt
   // ---- tensor-core path
   bool tc = (q->dtype == RTK_BF16 || q->dtype == RTK_F16) && D == 128 && rows16(q, 2) && (C == 0 || (rows16(k_text, fp8 ? 1 : 2) && rows16(v_text, fp8 ? 1 : 2)));
   if (Sv > 0)
-    tc = tc && (DK == 16 || DK == 32 || DK == 64) && rows16(R_partial, 2) && (delta_mu == nullptr || delta_mu->stride[2] == 1);
+    tc = tc && (DK == 16 || DK == 32 || DK == 64) && (delta_mu == nullptr || delta_mu->stride[2] == 1);
   rtk::PrefixMaps maps;
   std::memset(&maps, 0, sizeof(maps));
   if (tc && Sf > 0) tc = rtk::encode_rows_map(&maps.kf, k_full, 64, 64) && rtk::encode_rows_map(&maps.vf, v_full, 64, 64);
@@ -236,6 +236,7 @@ int rtk_shared_decode(const rtk_tensor *q, const rtk_tensor *R_partial, const rt
     rtk::PrefixParams pp;
     pp.s = p;
     pp.split = sp;
+    pp.R_rows = rows16(R_partial, 2);
     pp.ml = pml; pp.acc = pacc;
     pp.status = static_cast<unsigned int *>(status != nullptr ? status : workspace);
     e = rtk::launch_shared_prefix(maps, pp, st);

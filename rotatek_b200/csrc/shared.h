@@ -104,6 +104,7 @@ struct PrefixMaps {
 struct PrefixParams {
   SharedParams s;
   PrefixSplit split;
+  int R_rows;                   // R's rows can be read 16 bytes at a time
   float *ml, *acc;              // per slot: [128][2] and [128][128]
   unsigned int *status;
 };

@@ -344,15 +344,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (vis) {
           // R^T, K-major: row j holds column j of R
           const T *R = static_cast<const T *>(a.R.data) + pre * a.R.s[0] + h * a.R.s[1];
-          for (int e = tid; e < 128 * DK / 8; e += 256) {
-            const int d = e / (DK / 8), c = e % (DK / 8);
-            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(R + d * a.R.s[2] + c * 8));
-            const uint32_t words[4] = {v.x, v.y, v.z, v.w};
-            const uint32_t box = smem_u32(smem + L::kRot) + (d >> 6) * (DK * 128);
+          const uint32_t rt = smem_u32(smem + L::kRot);
+          if (p.R_rows) {                              // rows of R in 16-byte pieces
+            for (int e = tid; e < 128 * DK / 8; e += 256) {
+              const int d = e / (DK / 8), c = e % (DK / 8);
+              const uint4 v = __ldg(reinterpret_cast<const uint4 *>(R + d * a.R.s[2] + c * 8));
+              const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+              const uint32_t box = rt + (d >> 6) * (DK * 128);
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              st_shared_u16(box + swizzled_offset<128>(c * 8 + i, (d & 63) & ~7) + (d & 7) * 2,
-                            (uint16_t)(words[i >> 1] >> (16 * (i & 1))));
+              for (int i = 0; i < 8; ++i)
+                st_shared_u16(box + swizzled_offset<128>(c * 8 + i, (d & 63) & ~7) + (d & 7) * 2,
+                              (uint16_t)(words[i >> 1] >> (16 * (i & 1))));
+            }
+          } else {                                     // any strides; a transposed R reads along its columns
+#pragma unroll 8
+            for (int e = tid; e < 128 * DK; e += 256) {
+              const int d = e & 127, j = e >> 7;
+              st_shared_u16(rt + (d >> 6) * (DK * 128) + swizzled_offset<128>(j, (d & 63) & ~7) + (d & 7) * 2,
+                            __ldg(reinterpret_cast<const unsigned short *>(R + d * a.R.s[2] + j * a.R.s[3])));
+            }
           }
           if (tid < 128)
             dm_s[tid] = a.dm.data != nullptr
