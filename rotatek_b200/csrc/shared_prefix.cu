@@ -11,8 +11,7 @@
 //                       query q~ = q R is taken in fp32 and split into two 16-bit parts
 //                       (one part alone would move logits by 2^-9)
 //   x  = c (S + q . delta_mu),  c = log2(e) / sqrt(D)     (delta_mu: visual blocks)
-//   P  = 2^(x - m) rounded to 16 bits (the MMA's operand type), l += P as rounded, so a
-//        weight's rounding cancels where one token takes most of the sum
+//   P  = 2^(x - m) rounded to 16 bits, the MMA's operand type; l sums it unrounded
 //   O += P . V
 //
 // m follows the running maximum lazily: O and l are rescaled only when a maximum
@@ -25,8 +24,8 @@
 //   warps 8-11  softmax of the odd blocks
 // Even and odd blocks are two independent streams, each with its own S / P columns,
 // (m, l) and O accumulator in TMEM (2 x 128 + 2 x 128 = all 512 columns): while one
-// stream's softmax runs, the tensor core works for the other.  P goes back over S in
-// TMEM as the A operand of P . V.  At the end of a unit the streams are joined and
+// stream's softmax runs, the tensor core works for the other.  P goes back over S
+// (its upper half) in TMEM as the A operand of P . V.  At the end of a unit the streams are joined and
 // the partial result of (unit, CTA) is written for shared_merge.cu.
 #include <type_traits>
 
@@ -39,6 +38,7 @@ namespace {
 constexpr int kThreads = 384;
 constexpr int kFullTok = 64, kVisTok = 128;
 constexpr uint32_t kColsS = 128;                 // TMEM columns of a stream's S / P
+constexpr uint32_t kColP = 64;                   // P within them: over the upper half of S
 constexpr uint32_t kColO = 2 * kColsS;           // first column of the O accumulators
 constexpr float kLazy = 8.f;
 
@@ -64,88 +64,105 @@ struct PrefixSmem {
   static_assert(kBytes + 1024 <= 232448, "shared memory budget");
 };
 
-// TMEM columns -> per-element work on 32 columns at a time
-template <typename T>
-__device__ __forceinline__ float round_sum(uint32_t packed, float acc) {
-  float lo, hi;
-  unpack2<T>(packed, lo, hi);
-  return acc + (lo + hi);
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 struct RowStat {
   float m, l;
 };
 
-// One block of one stream for this thread's row: S in TMEM columns [s, s + NTOK),
-// P written over them, m / l / O brought along.  `valid` (NTOK bits in four words) marks
-// the tokens that count; `all` = every one does.
-template <typename T, int NTOK>
-__device__ __forceinline__ void softmax_block(uint32_t s, uint32_t o, bool first, float scale, float bias, bool all,
-                                              const uint32_t (&valid)[4], RowStat &st) {
-  constexpr int kChunks = NTOK / 32;
-  float mx = -INFINITY;
-#pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
-    uint32_t r[32];
-    tmem_ld32_nowait(s + 32 * c, r);
+// O of this warp's rows times each row's f.
+__device__ __forceinline__ void rescale_o(uint32_t o, float f) {
+#pragma unroll 1
+  for (int c = 0; c < 128; c += 16) {
+    uint32_t r[16];
+    tmem_ld16_nowait(o + c, r);
     tmem_wait_ld();
-    if (all) {
-      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(r[i]));
-      mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
-    } else {
+    for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
+    tmem_st16_nowait(o + c, r);
+  }
+}
+
+// 64 columns of S; those that do not count become -inf, whatever was there.
+__device__ __forceinline__ void load_half(uint32_t s, bool all, uint32_t v0, uint32_t v1, uint32_t (&r)[2][32]) {
+  tmem_ld32_nowait(s, r[0]);
+  tmem_ld32_nowait(s + 32, r[1]);
+  tmem_wait_ld();
+  if (!all) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        mx = fmaxf(mx, (valid[c] >> i) & 1u ? __uint_as_float(r[i]) : -INFINITY);
+    for (int i = 0; i < 32; ++i) {
+      if (!((v0 >> i) & 1u)) r[0][i] = 0xff800000u;
+      if (!((v1 >> i) & 1u)) r[1][i] = 0xff800000u;
     }
   }
-  const float top = fmaf(mx, scale, bias);         // scale > 0; -inf stays -inf
-  const bool grow = top > st.m + kLazy || (st.m == -INFINITY && top > -INFINITY);
+}
+
+__device__ __forceinline__ float max_half(const uint32_t (&r)[2][32]) {
+  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int i = 0; i < 32; i += 2)
+      mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1]));
+  return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+}
+
+// Weights of 64 columns: 32 columns of P (16-bit pairs) at `p`, their sum into l.
+template <typename T>
+__device__ __forceinline__ void weights_half(uint32_t p, const uint32_t (&r)[2][32], float2 scale, float2 off,
+                                             float2 (&l)[2]) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1])), scale, off);
+      x.x = fast_exp2(x.x);
+      x.y = fast_exp2(x.y);
+      l[i & 1] = __fadd2_rn(l[i & 1], x);
+      w[i] = pack2<T>(x.x, x.y);
+    }
+    tmem_st16_nowait(p + 16 * c, w);
+  }
+}
+
+// One block of one stream for this thread's row: S in TMEM columns [s, s + 64 or 128),
+// P written to [s + 64, s + 128), m / l / O brought along.  `valid` (a bit per token) marks the
+// tokens that count; `all` = every one does.  64 columns are in registers at a time;
+// of a visual block the upper half stays there from the maximum to the weights (P
+// goes over it) and the lower half is read again.
+template <typename T, bool VIS>
+__device__ __forceinline__ void softmax_block(uint32_t s, uint32_t o, bool first, float scale, float bias, bool all,
+                                              const uint32_t (&valid)[4], RowStat &st) {
+  uint32_t r[2][32];
+  load_half(s, all, valid[0], valid[1], r);
+  float mx = max_half(r);
+  if constexpr (VIS) {
+    load_half(s + 64, all, valid[2], valid[3], r);
+    mx = fmaxf(mx, max_half(r));
+  }
+  const float top = fmaf(mx, scale, bias);           // scale > 0; -inf stays -inf
+  const bool grow = top > st.m + kLazy;              // from -inf: whenever there is a maximum
   if (__any_sync(0xffffffffu, grow)) {
     const float m2 = grow ? top : st.m;
     const float f = grow ? fast_exp2(st.m - m2) : 1.f;      // first maximum: 2^-inf = 0
     st.m = m2;
     st.l *= f;
-    if (!first) {
-#pragma unroll
-      for (int c = 0; c < 128; c += 32) {
-        uint32_t r[32];
-        tmem_ld32_nowait(o + c, r);
-        tmem_wait_ld();
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t w[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(__uint_as_float(r[16 * h + i]) * f);
-          tmem_st16_nowait(o + c + 16 * h, w);
-        }
-      }
-    }
+    if (!first) rescale_o(o, f);
   }
   const float off = bias - (st.m > -INFINITY ? st.m : 0.f);
-  float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
-    uint32_t r[32];
-    tmem_ld32_nowait(s + 32 * c, r);
-    tmem_wait_ld();
-    uint32_t w[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float a = fast_exp2(fmaf(__uint_as_float(r[2 * i]), scale, off));
-      float b = fast_exp2(fmaf(__uint_as_float(r[2 * i + 1]), scale, off));
-      if (!all) {
-        a = (valid[c] >> (2 * i)) & 1u ? a : 0.f;
-        b = (valid[c] >> (2 * i + 1)) & 1u ? b : 0.f;
-      }
-      w[i] = pack2<T>(a, b);
-      if (i & 1) l1 = round_sum<T>(w[i], l1);
-      else l0 = round_sum<T>(w[i], l0);
-    }
-    tmem_st16_nowait(s + 16 * c, w);
+  const float2 scale2 = make_float2(scale, scale), off2 = make_float2(off, off);
+  float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  if constexpr (VIS) {
+    weights_half<T>(s + kColP + 32, r, scale2, off2, l2);
+    load_half(s, all, valid[0], valid[1], r);
   }
-  st.l += l0 + l1;
+  weights_half<T>(s + kColP, r, scale2, off2, l2);
+  st.l += (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
   tmem_wait_st();
 }
 
@@ -243,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr uint32_t kIdPv = idesc_f16(kFmt, 0, 1, 128, 128);
     const uint32_t q_addr = smem_u32(smem + L::kQ), rot_addr = smem_u32(smem + L::kRot);
     int it = 0;
-    uint32_t np[2] = {0, 0};                 // P blocks awaited so far, per stream
+    uint32_t np = 0;                         // parities of the next P block, a bit per stream
     for (int u = u0; u <= u1; ++u) {
       const long long w = (long long)u * sp.unit_weight;
       const int j0 = r0 > w ? sp.block_from((int)(r0 - w)) : 0;
@@ -290,12 +307,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (j0 + 1 < j1) issue_qk(j0 + 1, it + 1);
         for (int j = j0; j < j1; ++j, ++it) {
           const int x = (j - j0) & 1, stg = it % L::kStages;
-          mbar_wait_bounded(&p_bar[x], np[x] & 1, abort_flag, p.status);
-          ++np[x];
+          mbar_wait_bounded(&p_bar[x], (np >> x) & 1, abort_flag, p.status);
+          np ^= 1u << x;
           tc_fence_after();
           const bool vis = j >= sp.blocks_full;
           const uint32_t v_addr = smem_u32(smem + L::kRing + stg * L::kStage) + (vis ? L::kKeyBytes : 16384);
-          const uint32_t d = tmem + kColO + x * 128, pa = tmem + x * kColsS;
+          const uint32_t d = tmem + kColO + x * 128, pa = tmem + x * kColsS + kColP;
           const uint32_t half = vis ? 16384u : 8192u;
           const int steps = vis ? kVisTok / 16 : kFullTok / 16;
           for (int k = 0; k < steps; ++k)
@@ -469,15 +486,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           v += ((before + (j - j0)) % L::kStages) * L::kStage + 16384;
           for (int t = (warp & 3); t < kFullTok; t += 4)
-            if (!((valid[t >> 5] >> (t & 31)) & 1u))
+            if (!(((t < 32 ? valid[0] : valid[1]) >> (t & 31)) & 1u))
               *reinterpret_cast<uint2 *>(v + (lane >> 4) * 8192 + t * 128 + (lane & 15) * 8) = make_uint2(0, 0);
           fence_proxy_async_smem();
         }
         if (busy) {
           if (full)
-            softmax_block<T, kFullTok>(s_col, o_col, j - j0 < 2, a.scale_log2, 0.f, all, valid, st);
+            softmax_block<T, false>(s_col, o_col, j - j0 < 2, a.scale_log2, 0.f, all, valid, st);
           else
-            softmax_block<T, kVisTok>(s_col, o_col, j - j0 < 2, a.scale_log2, bias, all, valid, st);
+            softmax_block<T, true>(s_col, o_col, j - j0 < 2, a.scale_log2, bias, all, valid, st);
         }
         tc_fence_before();
         __syncwarp();
