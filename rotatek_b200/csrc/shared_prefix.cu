@@ -7,7 +7,7 @@
 // block of tokens:
 //
 //   S  = Q . K^T        prompt block, 64 tokens, K = 128 channels
-//   S  = [Qhi | Qlo] . [K~ | K~]^T    visual block, 128 tokens, K = 2 D_keep: the rotated
+//   S  = [Qhi | Qlo] . [K~ | K~]^T    visual block, 128 tokens (two sub-blocks), K = 2 D_keep: the rotated
 //                       query q~ = q R is taken in fp32 and split into two 16-bit parts
 //                       (one part alone would move logits by 2^-9)
 //   x  = c (S + q . delta_mu),  c = log2(e) / sqrt(D)     (delta_mu: visual blocks)
@@ -19,14 +19,17 @@
 //
 // CTA (one per SM, 12 warps):
 //   warp 0      TMA producer: a ring of stages, one block's K and V each
-//   warp 1      TMEM owner; one lane issues the MMAs
-//   warps 4-7   softmax of the even blocks: thread = query row (TMEM lane)
-//   warps 8-11  softmax of the odd blocks
-// Even and odd blocks are two independent streams, each with its own S / P columns,
-// (m, l) and O accumulator in TMEM (2 x 128 + 2 x 128 = all 512 columns): while one
-// stream's softmax runs, the tensor core works for the other.  P goes back over S
-// (its upper half) in TMEM as the A operand of P . V.  At the end of a unit the streams are joined and
-// the partial result of (unit, CTA) is written for shared_merge.cu.
+//   warps 1, 2  issue the MMAs of the even and the odd sub-blocks (one elected lane each:
+//               a single thread's instructions could not keep the tensor core fed); warp 1
+//               owns the TMEM
+//   warps 4-7   softmax of the even sub-blocks: thread = query row (TMEM lane)
+//   warps 8-11  softmax of the odd sub-blocks
+// A sub-block is 64 tokens: a prompt block, or half a visual block.  Even and odd
+// sub-blocks are two independent streams with their own (m, l) and O accumulator in
+// TMEM (2 x 128 columns), and two S buffers each (2 x 2 x 64 columns: all 512): while
+// a warp group works on one, the tensor core turns the other into the next S.  P goes
+// over S in TMEM as the A operand of P . V.  At the end of a unit the streams are
+// joined and the partial result of (unit, CTA) is written for shared_merge.cu.
 #include <type_traits>
 
 #include "shared.h"
@@ -36,10 +39,10 @@ namespace rtk {
 namespace {
 
 constexpr int kThreads = 384;
-constexpr int kFullTok = 64, kVisTok = 128;
-constexpr uint32_t kColsS = 128;                 // TMEM columns of a stream's S / P
-constexpr uint32_t kColP = 64;                   // P within them: over the upper half of S
-constexpr uint32_t kColO = 2 * kColsS;           // first column of the O accumulators
+constexpr int kFullTok = 64, kVisTok = 128;      // tokens of a block
+constexpr int kSub = 64;                         // tokens of a sub-block
+constexpr uint32_t kColsS = 64;                  // TMEM columns of an S buffer
+constexpr uint32_t kColO = 4 * kColsS;           // first column of the O accumulators
 constexpr float kLazy = 8.f;
 
 template <int DK>
@@ -56,8 +59,8 @@ struct PrefixSmem {
   static constexpr int kDm = kBias + 512;                          // float[128]
   static constexpr int kMl = kDm + 512;                            // float2[2][128]
   static constexpr int kBar = kMl + 2048;
-  // full[S], empty[S], s_ready[2], p_ready[2], rot, o_done
-  static constexpr int kNumBars = 2 * kStages + 6;
+  // full[S], empty[S], s_ready[4], p_ready[4], pv[2], rot, o_done
+  static constexpr int kNumBars = 2 * kStages + 12;
   static constexpr int kTmemSlot = kBar + kNumBars * 8;
   static constexpr int kAbort = kTmemSlot + 4;
   static constexpr int kBytes = kAbort + 4;
@@ -87,81 +90,56 @@ __device__ __forceinline__ void rescale_o(uint32_t o, float f) {
   }
 }
 
-// 64 columns of S; those that do not count become -inf, whatever was there.
-__device__ __forceinline__ void load_half(uint32_t s, bool all, uint32_t v0, uint32_t v1, uint32_t (&r)[2][32]) {
+// One sub-block for this thread's row: S in TMEM columns [s, s + 64), P written to
+// [s, s + 32), m and l brought along; rescale(f) multiplies O by each row's f when the
+// reference of any row of the warp moves.  v0, v1 (a bit per token) mark the tokens that
+// count; `all` = every one does.
+template <typename T, typename Rescale>
+__device__ __forceinline__ void softmax_sub(uint32_t s, float scale, float bias, bool all, uint32_t v0, uint32_t v1,
+                                            RowStat &st, Rescale rescale) {
+  uint32_t r[2][32];
   tmem_ld32_nowait(s, r[0]);
   tmem_ld32_nowait(s + 32, r[1]);
   tmem_wait_ld();
   if (!all) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
+    for (int i = 0; i < 32; ++i) {                   // -inf, whatever was there
       if (!((v0 >> i) & 1u)) r[0][i] = 0xff800000u;
       if (!((v1 >> i) & 1u)) r[1][i] = 0xff800000u;
     }
   }
-}
-
-__device__ __forceinline__ float max_half(const uint32_t (&r)[2][32]) {
   float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int c = 0; c < 2; ++c)
 #pragma unroll
     for (int i = 0; i < 32; i += 2)
       mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1]));
-  return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-}
-
-// Weights of 64 columns: 32 columns of P (16-bit pairs) at `p`, their sum into l.
-template <typename T>
-__device__ __forceinline__ void weights_half(uint32_t p, const uint32_t (&r)[2][32], float2 scale, float2 off,
-                                             float2 (&l)[2]) {
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    uint32_t w[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1])), scale, off);
-      x.x = fast_exp2(x.x);
-      x.y = fast_exp2(x.y);
-      l[i & 1] = __fadd2_rn(l[i & 1], x);
-      w[i] = pack2<T>(x.x, x.y);
-    }
-    tmem_st16_nowait(p + 16 * c, w);
-  }
-}
-
-// One block of one stream for this thread's row: S in TMEM columns [s, s + 64 or 128),
-// P written to [s + 64, s + 128), m / l / O brought along.  `valid` (a bit per token) marks the
-// tokens that count; `all` = every one does.  64 columns are in registers at a time;
-// of a visual block the upper half stays there from the maximum to the weights (P
-// goes over it) and the lower half is read again.
-template <typename T, bool VIS>
-__device__ __forceinline__ void softmax_block(uint32_t s, uint32_t o, bool first, float scale, float bias, bool all,
-                                              const uint32_t (&valid)[4], RowStat &st) {
-  uint32_t r[2][32];
-  load_half(s, all, valid[0], valid[1], r);
-  float mx = max_half(r);
-  if constexpr (VIS) {
-    load_half(s + 64, all, valid[2], valid[3], r);
-    mx = fmaxf(mx, max_half(r));
-  }
-  const float top = fmaf(mx, scale, bias);           // scale > 0; -inf stays -inf
+  // scale > 0; -inf stays -inf
+  const float top = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), scale, bias);
   const bool grow = top > st.m + kLazy;              // from -inf: whenever there is a maximum
   if (__any_sync(0xffffffffu, grow)) {
     const float m2 = grow ? top : st.m;
     const float f = grow ? fast_exp2(st.m - m2) : 1.f;      // first maximum: 2^-inf = 0
     st.m = m2;
     st.l *= f;
-    if (!first) rescale_o(o, f);
+    rescale(f);
   }
   const float off = bias - (st.m > -INFINITY ? st.m : 0.f);
   const float2 scale2 = make_float2(scale, scale), off2 = make_float2(off, off);
   float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-  if constexpr (VIS) {
-    weights_half<T>(s + kColP + 32, r, scale2, off2, l2);
-    load_half(s, all, valid[0], valid[1], r);
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1])), scale2, off2);
+      x.x = fast_exp2(x.x);
+      x.y = fast_exp2(x.y);
+      l2[i & 1] = __fadd2_rn(l2[i & 1], x);
+      w[i] = pack2<T>(x.x, x.y);
+    }
+    tmem_st16_nowait(s + 16 * c, w);
   }
-  weights_half<T>(s + kColP, r, scale2, off2, l2);
   st.l += (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
   tmem_wait_st();
 }
@@ -175,9 +153,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t *full_bar = reinterpret_cast<uint64_t *>(smem + L::kBar);
   uint64_t *empty_bar = full_bar + L::kStages;
-  uint64_t *s_bar = empty_bar + L::kStages;       // [2] S of the stream's block is in TMEM
-  uint64_t *p_bar = s_bar + 2;                    // [2] P of the stream's block is in TMEM
-  uint64_t *rot_bar = p_bar + 2;                  // rotated queries are in TMEM
+  uint64_t *s_bar = empty_bar + L::kStages;       // [stream + 2 buffer] S is in TMEM
+  uint64_t *p_bar = s_bar + 4;                    // [stream + 2 buffer] P is in TMEM
+  uint64_t *pv_bar = p_bar + 4;                   // [stream] the P . V before the stream's last is done
+  uint64_t *rot_bar = pv_bar + 2;                 // rotated queries are in TMEM
   uint64_t *o_bar = rot_bar + 1;                  // both O accumulators are complete
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::kTmemSlot);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::kAbort);
@@ -196,14 +175,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kStages; ++i) {
       mbar_init(&full_bar[i], 1);
-      mbar_init(&empty_bar[i], 1);
+      mbar_init(&empty_bar[i], 2);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&s_bar[i], 1);
       mbar_init(&p_bar[i], 4);
     }
+    for (int i = 0; i < 2; ++i) mbar_init(&pv_bar[i], 1);
     mbar_init(rot_bar, 1);
-    mbar_init(o_bar, 1);
+    mbar_init(o_bar, 2);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -251,79 +231,105 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_wait_bounded(&full_bar[k % L::kStages], (k / L::kStages) & 1, &dead, p.status);
       }
     }
-  } else if (warp == 1) {
-    // ---------------------------------------------------------------- MMA issuer
+  } else if (warp <= 2) {
+    // ---------------------------------------------------------------- MMA issuers, one per stream
+    const uint32_t x = warp - 1;
     constexpr uint32_t kFmt = kBf16 ? 1u : 0u;
     constexpr uint32_t kIdRot = idesc_f16(kFmt, 0, 0, 128, DK);
-    constexpr uint32_t kIdFull = idesc_f16(kFmt, 0, 0, 128, kFullTok);
-    constexpr uint32_t kIdVis = idesc_f16(kFmt, 0, 0, 128, kVisTok);
+    constexpr uint32_t kIdQk = idesc_f16(kFmt, 0, 0, 128, kSub);
     constexpr uint32_t kIdPv = idesc_f16(kFmt, 0, 1, 128, 128);
-    const uint32_t q_addr = smem_u32(smem + L::kQ), rot_addr = smem_u32(smem + L::kRot);
-    int it = 0;
-    uint32_t np = 0;                         // parities of the next P block, a bit per stream
+    constexpr uint32_t kStep = L::kStage >> 4;       // from stage to stage, in a descriptor
+    const uint32_t rot_addr = smem_u32(smem + L::kRot), ring = smem_u32(smem + L::kRing);
+    const uint64_t q_desc = smem_desc_kmajor<128>(smem_u32(smem + L::kQ)), rot_desc = smem_desc_kmajor<128>(rot_addr);
+    const uint64_t k_prompt = smem_desc_kmajor<128>(ring), v_prompt = smem_desc_sw128(ring + 16384, 8192, 1024);
+    const uint32_t d_o = tmem + kColO + x * 128;
+    int it = 0;                              // blocks of the segments before
+    uint32_t np = 0;                         // parity of the next P of each buffer
     for (int u = u0; u <= u1; ++u) {
       const long long w = (long long)u * sp.unit_weight;
       const int j0 = r0 > w ? sp.block_from((int)(r0 - w)) : 0;
       const int j1 = r1 - w >= sp.unit_weight ? sp.blocks() : sp.block_from((int)(r1 - w));
       if (j0 >= j1) continue;
-      named_barrier_sync(1, 288);            // Q and R^T are in shared memory
+      named_barrier_sync(1, 320);            // Q and R^T are in shared memory
       if (j1 > sp.blocks_full) {
-        if (lane == 0) {
+        if (x == 0 && elect_one()) {
           tc_fence_after();
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            umma_f16(tmem, smem_desc_kmajor<128>(q_addr + (k >> 2) * 16384 + (k & 3) * 32),
-                     smem_desc_kmajor<128>(rot_addr + (k >> 2) * (DK * 128) + (k & 3) * 32), kIdRot, k > 0);
+            umma_f16_ss(tmem, q_desc + (((k >> 2) * 16384 + (k & 3) * 32) >> 4),
+                        smem_desc_kmajor<128>(rot_addr + (k >> 2) * (DK * 128) + (k & 3) * 32), kIdRot, k > 0);
           umma_commit(rot_bar);
         }
         __syncwarp();
-        named_barrier_sync(1, 288);          // [Qhi | Qlo] is in shared memory
+        named_barrier_sync(1, 320);          // [Qhi | Qlo] is in shared memory
       }
-      if (lane == 0) {
+      if (elect_one()) {
         tc_fence_after();
-        auto issue_qk = [&](int j, int i) {
-          const int stg = i % L::kStages, x = (j - j0) & 1;
-          mbar_wait_bounded(&full_bar[stg], (i / L::kStages) & 1, abort_flag, p.status);
+        // Sub-block i of the segment: prompt blocks are one, visual blocks two; this
+        // stream takes every other one, i = x, x + 2, ...: whole prompt blocks, and always
+        // the same half of a visual block.  S runs two of them ahead of P . V: an S
+        // buffer is free once the P . V that reads it is issued (the tensor core works
+        // in order).  This thread's own instructions are what the tensor core waits for, so
+        // stages and parities are carried along instead of being computed.
+        const int nf = j0 < sp.blocks_full ? min(j1, sp.blocks_full) - j0 : 0;
+        const int subs = nf + 2 * (j1 - j0 - nf);
+        const uint32_t half = (x ^ (uint32_t)nf) & 1u;
+        const uint64_t k_vis = smem_desc_kmajor<DK * 2>(ring + half * (kSub * DK * 2));
+        const uint64_t v_vis = smem_desc_sw128(ring + L::kKeyBytes + half * 8192, 16384, 1024);
+        uint32_t q_stage = (it + (x == 1 && nf > 0)) % L::kStages;
+        uint32_t q_par = ((it + (x == 1 && nf > 0)) / L::kStages) & 1;
+        uint32_t p_stage = q_stage;
+        it += j1 - j0;
+        auto issue_qk = [&](int i, uint32_t buf) {
+          mbar_wait_bounded(&full_bar[q_stage], q_par, abort_flag, p.status);
           tc_fence_after();
-          const uint32_t k_addr = smem_u32(smem + L::kRing + stg * L::kStage);
-          const uint32_t d = tmem + x * kColsS;
-          if (j < sp.blocks_full) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              umma_f16(d, smem_desc_kmajor<128>(q_addr + (k >> 2) * 16384 + (k & 3) * 32),
-                       smem_desc_kmajor<128>(k_addr + (k >> 2) * 8192 + (k & 3) * 32), kIdFull, k > 0);
-          } else {
+          const uint32_t d = tmem + x * kColsS + buf * (2 * kColsS);
+          if (i >= nf) {
             constexpr int kSteps = DK / 16;
+            const uint64_t kd = k_vis + q_stage * kStep;
 #pragma unroll
             for (int k = 0; k < 2 * kSteps; ++k) {
               const int col = 16 * k;        // of [Qhi | Qlo]
-              umma_f16(d, smem_desc_kmajor<128>(rot_addr + (col >> 6) * 16384 + (col & 63) * 2),
-                       smem_desc_kmajor<DK * 2>(k_addr + (k % kSteps) * 32), kIdVis, k > 0);
+              umma_f16_ss(d, rot_desc + (((col >> 6) * 16384 + (col & 63) * 2) >> 4), kd + (((k % kSteps) * 32) >> 4),
+                          kIdQk, k > 0);
             }
+          } else {
+            const uint64_t kd = k_prompt + q_stage * kStep;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              umma_f16_ss(d, q_desc + (((k >> 2) * 16384 + (k & 3) * 32) >> 4),
+                          kd + (((k >> 2) * 8192 + (k & 3) * 32) >> 4), kIdQk, k > 0);
           }
-          umma_commit(&s_bar[x]);
+          umma_commit(&s_bar[x + 2 * buf]);
+          q_stage += i + 2 <= nf ? 2 : 1;
+          if (q_stage >= (uint32_t)L::kStages) {
+            q_stage -= L::kStages;
+            q_par ^= 1u;
+          }
         };
-        issue_qk(j0, it);
-        if (j0 + 1 < j1) issue_qk(j0 + 1, it + 1);
-        for (int j = j0; j < j1; ++j, ++it) {
-          const int x = (j - j0) & 1, stg = it % L::kStages;
-          mbar_wait_bounded(&p_bar[x], (np >> x) & 1, abort_flag, p.status);
-          np ^= 1u << x;
+        int i = x;
+        if (i < subs) issue_qk(i, 0);
+        if (i + 2 < subs) issue_qk(i + 2, 1);
+        for (uint32_t buf = 0; i < subs; i += 2, buf ^= 1u) {
+          mbar_wait_bounded(&p_bar[x + 2 * buf], (np >> buf) & 1u, abort_flag, p.status);
+          np ^= 1u << buf;
           tc_fence_after();
-          const bool vis = j >= sp.blocks_full;
-          const uint32_t v_addr = smem_u32(smem + L::kRing + stg * L::kStage) + (vis ? L::kKeyBytes : 16384);
-          const uint32_t d = tmem + kColO + x * 128, pa = tmem + x * kColsS + kColP;
-          const uint32_t half = vis ? 16384u : 8192u;
-          const int steps = vis ? kVisTok / 16 : kFullTok / 16;
-          for (int k = 0; k < steps; ++k)
-            umma_f16_ts(d, pa + 8 * k, smem_desc_sw128(v_addr + k * 2048, half, 1024), kIdPv, k > 0 || j - j0 > 1);
-          umma_commit(&empty_bar[stg]);
-          if (j + 1 == j1) umma_commit(o_bar);
-          if (j + 2 < j1) issue_qk(j + 2, it + 2);
+          const uint32_t pa = tmem + x * kColsS + buf * (2 * kColsS);
+          const uint64_t vd = (i >= nf ? v_vis : v_prompt) + p_stage * kStep;
+#pragma unroll
+          for (int k = 0; k < kSub / 16; ++k)
+            umma_f16_ts(d_o, pa + 8 * k, vd + ((k * 2048) >> 4), kIdPv, k > 0 || i > 1);
+          umma_commit(&empty_bar[p_stage]);            // two arrivals free a stage: one of each stream, or
+          if (i < nf) umma_commit(&empty_bar[p_stage]);    // both of the one that has the prompt block
+          p_stage += i + 2 <= nf ? 2 : 1;
+          if (p_stage >= (uint32_t)L::kStages) p_stage -= L::kStages;
+          if (i + 4 < subs) issue_qk(i + 4, buf);
+          else if (i + 2 < subs) umma_commit(&pv_bar[x]);  // the P . V before the stream's last
         }
+        umma_commit(o_bar);
       }
       __syncwarp();
-      named_barrier_sync(1, 288);            // the unit's partial has been read out
+      named_barrier_sync(1, 320);            // the unit's partial has been read out
     }
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- softmax
@@ -332,7 +338,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int row = tid & 127;                       // query row of the unit = TMEM lane
     const uint32_t lanes = (uint32_t)(row & ~31) << 16;
     const uint32_t s_col = tmem + lanes + x * kColsS, o_col = tmem + lanes + kColO + x * 128;
-    uint32_t ns = 0, nrot = 0, no = 0;
+    uint32_t ns = 0, npv = 0, nrot = 0, no = 0;      // parities (ns: one per buffer)
+    int it = 0;                                      // blocks of the units before
     for (int u = u0; u <= u1; ++u) {
       const long long w = (long long)u * sp.unit_weight;
       const int j0 = r0 > w ? sp.block_from((int)(r0 - w)) : 0;
@@ -388,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       fence_proxy_async_smem();
-      named_barrier_sync(1, 288);
+      named_barrier_sync(1, 320);
       if (vis) {
         if (x == 0) {
           // rotated queries out of TMEM, as two 16-bit parts into shared memory
@@ -440,66 +447,56 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ++nrot;
         fence_proxy_async_smem();
-        named_barrier_sync(1, 288);
+        named_barrier_sync(1, 320);
       }
       const float bias = vis ? bias_s[row] : 0.f;
       RowStat st{-INFINITY, 0.f};
       const bool busy = (row & ~31) < live;          // some row of this warp exists
-      for (int j = j0 + x; j < j1; j += 2, ++ns) {
-        uint32_t valid[4] = {~0u, ~0u, ~0u, ~0u};
-        bool all = true;
-        const bool full = j < sp.blocks_full;
-        if (full) {
-          const int tok = j * kFullTok, left = a.seq_full - tok;
-          if (a.mask.data != nullptr || left < kFullTok) {
-            const uint8_t *mk = static_cast<const uint8_t *>(a.mask.data) + pre * a.mask.s[0];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int t = 32 * i + lane;
-              const bool in = t < left && (a.mask.data == nullptr || mk[(tok + t) * a.mask.s[1]] != 0);
-              valid[i] = __ballot_sync(0xffffffffu, in);
-            }
-            all = (valid[0] & valid[1]) == ~0u;
-          }
-        } else {
-          const int left = a.seq_sparse - (j - sp.blocks_full) * kVisTok;
-          if (left < kVisTok) {
-            all = false;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int n = left - 32 * i;
-              valid[i] = n >= 32 ? ~0u : n > 0 ? (1u << n) - 1u : 0u;
-            }
-          }
+      const int nf = j0 < sp.blocks_full ? min(j1, sp.blocks_full) - j0 : 0;
+      const int subs = nf + 2 * (j1 - j0 - nf);
+      const int tok_vis = (max(j0, sp.blocks_full) - sp.blocks_full) * kVisTok;   // the segment's first visual token
+      for (int i = x; i < subs; i += 2) {
+        const int b = (i >> 1) & 1;
+        const bool prompt = i < nf;
+        const int tok = prompt ? (j0 + i) * kSub : tok_vis + (i - nf) * kSub;
+        const int left = (prompt ? a.seq_full : a.seq_sparse) - tok;
+        const bool masked = prompt && a.mask.data != nullptr;
+        uint32_t v0 = ~0u, v1 = ~0u;
+        if (masked || left < kSub) {
+          const uint8_t *mk = static_cast<const uint8_t *>(a.mask.data) + pre * a.mask.s[0];
+          v0 = __ballot_sync(0xffffffffu, lane < left && (!masked || mk[(tok + lane) * a.mask.s[1]] != 0));
+          v1 = __ballot_sync(0xffffffffu, lane + 32 < left && (!masked || mk[(tok + lane + 32) * a.mask.s[1]] != 0));
         }
-        mbar_wait_bounded(&s_bar[x], ns & 1, abort_flag, p.status);
+        const bool all = (v0 & v1) == ~0u;
+        mbar_wait_bounded(&s_bar[x + 2 * b], (ns >> b) & 1, abort_flag, p.status);
+        ns ^= 1u << b;
         tc_fence_after();
-        if (full && !all && a.mask.data != nullptr) {
+        if (masked && !all) {
           // a masked token's Values may hold anything, and 0 * NaN is NaN: zero them
-          unsigned char *v = smem + L::kRing;
-          // the stage of this block: blocks are numbered along the CTA's whole range
-          long long before = 0;
-          for (int q = u0; q < u; ++q) {
-            const long long wq = (long long)q * sp.unit_weight;
-            const int b0 = r0 > wq ? sp.block_from((int)(r0 - wq)) : 0;
-            before += sp.blocks() - b0;
-          }
-          v += ((before + (j - j0)) % L::kStages) * L::kStage + 16384;
-          for (int t = (warp & 3); t < kFullTok; t += 4)
-            if (!(((t < 32 ? valid[0] : valid[1]) >> (t & 31)) & 1u))
+          unsigned char *v = smem + L::kRing + (it + i) % L::kStages * L::kStage + 16384;
+          for (int t = (warp & 3); t < kSub; t += 4)
+            if (!(((t < 32 ? v0 : v1) >> (t & 31)) & 1u))
               *reinterpret_cast<uint2 *>(v + (lane >> 4) * 8192 + t * 128 + (lane & 15) * 8) = make_uint2(0, 0);
           fence_proxy_async_smem();
         }
-        if (busy) {
-          if (full)
-            softmax_block<T, false>(s_col, o_col, j - j0 < 2, a.scale_log2, 0.f, all, valid, st);
-          else
-            softmax_block<T, true>(s_col, o_col, j - j0 < 2, a.scale_log2, bias, all, valid, st);
-        }
+        if (busy)
+          softmax_sub<T>(s_col + 2 * b * kColsS, a.scale_log2, prompt ? 0.f : bias, all, v0, v1, st, [&](float f) {
+            if (i < 2) return;                       // nothing in O yet
+            // O is at rest once the P . V before this sub-block is done: the next S comes
+            // after it in the tensor core's order; before the last one it is signalled
+            if (i + 2 < subs)
+              mbar_wait_bounded(&s_bar[x + 2 * (b ^ 1)], (ns >> (b ^ 1)) & 1, abort_flag, p.status);
+            else
+              mbar_wait_bounded(&pv_bar[x], npv, abort_flag, p.status);
+            tc_fence_after();
+            rescale_o(o_col, f);
+          });
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_bar[x]);
+        if (lane == 0) mbar_arrive(&p_bar[x + 2 * b]);
       }
+      it += j1 - j0;
+      if (subs > x + 2) npv ^= 1u;                   // one signal per unit whose stream has two sub-blocks
       // join the two streams: each warp group writes 64 channels of the row
       ml_s[x * 128 + row] = make_float2(st.m, st.l);
       mbar_wait_bounded(o_bar, no & 1, abort_flag, p.status);
@@ -510,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float m = fmaxf(e0.x, e1.x);
       const float f0 = e0.x > -INFINITY ? fast_exp2(e0.x - m) : 0.f;
       const float f1 = e1.x > -INFINITY ? fast_exp2(e1.x - m) : 0.f;
-      const bool two = j1 - j0 > 1;                  // the odd stream had a block
+      const bool two = subs > 1;                     // the odd stream had a sub-block
       const long long slot = u + cta;
       if (busy) {
         float *out = p.acc + (slot * 128 + row) * 128 + 64 * x;
@@ -538,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           reinterpret_cast<float2 *>(p.ml)[slot * 128 + row] = make_float2(m, e0.y * f0 + e1.y * f1);
       }
       tc_fence_before();
-      named_barrier_sync(1, 288);
+      named_barrier_sync(1, 320);
     }
   }
   __syncthreads();
