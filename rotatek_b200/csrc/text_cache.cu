@@ -40,106 +40,114 @@ __device__ __forceinline__ float row_scale(float amax) {
   return amax > 0.f ? fmaxf(__fdiv_rn(amax, kE4m3Max), 1.17549435e-38f) : 1.f;
 }
 
-// Row r of the append: which cache (0 Keys, 1 Values), question, token, head.
-// Heads run fastest, the order in which a fused projection leaves the rows.
-struct AppendRow {
-  int side, b, t, h, pos;
-  bool live;
-};
-
-__device__ __forceinline__ AppendRow append_row(const AppendParams &p, unsigned r, unsigned total) {
-  AppendRow a;
-  a.live = r < 2u * total;
-  if (!a.live) r = 0;
-  a.side = r >= total;
-  unsigned i = a.side ? r - total : r;
-  a.h = i % p.heads;
-  i /= p.heads;
-  a.t = i % p.tokens;
-  a.b = i / p.tokens;
-  a.pos = p.lens[a.b * p.lens_s] + a.t;
-  const int count = p.counts != nullptr ? p.counts[a.b * p.counts_s] : p.tokens;
-  a.live = a.live && a.t < count && a.pos >= 0 && a.pos < p.cap;
-  return a;
-}
-
 __device__ __forceinline__ long long row_offset(const SharedTensor &x, int b, int h, int s) {
   return b * x.s[0] + h * x.s[1] + s * x.s[2];
 }
 
-// 8 channels of a row as floats (16 or 32 bytes)
+// 16 channels of a row (32 or 64 bytes)
 template <typename T>
-struct Eight {
-  uint4 raw[sizeof(T) / 2];
+struct Sixteen {
+  static constexpr int kWords = sizeof(T);           // 16-byte words
+  uint4 raw[kWords];
   __device__ __forceinline__ void load(const T *src) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = __ldg(reinterpret_cast<const uint4 *>(src) + i);
+    for (int i = 0; i < kWords; ++i) raw[i] = __ldg(reinterpret_cast<const uint4 *>(src) + i);
   }
   __device__ __forceinline__ void store(T *dst) const {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4 *>(dst)[i] = raw[i];
+    for (int i = 0; i < kWords; ++i) reinterpret_cast<uint4 *>(dst)[i] = raw[i];
   }
-  __device__ __forceinline__ void floats(float (&f)[8]) const {
-    if constexpr (sizeof(T) == 4) {
-      const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+  __device__ __forceinline__ void floats(float (&f)[16]) const {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
-    } else {
-      unpack2<T>(raw[0].x, f[0], f[1]);
-      unpack2<T>(raw[0].y, f[2], f[3]);
-      unpack2<T>(raw[0].z, f[4], f[5]);
-      unpack2<T>(raw[0].w, f[6], f[7]);
+    for (int i = 0; i < kWords; ++i) {
+      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (sizeof(T) == 4) f[4 * i + k] = __uint_as_float(w[k]);
+        else unpack2<T>(w[k], f[8 * i + 2 * k], f[8 * i + 2 * k + 1]);
+      }
     }
   }
 };
 
-// D = 128: 16 threads per row, kRows rows per thread.
+// x / s rounded to nearest for finite numbers, given r = 1 / s rounded to nearest: q = x r,
+// q + (x - q s) r (Markstein 1990: correctly rounded while the remainder x - q s is
+// exact, which s >= 2^-80 grants for every quotient that e4m3 does not round to 0).
+// The sign is x's (the sum would turn -0 into +0).
+__device__ __forceinline__ float divide(float x, float s, float r) {
+  const float q = x * r, e = fmaf(-q, s, x);
+  return __uint_as_float((__float_as_uint(fmaf(e, r, q)) & 0x7fffffffu) | (__float_as_uint(x) & 0x80000000u));
+}
+
+// D = 128: 8 threads per row of 16 channels each, kRows rows per thread.  A CTA takes
+// 32 kRows tokens of one head of one question's Keys or Values.  What it costs besides the
+// bytes is about ten instructions a channel (unpacking, the maximum, four for the
+// division, the conversion): 16 channels a thread so that the row's scale and its
+// reciprocal are worked out by 8 threads and not by 16.
 template <typename T, bool kQuantize, int kRows>
-__global__ void __launch_bounds__(256) append_rows_kernel(const AppendParams p) {
-  const unsigned total = (unsigned)p.batch * p.tokens * p.heads;
-  const int lane = threadIdx.x & 15;
-  const unsigned first = blockIdx.x * (16u * kRows) + (threadIdx.x >> 4);
-  AppendRow row[kRows];
-  Eight<T> x[kRows];
+__global__ void __launch_bounds__(256) append_rows_kernel(const AppendParams p, int ctas) {
+  const int lane = threadIdx.x & 7;
+  const int item = blockIdx.x / ctas, part = blockIdx.x % ctas;
+  const int side = item & 1, bh = item >> 1, b = bh / p.heads, h = bh % p.heads;
+  const int len = p.lens[b * p.lens_s];
+  int count = p.counts != nullptr ? min(p.counts[b * p.counts_s], p.tokens) : p.tokens;
+  count = (int)min((long long)count, (long long)p.cap - len);    // tokens below it fit
+  if (part * (32 * kRows) >= count) return;
+  const SharedTensor &src = p.src[side], &dst = p.dst[side], &scl = p.scale[side];
+  const int first = part * (32 * kRows) + (threadIdx.x >> 3);
+  const T *from = static_cast<const T *>(src.data) + row_offset(src, b, h, 0) + lane * 16;
+  const long long base = row_offset(dst, b, h, 0) + lane * 16;
+  Sixteen<T> x[kRows];
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
-    row[i] = append_row(p, first + 16u * i, total);
-    if (row[i].live)
-      x[i].load(static_cast<const T *>(p.src[row[i].side].data) +
-                row_offset(p.src[row[i].side], row[i].b, row[i].h, row[i].t) + lane * 8);
+    const int t = first + 32 * i;
+    if (t < count && t + len >= 0) x[i].load(from + t * src.s[2]);
   }
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
-    const AppendRow &a = row[i];
-    const SharedTensor &dst = p.dst[a.side];
+    const int t = first + 32 * i;
+    const bool live = t < count && t + len >= 0;
+    const long long to = base + (long long)(len + t) * dst.s[2];
     if constexpr (!kQuantize) {
-      if (a.live)
-        x[i].store(static_cast<T *>(const_cast<void *>(dst.data)) + row_offset(dst, a.b, a.h, a.pos) + lane * 8);
+      if (live) x[i].store(static_cast<T *>(const_cast<void *>(dst.data)) + to);
       continue;
     }
-    float f[8];
-    if (a.live) {
+    float f[16];
+    if (live) {
       x[i].floats(f);
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = 0.f;
+      for (int k = 0; k < 16; ++k) f[k] = 0.f;
     }
     float mx = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) mx = fmaxf(mx, finite_abs(f[k]));
+    for (int k = 0; k < 16; ++k) mx = fmaxf(mx, fabsf(f[k]));      // NaN is passed over
+    const bool infinite = !(mx < INFINITY);
+    if (infinite) {
+      mx = 0.f;
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      for (int k = 0; k < 16; ++k) mx = fmaxf(mx, finite_abs(f[k]));
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     const float sc = row_scale(mx);
-    uint2 o;
-    o.x = (uint32_t)e4m3x2(__fdiv_rn(f[0], sc), __fdiv_rn(f[1], sc)) |
-          ((uint32_t)e4m3x2(__fdiv_rn(f[2], sc), __fdiv_rn(f[3], sc)) << 16);
-    o.y = (uint32_t)e4m3x2(__fdiv_rn(f[4], sc), __fdiv_rn(f[5], sc)) |
-          ((uint32_t)e4m3x2(__fdiv_rn(f[6], sc), __fdiv_rn(f[7], sc)) << 16);
-    if (a.live) {
-      *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(const_cast<void *>(dst.data)) +
-                                 row_offset(dst, a.b, a.h, a.pos) + lane * 8) = o;
+    if (!infinite && sc >= 8.2718061e-25f) {
+      const float r = __frcp_rn(sc);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) f[k] = divide(f[k], sc, r);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) f[k] = __fdiv_rn(f[k], sc);
+    }
+    uint32_t o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      o[k] = (uint32_t)e4m3x2(f[4 * k], f[4 * k + 1]) | ((uint32_t)e4m3x2(f[4 * k + 2], f[4 * k + 3]) << 16);
+    if (live) {
+      *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(const_cast<void *>(dst.data)) + to) =
+          make_uint4(o[0], o[1], o[2], o[3]);
       if (lane == 0)
-        static_cast<float *>(const_cast<void *>(p.scale[a.side].data))[row_offset(p.scale[a.side], a.b, a.h, a.pos)] = sc;
+        static_cast<float *>(const_cast<void *>(scl.data))[row_offset(scl, b, h, 0) + (long long)(len + t) * scl.s[2]] = sc;
     }
   }
 }
@@ -149,11 +157,17 @@ template <typename T, bool kQuantize>
 __global__ void __launch_bounds__(256) append_any_kernel(const AppendParams p) {
   const unsigned total = (unsigned)p.batch * p.tokens * p.heads;
   const int lane = threadIdx.x & 31;
-  const AppendRow a = append_row(p, blockIdx.x * 8u + (threadIdx.x >> 5), total);
-  if (!a.live) return;                   // whole warp
-  const SharedTensor &src = p.src[a.side], &dst = p.dst[a.side];
-  const T *x = static_cast<const T *>(src.data) + row_offset(src, a.b, a.h, a.t);
-  const long long to = row_offset(dst, a.b, a.h, a.pos);
+  const unsigned r = blockIdx.x * 8u + (threadIdx.x >> 5);
+  if (r >= 2u * total) return;           // whole warp, here and below
+  const int side = r >= total;
+  unsigned i = side ? r - total : r;
+  const int h = i % p.heads;
+  i /= p.heads;
+  const int t = i % p.tokens, b = i / p.tokens, pos = p.lens[b * p.lens_s] + t;
+  if (t >= (p.counts != nullptr ? p.counts[b * p.counts_s] : p.tokens) || pos < 0 || pos >= p.cap) return;
+  const SharedTensor &src = p.src[side], &dst = p.dst[side];
+  const T *x = static_cast<const T *>(src.data) + row_offset(src, b, h, t);
+  const long long to = row_offset(dst, b, h, pos);
   if constexpr (!kQuantize) {
     T *y = static_cast<T *>(const_cast<void *>(dst.data)) + to;
     for (int d = lane; d < p.head_dim; d += 32) y[d * dst.s[3]] = x[d * src.s[3]];
@@ -167,17 +181,22 @@ __global__ void __launch_bounds__(256) append_any_kernel(const AppendParams p) {
     for (int d = lane; d < p.head_dim; d += 32)
       y[d * dst.s[3]] = (uint8_t)(e4m3x2(__fdiv_rn(to_f32(x[d * src.s[3]]), sc), 0.f) & 0xff);
     if (lane == 0)
-      static_cast<float *>(const_cast<void *>(p.scale[a.side].data))[row_offset(p.scale[a.side], a.b, a.h, a.pos)] = sc;
+      static_cast<float *>(const_cast<void *>(p.scale[side].data))[row_offset(p.scale[side], b, h, pos)] = sc;
   }
 }
 
 template <typename T, bool kQuantize>
 cudaError_t append(const AppendParams &p, bool rows128, cudaStream_t stream) {
-  const long long rows = 2ll * p.batch * p.tokens * p.heads;
+  const long long rows = 2ll * p.batch * p.heads * p.tokens;
+  const int items = 2 * p.batch * p.heads;
   if (!rows128) {
     append_any_kernel<T, kQuantize><<<(unsigned)((rows + 7) / 8), 256, 0, stream>>>(p);
-  } else {
-    append_rows_kernel<T, kQuantize, 1><<<(unsigned)((rows + 15) / 16), 256, 0, stream>>>(p);
+  } else if (rows <= 32 * 1024) {                    // few rows: spread them over the SMs
+    const int ctas = (p.tokens + 31) / 32;
+    append_rows_kernel<T, kQuantize, 1><<<items * ctas, 256, 0, stream>>>(p, ctas);
+  } else {                                           // many: two rows of a thread in flight
+    const int ctas = (p.tokens + 63) / 64;
+    append_rows_kernel<T, kQuantize, 2><<<items * ctas, 256, 0, stream>>>(p, ctas);
   }
   return cudaGetLastError();
 }
@@ -210,10 +229,69 @@ __global__ void __launch_bounds__(256) read_any_kernel(const ReadParams p) {
   for (int d = lane; d < p.head_dim; d += 32) y[d * dst.s[3]] = from_f32<T>(e4m3_value(x[d * src.s[3]]) * sc);
 }
 
+// D = 128: 8 threads per row (16 bytes each), kRows rows per thread, 32 kRows tokens of one
+// (question, head) of either cache per CTA.
+template <typename T, int kRows>
+__global__ void __launch_bounds__(256) read_rows_kernel(const ReadParams p, int ctas) {
+  const int item = blockIdx.x / ctas, part = blockIdx.x % ctas;
+  const int side = item & 1, bh = item >> 1, b = bh / p.heads, h = bh % p.heads;
+  const int lane = threadIdx.x & 7, first = part * (32 * kRows) + (threadIdx.x >> 3);
+  const int len = p.lens[b * p.lens_s];
+  const SharedTensor &src = p.src[side], &dst = p.dst[side], &scl = p.scale[side];
+  const uint8_t *x = static_cast<const uint8_t *>(src.data) + row_offset(src, b, h, 0) + lane * 16;
+  const float *sc = static_cast<const float *>(scl.data) + row_offset(scl, b, h, 0);
+  T *y = static_cast<T *>(const_cast<void *>(dst.data)) + row_offset(dst, b, h, 0) + lane * 16;
+  uint4 raw[kRows];
+  float scale[kRows];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int s = first + 32 * i;
+    const bool live = s < len && s < p.cap;
+    raw[i] = live ? __ldg(reinterpret_cast<const uint4 *>(x + s * src.s[2])) : make_uint4(0, 0, 0, 0);
+    scale[i] = live ? __ldg(sc + s * scl.s[2]) : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int s = first + 32 * i;
+    if (s >= p.cap) break;
+    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+    float f[16];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      uint32_t hh;
+      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hh) : "h"((uint16_t)(w[k >> 1] >> (16 * (k & 1)))));
+      unpack2<__half>(hh, f[2 * k], f[2 * k + 1]);
+      f[2 * k] *= scale[i];
+      f[2 * k + 1] *= scale[i];
+    }
+    uint4 *to = reinterpret_cast<uint4 *>(y + s * dst.s[2]);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        to[k] = make_uint4(__float_as_uint(f[4 * k]), __float_as_uint(f[4 * k + 1]), __float_as_uint(f[4 * k + 2]),
+                           __float_as_uint(f[4 * k + 3]));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        __stcs(to + k, make_uint4(pack2<T>(f[8 * k], f[8 * k + 1]), pack2<T>(f[8 * k + 2], f[8 * k + 3]),
+                                  pack2<T>(f[8 * k + 4], f[8 * k + 5]), pack2<T>(f[8 * k + 6], f[8 * k + 7])));
+    }
+  }
+}
+
 template <typename T>
-cudaError_t read(const ReadParams &p, cudaStream_t stream) {
+cudaError_t read(const ReadParams &p, bool rows128, cudaStream_t stream) {
   const long long rows = 2ll * p.batch * p.heads * p.cap;
-  read_any_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, stream>>>(p);
+  const int items = 2 * p.batch * p.heads;
+  if (!rows128) {
+    read_any_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, stream>>>(p);
+  } else if (rows <= 32 * 1024) {                    // few rows: spread them over the SMs
+    const int ctas = (p.cap + 31) / 32;
+    read_rows_kernel<T, 1><<<items * ctas, 256, 0, stream>>>(p, ctas);
+  } else {
+    const int ctas = (p.cap + 127) / 128;
+    read_rows_kernel<T, 4><<<items * ctas, 256, 0, stream>>>(p, ctas);
+  }
   return cudaGetLastError();
 }
 
@@ -232,7 +310,7 @@ cudaError_t launch_append_text(const AppendParams &p, cudaStream_t stream) {
   bool rows128 = p.head_dim == 128;
   for (int i = 0; i < 2; ++i)
     rows128 = rows128 && aligned_rows(p.src[i], esize, 16) &&
-              (p.quantize ? aligned_rows(p.dst[i], 1, 8) : aligned_rows(p.dst[i], esize, 16));
+              (p.quantize ? aligned_rows(p.dst[i], 1, 16) : aligned_rows(p.dst[i], esize, 16));
   if (p.quantize) {
     if (p.dtype == 0) return append<float, true>(p, rows128, stream);
     if (p.dtype == 1) return append<__nv_bfloat16, true>(p, rows128, stream);
@@ -245,9 +323,13 @@ cudaError_t launch_append_text(const AppendParams &p, cudaStream_t stream) {
 
 cudaError_t launch_read_text(const ReadParams &p, cudaStream_t stream) {
   if ((long long)p.batch * p.heads * p.cap == 0) return cudaSuccess;
-  if (p.dtype == 0) return read<float>(p, stream);
-  if (p.dtype == 1) return read<__nv_bfloat16>(p, stream);
-  return read<__half>(p, stream);
+  const int esize = p.dtype == 0 ? 4 : 2;
+  bool rows128 = p.head_dim == 128;
+  for (int i = 0; i < 2; ++i)
+    rows128 = rows128 && aligned_rows(p.src[i], 1, 16) && aligned_rows(p.dst[i], esize, 16);
+  if (p.dtype == 0) return read<float>(p, rows128, stream);
+  if (p.dtype == 1) return read<__nv_bfloat16>(p, rows128, stream);
+  return read<__half>(p, rows128, stream);
 }
 
 }  // namespace rtk
