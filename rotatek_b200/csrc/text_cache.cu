@@ -20,6 +20,8 @@
 
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 namespace rtk {
 namespace {
 
@@ -57,6 +59,27 @@ struct Sixteen {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) reinterpret_cast<uint4 *>(dst)[i] = raw[i];
   }
+  // the largest |x|, NaN passed over (16-bit types two at a time)
+  __device__ __forceinline__ float amax() const {
+    if constexpr (sizeof(T) == 4) {
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < kWords; ++i)
+        m = fmaxf(m, fmaxf(fmaxf(fabsf(__uint_as_float(raw[i].x)), fabsf(__uint_as_float(raw[i].y))),
+                           fmaxf(fabsf(__uint_as_float(raw[i].z)), fabsf(__uint_as_float(raw[i].w)))));
+      return m;
+    } else {
+      using T2 = typename std::conditional<std::is_same<T, __nv_bfloat16>::value, __nv_bfloat162, __half2>::type;
+      auto h2 = [](uint32_t w) { return __habs2(*reinterpret_cast<const T2 *>(&w)); };
+      T2 m = __hmax2(h2(raw[0].x), h2(raw[1].x));
+      m = __hmax2(m, __hmax2(h2(raw[0].y), h2(raw[1].y)));
+      m = __hmax2(m, __hmax2(h2(raw[0].z), h2(raw[1].z)));
+      m = __hmax2(m, __hmax2(h2(raw[0].w), h2(raw[1].w)));
+      float lo, hi;
+      unpack2<T>(*reinterpret_cast<const uint32_t *>(&m), lo, hi);
+      return fmaxf(fmaxf(lo, hi), 0.f);              // all NaN: 0
+    }
+  }
   __device__ __forceinline__ void floats(float (&f)[16]) const {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) {
@@ -71,12 +94,12 @@ struct Sixteen {
 };
 
 // x / s rounded to nearest for finite numbers, given r = 1 / s rounded to nearest: q = x r,
-// q + (x - q s) r (Markstein 1990: correctly rounded while the remainder x - q s is
+// q - (q s - x) r (Markstein 1990: correctly rounded while the remainder q s - x is
 // exact, which s >= 2^-80 grants for every quotient that e4m3 does not round to 0).
-// The sign is x's (the sum would turn -0 into +0).
+// Written with the remainder negated, -0 stays -0.
 __device__ __forceinline__ float divide(float x, float s, float r) {
-  const float q = x * r, e = fmaf(-q, s, x);
-  return __uint_as_float((__float_as_uint(fmaf(e, r, q)) & 0x7fffffffu) | (__float_as_uint(x) & 0x80000000u));
+  const float q = x * r;
+  return fmaf(-fmaf(q, s, -x), r, q);
 }
 
 // D = 128: 8 threads per row of 16 channels each, kRows rows per thread.  A CTA takes
@@ -112,16 +135,13 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const AppendParams p, 
       if (live) x[i].store(static_cast<T *>(const_cast<void *>(dst.data)) + to);
       continue;
     }
-    float f[16];
-    if (live) {
-      x[i].floats(f);
-    } else {
+    if (!live) {
 #pragma unroll
-      for (int k = 0; k < 16; ++k) f[k] = 0.f;
+      for (int k = 0; k < Sixteen<T>::kWords; ++k) x[i].raw[k] = make_uint4(0, 0, 0, 0);
     }
-    float mx = 0.f;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) mx = fmaxf(mx, fabsf(f[k]));      // NaN is passed over
+    float f[16];
+    x[i].floats(f);
+    float mx = x[i].amax();
     const bool infinite = !(mx < INFINITY);
     if (infinite) {
       mx = 0.f;

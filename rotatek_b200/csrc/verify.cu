@@ -14,11 +14,13 @@
 //           next token is the argmax of row k.
 //
 // Two kernels.  stats: a CTA per (row, chunk of the vocabulary) leaves the chunk's
-// running maximum and sum of exponentials (a greedy row: its maximum and where) --
-// one pass over every logits row.  pick: CTAs per (question, chunk) join a row's
-// chunks in chunk order, find k, and race over row k alone; the winners of the
-// chunks meet in a 64-bit atomicMax on (value, ~index), whose result does not depend
-// on the order of arrival.
+// maximum and sum of exponentials relative to it (a greedy row: its maximum and where): one
+// pass over every logits row that a decision can read, in 16-byte loads, bound by HBM.
+// pick: CTAs per (question, chunk) join a row's chunks (a warp per row, always in the
+// same tree), find k, and race over row k alone, which the first pass left in L2 or near
+// it; the chunks' winners meet in a 64-bit atomicMax on (value, ~index), whose result does
+// not depend on the order of arrival.  pick is launched while stats still runs and
+// waits for it on the device.
 #include "common.cuh"
 #include "shared.h"
 
@@ -30,22 +32,31 @@ constexpr int kMaxDrafts = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct VerifyLayout {
-  int chunk, chunks;           // vocabulary elements of a chunk, chunks of a row
-  long long rows;              // logits rows of a question: 2 T + 1
+  int chunk, chunks;           // vocabulary elements of a chunk, chunks of a row (stats)
+  int race, races;             // the same of the race (pick)
+  int rows;                    // logits rows of a question: 2 T + 1
 };
 
-__host__ __device__ inline VerifyLayout verify_layout(long long drafts, long long vocab) {
+// Chunks of at least 2048 elements (a 16-byte load of each thread), larger where there
+// are enough rows to fill the SMs several times over.
+__host__ __device__ inline VerifyLayout verify_layout(long long batch, long long drafts, long long vocab) {
   VerifyLayout l;
-  l.chunk = 8192;
+  l.rows = (int)(2 * drafts + 1);
+  const long long total = batch * l.rows * vocab;
+  l.chunk = 2048;
+  while (l.chunk < 16384 && total / l.chunk > 148 * 16) l.chunk *= 2;
   l.chunks = (int)((vocab + l.chunk - 1) / l.chunk);
-  l.rows = 2 * drafts + 1;
+  // pick: one wave of CTAs, since each of them joins and decides before it races
+  l.race = (int)((batch * vocab / (148 * 4) + 2047) / 2048 * 2048);
+  if (l.race < 2048) l.race = 2048;
+  l.races = (int)((vocab + l.race - 1) / l.race);
   return l;
 }
 
-// workspace: [B] race keys (residual), [B] race keys (p), [B] tickets, then
+// workspace: [B] race keys, [B] tickets, then
 // float4 (max, sum, argmax bits, -) per (b, row, chunk)
 struct VerifySpace {
-  unsigned long long *rest_key, *p_key;
+  unsigned long long *key;
   unsigned int *ticket;
   float4 *stats;
 };
@@ -55,10 +66,9 @@ __host__ __device__ inline long long align16(long long x) { return (x + 15) / 16
 __host__ __device__ inline VerifySpace verify_space(void *ws, long long batch) {
   VerifySpace s;
   unsigned char *p = static_cast<unsigned char *>(ws);
-  s.rest_key = reinterpret_cast<unsigned long long *>(p);
-  s.p_key = s.rest_key + batch;
-  s.ticket = reinterpret_cast<unsigned int *>(s.p_key + batch);
-  s.stats = reinterpret_cast<float4 *>(p + align16(batch * 20));
+  s.key = reinterpret_cast<unsigned long long *>(p);
+  s.ticket = reinterpret_cast<unsigned int *>(s.key + batch);
+  s.stats = reinterpret_cast<float4 *>(p + align16(batch * 12));
   return s;
 }
 
@@ -76,7 +86,7 @@ __device__ __forceinline__ const T *logits_row(const VerifyParams &p, int b, int
 __device__ __forceinline__ void join(float &m, float &z, float m2, float z2) {
   const float top = fmaxf(m, m2);
   if (top == -INFINITY) return;                  // nothing on either side
-  z = z * exp2f(m - top) + z2 * exp2f(m2 - top);
+  z = z * fast_exp2(m - top) + z2 * fast_exp2(m2 - top);
   m = top;
 }
 
@@ -85,17 +95,56 @@ __device__ __forceinline__ unsigned long long race_key(float v, unsigned i) {
   return ((unsigned long long)__float_as_uint(v) << 32) | (0xffffffffu - i);
 }
 
+// The chunk [i0, i1) of a row as visited by this thread: f(first index, n, values) with n
+// values at consecutive indices, ascending.  Whole aligned 16-byte words are loaded as
+// such, four of a thread in flight; what lies before and after them one by one.
+template <typename T, typename F>
+__device__ __forceinline__ void visit(const T *row, int i0, int i1, F f) {
+  constexpr int kVec = 16 / sizeof(T);
+  const int off = (int)((reinterpret_cast<uintptr_t>(row + i0) / sizeof(T)) % kVec);
+  const int head = min(i1 - i0, off ? kVec - off : 0);
+  const int words = (i1 - i0 - head) / kVec, tail = i0 + head + words * kVec;
+  float one[kVec];
+  if ((int)threadIdx.x < head) {
+    one[0] = to_f32(row[i0 + threadIdx.x]);
+    f(i0 + (int)threadIdx.x, 1, one);
+  }
+  const uint4 *body = reinterpret_cast<const uint4 *>(row + i0 + head);
+  for (int w = threadIdx.x; w < words; w += 4 * kThreads) {
+    uint4 raw[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (w + k * kThreads < words) raw[k] = __ldg(body + w + k * kThreads);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (w + k * kThreads >= words) break;
+      const uint32_t u[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+      float v[kVec];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (sizeof(T) == 4) v[e] = __uint_as_float(u[e]);
+        else unpack2<T>(u[e], v[2 * e], v[2 * e + 1]);
+      }
+      f(i0 + head + (w + k * kThreads) * kVec, kVec, v);
+    }
+  }
+  if (tail + (int)threadIdx.x < i1) {
+    one[0] = to_f32(row[tail + threadIdx.x]);
+    f(tail + (int)threadIdx.x, 1, one);
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads) verify_stats_kernel(const VerifyParams p) {
   __shared__ float m_s[kThreads / 32], z_s[kThreads / 32];
   __shared__ int i_s[kThreads / 32];
-  const VerifyLayout l = verify_layout(p.drafts, p.vocab);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const VerifyLayout l = verify_layout(p.batch, p.drafts, p.vocab);
   const VerifySpace ws = verify_space(p.workspace, p.batch);
   const int r = blockIdx.y, b = blockIdx.z, chunk = blockIdx.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (r == 0 && chunk == 0 && threadIdx.x == 0) {
-    ws.rest_key[b] = 0ull;
-    ws.p_key[b] = 0ull;
+    ws.key[b] = 0ull;
     ws.ticket[b] = 0u;
   }
   const int n = drafts_of(p, b);
@@ -105,23 +154,43 @@ __global__ void __launch_bounds__(kThreads) verify_stats_kernel(const VerifyPara
   if (is_draft ? (greedy || r - p.drafts - 1 >= n) : r > n) return;   // a row that no decision reads
   const T *row = logits_row<T>(p, b, r);
   const int i0 = chunk * l.chunk, i1 = min(p.vocab, i0 + l.chunk);
-  // base-2 logits relative to a running maximum, x = logit * log2(e) / h
-  const float c = greedy ? 1.f : kLog2e / fmaxf(heat, 1e-30f);
-  float m = -INFINITY, z = 0.f;
+  float m = -INFINITY, z = 0.f;                // the maximum logit; sum 2^((x - m) c)
   int at = i0;
-  for (int i = i0 + (int)threadIdx.x; i < i1; i += kThreads) {
-    const float x = to_f32(row[i]) * c;
-    if (greedy) {
-      if (x > m) {
-        m = x;
-        at = i;
+  const float c = greedy ? 1.f : kLog2e / fmaxf(heat, 1e-30f);
+  if (greedy) {
+    visit<T>(row, i0, i1, [&](int i, int cnt, const float *v) {
+#pragma unroll
+      for (int e = 0; e < 16 / (int)sizeof(T); ++e)
+        if (e < cnt && (v[e] > m || (v[e] == m && i + e < at))) {
+          m = v[e];
+          at = i + e;
+        }
+    });
+  } else {
+    visit<T>(row, i0, i1, [&](int, int cnt, const float *v) {
+      constexpr int kVec = 16 / sizeof(T);
+      if (cnt == kVec) {
+        float top = v[0];
+#pragma unroll
+        for (int e = 1; e < kVec; ++e) top = fmaxf(top, v[e]);
+        if (top > m) {
+          z *= fast_exp2((m - top) * c);       // nothing yet: 0
+          m = top;
+        }
+        if (m > -INFINITY) {
+          const float mc = -m * c;
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) z += fast_exp2(fmaf(v[e], c, mc));
+        }
+      } else {
+        if (v[0] > m) {
+          z *= fast_exp2((m - v[0]) * c);
+          m = v[0];
+        }
+        if (m > -INFINITY) z += fast_exp2((v[0] - m) * c);
       }
-    } else if (x > m) {
-      z = fmaf(z, exp2f(m - x), 1.f);
-      m = x;
-    } else if (m > -INFINITY) {
-      z += exp2f(x - m);
-    }
+    });
+    m *= c;                                    // from here on in base-2 units
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -159,31 +228,46 @@ __global__ void __launch_bounds__(kThreads) verify_stats_kernel(const VerifyPara
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) verify_pick_kernel(const VerifyParams p) {
-  __shared__ float m_s[2 * kMaxDrafts + 1], z_s[2 * kMaxDrafts + 1];
+  __shared__ float m_s[2 * kMaxDrafts + 1], z_s[2 * kMaxDrafts + 1];     // base-2 maximum, 1 / sum
   __shared__ int at_s[kMaxDrafts + 1];
   __shared__ int k_s;
   __shared__ bool last_s;
-  __shared__ unsigned long long rest_s[kThreads / 32], pk_s[kThreads / 32];
-  const VerifyLayout l = verify_layout(p.drafts, p.vocab);
+  __shared__ unsigned long long key_s[kThreads / 32];
+  const VerifyLayout l = verify_layout(p.batch, p.drafts, p.vocab);
   const VerifySpace ws = verify_space(p.workspace, p.batch);
   const int b = blockIdx.y, chunk = blockIdx.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n = drafts_of(p, b), T1 = p.drafts + 1;
   const float heat = p.temperature[b * p.temp_s];
   const bool greedy = !(heat > 0.f), soft_draft = p.draft.data != nullptr;
+  const float c = greedy ? 1.f : kLog2e / fmaxf(heat, 1e-30f);
   if (greedy && chunk > 0) return;
+  // what an acceptance needs besides the sums: a draft per thread
+  const int j = threadIdx.x;
+  long long x = -1;
+  float u = 0.f, tx = 0.f, dx = 0.f;
+  if (j < n) {
+    x = p.tokens[b * p.tok_s[0] + j * p.tok_s[1]];
+    u = p.uniforms[b * p.uni_s[0] + j * p.uni_s[1]];
+    if (x >= 0 && x < p.vocab && !greedy) {
+      tx = to_f32(logits_row<T>(p, b, j)[x]);
+      if (soft_draft) dx = to_f32(logits_row<T>(p, b, T1 + j)[x]);
+    }
+  }
+  if (threadIdx.x == 0) k_s = n;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  // join the chunks of every row a decision may read (in chunk order)
-  for (int r = threadIdx.x; r < (int)l.rows; r += kThreads) {
+  // join the chunks of every row a decision may read: a warp per row
+  for (int r = warp; r < l.rows; r += kThreads / 32) {
     const bool is_draft = r > p.drafts;
     if (is_draft ? (greedy || !soft_draft || r - T1 >= n) : r > n) continue;
     const float4 *st = ws.stats + ((long long)b * l.rows + r) * l.chunks;
     float m = -INFINITY, z = 0.f;
-    int at = 0;
-    for (int i = 0; i < l.chunks; ++i) {
-      const float4 v = st[i];
+    int at = 0x7fffffff;
+    for (int i = lane; i < l.chunks; i += 32) {
+      const float4 v = __ldcg(st + i);
       if (greedy) {
-        if (v.x > m) {                  // chunks come in index order: the first maximum stays
+        if (v.x > m || (v.x == m && __float_as_int(v.z) < at)) {
           m = v.x;
           at = __float_as_int(v.z);
         }
@@ -191,101 +275,135 @@ __global__ void __launch_bounds__(kThreads) verify_pick_kernel(const VerifyParam
         join(m, z, v.x, v.y);
       }
     }
-    m_s[r] = m;
-    z_s[r] = z;
-    if (!is_draft) at_s[r] = at;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), z2 = __shfl_xor_sync(0xffffffffu, z, o);
+      const int at2 = __shfl_xor_sync(0xffffffffu, at, o);
+      if (greedy) {
+        if (m2 > m || (m2 == m && at2 < at)) {
+          m = m2;
+          at = at2;
+        }
+      } else {
+        join(m, z, m2, z2);
+      }
+    }
+    if (lane == 0) {
+      m_s[r] = m;
+      z_s[r] = z > 0.f ? 1.f / z : 0.f;
+      if (!is_draft) at_s[r] = at;
+    }
   }
-  if (threadIdx.x == 0) k_s = n;
   __syncthreads();
-  const float c = greedy ? 1.f : kLog2e / fmaxf(heat, 1e-30f);
-  auto prob = [&](int r, float logit) {            // p (or q) of a token of row r
-    return m_s[r] > -INFINITY ? exp2f(logit * c - m_s[r]) / z_s[r] : 0.f;
+  // p (or q) of a token of row r
+  auto prob = [&](float m, float inv, float logit) {
+    return m > -INFINITY ? fast_exp2(fmaf(logit, c, -m)) * inv : 0.f;
   };
-  for (int j = threadIdx.x; j < n; j += kThreads) {
-    const long long x = p.tokens[b * p.tok_s[0] + j * p.tok_s[1]];
+  if (j < n) {
     bool ok = false;
     if (x >= 0 && x < p.vocab) {                    // anything else is no token: rejected
-      if (greedy) {
-        ok = x == at_s[j];
-      } else {
-        const float pj = prob(j, to_f32(logits_row<T>(p, b, j)[x]));
-        const float qj = soft_draft ? prob(T1 + j, to_f32(logits_row<T>(p, b, T1 + j)[x])) : 1.f;
-        ok = p.uniforms[b * p.uni_s[0] + j * p.uni_s[1]] * qj < pj;
-      }
+      if (greedy) ok = x == at_s[j];
+      else ok = u * (soft_draft ? prob(m_s[T1 + j], z_s[T1 + j], dx) : 1.f) < prob(m_s[j], z_s[j], tx);
     }
     if (!ok) atomicMin(&k_s, j);
   }
   __syncthreads();
   const int k = k_s;
-  unsigned long long rest = 0ull, whole = 0ull;
-  if (!greedy) {
-    const T *tr = logits_row<T>(p, b, k);
-    const bool rejected = k < n;
-    const T *dr = rejected && soft_draft ? logits_row<T>(p, b, T1 + k) : nullptr;
-    const long long drop = rejected && !soft_draft ? p.tokens[b * p.tok_s[0] + k * p.tok_s[1]] : -1;
-    const float *e = p.noise + b * p.noise_s;
-    const int i0 = chunk * l.chunk, i1 = min(p.vocab, i0 + l.chunk);
-    for (int i = i0 + (int)threadIdx.x; i < i1; i += kThreads) {
-      const float pi = prob(k, to_f32(tr[i]));
-      const float ei = e[i];
-      float w = pi;
-      if (dr != nullptr) w = fmaxf(pi - prob(T1 + k, to_f32(dr[i])), 0.f);
-      if (i == drop) w = fmaxf(pi - 1.f, 0.f);
-      if (w > 0.f) rest = max(rest, race_key(w / ei, (unsigned)i));
-      if (pi > 0.f) whole = max(whole, race_key(pi / ei, (unsigned)i));
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      rest = max(rest, __shfl_xor_sync(0xffffffffu, rest, o));
-      whole = max(whole, __shfl_xor_sync(0xffffffffu, whole, o));
-    }
-    if (lane == 0) {
-      rest_s[warp] = rest;
-      pk_s[warp] = whole;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int w = 1; w < kThreads / 32; ++w) {
-        rest = max(rest, rest_s[w]);
-        whole = max(whole, pk_s[w]);
+  const bool rejected = k < n;
+  const T *tr = logits_row<T>(p, b, k);
+  const T *dr = rejected && soft_draft ? logits_row<T>(p, b, T1 + k) : nullptr;
+  const long long gone = rejected && !soft_draft ? p.tokens[b * p.tok_s[0] + k * p.tok_s[1]] : -1;
+  const int drop = gone >= 0 && gone < p.vocab ? (int)gone : -1;
+  const float *noise = p.noise + b * p.noise_s;
+  const float mt = m_s[k], zt = z_s[k], md = dr != nullptr ? m_s[T1 + k] : 0.f, zd = dr != nullptr ? z_s[T1 + k] : 0.f;
+  // this thread's best runner of [i0, i1)
+  auto race = [&](int i0, int i1, bool rest) {
+    float top = 0.f;
+    int who = 0;
+    const bool minus = rest && dr != nullptr;
+    const int gone_at = rest ? drop : -1;
+    auto run = [&](int at, float t, float d, float e) {
+      float w = prob(mt, zt, t);
+      if (minus) w -= prob(md, zd, d);
+      if (at == gone_at) w -= 1.f;
+      const float v = __fdividef(w, e);
+      if (v > top) {                                // ascending indices: ties keep the lowest
+        top = v;
+        who = at;
       }
-      atomicMax(&ws.rest_key[b], rest);
-      atomicMax(&ws.p_key[b], whole);
+    };
+    constexpr int kU = 8;
+    int i = i0 + (int)threadIdx.x;
+    for (; i + (kU - 1) * kThreads < i1; i += kU * kThreads) {
+      float t[kU], d[kU], e[kU];
+#pragma unroll
+      for (int q = 0; q < kU; ++q) {
+        t[q] = to_f32(tr[i + q * kThreads]);
+        e[q] = __ldg(noise + i + q * kThreads);
+        d[q] = 0.f;
+      }
+      if (minus) {
+#pragma unroll
+        for (int q = 0; q < kU; ++q) d[q] = to_f32(dr[i + q * kThreads]);
+      }
+#pragma unroll
+      for (int q = 0; q < kU; ++q) run(i + q * kThreads, t[q], d[q], e[q]);
+    }
+    for (; i < i1; i += kThreads) run(i, to_f32(tr[i]), minus ? to_f32(dr[i]) : 0.f, __ldg(noise + i));
+    unsigned long long best = top > 0.f ? race_key(top, (unsigned)who) : 0ull;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+    if (lane == 0) key_s[warp] = best;
+    __syncthreads();
+    best = key_s[0];
+    for (int w = 1; w < kThreads / 32; ++w) best = max(best, key_s[w]);
+    return best;
+  };
+  long long next = at_s[greedy ? k : 0];
+  if (!greedy) {
+    const unsigned long long mine = race(chunk * l.race, min(p.vocab, (chunk + 1) * l.race), rejected);
+    if (threadIdx.x == 0) {
+      if (mine != 0ull) atomicMax(&ws.key[b], mine);
       __threadfence();
-      last_s = atomicAdd(&ws.ticket[b], 1u) == (unsigned)l.chunks - 1u;
+      last_s = atomicAdd(&ws.ticket[b], 1u) == (unsigned)l.races - 1u;
     }
     __syncthreads();
     if (!last_s) return;
+    // the question's last CTA writes the answer
     __threadfence();
-  }
-  // the question's last CTA writes the answer
-  long long next = at_s[greedy ? k : 0];
-  if (!greedy) {
-    unsigned long long key = atomicMax(&ws.rest_key[b], 0ull);
-    if (key == 0ull) key = atomicMax(&ws.p_key[b], 0ull);
+    unsigned long long key = __ldcg(&ws.key[b]);
+    if (key == 0ull && rejected) key = race(0, p.vocab, false);   // p - q left nothing: draw from p
     next = key == 0ull ? 0 : (long long)(0xffffffffu - (unsigned)(key & 0xffffffffull));
   }
-  for (int j = threadIdx.x; j < T1; j += kThreads)
-    p.out_tokens[(long long)b * T1 + j] = j < k ? p.tokens[b * p.tok_s[0] + j * p.tok_s[1]] : j == k ? next : -1ll;
+  for (int i = threadIdx.x; i < T1; i += kThreads)
+    p.out_tokens[(long long)b * T1 + i] = i < k ? p.tokens[b * p.tok_s[0] + i * p.tok_s[1]] : i == k ? next : -1ll;
   if (threadIdx.x == 0) p.accepted[b] = k;
 }
 
 template <typename T>
 cudaError_t verify(const VerifyParams &p, cudaStream_t stream) {
-  const VerifyLayout l = verify_layout(p.drafts, p.vocab);
-  const int rows = p.draft.data != nullptr ? (int)l.rows : p.drafts + 1;
+  const VerifyLayout l = verify_layout(p.batch, p.drafts, p.vocab);
+  const int rows = p.draft.data != nullptr ? l.rows : p.drafts + 1;
   verify_stats_kernel<T><<<dim3(l.chunks, rows, p.batch), kThreads, 0, stream>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  verify_pick_kernel<T><<<dim3(l.chunks, p.batch), kThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(l.races, p.batch);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, verify_pick_kernel<T>, p);
 }
 
 }  // namespace
 
 size_t verify_workspace_bytes(long long batch, long long drafts, long long vocab) {
-  const VerifyLayout l = verify_layout(drafts, vocab);
-  return (size_t)(align16(batch * 20) + batch * l.rows * l.chunks * 16);
+  const VerifyLayout l = verify_layout(batch, drafts, vocab);
+  return (size_t)(align16(batch * 12) + batch * l.rows * l.chunks * 16);
 }
 
 cudaError_t launch_verify(const VerifyParams &p, int sms, cudaStream_t stream) {
