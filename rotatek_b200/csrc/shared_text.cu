@@ -31,13 +31,15 @@ namespace rtk {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr float kLazy = 8.f;
 
 template <bool FP8, int kRT>
 struct TextSmem {
   static constexpr int kTok = FP8 ? 32 : 16;               // tokens of a block
   static constexpr int kRow = FP8 ? 128 : 256;             // bytes of a token's Key (or Value)
-  static constexpr int kStage = 2 * kTok * kRow;           // 8 KB
-  static constexpr int kStages = 3;
+  static constexpr int kScales = 2 * kTok * kRow;          // FP8: the tokens' Key scales, Value scales
+  static constexpr int kStage = kScales + (FP8 ? 2 * kTok * 4 : 0);   // 8 KB and the scales
+  static constexpr int kStages = 2;
   static constexpr int kQ = 0;                             // 16 kRT rows of 256 bytes
   static constexpr int kRing = kQ + kRT * 4096;
   static constexpr int kBytes = kRing + kWarps * kStages * kStage;
@@ -51,6 +53,11 @@ struct TextSmem {
 template <int kRow>
 __device__ __forceinline__ uint32_t at(int r, int c) {
   return (uint32_t)(r * kRow + ((c ^ (r & 7)) << 4));
+}
+
+// 4-byte global -> shared copy; zero where `in` is false
+__device__ __forceinline__ void cp_async_4_zfill(void *dst, const void *src, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 4 : 0) : "memory");
 }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -87,6 +94,8 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
   kbase += (b * a.kt.s[0] + h * a.kt.s[1]) * kEsize;
   vbase += (b * a.vt.s[0] + h * a.vt.s[1]) * kEsize;
   const long long ks = a.kt.s[2] * kEsize, vs = a.vt.s[2] * kEsize;
+  const float *ksc = FP8 ? static_cast<const float *>(a.ksc.data) + b * a.ksc.s[0] + h * a.ksc.s[1] : nullptr;
+  const float *vsc = FP8 ? static_cast<const float *>(a.vsc.data) + b * a.vsc.s[0] + h * a.vsc.s[1] : nullptr;
   auto fetch = [&](int blk, int stage) {
     unsigned char *dst = ring + stage * L::kStage;
     constexpr int kChunks = L::kRow / 16;
@@ -99,6 +108,11 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
       cp_async_16_zfill(dst + at<L::kRow>(r, c), kbase + (in ? tok * ks + c * 16 : 0), in ? 16 : 0);
       cp_async_16_zfill(dst + L::kTok * L::kRow + at<L::kRow>(r, c), vbase + (in ? tok * vs + c * 16 : 0), in ? 16 : 0);
     }
+    if constexpr (FP8) {                             // lane = token of the block
+      const bool in = first + lane < t1;
+      cp_async_4_zfill(dst + L::kScales + lane * 4, ksc + (in ? (first + lane) * a.ksc.s[2] : 0), in);
+      cp_async_4_zfill(dst + L::kScales + 128 + lane * 4, vsc + (in ? (first + lane) * a.vsc.s[2] : 0), in);
+    }
   };
 #pragma unroll
   for (int i = 0; i < L::kStages - 1; ++i) {
@@ -108,14 +122,21 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
 
   // queries: 16 kRT rows x 128 channels; per-row factor of the logits
   __shared__ float qscale_s[16 * kRT];
-  for (int e = warp; e < 16 * kRT; e += kWarps) {
-    const int r = row0 + e;
-    uint2 v = make_uint2(0, 0);                      // channels 4 lane .. 4 lane + 3
+  uint2 qv[4 * kRT];                                 // all in flight at once
+#pragma unroll
+  for (int k = 0; k < 4 * kRT; ++k) {
+    const int r = row0 + warp + kWarps * k;
+    qv[k] = make_uint2(0, 0);                        // channels 4 lane .. 4 lane + 3
     if (r < p.rows) {
       const int t = r / a.groups, gh = r % a.groups;
-      v = __ldg(reinterpret_cast<const uint2 *>(static_cast<const T *>(a.q.data) + b * a.q.s[0] + t * a.q.s[1] +
-                                                (h * a.groups + gh) * a.q.s[2] + lane * 4));
+      qv[k] = __ldg(reinterpret_cast<const uint2 *>(static_cast<const T *>(a.q.data) + b * a.q.s[0] + t * a.q.s[1] +
+                                                    (h * a.groups + gh) * a.q.s[2] + lane * 4));
     }
+  }
+#pragma unroll
+  for (int k = 0; k < 4 * kRT; ++k) {
+    const int e = warp + kWarps * k;
+    const uint2 v = qv[k];
     float f = a.scale_log2;
     if constexpr (FP8) {
       float x[4];
@@ -174,24 +195,12 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
       for (int i = 0; i < 4; ++i) acc[rt][n][i] = 0.f;
   }
   const uint32_t q_addr = smem_u32(smem + L::kQ);
-  const float *ksc = FP8 ? static_cast<const float *>(a.ksc.data) + b * a.ksc.s[0] + h * a.ksc.s[1] : nullptr;
-  const float *vsc = FP8 ? static_cast<const float *>(a.vsc.data) + b * a.vsc.s[0] + h * a.vsc.s[1] : nullptr;
 
   int stage = 0;
   for (int blk = warp; blk < blocks; blk += kWarps) {
     const int first = t0 + blk * L::kTok;
     constexpr int kNT = L::kTok / 8;                 // n-tiles of 8 tokens
     float kscale[kNT][2], vscale[kNT][2];
-    if constexpr (FP8) {
-#pragma unroll
-      for (int n = 0; n < kNT; ++n)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int tok = first + n * 8 + 2 * j4 + i;
-          kscale[n][i] = tok < t1 ? __ldg(ksc + tok * a.ksc.s[2]) : 0.f;
-          vscale[n][i] = tok < t1 ? __ldg(vsc + tok * a.vsc.s[2]) : 0.f;
-        }
-    }
     {
       const int next = blk + kWarps * (L::kStages - 1);
       int st2 = stage + L::kStages - 1;
@@ -204,6 +213,14 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
     const uint32_t k_addr = smem_u32(ring + stage * L::kStage), v_addr = k_addr + L::kTok * L::kRow;
 
     if constexpr (FP8) {
+      const unsigned char *sc = ring + stage * L::kStage + L::kScales;
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) {
+        const float2 k2 = *reinterpret_cast<const float2 *>(sc + (n * 8 + 2 * j4) * 4);
+        const float2 v2 = *reinterpret_cast<const float2 *>(sc + 128 + (n * 8 + 2 * j4) * 4);
+        kscale[n][0] = k2.x; kscale[n][1] = k2.y;
+        vscale[n][0] = v2.x; vscale[n][1] = v2.y;
+      }
       // the largest Value scale of the block, over the warp
       float top = 0.f;
 #pragma unroll
@@ -253,40 +270,55 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
           mma_16816<T>(s[1], qa, r[2], r[3]);
         }
       }
-      // logits in base 2; unseen tokens weigh nothing
+      // logits but for the row's factor; unseen tokens weigh nothing
       float mx[2] = {-INFINITY, -INFINITY};
+      if constexpr (FP8) {
+#pragma unroll
+        for (int n = 0; n < kNT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[n][i] *= kscale[n][i & 1];
+      }
+      if (first + L::kTok > all_see) {
+#pragma unroll
+        for (int n = 0; n < kNT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (first + n * 8 + 2 * j4 + (i & 1) >= limit[rt][i >> 1]) s[n][i] = -INFINITY;
+      }
 #pragma unroll
       for (int n = 0; n < kNT; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float x = s[n][i] * qf[rt][i >> 1];
-          if constexpr (FP8) x *= kscale[n][i & 1];
-          if (first + L::kTok > all_see && first + n * 8 + 2 * j4 + (i & 1) >= limit[rt][i >> 1]) x = -INFINITY;
-          s[n][i] = x;
-          mx[i >> 1] = fmaxf(mx[i >> 1], x);
-        }
-      float base[2];
+        for (int i = 0; i < 4; ++i) mx[i >> 1] = fmaxf(mx[i >> 1], s[n][i]);
+      // base-2 maxima of the rows; O and l move to a new one only when it is more than 2^8
+      // above the one in use
+      bool grow[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-        const float m2 = fmaxf(m[rt][i], mx[i]);
-        base[i] = m2 > -INFINITY ? m2 : 0.f;
-        const float f = fast_exp2(m[rt][i] - base[i]);         // nothing yet: 2^-inf = 0
-        m[rt][i] = m2;
-        l[rt][i] *= f;
+        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2)) * qf[rt][i];      // qf > 0
+        grow[i] = mx[i] > m[rt][i] + kLazy;          // from -inf: whenever there is a maximum
+      }
+      if (__any_sync(0xffffffffu, grow[0] || grow[1])) {
 #pragma unroll
-        for (int n = 0; n < 16; ++n) {
-          acc[rt][n][2 * i] *= f;
-          acc[rt][n][2 * i + 1] *= f;
+        for (int i = 0; i < 2; ++i) {
+          const float f = grow[i] ? fast_exp2(m[rt][i] - mx[i]) : 1.f;      // nothing yet: 2^-inf = 0
+          if (grow[i]) m[rt][i] = mx[i];
+          l[rt][i] *= f;
+#pragma unroll
+          for (int n = 0; n < 16; ++n) {
+            acc[rt][n][2 * i] *= f;
+            acc[rt][n][2 * i + 1] *= f;
+          }
         }
       }
+      const float base[2] = {m[rt][0] > -INFINITY ? m[rt][0] : 0.f, m[rt][1] > -INFINITY ? m[rt][1] : 0.f};
       uint32_t pa[kNT][2];                           // weights of rows g, g + 8
 #pragma unroll
       for (int n = 0; n < kNT; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float w0 = fast_exp2(s[n][2 * i] - base[i]), w1 = fast_exp2(s[n][2 * i + 1] - base[i]);
+          float w0 = fast_exp2(fmaf(s[n][2 * i], qf[rt][i], -base[i]));
+          float w1 = fast_exp2(fmaf(s[n][2 * i + 1], qf[rt][i], -base[i]));
           if constexpr (FP8) {
             l[rt][i] += w0 + w1;
             w0 *= vscale[n][0];
@@ -387,6 +419,286 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
   }
 }
 
+// ---- many rows (T G > 16): the warps of a CTA split the rows, 16 each, and share the
+// tokens, 32 at a time, so that 8-bit text is converted once for 64 rows (converting in
+// every warp's registers cost 3.4 times the instructions: 103 against 36 us for 64
+// questions x 8 heads of 64 rows on up to 1001 tokens).
+template <bool FP8>
+struct RowsSmem {
+  static constexpr int kTok = 32;
+  static constexpr int kScales = 2 * kTok * (FP8 ? 128 : 256);    // after a tile's Keys and Values as stored
+  static constexpr int kRaw = kScales + (FP8 ? 2 * kTok * 4 : 0);
+  static constexpr int kStages = 3;
+  static constexpr int kQ = 0;                                    // 64 rows of 256 bytes
+  static constexpr int kTile = kQ + kWarps * 4096;                // FP8: the tile as f16
+  static constexpr int kRing = kTile + (FP8 ? 2 * kTok * 256 : 0);
+  static constexpr int kBytes = kRing + kStages * kRaw;
+};
+
+template <typename T, bool FP8>
+__global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const TextParams p) {
+  using L = RowsSmem<FP8>;
+  using M = typename std::conditional<FP8, __half, T>::type;     // MMA operand type
+  extern __shared__ __align__(128) unsigned char smem[];
+  const SharedParams &a = p.s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, j4 = lane & 3;
+  const int chunk = blockIdx.y, bh = blockIdx.x, row0 = blockIdx.z * 64 + warp * 16;
+  const int b = bh / a.kv_heads, h = bh % a.kv_heads;
+  const int len = min(max(a.lens[b * a.lens_s], 0), a.cap);
+  const int t0 = chunk * kTextChunk;
+  if (t0 >= len) return;
+  const int t1 = min(len, t0 + kTextChunk);
+  const int tiles = (t1 - t0 + L::kTok - 1) / L::kTok;
+  constexpr int kEsize = FP8 ? 1 : 2, kRowBytes = 128 * kEsize, kChunks = kRowBytes / 16;
+  const unsigned char *kbase = static_cast<const unsigned char *>(a.kt.data) + (b * a.kt.s[0] + h * a.kt.s[1]) * kEsize;
+  const unsigned char *vbase = static_cast<const unsigned char *>(a.vt.data) + (b * a.vt.s[0] + h * a.vt.s[1]) * kEsize;
+  const long long ks = a.kt.s[2] * kEsize, vs = a.vt.s[2] * kEsize;
+  const float *ksc = FP8 ? static_cast<const float *>(a.ksc.data) + b * a.ksc.s[0] + h * a.ksc.s[1] : nullptr;
+  const float *vsc = FP8 ? static_cast<const float *>(a.vsc.data) + b * a.vsc.s[0] + h * a.vsc.s[1] : nullptr;
+  auto fetch = [&](int tile) {
+    unsigned char *dst = smem + L::kRing + tile % L::kStages * L::kRaw;
+    const int first = t0 + tile * L::kTok;
+#pragma unroll
+    for (int e = 0; e < L::kTok * kChunks / (32 * kWarps); ++e) {
+      const int i = e * 32 * kWarps + threadIdx.x, r = i / kChunks, c = i % kChunks;
+      const int tok = first + r;
+      const bool in = tok < t1;
+      cp_async_16_zfill(dst + at<kRowBytes>(r, c), kbase + (in ? tok * ks + c * 16 : 0), in ? 16 : 0);
+      cp_async_16_zfill(dst + L::kTok * kRowBytes + at<kRowBytes>(r, c), vbase + (in ? tok * vs + c * 16 : 0), in ? 16 : 0);
+    }
+    if (FP8 && warp < 2) {                           // lane = token of the tile
+      const bool in = first + lane < t1;
+      cp_async_4_zfill(dst + L::kScales + warp * 128 + lane * 4,
+                       warp == 0 ? ksc + (in ? (first + lane) * a.ksc.s[2] : 0) : vsc + (in ? (first + lane) * a.vsc.s[2] : 0),
+                       in);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < L::kStages - 1; ++i) {
+    if (i < tiles) fetch(i);
+    cp_async_commit();
+  }
+  // this warp's 16 queries, in the MMA's type (bf16 against 8-bit text: f16 scaled by a power of two)
+  __shared__ float qscale_s[kWarps * 16];
+  uint2 qv[16];                                      // all in flight at once
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int r = row0 + e;
+    qv[e] = make_uint2(0, 0);                        // channels 4 lane .. 4 lane + 3
+    if (r < p.rows) {
+      const int t = r / a.groups, gh = r % a.groups;
+      qv[e] = __ldg(reinterpret_cast<const uint2 *>(static_cast<const T *>(a.q.data) + b * a.q.s[0] + t * a.q.s[1] +
+                                                    (h * a.groups + gh) * a.q.s[2] + lane * 4));
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    uint2 v = qv[e];
+    float f = a.scale_log2;
+    if constexpr (FP8 && std::is_same<T, __nv_bfloat16>::value) {
+      float x[4];
+      unpack2<T>(v.x, x[0], x[1]);
+      unpack2<T>(v.y, x[2], x[3]);
+      float mx = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const uint32_t ex = min(max(__float_as_uint(mx) >> 23, 1u), 253u);
+      const float inv = __uint_as_float((254u - ex) << 23);
+      v.x = pack2<__half>(x[0] * inv, x[1] * inv);
+      v.y = pack2<__half>(x[2] * inv, x[3] * inv);
+      f *= __uint_as_float(ex << 23);
+    }
+    *reinterpret_cast<uint2 *>(smem + L::kQ + at<256>(warp * 16 + e, lane >> 1) + (lane & 1) * 8) = v;
+    if (lane == 0) qscale_s[warp * 16 + e] = f;
+  }
+  __syncwarp();
+  const bool busy = row0 < p.rows;
+  int limit[2];
+  float qf[2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, acc[16][4], vref = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = row0 + g + 8 * i;
+    limit[i] = r < p.rows ? len - (a.tokens - 1 - r / a.groups) : 0;
+    qf[i] = qscale_s[warp * 16 + g + 8 * i];
+  }
+#pragma unroll
+  for (int n = 0; n < 16; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+  const int all_see = len - (a.tokens - 1);          // every row sees tokens below this
+  const uint32_t q_addr = smem_u32(smem + L::kQ);
+
+  for (int tile = 0; tile < tiles; ++tile) {
+    const int first = t0 + tile * L::kTok;
+    constexpr int kNT = 4;
+    float kscale[kNT][2], vscale[kNT][2];
+    cp_async_wait_group<L::kStages - 2>();
+    __syncthreads();                                 // the tile has landed; the one before is done with
+    if (tile + L::kStages - 1 < tiles) fetch(tile + L::kStages - 1);
+    cp_async_commit();
+    uint32_t k_addr, v_addr;
+    const unsigned char *raw = smem + L::kRing + tile % L::kStages * L::kRaw;
+    if constexpr (FP8) {
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) {
+        const float2 k2 = *reinterpret_cast<const float2 *>(raw + L::kScales + (n * 8 + 2 * j4) * 4);
+        const float2 v2 = *reinterpret_cast<const float2 *>(raw + L::kScales + 128 + (n * 8 + 2 * j4) * 4);
+        kscale[n][0] = k2.x; kscale[n][1] = k2.y;
+        vscale[n][0] = v2.x; vscale[n][1] = v2.y;
+      }
+      // 16 bytes of a row become 16 f16: two chunks of the row's 256 bytes
+#pragma unroll
+      for (int e = 0; e < 2 * L::kTok * 8 / (32 * kWarps); ++e) {
+        const int i = e * 32 * kWarps + threadIdx.x, r = i >> 3, c = i & 7;   // rows 0-31 Keys, 32-63 Values
+        const uint4 w = *reinterpret_cast<const uint4 *>(raw + at<128>(r, c));
+        uint4 lo, hi;
+        lo.x = e4m3x2_f16x2((uint16_t)(w.x & 0xffffu)); lo.y = e4m3x2_f16x2((uint16_t)(w.x >> 16));
+        lo.z = e4m3x2_f16x2((uint16_t)(w.y & 0xffffu)); lo.w = e4m3x2_f16x2((uint16_t)(w.y >> 16));
+        hi.x = e4m3x2_f16x2((uint16_t)(w.z & 0xffffu)); hi.y = e4m3x2_f16x2((uint16_t)(w.z >> 16));
+        hi.z = e4m3x2_f16x2((uint16_t)(w.w & 0xffffu)); hi.w = e4m3x2_f16x2((uint16_t)(w.w >> 16));
+        *reinterpret_cast<uint4 *>(smem + L::kTile + at<256>(r, 2 * c)) = lo;
+        *reinterpret_cast<uint4 *>(smem + L::kTile + at<256>(r, 2 * c + 1)) = hi;
+      }
+      __syncthreads();
+      k_addr = smem_u32(smem + L::kTile);
+      v_addr = k_addr + L::kTok * 256;
+      float top = 0.f;                               // the tile's largest Value scale
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) top = fmaxf(top, fmaxf(vscale[n][0], vscale[n][1]));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      if (top > vref) {                              // the same in every lane
+        const float f = vref / top;
+        vref = top;
+#pragma unroll
+        for (int n = 0; n < 16; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[n][i] *= f;
+      }
+      const float inv = vref > 0.f ? 1.f / vref : 0.f;
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) {
+        vscale[n][0] *= inv;
+        vscale[n][1] *= inv;
+      }
+    } else {
+      k_addr = smem_u32(raw);
+      v_addr = k_addr + L::kTok * 256;
+    }
+    if (!busy) continue;
+    float s[kNT][4];
+#pragma unroll
+    for (int n = 0; n < kNT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {                    // 16 channels
+      uint32_t qa[4], r[4], r2[4];
+      ldmatrix_x4(q_addr + at<256>(warp * 16 + (lane & 15), 2 * k + (lane >> 4)), qa[0], qa[1], qa[2], qa[3]);
+      ldmatrix_x4(k_addr + at<256>((lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)), r[0], r[1], r[2], r[3]);
+      ldmatrix_x4(k_addr + at<256>(16 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)), r2[0], r2[1], r2[2],
+                  r2[3]);
+      mma_16816<M>(s[0], qa, r[0], r[1]);
+      mma_16816<M>(s[1], qa, r[2], r[3]);
+      mma_16816<M>(s[2], qa, r2[0], r2[1]);
+      mma_16816<M>(s[3], qa, r2[2], r2[3]);
+    }
+    if constexpr (FP8) {
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] *= kscale[n][i & 1];
+    }
+    if (first + L::kTok > all_see) {                 // unseen tokens weigh nothing
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (first + n * 8 + 2 * j4 + (i & 1) >= limit[i >> 1]) s[n][i] = -INFINITY;
+    }
+    bool grow[2];
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < kNT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx[i >> 1] = fmaxf(mx[i >> 1], s[n][i]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2)) * qf[i];
+      grow[i] = mx[i] > m[i] + kLazy;
+    }
+    if (__any_sync(0xffffffffu, grow[0] || grow[1])) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float f = grow[i] ? fast_exp2(m[i] - mx[i]) : 1.f;
+        if (grow[i]) m[i] = mx[i];
+        l[i] *= f;
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          acc[n][2 * i] *= f;
+          acc[n][2 * i + 1] *= f;
+        }
+      }
+    }
+    const float base[2] = {m[0] > -INFINITY ? m[0] : 0.f, m[1] > -INFINITY ? m[1] : 0.f};
+    uint32_t pa[kNT][2];
+#pragma unroll
+    for (int n = 0; n < kNT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float w0 = fast_exp2(fmaf(s[n][2 * i], qf[i], -base[i])), w1 = fast_exp2(fmaf(s[n][2 * i + 1], qf[i], -base[i]));
+        if constexpr (FP8) {
+          l[i] += w0 + w1;
+          pa[n][i] = pack2<M>(w0 * vscale[n][0], w1 * vscale[n][1]);
+        } else {
+          pa[n][i] = pack2<M>(w0, w1);
+          unpack2<M>(pa[n][i], w0, w1);
+          l[i] += w0 + w1;
+        }
+      }
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {                 // 16 tokens
+      const uint32_t pf[4] = {pa[2 * kk][0], pa[2 * kk][1], pa[2 * kk + 1][0], pa[2 * kk + 1][1]};
+#pragma unroll
+      for (int c = 0; c < 16; c += 2) {              // two chunks of 8 channels
+        uint32_t r[4];
+        ldmatrix_x4_trans(v_addr + at<256>(kk * 16 + (lane & 15), c + (lane >> 4)), r[0], r[1], r[2], r[3]);
+        mma_16816<M>(acc[c], pf, r[0], r[1]);
+        mma_16816<M>(acc[c + 1], pf, r[2], r[3]);
+      }
+    }
+  }
+  cp_async_wait_all();
+  const float scale_o = FP8 ? vref : 1.f;
+  const long long slot = ((long long)bh * p.chunks + chunk) * p.rows;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float ll = l[i];
+    ll += __shfl_xor_sync(0xffffffffu, ll, 1);
+    ll += __shfl_xor_sync(0xffffffffu, ll, 2);
+    const int r = row0 + g + 8 * i;
+    if (r < p.rows) {
+      float *out = p.acc + (slot + r) * 128 + 2 * j4;
+#pragma unroll
+      for (int n = 0; n < 16; ++n)
+        *reinterpret_cast<float2 *>(out + 8 * n) = make_float2(acc[n][2 * i] * scale_o, acc[n][2 * i + 1] * scale_o);
+      if (j4 == 0) reinterpret_cast<float2 *>(p.ml)[slot + r] = make_float2(m[i], ll);
+    }
+  }
+}
+
+template <typename T, bool FP8>
+cudaError_t launch_rows(const TextParams &p, cudaStream_t stream) {
+  const int smem = RowsSmem<FP8>::kBytes;
+  cudaError_t e = cudaFuncSetAttribute(shared_text_rows_kernel<T, FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  const dim3 grid(p.s.prefixes * p.s.questions * p.s.kv_heads, p.chunks, (p.rows + 63) / 64);
+  shared_text_rows_kernel<T, FP8><<<grid, kWarps * 32, smem, stream>>>(p);
+  return cudaGetLastError();
+}
+
 template <typename T, bool FP8, int kRT>
 cudaError_t launch(const TextParams &p, cudaStream_t stream) {
   const int smem = TextSmem<FP8, kRT>::kBytes;
@@ -399,8 +711,9 @@ cudaError_t launch(const TextParams &p, cudaStream_t stream) {
 
 template <typename T>
 cudaError_t launch_t(const TextParams &p, cudaStream_t stream) {
-  if (p.s.text_fp8) return launch<T, true, 1>(p, stream);
-  return launch<T, false, 1>(p, stream);
+  // few rows: the warps split the tokens; more than an MMA's 16: they split the rows
+  if (p.rows <= 16) return p.s.text_fp8 ? launch<T, true, 1>(p, stream) : launch<T, false, 1>(p, stream);
+  return p.s.text_fp8 ? launch_rows<T, true>(p, stream) : launch_rows<T, false>(p, stream);
 }
 
 }  // namespace
