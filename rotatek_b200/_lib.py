@@ -98,6 +98,31 @@ def load(path: str = LIB_PATH):
     return _lib
 
 
+_calls = None
+
+
+def calls():
+    """The module of direct calls (csrc/calls.c), bound to the loaded library."""
+    global _calls
+    if _calls is None:
+        load()
+        with _lock:
+            if _calls is None:
+                try:
+                    from rotatek_b200 import _calls as mod
+                except ImportError as e:
+                    raise RuntimeError("rotatek_b200/_calls.so is missing; build it with "
+                                       "`python -m rotatek_b200.csrc.build`") from e
+                mod.bind(_lib._name, _DTYPES)
+                _calls = mod
+    return _calls
+
+
+def raw_stream(device: torch.device) -> int:
+    """The current stream of `device` as an address."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def describe(t: Optional[torch.Tensor]):
     """rtk_tensor descriptor of a CUDA tensor (None -> NULL pointer)."""
     if t is None:
@@ -174,6 +199,23 @@ def workspace(device: torch.device, nbytes: int, counter_bytes: int) -> torch.Te
             buf[:counter_bytes].zero_()
         _zero_prefix[idx] = counter_bytes     # what follows is scratch after the call
         return buf
+
+
+_scratch = {}        # (device index, stream address) -> uint8 buffer
+
+
+def scratch(device: torch.device, stream: int, nbytes: int = 0) -> torch.Tensor:
+    """Scratch of a stream's own, at least `nbytes` long, for kernels that need nothing
+    zeroed and nothing kept: calls on one stream follow one another on the GPU, calls on
+    several do not share it.  Grown on demand; a call that is being captured gets a
+    buffer of the capture's own."""
+    if torch._C._cuda_isCurrentStreamCapturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    buf = _scratch.get((device.index, stream))
+    if buf is None or buf.numel() < nbytes:
+        buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+        _scratch[(device.index, stream)] = buf
+    return buf
 
 
 def status_word(device: torch.device) -> int:

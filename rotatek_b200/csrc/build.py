@@ -6,7 +6,9 @@ The library lands next to the package (rotatek_b200/librotatek_b200.so) so a
 snapshot of the source tree carries it.  The CUDA runtime is linked
 statically: the library does not depend on which libcudart the host process
 (e.g. torch) has loaded.  cuTensorMapEncodeTiled is resolved at run time
-through cudaGetDriverEntryPointByVersion, so there is no -lcuda.
+through cudaGetDriverEntryPointByVersion, so there is no -lcuda.  Beside it lands
+rotatek_b200/_calls.so, the CPython module that calls the shared-prefix entry
+points without ctypes.
 """
 from __future__ import annotations
 
@@ -15,11 +17,13 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 CSRC = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(CSRC)
 REPO = os.path.dirname(PKG)
 LIB_NAME = "librotatek_b200.so"
+CALLS_NAME = "_calls.so"          # CPython module over the C ABI (calls.c)
 SOURCES = ["capi.cu", "decode_tc.cu", "decode_simt.cu", "decode_static.cu", "quant_fp8.cu", "spark_pack.cu", "cov_tc.cu", "kproj_tc.cu", "eigen.cu",
            "rotate.cu", "selftest.cu", "capi_shared.cu", "shared_simt.cu", "shared_prefix.cu", "shared_text.cu", "shared_merge.cu", "text_cache.cu", "verify.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -49,6 +53,19 @@ def build(verbose: bool = False, out_dir: str = PKG) -> str:
     tmp = out + ".tmp"
     subprocess.run([nvcc()] + ARCH + ["-shared", "-cudart", "static", "-o", tmp] + objs, check=True)
     os.replace(tmp, out)
+    build_calls(out_dir)
+    return out
+
+
+def build_calls(out_dir: str = PKG) -> str:
+    """The Python module of direct calls: a C file against Python.h alone."""
+    out = os.path.join(out_dir, CALLS_NAME)
+    cc = os.environ.get("CC") or shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        raise RuntimeError("no C compiler found (set CC)")
+    subprocess.run([cc, "-O2", "-std=c11", "-Wall", "-shared", "-fPIC", "-I", sysconfig.get_paths()["include"],
+                    os.path.join(CSRC, "calls.c"), "-o", out + ".tmp", "-ldl"], check=True)
+    os.replace(out + ".tmp", out)
     return out
 
 

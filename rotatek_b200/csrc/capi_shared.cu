@@ -246,6 +246,7 @@ int rtk_shared_decode(const rtk_tensor *q, const rtk_tensor *R_partial, const rt
     rtk::TextParams tp;
     tp.s = p;
     tp.rows = (int)rows; tp.chunks = (int)chunks;
+    tp.beside = mp.has_prefix;
     tp.ml = tml; tp.acc = tacc;
     e = rtk::launch_shared_text(tp, st);
     if (e != cudaSuccess) return cuda_fail(e, "shared decode (text kernel) launch");

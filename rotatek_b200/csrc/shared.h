@@ -6,7 +6,24 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace rtk {
+
+// Let `kernel` use `bytes` of dynamic shared memory on the current device; asked once
+// per device.
+template <auto kernel>
+cudaError_t allow_shared_memory(int bytes) {
+  static std::atomic<unsigned long long> done{0};
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = device < 64 ? 1ull << device : 0ull;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 struct SharedTensor {
   const void *data;
@@ -115,6 +132,7 @@ constexpr int kTextChunk = 256;
 struct TextParams {
   SharedParams s;
   int rows, chunks;             // T G query rows, ceil(cap / kTextChunk)
+  int beside;                   // launched right after the prefix kernel, to run beside it
   float *ml, *acc;              // per (question, KV head, chunk): [rows][2] and [rows][128]
 };
 cudaError_t launch_shared_text(const TextParams &p, cudaStream_t stream);

@@ -3,7 +3,9 @@
 //   out = sum_i f_i O_i / sum_i f_i l_i,   f_i = 2^(m_i - max m),
 // in slot order (the same result every time); a row that saw nothing is 0.
 //
-// One warp per row, lane = 4 channels.  The partials are read once, from L2 mostly.
+// One warp per row, lane = 4 channels.  A row can have as many partials as there are
+// SMs, so their (m, l) are read 32 at a time, a lane each, and their O with eight loads
+// in flight; partials come from L2 mostly.
 #include "common.cuh"
 #include "shared.h"
 
@@ -15,6 +17,7 @@ constexpr int kWarps = 4;
 template <typename T>
 __global__ void __launch_bounds__(kWarps * 32) shared_merge_kernel(const MergeParams p) {
   const SharedParams &a = p.s;
+  wait_for_previous();
   const long long rows = (long long)a.prefixes * a.questions * a.tokens * a.q_heads;
   const long long idx = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (idx >= rows) return;
@@ -24,36 +27,73 @@ __global__ void __launch_bounds__(kWarps * 32) shared_merge_kernel(const MergePa
   const int t = (int)(bt % a.tokens), b = (int)(bt / a.tokens);
   const int h = hq / a.groups, g = hq % a.groups;
 
-  float m = -INFINITY, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto take = [&](float2 ml, const float *src) {
-    if (!(ml.x > -INFINITY) && !isnan(ml.x)) return;
-    const float m2 = fmaxf(m, ml.x);
-    const float f = fast_exp2(m - m2), fi = fast_exp2(ml.x - m2);
-    m = m2;
-    l = fmaf(l, f, ml.y * fi);
-    const float4 v = *reinterpret_cast<const float4 *>(src + lane * 4);
-    o.x = fmaf(o.x, f, v.x * fi);
-    o.y = fmaf(o.y, f, v.y * fi);
-    o.z = fmaf(o.z, f, v.z * fi);
-    o.w = fmaf(o.w, f, v.w * fi);
-  };
+  // partial i: the prefix's CTAs first, then the text's chunks
+  int prefixes = 0, total = 0;
+  long long at_p = 0, at_t = 0;
   if (p.has_prefix) {
     const int pre = b / a.questions, n = b % a.questions;
     const int r = (n * a.tokens + t) * a.groups + g;
     const int u = (pre * a.kv_heads + h) * p.split.row_tiles + r / 128;
-    const int c1 = p.split.last_cta(u);
-    for (int c = p.split.first_cta(u); c <= c1; ++c) {
-      const long long at = (long long)(u + c) * 128 + r % 128;
-      take(reinterpret_cast<const float2 *>(p.prefix_ml)[at], p.prefix_acc + at * 128);
-    }
+    const int c0 = p.split.first_cta(u);
+    prefixes = p.split.last_cta(u) - c0 + 1;
+    at_p = (long long)(u + c0) * 128 + r % 128;
   }
+  total = prefixes;
   if (p.has_text) {
     const int len = min(max(a.lens[b * a.lens_s], 0), a.cap);
-    const int r = t * a.groups + g;
-    for (int c = 0; c * kTextChunk < len; ++c) {
-      const long long at = (((long long)b * a.kv_heads + h) * p.text_chunks + c) * p.text_rows + r;
-      take(reinterpret_cast<const float2 *>(p.text_ml)[at], p.text_acc + at * 128);
+    total += (len + kTextChunk - 1) / kTextChunk;
+    at_t = ((long long)b * a.kv_heads + h) * p.text_chunks * p.text_rows + t * a.groups + g;
+  }
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int first = 0; first < total; first += 32) {
+    const int count = min(32, total - first);
+    float2 ml = make_float2(-INFINITY, 0.f);
+    const float *src = nullptr;
+    if (lane < count) {
+      const int i = first + lane;
+      if (i < prefixes) {
+        ml = __ldcg(reinterpret_cast<const float2 *>(p.prefix_ml) + at_p + i * 128ll);
+        src = p.prefix_acc + (at_p + i * 128ll) * 128;
+      } else {
+        const long long at = at_t + (long long)(i - prefixes) * p.text_rows;
+        ml = __ldcg(reinterpret_cast<const float2 *>(p.text_ml) + at);
+        src = p.text_acc + at * 128;
+      }
+    }
+    float top = ml.x;
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+    const float m2 = fmaxf(m, top), base = m2 > -INFINITY ? m2 : 0.f;
+    const float f = fast_exp2(m - base);              // nothing yet: 0
+    float w = fast_exp2(ml.x - base);                 // an empty partial: 0
+    float sum = w > 0.f || isnan(w) ? w * ml.y : 0.f;
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+    m = m2;
+    l = fmaf(l, f, sum);
+    o.x *= f;
+    o.y *= f;
+    o.z *= f;
+    o.w *= f;
+    for (int i = 0; i < count; i += 8) {
+      float4 v[8];
+      float wi[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int from = i + k < count ? i + k : i;
+        wi[k] = __shfl_sync(0xffffffffu, w, from);
+        const float *q = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, reinterpret_cast<long long>(src), from));
+        if (i + k >= count) wi[k] = 0.f;
+        v[k] = wi[k] != 0.f ? __ldcg(reinterpret_cast<const float4 *>(q + lane * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {                   // an empty partial's O was never written
+        o.x = fmaf(wi[k], v[k].x, o.x);
+        o.y = fmaf(wi[k], v[k].y, o.y);
+        o.z = fmaf(wi[k], v[k].z, o.z);
+        o.w = fmaf(wi[k], v[k].w, o.w);
+      }
     }
   }
   const float inv = l != 0.f ? 1.f / l : 0.f;
@@ -72,9 +112,8 @@ __global__ void __launch_bounds__(kWarps * 32) shared_merge_kernel(const MergePa
 cudaError_t launch_shared_merge(const MergeParams &p, cudaStream_t stream) {
   const long long rows = (long long)p.s.prefixes * p.s.questions * p.s.tokens * p.s.q_heads;
   const unsigned grid = (unsigned)((rows + kWarps - 1) / kWarps);
-  if (p.s.dtype == 1) shared_merge_kernel<__nv_bfloat16><<<grid, kWarps * 32, 0, stream>>>(p);
-  else shared_merge_kernel<__half><<<grid, kWarps * 32, 0, stream>>>(p);
-  return cudaGetLastError();
+  return p.s.dtype == 1 ? launch_overlapping(shared_merge_kernel<__nv_bfloat16>, dim3(grid), dim3(kWarps * 32), 0, stream, p)
+                        : launch_overlapping(shared_merge_kernel<__half>, dim3(grid), dim3(kWarps * 32), 0, stream, p);
 }
 
 }  // namespace rtk

@@ -165,6 +165,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   float *dm_s = reinterpret_cast<float *>(smem + L::kDm);
   float2 *ml_s = reinterpret_cast<float2 *>(smem + L::kMl);
 
+  launch_dependents();
   const PrefixSplit &sp = p.split;
   const SharedParams &a = p.s;
   const int cta = blockIdx.x;
@@ -556,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <typename T, int DK>
 cudaError_t launch(const PrefixMaps &maps, const PrefixParams &p, cudaStream_t stream) {
   const int smem = PrefixSmem<DK>::kBytes + 1024;
-  cudaError_t e = cudaFuncSetAttribute(shared_prefix_kernel<T, DK>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = allow_shared_memory<shared_prefix_kernel<T, DK>>(smem);
   if (e != cudaSuccess) return e;
   shared_prefix_kernel<T, DK><<<p.split.grid, kThreads, smem, stream>>>(maps, p);
   return cudaGetLastError();

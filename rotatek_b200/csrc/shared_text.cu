@@ -22,6 +22,10 @@
 // so weights stay within f16 whatever the scales are.
 //
 // Tokens past the length are zero-filled on the way in (cp.async reads nothing there).
+//
+// The kernel may run beside the prefix kernel launched before it (it needs nothing of it);
+// every CTA waits for that one before it ends, so that the join, which waits for this
+// kernel, finds both done.
 #include <type_traits>
 
 #include "common.cuh"
@@ -75,6 +79,7 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
   using L = TextSmem<FP8, kRT>;
   using M = typename std::conditional<FP8, __half, T>::type;   // MMA operand type
   extern __shared__ __align__(128) unsigned char smem[];
+  launch_dependents();
   const SharedParams &a = p.s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, j4 = lane & 3;
@@ -82,7 +87,10 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
   const int b = bh / a.kv_heads, h = bh % a.kv_heads;
   const int len = min(max(a.lens[b * a.lens_s], 0), a.cap);
   const int t0 = chunk * kTextChunk;
-  if (t0 >= len) return;
+  if (t0 >= len) {
+    wait_for_previous();
+    return;
+  }
   const int t1 = min(len, t0 + kTextChunk);
   const int blocks = (t1 - t0 + L::kTok - 1) / L::kTok;
 
@@ -417,6 +425,7 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
     *reinterpret_cast<float4 *>(p.acc + (slot + r) * 128 + lane * 4) = o;
     if (lane == 0) reinterpret_cast<float2 *>(p.ml)[slot + r] = make_float2(mm, ll);
   }
+  wait_for_previous();
 }
 
 // ---- many rows (T G > 16): the warps of a CTA split the rows, 16 each, and share the
@@ -440,6 +449,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
   using L = RowsSmem<FP8>;
   using M = typename std::conditional<FP8, __half, T>::type;     // MMA operand type
   extern __shared__ __align__(128) unsigned char smem[];
+  launch_dependents();
   const SharedParams &a = p.s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, j4 = lane & 3;
@@ -447,7 +457,10 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
   const int b = bh / a.kv_heads, h = bh % a.kv_heads;
   const int len = min(max(a.lens[b * a.lens_s], 0), a.cap);
   const int t0 = chunk * kTextChunk;
-  if (t0 >= len) return;
+  if (t0 >= len) {
+    wait_for_previous();
+    return;
+  }
   const int t1 = min(len, t0 + kTextChunk);
   const int tiles = (t1 - t0 + L::kTok - 1) / L::kTok;
   constexpr int kEsize = FP8 ? 1 : 2, kRowBytes = 128 * kEsize, kChunks = kRowBytes / 16;
@@ -687,14 +700,16 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
       if (j4 == 0) reinterpret_cast<float2 *>(p.ml)[slot + r] = make_float2(m[i], ll);
     }
   }
+  wait_for_previous();
 }
 
 template <typename T, bool FP8>
 cudaError_t launch_rows(const TextParams &p, cudaStream_t stream) {
   const int smem = RowsSmem<FP8>::kBytes;
-  cudaError_t e = cudaFuncSetAttribute(shared_text_rows_kernel<T, FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = allow_shared_memory<shared_text_rows_kernel<T, FP8>>(smem);
   if (e != cudaSuccess) return e;
   const dim3 grid(p.s.prefixes * p.s.questions * p.s.kv_heads, p.chunks, (p.rows + 63) / 64);
+  if (p.beside) return launch_overlapping(shared_text_rows_kernel<T, FP8>, grid, dim3(kWarps * 32), smem, stream, p);
   shared_text_rows_kernel<T, FP8><<<grid, kWarps * 32, smem, stream>>>(p);
   return cudaGetLastError();
 }
@@ -702,9 +717,10 @@ cudaError_t launch_rows(const TextParams &p, cudaStream_t stream) {
 template <typename T, bool FP8, int kRT>
 cudaError_t launch(const TextParams &p, cudaStream_t stream) {
   const int smem = TextSmem<FP8, kRT>::kBytes;
-  cudaError_t e = cudaFuncSetAttribute(shared_text_kernel<T, FP8, kRT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = allow_shared_memory<shared_text_kernel<T, FP8, kRT>>(smem);
   if (e != cudaSuccess) return e;
   const dim3 grid(p.s.prefixes * p.s.questions * p.s.kv_heads, p.chunks, (p.rows + 16 * kRT - 1) / (16 * kRT));
+  if (p.beside) return launch_overlapping(shared_text_kernel<T, FP8, kRT>, grid, dim3(kWarps * 32), smem, stream, p);
   shared_text_kernel<T, FP8, kRT><<<grid, kWarps * 32, smem, stream>>>(p);
   return cudaGetLastError();
 }

@@ -138,7 +138,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) verify_stats_kernel(const VerifyParams p) {
   __shared__ float m_s[kThreads / 32], z_s[kThreads / 32];
   __shared__ int i_s[kThreads / 32];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  launch_dependents();
   const VerifyLayout l = verify_layout(p.batch, p.drafts, p.vocab);
   const VerifySpace ws = verify_space(p.workspace, p.batch);
   const int r = blockIdx.y, b = blockIdx.z, chunk = blockIdx.x;
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(kThreads) verify_pick_kernel(const VerifyParam
     }
   }
   if (threadIdx.x == 0) k_s = n;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_previous();
 
   // join the chunks of every row a decision may read: a warp per row
   for (int r = warp; r < l.rows; r += kThreads / 32) {
@@ -387,16 +387,7 @@ cudaError_t verify(const VerifyParams &p, cudaStream_t stream) {
   verify_stats_kernel<T><<<dim3(l.chunks, rows, p.batch), kThreads, 0, stream>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(l.races, p.batch);
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, verify_pick_kernel<T>, p);
+  return launch_overlapping(verify_pick_kernel<T>, dim3(l.races, p.batch), dim3(kThreads), 0, stream, p);
 }
 
 }  // namespace

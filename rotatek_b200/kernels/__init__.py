@@ -347,26 +347,45 @@ def rotatek_shared_decode(
         raise ValueError("R_partial must be [P, H_kv, D, D_keep]")
     if k_scale is not None:
         k_text, v_text = _as_u8(k_text), _as_u8(v_text)
-    dev = _lib.require_one_device(q, R_partial, delta_mu, k_full, v_full, mask_full, k_sparse, v_sparse, k_text,
-                                  v_text, text_lens, k_scale, v_scale, out)
-    lib = _lib.load()
+    dev = q.device
+    if not q.is_cuda:
+        _lib.require_one_device(q)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return rotatek_shared_decode(q, R_partial, delta_mu, k_full, v_full, mask_full, k_sparse, v_sparse, k_text,
+                                         v_text, text_lens, num_kv_groups, k_scale=k_scale, v_scale=v_scale, out=out)
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    b, t, heads, _ = q.shape
-    key = ("sh", R_partial.shape[0], b, t, heads, R_partial.shape[1], k_full.shape[-2], k_sparse.shape[-2],
-           k_text.shape[-2], dev.index)
-    need = _ws_size_cache.get(key)
-    if need is None:
-        need = _ws_size_cache[key] = lib.rtk_shared_decode_workspace_size(*key[1:])
-    # scratch of this call alone, from the stream's own pool: calls on several
-    # streams do not share it
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    D = _lib.describe
-    _lib.check(lib.rtk_shared_decode(
-        D(q), D(R_partial), D(delta_mu), D(k_full), D(v_full), D(mask_full), D(k_sparse), D(v_sparse), D(k_text),
-        D(v_text), D(k_scale), D(v_scale), D(text_lens), num_kv_groups, D(out), ws.data_ptr(), need,
-        _lib.status_word(dev), _stream(dev)))
+    calls = _lib.calls()
+    stream = _lib.raw_stream(dev)
+    need = 0
+    while True:
+        ws = _lib.scratch(dev, stream, need)
+        code = calls.shared_decode(q, R_partial, delta_mu, k_full, v_full, mask_full, k_sparse, v_sparse, k_text, v_text,
+                                   k_scale, v_scale, text_lens, out, num_kv_groups, ws.data_ptr(), ws.numel(),
+                                   _lib.status_word(dev), stream)
+        if code != _lib.RTK_ERR_WORKSPACE or need:
+            break
+        # the arguments are good, the stream's scratch is too small: nothing was launched
+        need = _lib.load().rtk_shared_decode_workspace_size(
+            R_partial.shape[0], *q.shape[:3], R_partial.shape[1], k_full.shape[2], k_sparse.shape[2], k_text.shape[2],
+            dev.index)
+    if code:
+        _raise(code, q, R_partial, delta_mu, k_full, v_full, mask_full, k_sparse, v_sparse, k_text, v_text, k_scale,
+               v_scale, text_lens, out)
     return out
+
+
+def _elsewhere(dev: torch.device) -> bool:
+    """Whether another device than `dev` is current: kernels are launched on the current one."""
+    return torch._C._cuda_getDevice() != dev.index
+
+
+def _raise(code: int, *tensors) -> None:
+    """The error behind a direct call's nonzero code."""
+    if code < 0:
+        _lib.require_one_device(*tensors)
+    _lib.check(code)
 
 
 def append_text(
@@ -394,10 +413,15 @@ def append_text(
         raise ValueError("k_new must be [B, H_kv, T, D]")
     if k_scale is not None:
         k_text, v_text = _as_u8(k_text), _as_u8(v_text)
-    dev = _lib.require_one_device(k_new, v_new, text_lens, k_text, v_text, k_scale, v_scale, counts)
-    D = _lib.describe
-    _lib.check(_lib.load().rtk_append_text(D(k_new), D(v_new), D(text_lens), D(counts), D(k_text), D(v_text),
-                                           D(k_scale), D(v_scale), _stream(dev)))
+    if not k_new.is_cuda:
+        _lib.require_one_device(k_new)
+    if _elsewhere(k_new.device):
+        with torch.cuda.device(k_new.device):
+            return append_text(k_new, v_new, text_lens, k_text, v_text, k_scale=k_scale, v_scale=v_scale, counts=counts)
+    code = _lib.calls().append_text(k_new, v_new, text_lens, counts, k_text, v_text, k_scale, v_scale,
+                                    _lib.raw_stream(k_new.device))
+    if code:
+        _raise(code, k_new, v_new, text_lens, counts, k_text, v_text, k_scale, v_scale)
 
 
 def read_text(
@@ -415,12 +439,17 @@ def read_text(
     if k_text.dim() != 4:
         raise ValueError("k_text must be a uint8 (e4m3) [B, H_kv, C, D]")
     k_text, v_text = _as_u8(k_text), _as_u8(v_text)
-    dev = _lib.require_one_device(k_text, v_text, text_lens, k_scale, v_scale)
+    if not k_text.is_cuda:
+        _lib.require_one_device(k_text)
+    dev = k_text.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return read_text(k_text, v_text, text_lens, k_scale=k_scale, v_scale=v_scale, dtype=dtype)
     k = torch.empty(k_text.shape, dtype=dtype, device=dev)
     v = torch.empty(k_text.shape, dtype=dtype, device=dev)
-    D = _lib.describe
-    _lib.check(_lib.load().rtk_read_text(D(k_text), D(v_text), D(k_scale), D(v_scale), D(text_lens), D(k), D(v),
-                                         _stream(dev)))
+    code = _lib.calls().read_text(k_text, v_text, k_scale, v_scale, text_lens, k, v, _lib.raw_stream(dev))
+    if code:
+        _raise(code, k_text, v_text, k_scale, v_scale, text_lens, k, v)
     return k, v
 
 
@@ -450,20 +479,28 @@ def verify_drafts(
     fp32, bf16 or fp16 logits; no host synchronisation."""
     if target_logits.dim() != 3:
         raise ValueError("target_logits must be [B, T + 1, V]")
-    dev = _lib.require_one_device(target_logits, draft_tokens, draft_logits, uniforms, noise, temperature, draft_lens)
+    if not target_logits.is_cuda:
+        _lib.require_one_device(target_logits)
+    dev = target_logits.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return verify_drafts(target_logits, draft_tokens, draft_logits, uniforms, noise, temperature,
+                                 draft_lens=draft_lens)
     b, rows, vocab = target_logits.shape
-    lib = _lib.load()
-    tokens = torch.empty(b, rows, dtype=torch.int64, device=dev)
+    calls = _lib.calls()
+    tokens = torch.empty((b, rows), dtype=torch.int64, device=dev)
     accepted = torch.empty(b, dtype=torch.int32, device=dev)
-    key = ("vd", b, rows - 1, vocab)
-    need = _ws_size_cache.get(key)
-    if need is None:
-        need = _ws_size_cache[key] = lib.rtk_verify_drafts_workspace_size(*key[1:])
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    D = _lib.describe
-    _lib.check(lib.rtk_verify_drafts(D(target_logits), D(draft_tokens), D(draft_logits), D(uniforms), D(noise),
-                                     D(temperature), D(draft_lens), D(tokens), D(accepted), ws.data_ptr(), need,
-                                     _stream(dev)))
+    stream = _lib.raw_stream(dev)
+    need = 0
+    while True:
+        ws = _lib.scratch(dev, stream, need)
+        code = calls.verify_drafts(target_logits, draft_tokens, draft_logits, uniforms, noise, temperature, draft_lens,
+                                   tokens, accepted, ws.data_ptr(), ws.numel(), stream)
+        if code != _lib.RTK_ERR_WORKSPACE or need:
+            break
+        need = _lib.load().rtk_verify_drafts_workspace_size(b, rows - 1, vocab)   # nothing was launched
+    if code:
+        _raise(code, target_logits, draft_tokens, draft_logits, uniforms, noise, temperature, draft_lens)
     return tokens, accepted
 
 
