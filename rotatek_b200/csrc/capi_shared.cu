@@ -114,7 +114,8 @@ size_t rtk_shared_decode_workspace_size(int64_t prefixes, int64_t batch, int64_t
   if (prefixes < 1 || kv_heads < 1 || batch < 0 || tokens < 0) return 0;
   const int64_t groups = q_heads / kv_heads;
   const rtk::PrefixSplit sp =
-      rtk::prefix_split(prefixes, batch / prefixes, tokens, groups, kv_heads, seq_full, seq_sparse, rtk::device_sms(device));
+      rtk::prefix_split(prefixes, batch / prefixes, tokens, groups, kv_heads, seq_full, seq_sparse, text_cap,
+                        rtk::device_sms(device));
   return shared_space(sp, batch, kv_heads, tokens * groups, text_chunks(text_cap)).bytes;
 }
 
@@ -209,7 +210,7 @@ int rtk_shared_decode(const rtk_tensor *q, const rtk_tensor *R_partial, const rt
   }
   const int device = current_device();
   const rtk::PrefixSplit sp =
-      rtk::prefix_split(P, B / P, T, num_kv_groups, Hkv, Sf, Sv, rtk::device_sms(device));
+      rtk::prefix_split(P, B / P, T, num_kv_groups, Hkv, Sf, Sv, C, rtk::device_sms(device));
   const int64_t rows = T * num_kv_groups, chunks = text_chunks(C);
   if ((int64_t)sp.rows != B / P * rows || (int64_t)P * Hkv * sp.row_tiles > kMaxInt / 256 || chunks > 65535 ||
       rows > 65535 * 16 || B * Hkv > kMaxInt)
@@ -236,7 +237,10 @@ int rtk_shared_decode(const rtk_tensor *q, const rtk_tensor *R_partial, const rt
     rtk::PrefixParams pp;
     pp.s = p;
     pp.split = sp;
-    pp.R_rows = rows16(R_partial, 2);
+    rtk_tensor Rt = *R_partial;                      // its columns as rows
+    std::swap(Rt.shape[2], Rt.shape[3]);
+    std::swap(Rt.stride[2], Rt.stride[3]);
+    pp.R_layout = rows16(R_partial, 2) ? 1 : rows16(&Rt, 2) ? 2 : 0;
     pp.ml = pml; pp.acc = pacc;
     pp.status = static_cast<unsigned int *>(status != nullptr ? status : workspace);
     e = rtk::launch_shared_prefix(maps, pp, st);

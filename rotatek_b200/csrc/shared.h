@@ -101,7 +101,7 @@ struct PrefixSplit {
 };
 
 inline PrefixSplit prefix_split(long long prefixes, long long questions, long long tokens, long long groups,
-                                long long kv_heads, long long seq_full, long long seq_sparse, int sms) {
+                                long long kv_heads, long long seq_full, long long seq_sparse, long long text_cap, int sms) {
   PrefixSplit s;
   s.rows = (int)(questions * tokens * groups);
   s.row_tiles = (s.rows + 127) / 128;
@@ -110,6 +110,9 @@ inline PrefixSplit prefix_split(long long prefixes, long long questions, long lo
   s.blocks_vis = (int)((seq_sparse + 127) / 128);
   s.unit_weight = PrefixSplit::kUnitStart + s.blocks_full + 2 * s.blocks_vis;
   s.total = (long long)s.units * s.unit_weight;
+  // Ranges of a few blocks: a quarter of the SMs is left to the text kernel, which then runs
+  // beside this one instead of after it (a block costs 0.75 us, the text of a step 5 to 8).
+  if (text_cap > 0 && s.total < 16ll * sms) sms = sms - sms / 4;
   s.grid = (int)(s.total / 2 < sms ? (s.total / 2 > 0 ? s.total / 2 : 1) : sms);
   return s;
 }
@@ -121,8 +124,8 @@ struct PrefixMaps {
 struct PrefixParams {
   SharedParams s;
   PrefixSplit split;
-  int R_rows;                   // R's rows can be read 16 bytes at a time
-  float *ml, *acc;              // per slot: [128][2] and [128][128]
+  int R_layout;                 // R can be read 16 bytes at a time: 1 along its rows, 2 along its columns, 0 not
+  float *ml, *acc;              // per slot: [128 rows][2] and [32 groups of 4 channels][128 rows][4]
   unsigned int *status;
 };
 cudaError_t launch_shared_prefix(const PrefixMaps &maps, const PrefixParams &p, cudaStream_t stream);
@@ -133,7 +136,7 @@ struct TextParams {
   SharedParams s;
   int rows, chunks;             // T G query rows, ceil(cap / kTextChunk)
   int beside;                   // launched right after the prefix kernel, to run beside it
-  float *ml, *acc;              // per (question, KV head, chunk): [rows][2] and [rows][128]
+  float *ml, *acc;              // per (question, KV head, chunk): [rows][2] and [32 groups of 4 channels][rows][4]
 };
 cudaError_t launch_shared_text(const TextParams &p, cudaStream_t stream);
 

@@ -17,19 +17,22 @@
 // m follows the running maximum lazily: O and l are rescaled only when a maximum
 // grows by more than 2^8 over the one in use (P stays below 2^8, O and l are fp32).
 //
-// CTA (one per SM, 12 warps):
-//   warp 0      TMA producer: a ring of stages, one block's K and V each
-//   warps 1, 2  issue the MMAs of the even and the odd sub-blocks (one elected lane each:
-//               a single thread's instructions could not keep the tensor core fed); warp 1
-//               owns the TMEM
-//   warps 4-7   softmax of the even sub-blocks: thread = query row (TMEM lane)
-//   warps 8-11  softmax of the odd sub-blocks
-// A sub-block is 64 tokens: a prompt block, or half a visual block.  Even and odd
-// sub-blocks are two independent streams with their own (m, l) and O accumulator in
-// TMEM (2 x 128 columns), and two S buffers each (2 x 2 x 64 columns: all 512): while
-// a warp group works on one, the tensor core turns the other into the next S.  P goes
-// over S in TMEM as the A operand of P . V.  At the end of a unit the streams are
-// joined and the partial result of (unit, CTA) is written for shared_merge.cu.
+// CTA (one per SM, 11 warps):
+//   warps 0-3   softmax of the even blocks: thread = query row (TMEM lane)
+//   warps 4-7   softmax of the odd blocks
+//   warp 8      TMA producer: a ring of stages, one block's K and V each
+//   warp 9      issues the MMAs of S (one elected lane); owns the TMEM
+//   warp 10     issues those of O: a single thread's instructions could not keep the
+//               tensor core fed
+// TMEM (all 512 columns): three S buffers of 128, O of 128.  The S of the next blocks is made
+// while two blocks are in the softmax; P goes over the upper half of its S as the A
+// operand of P . V.  The two softmax groups settle m in the order of the blocks, through
+// shared memory; only where m moves does the group wait for the P . V before and rescale O.
+// At the end of a unit the partial result of (unit, CTA) is written for shared_merge.cu.
+//
+// What bounds it: with many rows the exponential unit, 128 x 128 a block at 16 a cycle,
+// and what a warp does between two blocks' exponentials (waiting for S, reading it,
+// its maximum, handing P over); with few rows, HBM.
 #include <type_traits>
 
 #include "shared.h"
@@ -38,12 +41,13 @@
 namespace rtk {
 namespace {
 
-constexpr int kThreads = 384;
+constexpr int kThreads = 352;
 constexpr int kFullTok = 64, kVisTok = 128;      // tokens of a block
-constexpr int kSub = 64;                         // tokens of a sub-block
-constexpr uint32_t kColsS = 64;                  // TMEM columns of an S buffer
-constexpr uint32_t kColO = 4 * kColsS;           // first column of the O accumulators
+constexpr uint32_t kColsS = 128;                 // TMEM columns of an S buffer
+constexpr uint32_t kColP = 64;                   // P within it
+constexpr uint32_t kColO = 3 * kColsS;           // the O accumulator
 constexpr float kLazy = 8.f;
+constexpr int kPolyOf = 4;                       // one pair of exponentials in this many goes to the FMA units
 
 template <int DK>
 struct PrefixSmem {
@@ -57,10 +61,11 @@ struct PrefixSmem {
   static constexpr int kRing = kRot + kRotBytes;
   static constexpr int kBias = kRing + kStages * kStage;           // float[128]
   static constexpr int kDm = kBias + 512;                          // float[128]
-  static constexpr int kMl = kDm + 512;                            // float2[2][128]
+  static constexpr int kRef = kDm + 512;                           // float[128]: m
+  static constexpr int kMl = kRef + 512;                           // float2[2][128]: a group's m, l
   static constexpr int kBar = kMl + 2048;
-  // full[S], empty[S], s_ready[4], p_ready[4], pv[2], rot, o_done
-  static constexpr int kNumBars = 2 * kStages + 12;
+  // full[S], empty[S], s_ready[3], p_ready[3], pv_done[3], rot, o_done
+  static constexpr int kNumBars = 2 * kStages + 11;
   static constexpr int kTmemSlot = kBar + kNumBars * 8;
   static constexpr int kAbort = kTmemSlot + 4;
   static constexpr int kBytes = kAbort + 4;
@@ -73,10 +78,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-struct RowStat {
-  float m, l;
-};
-
 // O of this warp's rows times each row's f.
 __device__ __forceinline__ void rescale_o(uint32_t o, float f) {
 #pragma unroll 1
@@ -88,44 +89,72 @@ __device__ __forceinline__ void rescale_o(uint32_t o, float f) {
     for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
     tmem_st16_nowait(o + c, r);
   }
+  tmem_wait_st();
 }
 
-// One sub-block for this thread's row: S in TMEM columns [s, s + 64), P written to
-// [s, s + 32), m and l brought along; rescale(f) multiplies O by each row's f when the
-// reference of any row of the warp moves; before() comes before the exponentials.  v0, v1 (a bit per token) mark the tokens that
-// count; `all` = every one does.
-template <typename T, typename Rescale, typename Before>
-__device__ __forceinline__ void softmax_sub(uint32_t s, float scale, float bias, bool all, uint32_t v0, uint32_t v1,
-                                            RowStat &st, Rescale rescale, Before before) {
-  uint32_t r[2][32];
+// 2^x of two numbers without the exponential unit, for x in [-inf, 126]: x = n + f with n the
+// nearest integer (added in, and left in, the low bits of 1.5 * 2^23) and f in
+// [-1/2, 1/2], 2^f by a polynomial whose coefficients minimise the largest relative
+// error there (Remez; degree 3: 7.5e-5, degree 4: 2.6e-6 -- against 2^-9 and 2^-12 that
+// rounding to 16 bits costs), n added to its exponent.  Below 2^-126: 2^-126.
+template <typename T>
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  constexpr float kMagic = 12582912.f;
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
+  const float2 t = __fadd2_rn(x, make_float2(kMagic, kMagic));
+  const float2 n = __fadd2_rn(t, make_float2(-kMagic, -kMagic));
+  const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+  float2 y;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    y = __ffma2_rn(f, make_float2(0x1.c3f76p-5f, 0x1.c3f76p-5f), make_float2(0x1.f0de1cp-3f, 0x1.f0de1cp-3f));
+    y = __ffma2_rn(f, y, make_float2(0x1.62f31ap-1f, 0x1.62f31ap-1f));
+    y = __ffma2_rn(f, y, make_float2(0x1.fff692p-1f, 0x1.fff692p-1f));
+  } else {
+    y = __ffma2_rn(f, make_float2(0x1.3997d4p-7f, 0x1.3997d4p-7f), make_float2(0x1.ca1442p-5f, 0x1.ca1442p-5f));
+    y = __ffma2_rn(f, y, make_float2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+    y = __ffma2_rn(f, y, make_float2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+    y = __ffma2_rn(f, y, make_float2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+  }
+  return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
+}
+
+// Columns [s, s + 64) of S whose token does not count become -inf, whatever was there.
+__device__ __forceinline__ void mask_s(uint32_t s, uint32_t v0, uint32_t v1) {
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    const uint32_t v = (c < 2 ? v0 : v1) >> (16 * (c & 1));
+    uint32_t r[16];
+    tmem_ld16_nowait(s + 16 * c, r);
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (!((v >> i) & 1u)) r[i] = 0xff800000u;
+    tmem_st16_nowait(s + 16 * c, r);
+  }
+  tmem_wait_st();
+}
+
+__device__ __forceinline__ void load_half(uint32_t s, uint32_t (&r)[2][32]) {
   tmem_ld32_nowait(s, r[0]);
   tmem_ld32_nowait(s + 32, r[1]);
   tmem_wait_ld();
-  if (!all) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {                   // -inf, whatever was there
-      if (!((v0 >> i) & 1u)) r[0][i] = 0xff800000u;
-      if (!((v1 >> i) & 1u)) r[1][i] = 0xff800000u;
-    }
-  }
+}
+
+__device__ __forceinline__ float max_half(const uint32_t (&r)[2][32]) {
   float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int c = 0; c < 2; ++c)
 #pragma unroll
     for (int i = 0; i < 32; i += 2)
       mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1]));
-  // scale > 0; -inf stays -inf
-  const float top = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), scale, bias);
-  const bool grow = top > st.m + kLazy;              // from -inf: whenever there is a maximum
-  if (__any_sync(0xffffffffu, grow)) {
-    const float m2 = grow ? top : st.m;
-    const float f = grow ? fast_exp2(st.m - m2) : 1.f;      // first maximum: 2^-inf = 0
-    st.m = m2;
-    st.l *= f;
-    rescale(f);
-  }
-  before();
-  const float off = bias - (st.m > -INFINITY ? st.m : 0.f);
+  return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+}
+
+// Weights of 64 columns: 32 columns of P (16-bit pairs) at `p`; returns their sum.
+template <typename T>
+__device__ __forceinline__ float weights_half(uint32_t p, const uint32_t (&r)[2][32], float scale, float off) {
   const float2 scale2 = make_float2(scale, scale), off2 = make_float2(off, off);
   float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -134,15 +163,18 @@ __device__ __forceinline__ void softmax_sub(uint32_t s, float scale, float bias,
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1])), scale2, off2);
-      x.x = fast_exp2(x.x);
-      x.y = fast_exp2(x.y);
+      if (i % kPolyOf == kPolyOf - 1) {
+        x = exp2_poly<T>(x);
+      } else {
+        x.x = fast_exp2(x.x);
+        x.y = fast_exp2(x.y);
+      }
       l2[i & 1] = __fadd2_rn(l2[i & 1], x);
       w[i] = pack2<T>(x.x, x.y);
     }
-    tmem_st16_nowait(s + 16 * c, w);
+    tmem_st16_nowait(p + 16 * c, w);
   }
-  st.l += (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
-  tmem_wait_st();
+  return (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
 }
 
 template <typename T, int DK>
@@ -154,15 +186,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t *full_bar = reinterpret_cast<uint64_t *>(smem + L::kBar);
   uint64_t *empty_bar = full_bar + L::kStages;
-  uint64_t *s_bar = empty_bar + L::kStages;       // [stream + 2 buffer] S is in TMEM
-  uint64_t *p_bar = s_bar + 4;                    // [stream + 2 buffer] P is in TMEM
-  uint64_t *pv_bar = p_bar + 4;                   // [stream] the P . V before the stream's last is done
-  uint64_t *rot_bar = pv_bar + 2;                 // rotated queries are in TMEM
-  uint64_t *o_bar = rot_bar + 1;                  // both O accumulators are complete
+  uint64_t *s_bar = empty_bar + L::kStages;       // [buffer] S is in TMEM
+  uint64_t *p_bar = s_bar + 3;                    // [buffer] P is in TMEM
+  uint64_t *pv_bar = p_bar + 3;                   // [buffer] its P . V is done
+  uint64_t *rot_bar = pv_bar + 3;                 // rotated queries are in TMEM
+  uint64_t *o_bar = rot_bar + 1;                  // the O accumulator is complete
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::kTmemSlot);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::kAbort);
   float *bias_s = reinterpret_cast<float *>(smem + L::kBias);
   float *dm_s = reinterpret_cast<float *>(smem + L::kDm);
+  float *ref_s = reinterpret_cast<float *>(smem + L::kRef);
   float2 *ml_s = reinterpret_cast<float2 *>(smem + L::kMl);
 
   launch_dependents();
@@ -177,25 +210,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kStages; ++i) {
       mbar_init(&full_bar[i], 1);
-      mbar_init(&empty_bar[i], 2);
+      mbar_init(&empty_bar[i], 1);
     }
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 3; ++i) {
       mbar_init(&s_bar[i], 1);
       mbar_init(&p_bar[i], 4);
+      mbar_init(&pv_bar[i], 1);
     }
-    for (int i = 0; i < 2; ++i) mbar_init(&pv_bar[i], 1);
     mbar_init(rot_bar, 1);
-    mbar_init(o_bar, 2);
+    mbar_init(o_bar, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 1) tmem_alloc(tmem_slot, 512);
+  if (warp == 9) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 0) {
+  if (warp == 8) {
     // ---------------------------------------------------------------- producer
     if (lane == 0) {
       int it = 0;
@@ -233,20 +266,32 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_wait_bounded(&full_bar[k % L::kStages], (k / L::kStages) & 1, &dead, p.status);
       }
     }
-  } else if (warp <= 2) {
-    // ---------------------------------------------------------------- MMA issuers, one per stream
-    const uint32_t x = warp - 1;
+  } else if (warp >= 9) {
+    // ---------------------------------------------------------------- MMA issuers
+    const bool for_s = warp == 9;
     constexpr uint32_t kFmt = kBf16 ? 1u : 0u;
     constexpr uint32_t kIdRot = idesc_f16(kFmt, 0, 0, 128, DK);
-    constexpr uint32_t kIdQk = idesc_f16(kFmt, 0, 0, 128, kSub);
+    constexpr uint32_t kIdFull = idesc_f16(kFmt, 0, 0, 128, kFullTok);
+    constexpr uint32_t kIdVis = idesc_f16(kFmt, 0, 0, 128, kVisTok);
     constexpr uint32_t kIdPv = idesc_f16(kFmt, 0, 1, 128, 128);
     constexpr uint32_t kStep = L::kStage >> 4;       // from stage to stage, in a descriptor
     const uint32_t rot_addr = smem_u32(smem + L::kRot), ring = smem_u32(smem + L::kRing);
     const uint64_t q_desc = smem_desc_kmajor<128>(smem_u32(smem + L::kQ)), rot_desc = smem_desc_kmajor<128>(rot_addr);
     const uint64_t k_prompt = smem_desc_kmajor<128>(ring), v_prompt = smem_desc_sw128(ring + 16384, 8192, 1024);
-    const uint32_t d_o = tmem + kColO + x * 128;
-    int it = 0;                              // blocks of the segments before
-    uint32_t np = 0;                         // parity of the next P of each buffer
+    const uint64_t k_vis = smem_desc_kmajor<DK * 2>(ring), v_vis = smem_desc_sw128(ring + L::kKeyBytes, 16384, 1024);
+    // stage and S buffer of the next block, and the parities of their rounds.  Issuing is
+    // what the tensor core waits for, so they are carried along, not computed.
+    uint32_t stage = 0, stage_par = 0, buf = 0, buf_par = 0;
+    auto next = [&] {
+      if (++stage == (uint32_t)L::kStages) {
+        stage = 0;
+        stage_par ^= 1u;
+      }
+      if (++buf == 3u) {
+        buf = 0;
+        buf_par ^= 1u;
+      }
+    };
     for (int u = u0; u <= u1; ++u) {
       const long long w = (long long)u * sp.unit_weight;
       const int j0 = r0 > w ? sp.block_from((int)(r0 - w)) : 0;
@@ -254,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (j0 >= j1) continue;
       named_barrier_sync(1, 320);            // Q and R^T are in shared memory
       if (j1 > sp.blocks_full) {
-        if (x == 0 && elect_one()) {
+        if (for_s && elect_one()) {
           tc_fence_after();
 #pragma unroll
           for (int k = 0; k < 8; ++k)
@@ -267,80 +312,67 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (elect_one()) {
         tc_fence_after();
-        // Sub-block i of the segment: prompt blocks are one, visual blocks two; this
-        // stream takes every other one, i = x, x + 2, ...: whole prompt blocks, and always
-        // the same half of a visual block.  S runs two of them ahead of P . V: an S
-        // buffer is free once the P . V that reads it is issued (the tensor core works
-        // in order).  This thread's own instructions are what the tensor core waits for, so
-        // stages and parities are carried along instead of being computed.
-        const int nf = j0 < sp.blocks_full ? min(j1, sp.blocks_full) - j0 : 0;
-        const int subs = nf + 2 * (j1 - j0 - nf);
-        const uint32_t half = (x ^ (uint32_t)nf) & 1u;
-        const uint64_t k_vis = smem_desc_kmajor<DK * 2>(ring + half * (kSub * DK * 2));
-        const uint64_t v_vis = smem_desc_sw128(ring + L::kKeyBytes + half * 8192, 16384, 1024);
-        uint32_t q_stage = (it + (x == 1 && nf > 0)) % L::kStages;
-        uint32_t q_par = ((it + (x == 1 && nf > 0)) / L::kStages) & 1;
-        uint32_t p_stage = q_stage;
-        it += j1 - j0;
-        auto issue_qk = [&](int i, uint32_t buf) {
-          mbar_wait_bounded(&full_bar[q_stage], q_par, abort_flag, p.status);
-          tc_fence_after();
-          const uint32_t d = tmem + x * kColsS + buf * (2 * kColsS);
-          if (i >= nf) {
-            constexpr int kSteps = DK / 16;
-            const uint64_t kd = k_vis + q_stage * kStep;
+        if (for_s) {
+          for (int j = j0; j < j1; ++j) {
+            // the buffer's last P has been used (the first round finds its parity done)
+            mbar_wait_bounded(&pv_bar[buf], buf_par ^ 1u, abort_flag, p.status);
+            mbar_wait_bounded(&full_bar[stage], stage_par, abort_flag, p.status);
+            tc_fence_after();
+            const uint32_t d = tmem + buf * kColsS;
+            if (j >= sp.blocks_full) {
+              constexpr int kSteps = DK / 16;
+              const uint64_t kd = k_vis + stage * kStep;
 #pragma unroll
-            for (int k = 0; k < 2 * kSteps; ++k) {
-              const int col = 16 * k;        // of [Qhi | Qlo]
-              umma_f16_ss(d, rot_desc + (((col >> 6) * 16384 + (col & 63) * 2) >> 4), kd + (((k % kSteps) * 32) >> 4),
-                          kIdQk, k > 0);
+              for (int k = 0; k < 2 * kSteps; ++k) {
+                const int col = 16 * k;      // of [Qhi | Qlo]
+                umma_f16_ss(d, rot_desc + (((col >> 6) * 16384 + (col & 63) * 2) >> 4),
+                            kd + (((k % kSteps) * 32) >> 4), kIdVis, k > 0);
+              }
+            } else {
+              const uint64_t kd = k_prompt + stage * kStep;
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                umma_f16_ss(d, q_desc + (((k >> 2) * 16384 + (k & 3) * 32) >> 4),
+                            kd + (((k >> 2) * 8192 + (k & 3) * 32) >> 4), kIdFull, k > 0);
             }
-          } else {
-            const uint64_t kd = k_prompt + q_stage * kStep;
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              umma_f16_ss(d, q_desc + (((k >> 2) * 16384 + (k & 3) * 32) >> 4),
-                          kd + (((k >> 2) * 8192 + (k & 3) * 32) >> 4), kIdQk, k > 0);
+            umma_commit(&s_bar[buf]);
+            next();
           }
-          umma_commit(&s_bar[x + 2 * buf]);
-          q_stage += i + 2 <= nf ? 2 : 1;
-          if (q_stage >= (uint32_t)L::kStages) {
-            q_stage -= L::kStages;
-            q_par ^= 1u;
-          }
-        };
-        int i = x;
-        if (i < subs) issue_qk(i, 0);
-        if (i + 2 < subs) issue_qk(i + 2, 1);
-        for (uint32_t buf = 0; i < subs; i += 2, buf ^= 1u) {
-          mbar_wait_bounded(&p_bar[x + 2 * buf], (np >> buf) & 1u, abort_flag, p.status);
-          np ^= 1u << buf;
-          tc_fence_after();
-          const uint32_t pa = tmem + x * kColsS + buf * (2 * kColsS);
-          const uint64_t vd = (i >= nf ? v_vis : v_prompt) + p_stage * kStep;
+        } else {
+          for (int j = j0; j < j1; ++j) {
+            mbar_wait_bounded(&full_bar[stage], stage_par, abort_flag, p.status);
+            mbar_wait_bounded(&p_bar[buf], buf_par, abort_flag, p.status);
+            tc_fence_after();
+            const uint32_t pa = tmem + buf * kColsS + kColP, first = j > j0;
+            if (j >= sp.blocks_full) {
+              const uint64_t vd = v_vis + stage * kStep;
 #pragma unroll
-          for (int k = 0; k < kSub / 16; ++k)
-            umma_f16_ts(d_o, pa + 8 * k, vd + ((k * 2048) >> 4), kIdPv, k > 0 || i > 1);
-          umma_commit(&empty_bar[p_stage]);            // two arrivals free a stage: one of each stream, or
-          if (i < nf) umma_commit(&empty_bar[p_stage]);    // both of the one that has the prompt block
-          p_stage += i + 2 <= nf ? 2 : 1;
-          if (p_stage >= (uint32_t)L::kStages) p_stage -= L::kStages;
-          if (i + 4 < subs) issue_qk(i + 4, buf);
-          else if (i + 2 < subs) umma_commit(&pv_bar[x]);  // the P . V before the stream's last
+              for (int k = 0; k < kVisTok / 16; ++k)
+                umma_f16_ts(tmem + kColO, pa + 8 * k, vd + ((k * 2048) >> 4), kIdPv, k > 0 ? 1u : first);
+            } else {
+              const uint64_t vd = v_prompt + stage * kStep;
+#pragma unroll
+              for (int k = 0; k < kFullTok / 16; ++k)
+                umma_f16_ts(tmem + kColO, pa + 8 * k, vd + ((k * 2048) >> 4), kIdPv, k > 0 ? 1u : first);
+            }
+            umma_commit(&pv_bar[buf]);
+            umma_commit(&empty_bar[stage]);
+            next();
+          }
+          umma_commit(o_bar);
         }
-        umma_commit(o_bar);
       }
       __syncwarp();
       named_barrier_sync(1, 320);            // the unit's partial has been read out
     }
-  } else if (warp >= 4) {
+  } else {
     // ---------------------------------------------------------------- softmax
-    const int x = (warp - 4) >> 2;                   // stream
-    const int tid = threadIdx.x - 128;               // 0 .. 255
+    const int x = warp >> 2;                         // group: even or odd blocks of a unit
+    const int tid = threadIdx.x;                     // 0 .. 255
     const int row = tid & 127;                       // query row of the unit = TMEM lane
     const uint32_t lanes = (uint32_t)(row & ~31) << 16;
-    const uint32_t s_col = tmem + lanes + x * kColsS, o_col = tmem + lanes + kColO + x * 128;
-    uint32_t ns = 0, npv = 0, nrot = 0, no = 0;      // parities (ns: one per buffer)
+    const uint32_t o_col = tmem + lanes + kColO;
+    uint32_t nrot = 0, no = 0;                       // parities
     int it = 0;                                      // blocks of the units before
     for (int u = u0; u <= u1; ++u) {
       const long long w = (long long)u * sp.unit_weight;
@@ -352,48 +384,67 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int live = min(128, sp.rows - base);     // rows of this unit
       const bool vis = j1 > sp.blocks_full;
       {
-        // queries: thread = half a row (8 chunks of 16 bytes)
+        // queries: thread = half a row (8 chunks of 16 bytes).  Every load of the prologue is
+        // in flight before the first is stored: beside the tiles' stream each round trip
+        // takes microseconds.
         const int qrow = tid >> 1, half = tid & 1;
-        const bool there = qrow < live;
         const T *src = nullptr;
-        if (there) {
+        if (qrow < live) {
           const int r = base + qrow, g = r % a.groups, nt = r / a.groups;
           src = static_cast<const T *>(a.q.data) + ((long long)pre * a.questions + nt / a.tokens) * a.q.s[0] +
                 (nt % a.tokens) * a.q.s[1] + (h * a.groups + g) * a.q.s[2] + half * 64;
         }
+        const T *R = static_cast<const T *>(a.R.data) + pre * a.R.s[0] + h * a.R.s[1];
+        uint4 qv[8], rv[DK / 16];
+        float dm = 0.f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          qv[c] = src != nullptr ? __ldg(reinterpret_cast<const uint4 *>(src) + c) : make_uint4(0, 0, 0, 0);
+        if (vis) {
+#pragma unroll
+          for (int i = 0; i < DK / 16; ++i) {
+            const int e = tid + 256 * i;
+            if (p.R_layout == 1)                       // rows of R, 8 columns at a time
+              rv[i] = __ldg(reinterpret_cast<const uint4 *>(R + (e / (DK / 8)) * a.R.s[2] + (e % (DK / 8)) * 8));
+            else if (p.R_layout == 2)                  // columns of R, 8 rows at a time
+              rv[i] = __ldg(reinterpret_cast<const uint4 *>(R + (e >> 4) * a.R.s[3] + (e & 15) * 8));
+          }
+          if (tid < 128 && a.dm.data != nullptr)
+            dm = to_f32(static_cast<const T *>(a.dm.data)[pre * a.dm.s[0] + h * a.dm.s[1] + tid]);
+        }
         unsigned char *dst = smem + L::kQ + half * 16384;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const uint4 v = there ? __ldg(reinterpret_cast<const uint4 *>(src) + c) : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4 *>(dst + swizzled_offset<128>(qrow, c * 8)) = v;
-        }
+        for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4 *>(dst + swizzled_offset<128>(qrow, c * 8)) = qv[c];
         if (vis) {
           // R^T, K-major: row j holds column j of R
-          const T *R = static_cast<const T *>(a.R.data) + pre * a.R.s[0] + h * a.R.s[1];
           const uint32_t rt = smem_u32(smem + L::kRot);
-          if (p.R_rows) {                              // rows of R in 16-byte pieces
-            for (int e = tid; e < 128 * DK / 8; e += 256) {
-              const int d = e / (DK / 8), c = e % (DK / 8);
-              const uint4 v = __ldg(reinterpret_cast<const uint4 *>(R + d * a.R.s[2] + c * 8));
-              const uint32_t words[4] = {v.x, v.y, v.z, v.w};
-              const uint32_t box = rt + (d >> 6) * (DK * 128);
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                st_shared_u16(box + swizzled_offset<128>(c * 8 + i, (d & 63) & ~7) + (d & 7) * 2,
-                              (uint16_t)(words[i >> 1] >> (16 * (i & 1))));
-            }
-          } else {                                     // any strides; a transposed R reads along its columns
+          if (p.R_layout == 0) {                       // any strides
 #pragma unroll 8
             for (int e = tid; e < 128 * DK; e += 256) {
               const int d = e & 127, j = e >> 7;
               st_shared_u16(rt + (d >> 6) * (DK * 128) + swizzled_offset<128>(j, (d & 63) & ~7) + (d & 7) * 2,
                             __ldg(reinterpret_cast<const unsigned short *>(R + d * a.R.s[2] + j * a.R.s[3])));
             }
+          } else {
+#pragma unroll
+            for (int i = 0; i < DK / 16; ++i) {
+              const int e = tid + 256 * i;
+              if (p.R_layout == 1) {
+                const int d = e / (DK / 8), c = e % (DK / 8);
+                const uint32_t words[4] = {rv[i].x, rv[i].y, rv[i].z, rv[i].w};
+                const uint32_t box = rt + (d >> 6) * (DK * 128);
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                  st_shared_u16(box + swizzled_offset<128>(c * 8 + k, (d & 63) & ~7) + (d & 7) * 2,
+                                (uint16_t)(words[k >> 1] >> (16 * (k & 1))));
+              } else {
+                const int j = e >> 4, c = e & 15;
+                st_shared_v4(rt + (c >> 3) * (DK * 128) + swizzled_offset<128>(j, (c & 7) * 8), rv[i].x, rv[i].y, rv[i].z,
+                             rv[i].w);
+              }
+            }
           }
-          if (tid < 128)
-            dm_s[tid] = a.dm.data != nullptr
-                            ? to_f32(static_cast<const T *>(a.dm.data)[pre * a.dm.s[0] + h * a.dm.s[1] + tid])
-                            : 0.f;
+          if (tid < 128) dm_s[tid] = dm;
         }
       }
       fence_proxy_async_smem();
@@ -452,103 +503,126 @@ __global__ void __launch_bounds__(kThreads, 1)
         named_barrier_sync(1, 320);
       }
       const float bias = vis ? bias_s[row] : 0.f;
-      RowStat st{-INFINITY, 0.f};
+      float m = -INFINITY, l = 0.f;                  // what this group's last weights were relative to; their sum
       const bool busy = (row & ~31) < live;          // some row of this warp exists
-      const int nf = j0 < sp.blocks_full ? min(j1, sp.blocks_full) - j0 : 0;
-      const int subs = nf + 2 * (j1 - j0 - nf);
-      const int tok_vis = (max(j0, sp.blocks_full) - sp.blocks_full) * kVisTok;   // the segment's first visual token
-      for (int i = x; i < subs; i += 2) {
-        const int b = (i >> 1) & 1;
-        const bool prompt = i < nf;
-        const int tok = prompt ? (j0 + i) * kSub : tok_vis + (i - nf) * kSub;
-        const int left = (prompt ? a.seq_full : a.seq_sparse) - tok;
+      const int blocks = j1 - j0;
+      for (int k = x; k < blocks; k += 2) {
+        const int j = j0 + k, buf = (it + k) % 3;
+        const uint32_t par = ((it + k) / 3) & 1;
+        const bool prompt = j < sp.blocks_full;
+        const int left = prompt ? a.seq_full - j * kFullTok : a.seq_sparse - (j - sp.blocks_full) * kVisTok;
         const bool masked = prompt && a.mask.data != nullptr;
         uint32_t v0 = ~0u, v1 = ~0u;
-        if (masked || left < kSub) {
+        if (masked) {
           const uint8_t *mk = static_cast<const uint8_t *>(a.mask.data) + pre * a.mask.s[0];
-          v0 = __ballot_sync(0xffffffffu, lane < left && (!masked || mk[(tok + lane) * a.mask.s[1]] != 0));
-          v1 = __ballot_sync(0xffffffffu, lane + 32 < left && (!masked || mk[(tok + lane + 32) * a.mask.s[1]] != 0));
+          const long long tok = j * kFullTok + lane;
+          v0 = __ballot_sync(0xffffffffu, lane < left && mk[tok * a.mask.s[1]] != 0);
+          v1 = __ballot_sync(0xffffffffu, lane + 32 < left && mk[(tok + 32) * a.mask.s[1]] != 0);
         }
-        const bool all = (v0 & v1) == ~0u;
-        mbar_wait_bounded(&s_bar[x + 2 * b], (ns >> b) & 1, abort_flag, p.status);
-        ns ^= 1u << b;
+        mbar_wait_bounded(&s_bar[buf], par, abort_flag, p.status);
         tc_fence_after();
-        if (masked && !all) {
+        const uint32_t s = tmem + lanes + buf * kColsS;
+        if (masked && (v0 & v1) != ~0u) {
           // a masked token's Values may hold anything, and 0 * NaN is NaN: zero them
-          unsigned char *v = smem + L::kRing + (it + i) % L::kStages * L::kStage + 16384;
-          for (int t = (warp & 3); t < kSub; t += 4)
+          unsigned char *v = smem + L::kRing + (it + k) % L::kStages * L::kStage + 16384;
+          for (int t = (warp & 3); t < kFullTok; t += 4)
             if (!(((t < 32 ? v0 : v1) >> (t & 31)) & 1u))
               *reinterpret_cast<uint2 *>(v + (lane >> 4) * 8192 + t * 128 + (lane & 15) * 8) = make_uint2(0, 0);
           fence_proxy_async_smem();
+          mask_s(s, v0, v1);
+        } else if (left < (prompt ? kFullTok : kVisTok)) {
+          auto bits = [&](int n) { return n >= 32 ? ~0u : n > 0 ? (1u << n) - 1u : 0u; };
+          mask_s(s, bits(left), bits(left - 32));
+          if (!prompt) mask_s(s + 64, bits(left - 64), bits(left - 96));
         }
-        if (busy)
-          softmax_sub<T>(s_col + 2 * b * kColsS, a.scale_log2, prompt ? 0.f : bias, all, v0, v1, st, [&](float f) {
-            if (i < 2) return;                       // nothing in O yet
-            // O is at rest once the P . V before this sub-block is done: the next S comes
-            // after it in the tensor core's order; before the last one it is signalled
-            if (i + 2 < subs)
-              mbar_wait_bounded(&s_bar[x + 2 * (b ^ 1)], (ns >> (b ^ 1)) & 1, abort_flag, p.status);
-            else
-              mbar_wait_bounded(&pv_bar[x], npv, abort_flag, p.status);
-            tc_fence_after();
-            rescale_o(o_col, f);
-          }, [&] {
-            // The two streams' warps of a scheduler take turns with its exponential unit: while
-            // one computes weights the other waits for S, reads it and finds its maximum
-            // (left to themselves they run in step, and want the unit, and leave it idle, at
-            // the same time: 490 -> 409 us for 4096 rows on 32,768 tokens of 8 heads).
-            if (i > 0) named_barrier_sync(3 + (warp & 3) + 4 * (x ^ 1), 64);
-          });
-        if (busy && i + 1 < subs) asm volatile("bar.arrive %0, 64;" ::"r"(3 + (warp & 3) + 4 * x) : "memory");
+        if (busy) {
+          uint32_t r[2][32];
+          load_half(s, r);
+          float mx = max_half(r);
+          if (!prompt) {                             // the upper half stays in registers
+            load_half(s + 64, r);
+            mx = fmaxf(mx, max_half(r));
+          }
+          const float bi = prompt ? 0.f : bias;
+          const float top = fmaf(mx, a.scale_log2, bi);     // scale > 0; -inf stays -inf
+          // m, as the block before has settled it
+          float now = -INFINITY;
+          if (k > 0) {
+            named_barrier_sync(3 + (warp & 3) + 4 * (x ^ 1), 64);
+            now = ref_s[row];
+          }
+          const bool grow = top > now + kLazy;       // from -inf: whenever there is a maximum
+          if (__any_sync(0xffffffffu, grow)) {
+            const float f = grow ? fast_exp2(now - top) : 1.f;      // first maximum: 2^-inf = 0
+            if (grow) now = top;
+            if (k > 0) {                             // O is at rest when the P . V before is done
+              const int g = it + k - 1;
+              mbar_wait_bounded(&pv_bar[g % 3], (g / 3) & 1, abort_flag, p.status);
+              tc_fence_after();
+              rescale_o(o_col, f);
+              tc_fence_before();
+            }
+            ref_s[row] = now;
+          } else if (k == 0) {
+            ref_s[row] = now;
+          }
+          if (k + 1 < blocks) asm volatile("bar.arrive %0, 64;" ::"r"(3 + (warp & 3) + 4 * x) : "memory");
+          if (__any_sync(0xffffffffu, m != now)) {   // the other group moves it too
+            l *= m > -INFINITY ? fast_exp2(m - now) : 0.f;
+            m = now;
+          }
+          const float off = bi - (m > -INFINITY ? m : 0.f);
+          if (!prompt) {
+            l += weights_half<T>(s + kColP + 32, r, a.scale_log2, off);
+            load_half(s, r);
+          }
+          l += weights_half<T>(s + kColP, r, a.scale_log2, off);
+          tmem_wait_st();
+        }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_bar[x + 2 * b]);
+        if (lane == 0) mbar_arrive(&p_bar[buf]);
       }
-      it += j1 - j0;
-      if (subs > x + 2) npv ^= 1u;                   // one signal per unit whose stream has two sub-blocks
-      // join the two streams: each warp group writes 64 channels of the row
-      ml_s[x * 128 + row] = make_float2(st.m, st.l);
+      it += blocks;
+      // the partial result: each group writes 64 channels of the row
+      ml_s[x * 128 + row] = make_float2(m, l);
       mbar_wait_bounded(o_bar, no & 1, abort_flag, p.status);
       ++no;
       tc_fence_after();
       named_barrier_sync(2, 256);
-      const float2 e0 = ml_s[row], e1 = ml_s[128 + row];
-      const float m = fmaxf(e0.x, e1.x);
-      const float f0 = e0.x > -INFINITY ? fast_exp2(e0.x - m) : 0.f;
-      const float f1 = e1.x > -INFINITY ? fast_exp2(e1.x - m) : 0.f;
-      const bool two = subs > 1;                     // the odd stream had a sub-block
       const long long slot = u + cta;
       if (busy) {
-        float *out = p.acc + (slot * 128 + row) * 128 + 64 * x;
-        const uint32_t c0 = tmem + lanes + kColO + 64 * x, c1 = c0 + 128;
+        const float ref = ref_s[row];
+        // four channels of a row together, rows side by side: a warp's stores are whole lines
+        float4 *out = reinterpret_cast<float4 *>(p.acc) + (slot * 32 + 16 * x) * 128 + row;
 #pragma unroll
         for (int c = 0; c < 64; c += 16) {
-          uint32_t ra[16], rb[16];
-          tmem_ld16_nowait(c0 + c, ra);
-          if (two) tmem_ld16_nowait(c1 + c, rb);
+          uint32_t r[16];
+          tmem_ld16_nowait(o_col + 64 * x + c, r);
           tmem_wait_ld();
           if (row < live) {
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-              float v[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                v[k] = f0 > 0.f ? __uint_as_float(ra[i + k]) * f0 : 0.f;
-                if (two && f1 > 0.f) v[k] = fmaf(__uint_as_float(rb[i + k]), f1, v[k]);
-              }
-              *reinterpret_cast<float4 *>(out + c + i) = make_float4(v[0], v[1], v[2], v[3]);
-            }
+            for (int i = 0; i < 4; ++i)
+              out[(c / 4 + i) * 128] = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]),
+                                                   __uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
           }
         }
-        if (x == 0 && row < live)
-          reinterpret_cast<float2 *>(p.ml)[slot * 128 + row] = make_float2(m, e0.y * f0 + e1.y * f1);
+        if (x == 0 && row < live) {
+          float sum = 0.f;
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const float2 e = ml_s[g * 128 + row];
+            if (e.x > -INFINITY) sum = fmaf(e.y, fast_exp2(e.x - ref), sum);
+          }
+          reinterpret_cast<float2 *>(p.ml)[slot * 128 + row] = make_float2(ref, sum);
+        }
       }
       tc_fence_before();
       named_barrier_sync(1, 320);
     }
   }
   __syncthreads();
-  if (warp == 1) {
+  if (warp == 9) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }

@@ -399,31 +399,42 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
       }
     }
   __syncthreads();
-  const long long slot = ((long long)bh * p.chunks + chunk) * p.rows;
-  for (int e = warp; e < 16 * kRT; e += kWarps) {
-    const int r = row0 + e;
-    if (r >= p.rows) break;
-    float mm = -INFINITY, ll = 0.f;
+  // the rows' factors of each warp's partial, over the warps' own (m, l)
+  const int rows = min(p.rows - row0, 16 * kRT);
+  const long long slot = (long long)bh * p.chunks + chunk;
+  if ((int)threadIdx.x < rows) {
+    const int e = threadIdx.x;
     float2 st[kWarps];
+    float mm = -INFINITY, ll = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       st[w] = ml_s[w * kRT * 16 + e];
       mm = fmaxf(mm, st[w].x);
     }
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = st[w].x > -INFINITY ? fast_exp2(st[w].x - mm) : 0.f;
+      ll = fmaf(st[w].y, f, ll);
+      ml_s[w * kRT * 16 + e].x = f;
+    }
+    reinterpret_cast<float2 *>(p.ml)[slot * p.rows + row0 + e] = make_float2(mm, ll);
+  }
+  __syncthreads();
+  float4 *out = reinterpret_cast<float4 *>(p.acc) + slot * 32 * p.rows + row0;
+  for (int i = threadIdx.x; i < rows * 32; i += 32 * kWarps) {
+    const int c4 = i / rows, e = i - c4 * rows;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      if (!(st[w].x > -INFINITY)) continue;
-      const float f = fast_exp2(st[w].x - mm);
-      ll = fmaf(st[w].y, f, ll);
-      const float4 v = *reinterpret_cast<const float4 *>(o_s + (w * kRT * 16 + e) * 128 + lane * 4);
+      const float f = ml_s[w * kRT * 16 + e].x;
+      if (f == 0.f) continue;
+      const float4 v = *reinterpret_cast<const float4 *>(o_s + (w * kRT * 16 + e) * 128 + c4 * 4);
       o.x = fmaf(v.x, f, o.x);
       o.y = fmaf(v.y, f, o.y);
       o.z = fmaf(v.z, f, o.z);
       o.w = fmaf(v.w, f, o.w);
     }
-    *reinterpret_cast<float4 *>(p.acc + (slot + r) * 128 + lane * 4) = o;
-    if (lane == 0) reinterpret_cast<float2 *>(p.ml)[slot + r] = make_float2(mm, ll);
+    out[(long long)c4 * p.rows + e] = o;
   }
   wait_for_previous();
 }
@@ -685,7 +696,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
   }
   cp_async_wait_all();
   const float scale_o = FP8 ? vref : 1.f;
-  const long long slot = ((long long)bh * p.chunks + chunk) * p.rows;
+  const long long slot = (long long)bh * p.chunks + chunk;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     float ll = l[i];
@@ -693,11 +704,13 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
     ll += __shfl_xor_sync(0xffffffffu, ll, 2);
     const int r = row0 + g + 8 * i;
     if (r < p.rows) {
-      float *out = p.acc + (slot + r) * 128 + 2 * j4;
+      // channels 8 n + 2 j4, + 1: half of channel group 2 n + j4 / 2
+      float *out = p.acc + ((slot * 32 + (j4 >> 1)) * p.rows + r) * 4 + 2 * (j4 & 1);
 #pragma unroll
       for (int n = 0; n < 16; ++n)
-        *reinterpret_cast<float2 *>(out + 8 * n) = make_float2(acc[n][2 * i] * scale_o, acc[n][2 * i + 1] * scale_o);
-      if (j4 == 0) reinterpret_cast<float2 *>(p.ml)[slot + r] = make_float2(m[i], ll);
+        *reinterpret_cast<float2 *>(out + 8ll * n * p.rows) =
+            make_float2(acc[n][2 * i] * scale_o, acc[n][2 * i + 1] * scale_o);
+      if (j4 == 0) reinterpret_cast<float2 *>(p.ml)[slot * p.rows + r] = make_float2(m[i], ll);
     }
   }
   wait_for_previous();
