@@ -30,9 +30,11 @@
 // shared memory; only where m moves does the group wait for the P . V before and rescale O.
 // At the end of a unit the partial result of (unit, CTA) is written for shared_merge.cu.
 //
-// What bounds it: with many rows the exponential unit, 128 x 128 a block at 16 a cycle,
-// and what a warp does between two blocks' exponentials (waiting for S, reading it,
-// its maximum, handing P over); with few rows, HBM.
+// What bounds it: with many rows the exponential unit (128 x 128 a block at 16 a cycle: 1024
+// of the 1370 cycles a block takes) and what a warp does between two blocks'
+// exponentials (waiting for S, reading it, its maximum, handing P over); with few
+// rows, HBM.  A quarter or less of the exponentials as polynomials on the FMA units made it
+// slower (373 -> 378 to 404 us).
 #include <type_traits>
 
 #include "shared.h"
@@ -47,7 +49,6 @@ constexpr uint32_t kColsS = 128;                 // TMEM columns of an S buffer
 constexpr uint32_t kColP = 64;                   // P within it
 constexpr uint32_t kColO = 3 * kColsS;           // the O accumulator
 constexpr float kLazy = 8.f;
-constexpr int kPolyOf = 4;                       // one pair of exponentials in this many goes to the FMA units
 
 template <int DK>
 struct PrefixSmem {
@@ -64,8 +65,8 @@ struct PrefixSmem {
   static constexpr int kRef = kDm + 512;                           // float[128]: m
   static constexpr int kMl = kRef + 512;                           // float2[2][128]: a group's m, l
   static constexpr int kBar = kMl + 2048;
-  // full[S], empty[S], s_ready[3], p_ready[3], pv_done[3], rot, o_done
-  static constexpr int kNumBars = 2 * kStages + 11;
+  // full[S], empty[S], s_ready[3], p_ready[3], pv_done[3], rot, o_done, q_here
+  static constexpr int kNumBars = 2 * kStages + 12;
   static constexpr int kTmemSlot = kBar + kNumBars * 8;
   static constexpr int kAbort = kTmemSlot + 4;
   static constexpr int kBytes = kAbort + 4;
@@ -90,34 +91,6 @@ __device__ __forceinline__ void rescale_o(uint32_t o, float f) {
     tmem_st16_nowait(o + c, r);
   }
   tmem_wait_st();
-}
-
-// 2^x of two numbers without the exponential unit, for x in [-inf, 126]: x = n + f with n the
-// nearest integer (added in, and left in, the low bits of 1.5 * 2^23) and f in
-// [-1/2, 1/2], 2^f by a polynomial whose coefficients minimise the largest relative
-// error there (Remez; degree 3: 7.5e-5, degree 4: 2.6e-6 -- against 2^-9 and 2^-12 that
-// rounding to 16 bits costs), n added to its exponent.  Below 2^-126: 2^-126.
-template <typename T>
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-  constexpr float kMagic = 12582912.f;
-  x.x = fmaxf(x.x, -126.f);
-  x.y = fmaxf(x.y, -126.f);
-  const float2 t = __fadd2_rn(x, make_float2(kMagic, kMagic));
-  const float2 n = __fadd2_rn(t, make_float2(-kMagic, -kMagic));
-  const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
-  float2 y;
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    y = __ffma2_rn(f, make_float2(0x1.c3f76p-5f, 0x1.c3f76p-5f), make_float2(0x1.f0de1cp-3f, 0x1.f0de1cp-3f));
-    y = __ffma2_rn(f, y, make_float2(0x1.62f31ap-1f, 0x1.62f31ap-1f));
-    y = __ffma2_rn(f, y, make_float2(0x1.fff692p-1f, 0x1.fff692p-1f));
-  } else {
-    y = __ffma2_rn(f, make_float2(0x1.3997d4p-7f, 0x1.3997d4p-7f), make_float2(0x1.ca1442p-5f, 0x1.ca1442p-5f));
-    y = __ffma2_rn(f, y, make_float2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
-    y = __ffma2_rn(f, y, make_float2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
-    y = __ffma2_rn(f, y, make_float2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
-  }
-  return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
 }
 
 // Columns [s, s + 64) of S whose token does not count become -inf, whatever was there.
@@ -163,12 +136,8 @@ __device__ __forceinline__ float weights_half(uint32_t p, const uint32_t (&r)[2]
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1])), scale2, off2);
-      if (i % kPolyOf == kPolyOf - 1) {
-        x = exp2_poly<T>(x);
-      } else {
-        x.x = fast_exp2(x.x);
-        x.y = fast_exp2(x.y);
-      }
+      x.x = fast_exp2(x.x);
+      x.y = fast_exp2(x.y);
       l2[i & 1] = __fadd2_rn(l2[i & 1], x);
       w[i] = pack2<T>(x.x, x.y);
     }
@@ -191,6 +160,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t *pv_bar = p_bar + 3;                   // [buffer] its P . V is done
   uint64_t *rot_bar = pv_bar + 3;                 // rotated queries are in TMEM
   uint64_t *o_bar = rot_bar + 1;                  // the O accumulator is complete
+  uint64_t *q_bar = o_bar + 1;                    // the first unit's queries are here
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::kTmemSlot);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::kAbort);
   float *bias_s = reinterpret_cast<float *>(smem + L::kBias);
@@ -219,6 +189,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(rot_bar, 1);
     mbar_init(o_bar, 1);
+    mbar_init(q_bar, 8);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -230,7 +201,25 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 8) {
     // ---------------------------------------------------------------- producer
-    if (lane == 0) {
+    if (lane > 0) {
+      // the queries and R of the CTA's later units, into L2 before they are asked for
+      for (int u = u0 + 1; u <= u1; ++u) {
+        const int ph = u / sp.row_tiles, pre = ph / a.kv_heads, h = ph % a.kv_heads;
+        const int base = (u % sp.row_tiles) * 128, live = min(128, sp.rows - base);
+        for (int e = lane - 1; e < 2 * live; e += 31) {
+          const int r = base + (e >> 1), g = r % a.groups, nt = r / a.groups;
+          prefetch_l2(static_cast<const T *>(a.q.data) + ((long long)pre * a.questions + nt / a.tokens) * a.q.s[0] +
+                      (nt % a.tokens) * a.q.s[1] + (h * a.groups + g) * a.q.s[2] + (e & 1) * 64);
+        }
+        if (sp.blocks_vis > 0 && p.R_layout != 0) {
+          const T *R = static_cast<const T *>(a.R.data) + pre * a.R.s[0] + h * a.R.s[1];
+          if (p.R_layout == 1)
+            for (int d = lane - 1; d < 128; d += 31) prefetch_l2(R + d * a.R.s[2]);
+          else
+            for (int e = lane - 1; e < 2 * DK; e += 31) prefetch_l2(R + (e >> 1) * a.R.s[3] + (e & 1) * 64);
+        }
+      }
+    } else {
       int it = 0;
       bool ok = true;
       for (int u = u0; u <= u1 && ok; ++u) {
@@ -240,6 +229,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int ph = u / sp.row_tiles, pre = ph / a.kv_heads, h = ph % a.kv_heads;
         for (int j = j0; j < j1; ++j, ++it) {
           const int stg = it % L::kStages;
+          // one block ahead of the queries, the rest of the ring after them: every CTA's whole
+          // ring would queue at HBM in front of them
+          if (it == 1) mbar_wait_bounded(q_bar, 0, abort_flag, p.status);
           if (!mbar_wait_bounded(&empty_bar[stg], ((it / L::kStages) & 1) ^ 1, abort_flag, p.status)) {
             ok = false;
             break;
@@ -446,6 +438,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (tid < 128) dm_s[tid] = dm;
         }
+      }
+      if (it == 0) {                                   // the first unit of this CTA
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_bar);
       }
       fence_proxy_async_smem();
       named_barrier_sync(1, 320);
