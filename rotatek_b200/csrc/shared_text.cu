@@ -64,6 +64,11 @@ __device__ __forceinline__ void cp_async_4_zfill(void *dst, const void *src, boo
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 4 : 0) : "memory");
 }
 
+// Chunk c of this lane's row of an ldmatrix, given the address of its chunk `odd` (0 or 1)
+// there: c = even + odd, and XOR with an even chunk number is one instruction (rows start
+// at multiples of 256 bytes).
+__device__ __forceinline__ uint32_t even(uint32_t lane_addr, int even_chunk) { return lane_addr ^ (even_chunk << 4); }
+
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   mma_16816<__half>(d, a, b0, b1);
 }
@@ -78,7 +83,7 @@ template <typename T, bool FP8, int kRT>
 __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextParams p) {
   using L = TextSmem<FP8, kRT>;
   using M = typename std::conditional<FP8, __half, T>::type;   // MMA operand type
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ __align__(1024) unsigned char smem[];
   launch_dependents();
   const SharedParams &a = p.s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -202,7 +207,8 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[rt][n][i] = 0.f;
   }
-  const uint32_t q_addr = smem_u32(smem + L::kQ);
+  const uint32_t q_lane = smem_u32(smem + L::kQ) + at<256>(lane & 15, lane >> 4);
+  const uint32_t k_at = at<256>((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1), v_at = at<256>(lane & 15, lane >> 4);
 
   int stage = 0;
   for (int blk = warp; blk < blocks; blk += kWarps) {
@@ -262,7 +268,7 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
 #pragma unroll
       for (int k = 0; k < 8; ++k) {                  // 16 channels
         uint32_t qa[4];
-        ldmatrix_x4(q_addr + at<256>(rt * 16 + (lane & 15), 2 * k + (lane >> 4)), qa[0], qa[1], qa[2], qa[3]);
+        ldmatrix_x4(even(q_lane + rt * 4096, 2 * k), qa[0], qa[1], qa[2], qa[3]);
         if constexpr (FP8) {
           // four n-tiles of 8 tokens, the 16-byte chunk k of each
           uint32_t r[4];
@@ -273,7 +279,7 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
         } else {
           // two n-tiles, the chunks 2k and 2k + 1
           uint32_t r[4];
-          ldmatrix_x4(k_addr + at<256>((lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)), r[0], r[1], r[2], r[3]);
+          ldmatrix_x4(even(k_addr + k_at, 2 * k), r[0], r[1], r[2], r[3]);
           mma_16816<T>(s[0], qa, r[0], r[1]);
           mma_16816<T>(s[1], qa, r[2], r[3]);
         }
@@ -359,7 +365,7 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
 #pragma unroll
           for (int c = 0; c < 16; c += 2) {          // two chunks of 8 channels
             uint32_t r[4];
-            ldmatrix_x4_trans(v_addr + at<256>(kk * 16 + (lane & 15), c + (lane >> 4)), r[0], r[1], r[2], r[3]);
+            ldmatrix_x4_trans(even(v_addr + v_at + kk * 4096, c), r[0], r[1], r[2], r[3]);
             mma_16816<T>(acc[rt][c], pf, r[0], r[1]);
             mma_16816<T>(acc[rt][c + 1], pf, r[2], r[3]);
           }
@@ -459,7 +465,7 @@ template <typename T, bool FP8>
 __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const TextParams p) {
   using L = RowsSmem<FP8>;
   using M = typename std::conditional<FP8, __half, T>::type;     // MMA operand type
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ __align__(1024) unsigned char smem[];
   launch_dependents();
   const SharedParams &a = p.s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -480,16 +486,21 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
   const long long ks = a.kt.s[2] * kEsize, vs = a.vt.s[2] * kEsize;
   const float *ksc = FP8 ? static_cast<const float *>(a.ksc.data) + b * a.ksc.s[0] + h * a.ksc.s[1] : nullptr;
   const float *vsc = FP8 ? static_cast<const float *>(a.vsc.data) + b * a.vsc.s[0] + h * a.vsc.s[1] : nullptr;
-  auto fetch = [&](int tile) {
-    unsigned char *dst = smem + L::kRing + tile % L::kStages * L::kRaw;
-    const int first = t0 + tile * L::kTok;
+  // this thread's first row of a tile and its 16 bytes of it; further rows kRowStep apart
+  constexpr int kRowStep = 32 * kWarps / kChunks, kRows = L::kTok / kRowStep;
+  const int my_row = threadIdx.x / kChunks, my_chunk = threadIdx.x % kChunks;
+  const unsigned char *kp = kbase + (t0 + my_row) * ks + my_chunk * 16, *vp = vbase + (t0 + my_row) * vs + my_chunk * 16;
+  int fetched = 0;                                   // tiles asked for so far, one after another
+  uint32_t fetch_stage = 0;
+  auto fetch = [&] {
+    unsigned char *dst = smem + L::kRing + fetch_stage * L::kRaw;
+    const int first = t0 + fetched * L::kTok;
 #pragma unroll
-    for (int e = 0; e < L::kTok * kChunks / (32 * kWarps); ++e) {
-      const int i = e * 32 * kWarps + threadIdx.x, r = i / kChunks, c = i % kChunks;
-      const int tok = first + r;
-      const bool in = tok < t1;
-      cp_async_16_zfill(dst + at<kRowBytes>(r, c), kbase + (in ? tok * ks + c * 16 : 0), in ? 16 : 0);
-      cp_async_16_zfill(dst + L::kTok * kRowBytes + at<kRowBytes>(r, c), vbase + (in ? tok * vs + c * 16 : 0), in ? 16 : 0);
+    for (int e = 0; e < kRows; ++e) {
+      const int r = my_row + e * kRowStep;
+      const bool in = first + r < t1;
+      cp_async_16_zfill(dst + at<kRowBytes>(r, my_chunk), in ? kp + e * kRowStep * ks : kbase, in ? 16 : 0);
+      cp_async_16_zfill(dst + L::kTok * kRowBytes + at<kRowBytes>(r, my_chunk), in ? vp + e * kRowStep * vs : vbase, in ? 16 : 0);
     }
     if (FP8 && warp < 2) {                           // lane = token of the tile
       const bool in = first + lane < t1;
@@ -497,10 +508,14 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
                        warp == 0 ? ksc + (in ? (first + lane) * a.ksc.s[2] : 0) : vsc + (in ? (first + lane) * a.vsc.s[2] : 0),
                        in);
     }
+    kp += L::kTok * ks;
+    vp += L::kTok * vs;
+    ++fetched;
+    if (++fetch_stage == (uint32_t)L::kStages) fetch_stage = 0;
   };
 #pragma unroll
   for (int i = 0; i < L::kStages - 1; ++i) {
-    if (i < tiles) fetch(i);
+    if (i < tiles) fetch();
     cp_async_commit();
   }
   // this warp's 16 queries, in the MMA's type (bf16 against 8-bit text: f16 scaled by a power of two)
@@ -551,7 +566,8 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
   const int all_see = len - (a.tokens - 1);          // every row sees tokens below this
-  const uint32_t q_addr = smem_u32(smem + L::kQ);
+  const uint32_t q_lane = smem_u32(smem + L::kQ) + at<256>(warp * 16 + (lane & 15), lane >> 4);
+  const uint32_t k_at = at<256>((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1), v_at = at<256>(lane & 15, lane >> 4);
 
   for (int tile = 0; tile < tiles; ++tile) {
     const int first = t0 + tile * L::kTok;
@@ -559,7 +575,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
     float kscale[kNT][2], vscale[kNT][2];
     cp_async_wait_group<L::kStages - 2>();
     __syncthreads();                                 // the tile has landed; the one before is done with
-    if (tile + L::kStages - 1 < tiles) fetch(tile + L::kStages - 1);
+    if (fetched < tiles) fetch();
     cp_async_commit();
     uint32_t k_addr, v_addr;
     const unsigned char *raw = smem + L::kRing + tile % L::kStages * L::kRaw;
@@ -616,13 +632,13 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
     for (int n = 0; n < kNT; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
+    const uint32_t k_lane = k_addr + k_at, k_lane2 = k_lane + 16 * 256, v_lane = v_addr + v_at, v_lane2 = v_lane + 16 * 256;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {                    // 16 channels
       uint32_t qa[4], r[4], r2[4];
-      ldmatrix_x4(q_addr + at<256>(warp * 16 + (lane & 15), 2 * k + (lane >> 4)), qa[0], qa[1], qa[2], qa[3]);
-      ldmatrix_x4(k_addr + at<256>((lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)), r[0], r[1], r[2], r[3]);
-      ldmatrix_x4(k_addr + at<256>(16 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)), r2[0], r2[1], r2[2],
-                  r2[3]);
+      ldmatrix_x4(even(q_lane, 2 * k), qa[0], qa[1], qa[2], qa[3]);
+      ldmatrix_x4(even(k_lane, 2 * k), r[0], r[1], r[2], r[3]);
+      ldmatrix_x4(even(k_lane2, 2 * k), r2[0], r2[1], r2[2], r2[3]);
       mma_16816<M>(s[0], qa, r[0], r[1]);
       mma_16816<M>(s[1], qa, r[2], r[3]);
       mma_16816<M>(s[2], qa, r2[0], r2[1]);
@@ -688,7 +704,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
 #pragma unroll
       for (int c = 0; c < 16; c += 2) {              // two chunks of 8 channels
         uint32_t r[4];
-        ldmatrix_x4_trans(v_addr + at<256>(kk * 16 + (lane & 15), c + (lane >> 4)), r[0], r[1], r[2], r[3]);
+        ldmatrix_x4_trans(even(kk ? v_lane2 : v_lane, c), r[0], r[1], r[2], r[3]);
         mma_16816<M>(acc[c], pf, r[0], r[1]);
         mma_16816<M>(acc[c + 1], pf, r[2], r[3]);
       }
