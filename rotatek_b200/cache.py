@@ -139,4 +139,86 @@ class SpanKVCache:
         return L.s_prompt + L.s_vision + L.s_text
 
 
-__all__ = ["SpanKVCache"]
+class SharedPrefixCache:
+    """Text caches of many questions on shared prefixes.
+
+    ``prefix`` is the ``SpanKVCache`` that the prefill of P images left (its prompt,
+    rotated visual Keys and Values; stored once), each serving ``questions``
+    questions: B = P * questions rows, row b on prefix b // questions.  Each layer
+    of each row has room for ``capacity`` text tokens, stored as e4m3 rows with one
+    scale each (``fp8``: half the bytes) or in the prefix's dtype:
+
+        k_text, v_text    [B, H_kv, capacity, D]
+        k_scale, v_scale  [B, H_kv, capacity] float32 (fp8)
+
+    ``lens`` [B] int32 lives on the device, so that a captured step can be
+    replayed.  A step appends T tokens to every layer (``append``) and attends with
+    them (``attend``); ``advance`` then moves the lengths.  Drafted tokens that a
+    step did not accept need no undoing: their rows lie past the new length and are
+    overwritten by the next append.  The host cannot see the lengths, so it counts
+    the most that a row can have reached; ``append`` refuses what might not fit."""
+
+    def __init__(self, prefix: SpanKVCache, questions: int, capacity: int, fp8: bool = True):
+        if len(prefix) == 0:
+            raise ValueError("the prefix has no layers")
+        if questions < 1 or capacity < 1:
+            raise ValueError("questions and capacity must be positive")
+        self.prefix, self.questions, self.capacity, self.fp8 = prefix, questions, capacity, fp8
+        keys = prefix.layers[0].keys_full
+        p, h, _, d = keys.shape
+        self.batch, dev = p * questions, keys.device
+        kind = torch.uint8 if fp8 else keys.dtype
+        self.text = []
+        for _ in prefix.layers:
+            k, v = (torch.zeros(self.batch, h, capacity, d, dtype=kind, device=dev) for _ in range(2))
+            scales = (torch.zeros(self.batch, h, capacity, device=dev) for _ in range(2)) if fp8 else (None, None)
+            self.text.append((k, v, *scales))
+        self.lens = torch.zeros(self.batch, dtype=torch.int32, device=dev)
+        self.reach = 0                 # no row is longer than this
+
+    def append(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int,
+               counts: Optional[torch.Tensor] = None, at: Optional[torch.Tensor] = None) -> None:
+        """Write [B, H_kv, T, D] new Keys and Values of a layer behind the lengths
+        (``at`` [B] int32: behind these instead); ``counts`` [B] int32: only the
+        first counts[b] of them."""
+        from rotatek_b200.kernels import append_text
+        t = key_states.shape[2]
+        if self.reach + t > self.capacity:
+            raise ValueError(f"text caches full: {self.reach} + {t} tokens > capacity {self.capacity}")
+        k, v, ks, vs = self.text[layer_idx]
+        append_text(key_states, value_states, self.lens if at is None else at, k, v, k_scale=ks, v_scale=vs,
+                    counts=counts)
+
+    def attend(self, q: torch.Tensor, layer_idx: int, lens: torch.Tensor, num_kv_groups: int) -> torch.Tensor:
+        """Attention of q [B, T, H_q, D] over the prefix and the first ``lens`` [B]
+        text rows, the T new ones among them; [B, T, H_q, D]."""
+        from rotatek_b200.kernels import rotatek_shared_decode
+        a = self.prefix.decode_args(layer_idx)
+        k, v, ks, vs = self.text[layer_idx]
+        return rotatek_shared_decode(q, a["R_partial"], a["delta_mu"], a["k_full"], a["v_full"], a["mask_full"],
+                                     a["k_sparse"], a["v_sparse"], k, v, lens, num_kv_groups, k_scale=ks, v_scale=vs)
+
+    def advance(self, tokens: torch.Tensor, most: int) -> None:
+        """Lengthen every row by tokens[b] (device int32 [B], each at most ``most``)."""
+        if self.reach + most > self.capacity:
+            raise ValueError(f"text caches full: {self.reach} + {most} tokens > capacity {self.capacity}")
+        self.lens += tokens
+        self.reach += most
+
+    def settle(self) -> None:
+        """Read the lengths back, so that the host's count is exact again (one
+        synchronisation)."""
+        self.reach = int(self.lens.max())
+
+    def read(self, layer_idx: int, dtype: Optional[torch.dtype] = None):
+        """A layer's text as plain tensors (k, v), zero past each length."""
+        from rotatek_b200.kernels import read_text
+        k, v, ks, vs = self.text[layer_idx]
+        if self.fp8:
+            return read_text(k, v, self.lens, k_scale=ks, v_scale=vs,
+                             dtype=dtype or self.prefix.layers[0].keys_full.dtype)
+        there = (torch.arange(self.capacity, device=k.device) < self.lens[:, None])[:, None, :, None]
+        return tuple(torch.where(there, x, 0).to(dtype or x.dtype) for x in (k, v))
+
+
+__all__ = ["SpanKVCache", "SharedPrefixCache"]
