@@ -214,9 +214,9 @@ cudaError_t append(const AppendParams &p, bool rows128, cudaStream_t stream) {
   } else if (rows <= 32 * 1024) {                    // few rows: spread them over the SMs
     const int ctas = (p.tokens + 31) / 32;
     append_rows_kernel<T, kQuantize, 1><<<items * ctas, 256, 0, stream>>>(p, ctas);
-  } else {                                           // many: two rows of a thread in flight
-    const int ctas = (p.tokens + 63) / 64;
-    append_rows_kernel<T, kQuantize, 2><<<items * ctas, 256, 0, stream>>>(p, ctas);
+  } else {                                           // many: four rows of a thread in flight
+    const int ctas = (p.tokens + 127) / 128;
+    append_rows_kernel<T, kQuantize, 4><<<items * ctas, 256, 0, stream>>>(p, ctas);
   }
   return cudaGetLastError();
 }
@@ -309,8 +309,8 @@ cudaError_t read(const ReadParams &p, bool rows128, cudaStream_t stream) {
     const int ctas = (p.cap + 31) / 32;
     read_rows_kernel<T, 1><<<items * ctas, 256, 0, stream>>>(p, ctas);
   } else {
-    const int ctas = (p.cap + 127) / 128;
-    read_rows_kernel<T, 4><<<items * ctas, 256, 0, stream>>>(p, ctas);
+    const int ctas = (p.cap + 63) / 64;
+    read_rows_kernel<T, 2><<<items * ctas, 256, 0, stream>>>(p, ctas);
   }
   return cudaGetLastError();
 }

@@ -44,7 +44,7 @@ __host__ __device__ inline VerifyLayout verify_layout(long long batch, long long
   l.rows = (int)(2 * drafts + 1);
   const long long total = batch * l.rows * vocab;
   l.chunk = 2048;
-  while (l.chunk < 16384 && total / l.chunk > 148 * 16) l.chunk *= 2;
+  while (l.chunk < 65536 && total / l.chunk > 148 * 16) l.chunk *= 2;
   l.chunks = (int)((vocab + l.chunk - 1) / l.chunk);
   // pick: one wave of CTAs, since each of them joins and decides before it races
   l.race = (int)((batch * vocab / (148 * 4) + 2047) / 2048 * 2048);

@@ -355,7 +355,7 @@ def rotatek_shared_decode(
             return rotatek_shared_decode(q, R_partial, delta_mu, k_full, v_full, mask_full, k_sparse, v_sparse, k_text,
                                          v_text, text_lens, num_kv_groups, k_scale=k_scale, v_scale=v_scale, out=out)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     calls = _lib.calls()
     stream = _lib.raw_stream(dev)
     need = 0
@@ -445,8 +445,8 @@ def read_text(
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return read_text(k_text, v_text, text_lens, k_scale=k_scale, v_scale=v_scale, dtype=dtype)
-    k = torch.empty(k_text.shape, dtype=dtype, device=dev)
-    v = torch.empty(k_text.shape, dtype=dtype, device=dev)
+    k = torch.empty_like(k_text, dtype=dtype, memory_format=torch.contiguous_format)
+    v = torch.empty_like(k_text, dtype=dtype, memory_format=torch.contiguous_format)
     code = _lib.calls().read_text(k_text, v_text, k_scale, v_scale, text_lens, k, v, _lib.raw_stream(dev))
     if code:
         _raise(code, k_text, v_text, k_scale, v_scale, text_lens, k, v)
@@ -489,7 +489,7 @@ def verify_drafts(
     b, rows, vocab = target_logits.shape
     calls = _lib.calls()
     tokens = torch.empty((b, rows), dtype=torch.int64, device=dev)
-    accepted = torch.empty(b, dtype=torch.int32, device=dev)
+    accepted = torch.empty_like(temperature, dtype=torch.int32, memory_format=torch.contiguous_format)
     stream = _lib.raw_stream(dev)
     need = 0
     while True:
