@@ -96,7 +96,10 @@ SharedSpace shared_space(const rtk::PrefixSplit &sp, int64_t batch, int64_t kv_h
   return w;
 }
 
-int64_t text_chunks(int64_t cap) { return (cap + rtk::kTextChunk - 1) / rtk::kTextChunk; }
+int64_t text_chunks(int64_t batch, int64_t kv_heads, int64_t rows, int64_t cap) {
+  const int64_t chunk = rtk::text_chunk(batch, kv_heads, rows, cap);
+  return (cap + chunk - 1) / chunk;
+}
 
 int current_device() {
   int d = 0;
@@ -116,7 +119,7 @@ size_t rtk_shared_decode_workspace_size(int64_t prefixes, int64_t batch, int64_t
   const rtk::PrefixSplit sp =
       rtk::prefix_split(prefixes, batch / prefixes, tokens, groups, kv_heads, seq_full, seq_sparse, text_cap,
                         rtk::device_sms(device));
-  return shared_space(sp, batch, kv_heads, tokens * groups, text_chunks(text_cap)).bytes;
+  return shared_space(sp, batch, kv_heads, tokens * groups, text_chunks(batch, kv_heads, tokens * groups, text_cap)).bytes;
 }
 
 int rtk_shared_decode(const rtk_tensor *q, const rtk_tensor *R_partial, const rtk_tensor *delta_mu,
@@ -211,7 +214,7 @@ int rtk_shared_decode(const rtk_tensor *q, const rtk_tensor *R_partial, const rt
   const int device = current_device();
   const rtk::PrefixSplit sp =
       rtk::prefix_split(P, B / P, T, num_kv_groups, Hkv, Sf, Sv, C, rtk::device_sms(device));
-  const int64_t rows = T * num_kv_groups, chunks = text_chunks(C);
+  const int64_t rows = T * num_kv_groups, chunks = text_chunks(B, Hkv, rows, C);
   if ((int64_t)sp.rows != B / P * rows || (int64_t)P * Hkv * sp.row_tiles > kMaxInt / 256 || chunks > 65535 ||
       rows > 65535 * 16 || B * Hkv > kMaxInt)
     return fail(RTK_ERR_UNSUPPORTED, "too many query rows or text tokens");
@@ -229,7 +232,7 @@ int rtk_shared_decode(const rtk_tensor *q, const rtk_tensor *R_partial, const rt
   mp.split = sp;
   mp.has_prefix = Sf + Sv > 0;
   mp.has_text = C > 0;
-  mp.text_rows = (int)rows; mp.text_chunks = (int)chunks;
+  mp.text_rows = (int)rows; mp.text_chunk = rtk::text_chunk(B, Hkv, rows, C); mp.text_chunks = (int)chunks;
   float *pml = reinterpret_cast<float *>(ws + w.prefix_ml), *pacc = reinterpret_cast<float *>(ws + w.prefix_acc);
   float *tml = reinterpret_cast<float *>(ws + w.text_ml), *tacc = reinterpret_cast<float *>(ws + w.text_acc);
   mp.prefix_ml = pml; mp.prefix_acc = pacc; mp.text_ml = tml; mp.text_acc = tacc;
@@ -249,7 +252,7 @@ int rtk_shared_decode(const rtk_tensor *q, const rtk_tensor *R_partial, const rt
   if (mp.has_text) {
     rtk::TextParams tp;
     tp.s = p;
-    tp.rows = (int)rows; tp.chunks = (int)chunks;
+    tp.rows = (int)rows; tp.chunk = mp.text_chunk; tp.chunks = (int)chunks;
     tp.beside = mp.has_prefix;
     tp.ml = tml; tp.acc = tacc;
     e = rtk::launch_shared_text(tp, st);

@@ -130,11 +130,19 @@ struct PrefixParams {
 };
 cudaError_t launch_shared_prefix(const PrefixMaps &maps, const PrefixParams &p, cudaStream_t stream);
 
-// Text: CTAs per (question, KV head, chunk of kTextChunk tokens, 16 or 32 query rows).
-constexpr int kTextChunk = 256;
+// Text: CTAs per (question, KV head, chunk of tokens, 16 or 64 query rows).  Chunks of 256
+// tokens, so that few questions use many SMs; longer where that makes several waves of
+// CTAs (their prologues and partials cost more than the balance they bring).
+inline int text_chunk(long long batch, long long kv_heads, long long rows, long long cap) {
+  const long long tiles = rows <= 16 ? 1 : (rows + 63) / 64;
+  int chunk = 256;
+  while (chunk < 1024 && batch * kv_heads * tiles * ((cap + chunk - 1) / chunk) > 148 * 8) chunk *= 2;
+  return chunk;
+}
+
 struct TextParams {
   SharedParams s;
-  int rows, chunks;             // T G query rows, ceil(cap / kTextChunk)
+  int rows, chunk, chunks;      // T G query rows; tokens of a chunk, ceil(cap / chunk)
   int beside;                   // launched right after the prefix kernel, to run beside it
   float *ml, *acc;              // per (question, KV head, chunk): [rows][2] and [32 groups of 4 channels][rows][4]
 };
@@ -144,7 +152,7 @@ struct MergeParams {
   SharedParams s;
   PrefixSplit split;
   int has_prefix, has_text;
-  int text_rows, text_chunks;
+  int text_rows, text_chunk, text_chunks;
   const float *prefix_ml, *prefix_acc, *text_ml, *text_acc;
 };
 cudaError_t launch_shared_merge(const MergeParams &p, cudaStream_t stream);

@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(1024 / kQuads) shared_merge_kernel(const Merge
     const long long first = ((long long)b * a.kv_heads + h) * p.text_chunks;
     const float2 *ml = reinterpret_cast<const float2 *>(p.text_ml) + first * p.text_rows + row;
     const float4 *acc = reinterpret_cast<const float4 *>(p.text_acc) + first * 32 * p.text_rows + row;
-    join((len + kTextChunk - 1) / kTextChunk, [&](int i) { return ml + (long long)i * p.text_rows; },
+    join((len + p.text_chunk - 1) / p.text_chunk, [&](int i) { return ml + (long long)i * p.text_rows; },
          [&](int i, int c4) { return acc + (i * 32ll + c4) * p.text_rows; });
   }
   const float inv = l != 0.f ? 1.f / l : 0.f;
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(128) shared_merge_rows_kernel(const MergeParam
   total = prefixes;
   if (p.has_text) {
     const int len = min(max(a.lens[b * a.lens_s], 0), a.cap);
-    total += (len + kTextChunk - 1) / kTextChunk;
+    total += (len + p.text_chunk - 1) / p.text_chunk;
     text0 = ((long long)b * a.kv_heads + h) * p.text_chunks;
     at_t = text0 * p.text_rows + t * a.groups + g;
   }

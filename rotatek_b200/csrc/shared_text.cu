@@ -3,7 +3,7 @@
 //
 // A question's text belongs to it alone, so its Keys and Values are read once for a
 // handful of rows: the bound is HBM, and the work is cut so that bytes stay in
-// flight.  A CTA takes (question, KV head, 256 tokens, up to 16 kRT query rows); its
+// flight.  A CTA takes (question, KV head, a chunk of tokens, up to 16 kRT query rows); its
 // four warps take every fourth block of tokens through cp.async rings of their own
 // (no CTA-wide barrier in the loop), keep (m, l, O) in registers, and meet once at the
 // end.  Per block a warp runs m16n8k16 MMAs: S = Q . K^T with the query rows as M, and
@@ -91,12 +91,12 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
   const int chunk = blockIdx.y, bh = blockIdx.x, row0 = blockIdx.z * 16 * kRT;
   const int b = bh / a.kv_heads, h = bh % a.kv_heads;
   const int len = min(max(a.lens[b * a.lens_s], 0), a.cap);
-  const int t0 = chunk * kTextChunk;
+  const int t0 = chunk * p.chunk;
   if (t0 >= len) {
     wait_for_previous();
     return;
   }
-  const int t1 = min(len, t0 + kTextChunk);
+  const int t1 = min(len, t0 + p.chunk);
   const int blocks = (t1 - t0 + L::kTok - 1) / L::kTok;
 
   // this warp's ring
@@ -473,12 +473,12 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
   const int chunk = blockIdx.y, bh = blockIdx.x, row0 = blockIdx.z * 64 + warp * 16;
   const int b = bh / a.kv_heads, h = bh % a.kv_heads;
   const int len = min(max(a.lens[b * a.lens_s], 0), a.cap);
-  const int t0 = chunk * kTextChunk;
+  const int t0 = chunk * p.chunk;
   if (t0 >= len) {
     wait_for_previous();
     return;
   }
-  const int t1 = min(len, t0 + kTextChunk);
+  const int t1 = min(len, t0 + p.chunk);
   const int tiles = (t1 - t0 + L::kTok - 1) / L::kTok;
   constexpr int kEsize = FP8 ? 1 : 2, kRowBytes = 128 * kEsize, kChunks = kRowBytes / 16;
   const unsigned char *kbase = static_cast<const unsigned char *>(a.kt.data) + (b * a.kt.s[0] + h * a.kt.s[1]) * kEsize;
