@@ -492,3 +492,49 @@ def test_verify_captured():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("up", [True, False])
+def test_decode_maximum_that_keeps_moving(dtype, up):
+    """Logits that climb (or fall) by hundreds along the prefix, in every block anew, for
+    more than one tile of rows: the accumulators are rescaled again and again."""
+    a = make(1, 40, 1, 14, 2, 2000, 200, 30, 32, dtype=dtype, seed=23, bias=False)
+    ramp = torch.linspace(-1, 1, 2000, device=DEV) * (1 if up else -1)
+    row = torch.zeros(32, device=DEV)
+    row[0] = 1.0
+    direction = a["R_partial"][0, :, :, 0].float()                       # q . R column 0 = 20 for every query
+    q = a["q"].float() * 0.05
+    q = q + 20.0 * direction.repeat_interleave(7, 0)
+    a["q"] = q.to(dtype)
+    a["k_sparse"] = (a["k_sparse"].float() * 0.05 + 60.0 * ramp[:, None] * row).to(dtype)
+    a["k_full"] = (a["k_full"].float() * 0.1).to(dtype)
+    from rotatek_b200.kernels import rotatek_shared_decode
+    got = rotatek_shared_decode(**a).cpu().double()
+    want, mag = osh.shared_decode(**a)
+    # logits reach 106 with the rotated query in two 16-bit parts (2^-16): weights move by
+    # up to 2 * 106 * 2^-16 * log2(e) < 2^-7.7
+    u = HALF_ULP[dtype]
+    assert ((got - want).abs() <= u * want.abs() + (2 * u + 2.0 ** -7) * mag + 2.0 ** -25).all()
+
+
+def test_decode_many_units_and_short_ranges():
+    """Grids where a CTA's share is a block, less than a block's weight apart, or several
+    units; more units than SMs."""
+    for shape in [(3, 1, 1, 8, 8, 1, 1, 2, 16), (40, 1, 1, 8, 8, 130, 3, 2, 16), (5, 30, 2, 40, 8, 129, 0, 3, 32)]:
+        check(make(*shape, seed=shape[0]))
+
+
+def test_verify_large_noise_and_tiny_temperature():
+    """Temperatures near zero pick the argmax; enormous and tiny noise stay finite."""
+    from rotatek_b200.kernels import verify_drafts
+    a = make_verify(6, 2, 3000, torch.float32, False, 12)
+    a["temperature"] = torch.full((6,), 1e-4, device=DEV)
+    a["draft_lens"] = torch.zeros(6, dtype=torch.int32, device=DEV)
+    a["noise"][::2] *= 1e30
+    a["noise"][1::2] *= 1e-25
+    tokens, _ = verify_drafts(**a)
+    best = a["target_logits"][:, 0].argmax(-1)
+    top = a["target_logits"][:, 0].topk(2).values
+    clear = (top[:, 0] - top[:, 1]) > 0.01          # e^100 outweighs any noise ratio here
+    assert clear.any() and torch.equal(tokens[clear, 0], best[clear])
