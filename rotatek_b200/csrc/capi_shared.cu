@@ -398,7 +398,7 @@ int rtk_verify_drafts(const rtk_tensor *target_logits, const rtk_tensor *draft_t
   p.out_tokens = static_cast<long long *>(tokens_out->data);
   p.accepted = static_cast<int *>(accepted_out->data);
   p.workspace = workspace;
-  const cudaError_t e = rtk::launch_verify(p, 148, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = rtk::launch_verify(p, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "draft verification launch");
   return RTK_OK;
 }

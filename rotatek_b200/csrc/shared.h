@@ -198,6 +198,6 @@ struct VerifyParams {
 int device_sms(int device);
 
 size_t verify_workspace_bytes(long long batch, long long drafts, long long vocab);
-cudaError_t launch_verify(const VerifyParams &p, int sms, cudaStream_t stream);
+cudaError_t launch_verify(const VerifyParams &p, cudaStream_t stream);
 
 }  // namespace rtk

@@ -20,7 +20,6 @@ __global__ void __launch_bounds__(1024 / kQuads) shared_merge_kernel(const Merge
   constexpr int kWarps = 32 / kQuads;
   __shared__ __align__(16) T out_s[32][128 + 8];
   const SharedParams &a = p.s;
-  wait_for_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;    // channel groups warp + kWarps q
   const int u = blockIdx.x / 4, in_unit = (blockIdx.x % 4) * 32;
   const int ph = u / p.split.row_tiles, pre = ph / a.kv_heads, h = ph % a.kv_heads;
@@ -77,22 +76,27 @@ __global__ void __launch_bounds__(1024 / kQuads) shared_merge_kernel(const Merge
       }
     }
   };
+  int prefixes = 0, chunks = 0;
+  long long slot = 0, first = 0;
+  const int row = t * a.groups + g;
   if (live && p.has_prefix) {
     const int c0 = p.split.first_cta(u);
-    const long long slot = u + c0;
-    const float2 *ml = reinterpret_cast<const float2 *>(p.prefix_ml) + slot * 128 + in_unit + lane;
-    const float4 *acc = reinterpret_cast<const float4 *>(p.prefix_acc) + slot * 4096 + in_unit + lane;
-    join(p.split.last_cta(u) - c0 + 1, [&](int i) { return ml + i * 128; },
-         [&](int i, int c4) { return acc + (i * 32ll + c4) * 128; });
+    prefixes = p.split.last_cta(u) - c0 + 1;
+    slot = u + c0;
   }
   if (live && p.has_text) {
-    const int len = min(max(a.lens[b * a.lens_s], 0), a.cap), row = t * a.groups + g;
-    const long long first = ((long long)b * a.kv_heads + h) * p.text_chunks;
-    const float2 *ml = reinterpret_cast<const float2 *>(p.text_ml) + first * p.text_rows + row;
-    const float4 *acc = reinterpret_cast<const float4 *>(p.text_acc) + first * 32 * p.text_rows + row;
-    join((len + p.text_chunk - 1) / p.text_chunk, [&](int i) { return ml + (long long)i * p.text_rows; },
-         [&](int i, int c4) { return acc + (i * 32ll + c4) * p.text_rows; });
+    const int len = min(max(a.lens[b * a.lens_s], 0), a.cap);
+    chunks = (len + p.text_chunk - 1) / p.text_chunk;
+    first = ((long long)b * a.kv_heads + h) * p.text_chunks;
   }
+  wait_for_previous();                               // where the partials are is known by then
+  const float2 *ml_p = reinterpret_cast<const float2 *>(p.prefix_ml) + slot * 128 + in_unit + lane;
+  const float4 *acc_p = reinterpret_cast<const float4 *>(p.prefix_acc) + slot * 4096 + in_unit + lane;
+  join(prefixes, [&](int i) { return ml_p + i * 128; }, [&](int i, int c4) { return acc_p + (i * 32ll + c4) * 128; });
+  const float2 *ml_t = reinterpret_cast<const float2 *>(p.text_ml) + first * p.text_rows + row;
+  const float4 *acc_t = reinterpret_cast<const float4 *>(p.text_acc) + first * 32 * p.text_rows + row;
+  join(chunks, [&](int i) { return ml_t + (long long)i * p.text_rows; },
+       [&](int i, int c4) { return acc_t + (i * 32ll + c4) * p.text_rows; });
   const float inv = l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
   for (int q = 0; q < kQuads; ++q)
@@ -115,121 +119,111 @@ __global__ void __launch_bounds__(1024 / kQuads) shared_merge_kernel(const Merge
   }
 }
 
-// Few units on many SMs: a CTA per row, lane = four channels.  Its four warps take a quarter
-// of the partials each -- their (m, l) 32 at a time, a lane each, their O with eight
-// loads in flight -- and are joined in warp order.
+// Few units on many SMs: a row has many partials.  A CTA takes 8 rows of a unit and 8 groups
+// of four channels; a warp's load is 4 groups of 8 rows (whole lines: a CTA per row, with
+// lane = group, asked for 32 lines per load, and where CTAs crowded on the SMs that the prefix
+// had left free they queued for 5 us).  Two warps side by side, four pairs for every fourth
+// partial each, eight partials in flight; the pairs are joined in order.
+constexpr int kSplitRows = 8, kSplitWays = 4, kSplitDepth = 8;
+
 template <typename T>
-__global__ void __launch_bounds__(128) shared_merge_rows_kernel(const MergeParams p) {
+__global__ void __launch_bounds__(64 * kSplitWays) shared_merge_split_kernel(const MergeParams p) {
+  __shared__ float2 ml_s[kSplitWays][kSplitRows];
+  __shared__ float4 o_s[kSplitWays][64];
   const SharedParams &a = p.s;
-  wait_for_previous();
-  __shared__ float2 ml_s[4];
-  __shared__ float4 o_s[4][32];
-  const long long idx = blockIdx.x;
-  const int lane = threadIdx.x & 31;
-  const int hq = (int)(idx % a.q_heads);
-  const long long bt = idx / a.q_heads;
-  const int t = (int)(bt % a.tokens), b = (int)(bt / a.tokens);
-  const int h = hq / a.groups, g = hq % a.groups;
+  const int lane = threadIdx.x & 31, side = (threadIdx.x >> 5) & 1, way = threadIdx.x >> 6;
+  const int groups = (min(p.split.rows, 128) + kSplitRows - 1) / kSplitRows;      // of rows, in a unit
+  const int c4 = (blockIdx.x & 3) * 8 + side * 4 + (lane >> 3);                   // group of four channels
+  const int u = (int)(blockIdx.x >> 2) / groups, in_unit = (int)(blockIdx.x >> 2) % groups * kSplitRows;
+  const int ph = u / p.split.row_tiles, pre = ph / a.kv_heads, h = ph % a.kv_heads;
+  const int r = (u % p.split.row_tiles) * 128 + in_unit + (lane & 7);
+  const bool live = r < p.split.rows;
+  // row r is head g of token t of question n
+  const int g = r % a.groups, nt = r / a.groups, t = nt % a.tokens, b = pre * a.questions + nt / a.tokens;
 
   // partial i: the prefix's CTAs first, then the text's chunks
   int prefixes = 0, total = 0;
-  long long at_p = 0, at_t = 0, slot0 = 0, text0 = 0, r0 = 0;
-  if (p.has_prefix) {
-    const int pre = b / a.questions, n = b % a.questions;
-    const int r = (n * a.tokens + t) * a.groups + g;
-    const int u = (pre * a.kv_heads + h) * p.split.row_tiles + r / 128;
+  const float2 *ml_p = nullptr, *ml_t = nullptr;
+  const float4 *acc_p = nullptr, *acc_t = nullptr;
+  if (live && p.has_prefix) {
     const int c0 = p.split.first_cta(u);
     prefixes = p.split.last_cta(u) - c0 + 1;
-    slot0 = u + c0;
-    r0 = r % 128;
-    at_p = slot0 * 128 + r0;
+    const long long slot = u + c0;
+    ml_p = reinterpret_cast<const float2 *>(p.prefix_ml) + slot * 128 + r % 128;
+    acc_p = reinterpret_cast<const float4 *>(p.prefix_acc) + (slot * 32 + c4) * 128 + r % 128;
   }
   total = prefixes;
-  if (p.has_text) {
-    const int len = min(max(a.lens[b * a.lens_s], 0), a.cap);
+  if (live && p.has_text) {
+    const int len = min(max(a.lens[b * a.lens_s], 0), a.cap), row = t * a.groups + g;
     total += (len + p.text_chunk - 1) / p.text_chunk;
-    text0 = ((long long)b * a.kv_heads + h) * p.text_chunks;
-    at_t = text0 * p.text_rows + t * a.groups + g;
+    const long long first = ((long long)b * a.kv_heads + h) * p.text_chunks;
+    ml_t = reinterpret_cast<const float2 *>(p.text_ml) + first * p.text_rows + row;
+    acc_t = reinterpret_cast<const float4 *>(p.text_acc) + (first * 32 + c4) * p.text_rows + row;
   }
+  wait_for_previous();
+
   float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  const int warp = threadIdx.x >> 5, quarter = (total + 3) / 4, last = min(total, (warp + 1) * quarter);
-  for (int first = warp * quarter; first < last; first += 32) {
-    const int count = min(32, last - first);
-    float2 ml = make_float2(-INFINITY, 0.f);
-    const float *src = nullptr;
-    int stride = 0;                                   // from one group of four channels to the next
-    if (lane < count) {
-      const int i = first + lane;
+  for (int first = way; first < total; first += kSplitWays * kSplitDepth) {
+    float2 e[kSplitDepth];
+    float4 v[kSplitDepth];
+#pragma unroll
+    for (int k = 0; k < kSplitDepth; ++k) {
+      const int i = first + kSplitWays * k;
+      e[k] = make_float2(-INFINITY, 0.f);
       if (i < prefixes) {
-        ml = __ldcg(reinterpret_cast<const float2 *>(p.prefix_ml) + at_p + i * 128ll);
-        src = p.prefix_acc + ((slot0 + i) * 32 * 128 + r0) * 4;
-        stride = 128 * 4;
-      } else {
-        const long long at = at_t + (long long)(i - prefixes) * p.text_rows;
-        ml = __ldcg(reinterpret_cast<const float2 *>(p.text_ml) + at);
-        src = p.text_acc + ((text0 + i - prefixes) * 32 * p.text_rows + t * a.groups + g) * 4;
-        stride = p.text_rows * 4;
+        e[k] = __ldcg(ml_p + i * 128);
+        v[k] = __ldcg(acc_p + i * 4096ll);
+      } else if (i < total) {
+        e[k] = __ldcg(ml_t + (long long)(i - prefixes) * p.text_rows);
+        v[k] = __ldcg(acc_t + (i - prefixes) * 32ll * p.text_rows);
       }
     }
-    float top = ml.x;
+    float m2 = m;
 #pragma unroll
-    for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-    const float m2 = fmaxf(m, top), base = m2 > -INFINITY ? m2 : 0.f;
-    const float f = fast_exp2(m - base);              // nothing yet: 0
-    float w = fast_exp2(ml.x - base);                 // an empty partial: 0
-    float sum = w > 0.f || isnan(w) ? w * ml.y : 0.f;
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+    for (int k = 0; k < kSplitDepth; ++k) m2 = fmaxf(m2, e[k].x);
+    const float ref = m2 > -INFINITY ? m2 : 0.f;
+    const float f = fast_exp2(m - ref);              // nothing yet: 0
     m = m2;
-    l = fmaf(l, f, sum);
+    l *= f;
     o.x *= f;
     o.y *= f;
     o.z *= f;
     o.w *= f;
-    for (int i = 0; i < count; i += 8) {
-      float4 v[8];
-      float wi[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int from = i + k < count ? i + k : i;
-        wi[k] = __shfl_sync(0xffffffffu, w, from);
-        const float *q = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, reinterpret_cast<long long>(src), from));
-        const int st = __shfl_sync(0xffffffffu, stride, from);
-        if (i + k >= count) wi[k] = 0.f;
-        v[k] = wi[k] != 0.f ? __ldcg(reinterpret_cast<const float4 *>(q + (long long)lane * st)) : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {                   // an empty partial's O was never written
-        o.x = fmaf(wi[k], v[k].x, o.x);
-        o.y = fmaf(wi[k], v[k].y, o.y);
-        o.z = fmaf(wi[k], v[k].z, o.z);
-        o.w = fmaf(wi[k], v[k].w, o.w);
-      }
+    for (int k = 0; k < kSplitDepth; ++k) {
+      const float w = fast_exp2(e[k].x - ref);
+      if (w == 0.f) continue;                        // a partial that saw nothing: its O may be anything
+      l = fmaf(w, e[k].y, l);
+      o.x = fmaf(w, v[k].x, o.x);
+      o.y = fmaf(w, v[k].y, o.y);
+      o.z = fmaf(w, v[k].z, o.z);
+      o.w = fmaf(w, v[k].w, o.w);
     }
   }
-  if (lane == 0) ml_s[warp] = make_float2(m, l);
-  o_s[warp][lane] = o;
+  if (side == 0 && lane < kSplitRows) ml_s[way][lane] = make_float2(isnan(l) ? l : m, l);
+  o_s[way][side * 32 + lane] = o;
   __syncthreads();
-  if (warp > 0) return;
-  float top = m;
+  if (way > 0 || !live) return;
+  float top = -INFINITY;
 #pragma unroll
-  for (int w = 1; w < 4; ++w) top = fmaxf(top, ml_s[w].x);
+  for (int w = 0; w < kSplitWays; ++w) top = fmaxf(top, ml_s[w][lane & 7].x);
+  const float ref = top > -INFINITY ? top : 0.f;
   l = 0.f;
   o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if (!(ml_s[w].x > -INFINITY)) continue;
-    const float f = fast_exp2(ml_s[w].x - top);
-    const float4 v = o_s[w][lane];
-    l = fmaf(f, ml_s[w].y, l);
+  for (int w = 0; w < kSplitWays; ++w) {
+    const float2 e = ml_s[w][lane & 7];
+    const float f = fast_exp2(e.x - ref);            // nothing there: 0
+    const float4 v = o_s[w][side * 32 + lane];
+    l = fmaf(f, e.y, l);
     o.x = fmaf(f, v.x, o.x);
     o.y = fmaf(f, v.y, o.y);
     o.z = fmaf(f, v.z, o.z);
     o.w = fmaf(f, v.w, o.w);
   }
   const float inv = l != 0.f ? 1.f / l : 0.f;
-  T *out = static_cast<T *>(a.out) + b * a.o_s[0] + t * a.o_s[1] + hq * a.o_s[2] + lane * 4 * a.o_s[3];
+  T *out = static_cast<T *>(a.out) + b * a.o_s[0] + t * a.o_s[1] + (h * a.groups + g) * a.o_s[2] + c4 * 4 * a.o_s[3];
   const float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
   if (a.o_s[3] == 1 && reinterpret_cast<uintptr_t>(out) % 8 == 0) {
     *reinterpret_cast<uint2 *>(out) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
@@ -241,12 +235,12 @@ __global__ void __launch_bounds__(128) shared_merge_rows_kernel(const MergeParam
 
 template <typename T>
 cudaError_t launch(const MergeParams &p, cudaStream_t stream) {
+  const int rows = p.split.rows < 128 ? p.split.rows : 128;        // of a unit
+  if (p.split.units * ((rows + 31) / 32) < 96)                     // 32-row CTAs with work
+    return launch_overlapping(shared_merge_split_kernel<T>,
+                              dim3((unsigned)p.split.units * ((rows + kSplitRows - 1) / kSplitRows) * 4),
+                              dim3(64 * kSplitWays), 0, stream, p);
   const dim3 grid((unsigned)p.split.units * 4u);
-  // partials of a row from the prefix: about grid / units
-  if (p.split.grid > 4 * p.split.units) {
-    const long long rows = (long long)p.s.prefixes * p.s.questions * p.s.tokens * p.s.q_heads;
-    return launch_overlapping(shared_merge_rows_kernel<T>, dim3((unsigned)rows), dim3(128), 0, stream, p);
-  }
   return launch_overlapping(shared_merge_kernel<T, 4, 2>, grid, dim3(256), 0, stream, p);
 }
 

@@ -608,9 +608,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
             const float2 e = ml_s[g * 128 + row];
-            if (e.x > -INFINITY) sum = fmaf(e.y, fast_exp2(e.x - ref), sum);
+            sum = fmaf(e.y, e.x > -INFINITY ? fast_exp2(e.x - ref) : 0.f, sum);
           }
-          reinterpret_cast<float2 *>(p.ml)[slot * 128 + row] = make_float2(ref, sum);
+          // a row whose logits are NaN stays one: m NaN, as no weight may drop it
+          reinterpret_cast<float2 *>(p.ml)[slot * 128 + row] = make_float2(isnan(sum) ? sum : ref, sum);
         }
       }
       tc_fence_before();

@@ -1,29 +1,44 @@
 // Shared-prefix attention, the text part: each question's T tokens and G heads of a
 // KV head (rows = T G, few) over that question's own text cache.
 //
-// A question's text belongs to it alone, so its Keys and Values are read once for a
-// handful of rows: the bound is HBM, and the work is cut so that bytes stay in
-// flight.  A CTA takes (question, KV head, a chunk of tokens, up to 16 kRT query rows); its
-// four warps take every fourth block of tokens through cp.async rings of their own
-// (no CTA-wide barrier in the loop), keep (m, l, O) in registers, and meet once at the
-// end.  Per block a warp runs m16n8k16 MMAs: S = Q . K^T with the query rows as M, and
-// O += P . V with P straight out of S's registers.
+//   x_s = c s_k[s] (q . k[s]),  c = log2(e) / sqrt(D);   O = sum 2^(x_s - m) s_v[s] v[s]
+// (s_k, s_v: the scales of 8-bit rows, 1 otherwise), over the tokens that query t sees.
 //
-// 16-bit text: blocks of 16 tokens.  P is rounded to 16 bits, l sums P as rounded.
-// 8-bit text: blocks of 32 tokens, the e4m3 bytes converted in registers to f16
-// (exact).  ldmatrix of Key bytes gives lane (g, j) bytes 4j .. 4j+3 of token g: the
-// MMA's k index runs over a 16-channel group in the order 0 1 4 5 8 9 12 13 2 3 6 7 10 11
-// 14 15, and the queries are stored in that order.  ldmatrix.trans of Value bytes
-// pairs two tokens' bytes of channels (2g, 2g+1): one byte permute separates them into
-// B fragments of an "even" and an "odd" n-tile.  Queries go in as f16 scaled by a
-// power of two per row (bf16 has more range, f16 more bits: exact but for what lies
-// 2^-24 below the row's largest).  A token's Key scale multiplies its logit; its Value
-// scale multiplies its weight relative to the largest Value scale met so far (`vref`),
-// so weights stay within f16 whatever the scales are.
+// A question's text belongs to it alone: its bytes are read once for a handful of rows.  The
+// work is cut into (question, KV head, chunk of tokens), so that bytes stay in flight on every
+// SM, and m16n8k16 MMAs take the rows as M: S = Q . K^T, and O += P . V with P straight out of
+// S's registers.  m follows the maximum lazily (it moves when a maximum is more than 2^8 above
+// it).  Two kernels:
+//
+// - The warps split the rows, 16 each (64 of a CTA), and share tiles of 32 tokens through one
+//   cp.async ring; an 8-bit tile is converted to f16 in shared memory once for all of them.
+// - 8-bit text of at most 16 rows: the warps split the tokens, blocks of 32 in rings of their
+//   own (no CTA-wide barrier in the loop), convert in registers, and join at the end.
+//
+// Measured (the whole attention of a step, prefix of 1064 tokens): 8-bit, 64 questions, 8 heads
+// of 8 rows, up to 4096 tokens 93 us with split tokens, 169 with split rows; 256 questions, 8
+// heads of 4, 512 tokens 74 and 109.  16-bit, the same two 113.8 and 112.8, 80.0 and 75.5: no
+// conversion to share, and the rows' kernel ends with less to join, so 16-bit text always
+// takes that one.  64 rows (64 questions, 8 heads, up to 1001 tokens of 8 bits): 119 us when
+// split by tokens, 16 rows a CTA, 82 by rows.
+//
+// What bounds it: HBM where questions are many and their text 16-bit (537 MB in 84 us, 6.4
+// TB/s); with 8-bit text the conversions and their shuffling (4.1 TB/s); with few questions
+// the latency of a chunk.
+//
+// 8-bit operands: e4m3 is exact in f16.  Queries go in as f16 scaled by a power of two per row
+// (bf16 has more range, f16 more bits: exact but for what lies 2^-24 below the row's largest).
+// A token's Key scale multiplies its logit; its Value scale multiplies its weight relative to
+// the largest Value scale met so far (`vref`), so weights stay within f16 whatever the scales.
+// In registers: ldmatrix of Key bytes gives lane (g, j) bytes 4j .. 4j+3 of token g: the MMA's
+// k index runs over a 16-channel group in the order 0 1 4 5 8 9 12 13 2 3 6 7 10 11 14 15, and
+// the queries are stored in that order.  ldmatrix.trans of Value bytes pairs two tokens' bytes
+// of channels (2g, 2g+1): one byte permute separates them into B fragments of an "even" and
+// an "odd" n-tile.  16-bit operands: P is rounded to 16 bits, l sums P as rounded.
 //
 // Tokens past the length are zero-filled on the way in (cp.async reads nothing there).
 //
-// The kernel may run beside the prefix kernel launched before it (it needs nothing of it);
+// The kernels may run beside the prefix kernel launched before (they need nothing of it);
 // every CTA waits for that one before it ends, so that the join, which waits for this
 // kernel, finds both done.
 #include <type_traits>
@@ -37,18 +52,18 @@ namespace {
 constexpr int kWarps = 4;
 constexpr float kLazy = 8.f;
 
-template <bool FP8, int kRT>
+// ---- the warps split the tokens: 8-bit text of at most 16 rows
 struct TextSmem {
-  static constexpr int kTok = FP8 ? 32 : 16;               // tokens of a block
-  static constexpr int kRow = FP8 ? 128 : 256;             // bytes of a token's Key (or Value)
-  static constexpr int kScales = 2 * kTok * kRow;          // FP8: the tokens' Key scales, Value scales
-  static constexpr int kStage = kScales + (FP8 ? 2 * kTok * 4 : 0);   // 8 KB and the scales
+  static constexpr int kTok = 32;                          // tokens of a block
+  static constexpr int kRow = 128;                         // bytes of a token's Key (or Value)
+  static constexpr int kScales = 2 * kTok * kRow;          // the tokens' Key scales, Value scales
+  static constexpr int kStage = kScales + 2 * kTok * 4;           // 8 KB and the scales
   static constexpr int kStages = 2;
-  static constexpr int kQ = 0;                             // 16 kRT rows of 256 bytes
-  static constexpr int kRing = kQ + kRT * 4096;
+  static constexpr int kQ = 0;                             // 16 rows of 256 bytes
+  static constexpr int kRing = kQ + 4096;
   static constexpr int kBytes = kRing + kWarps * kStages * kStage;
-  // after the loop: O [4][16 kRT][128] and (m, l) [4][16 kRT], over the ring
-  static constexpr int kMerge = kWarps * kRT * 16 * (128 + 2) * 4;
+  // after the loop: O [4][16][128] and (m, l) [4][16], over the ring
+  static constexpr int kMerge = kWarps * 16 * (128 + 2) * 4;
   static_assert(kMerge <= kWarps * kStages * kStage, "merge area");
 };
 
@@ -79,16 +94,15 @@ __device__ __forceinline__ uint32_t e4m3x2_f16x2(uint16_t v) {
   return r;
 }
 
-template <typename T, bool FP8, int kRT>
+template <typename T>
 __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextParams p) {
-  using L = TextSmem<FP8, kRT>;
-  using M = typename std::conditional<FP8, __half, T>::type;   // MMA operand type
+  using L = TextSmem;
   extern __shared__ __align__(1024) unsigned char smem[];
   launch_dependents();
   const SharedParams &a = p.s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, j4 = lane & 3;
-  const int chunk = blockIdx.y, bh = blockIdx.x, row0 = blockIdx.z * 16 * kRT;
+  const int chunk = blockIdx.y, bh = blockIdx.x;
   const int b = bh / a.kv_heads, h = bh % a.kv_heads;
   const int len = min(max(a.lens[b * a.lens_s], 0), a.cap);
   const int t0 = chunk * p.chunk;
@@ -101,14 +115,11 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
 
   // this warp's ring
   unsigned char *ring = smem + L::kRing + warp * L::kStages * L::kStage;
-  const unsigned char *kbase = static_cast<const unsigned char *>(a.kt.data);
-  const unsigned char *vbase = static_cast<const unsigned char *>(a.vt.data);
-  constexpr int kEsize = FP8 ? 1 : 2;
-  kbase += (b * a.kt.s[0] + h * a.kt.s[1]) * kEsize;
-  vbase += (b * a.vt.s[0] + h * a.vt.s[1]) * kEsize;
-  const long long ks = a.kt.s[2] * kEsize, vs = a.vt.s[2] * kEsize;
-  const float *ksc = FP8 ? static_cast<const float *>(a.ksc.data) + b * a.ksc.s[0] + h * a.ksc.s[1] : nullptr;
-  const float *vsc = FP8 ? static_cast<const float *>(a.vsc.data) + b * a.vsc.s[0] + h * a.vsc.s[1] : nullptr;
+  const unsigned char *kbase = static_cast<const unsigned char *>(a.kt.data) + b * a.kt.s[0] + h * a.kt.s[1];
+  const unsigned char *vbase = static_cast<const unsigned char *>(a.vt.data) + b * a.vt.s[0] + h * a.vt.s[1];
+  const long long ks = a.kt.s[2], vs = a.vt.s[2];
+  const float *ksc = static_cast<const float *>(a.ksc.data) + b * a.ksc.s[0] + h * a.ksc.s[1];
+  const float *vsc = static_cast<const float *>(a.vsc.data) + b * a.vsc.s[0] + h * a.vsc.s[1];
   auto fetch = [&](int blk, int stage) {
     unsigned char *dst = ring + stage * L::kStage;
     constexpr int kChunks = L::kRow / 16;
@@ -121,11 +132,10 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
       cp_async_16_zfill(dst + at<L::kRow>(r, c), kbase + (in ? tok * ks + c * 16 : 0), in ? 16 : 0);
       cp_async_16_zfill(dst + L::kTok * L::kRow + at<L::kRow>(r, c), vbase + (in ? tok * vs + c * 16 : 0), in ? 16 : 0);
     }
-    if constexpr (FP8) {                             // lane = token of the block
-      const bool in = first + lane < t1;
-      cp_async_4_zfill(dst + L::kScales + lane * 4, ksc + (in ? (first + lane) * a.ksc.s[2] : 0), in);
-      cp_async_4_zfill(dst + L::kScales + 128 + lane * 4, vsc + (in ? (first + lane) * a.vsc.s[2] : 0), in);
-    }
+    // lane = token of the block
+    const bool in = first + lane < t1;
+    cp_async_4_zfill(dst + L::kScales + lane * 4, ksc + (in ? (first + lane) * a.ksc.s[2] : 0), in);
+    cp_async_4_zfill(dst + L::kScales + 128 + lane * 4, vsc + (in ? (first + lane) * a.vsc.s[2] : 0), in);
   };
 #pragma unroll
   for (int i = 0; i < L::kStages - 1; ++i) {
@@ -133,12 +143,12 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
     cp_async_commit();
   }
 
-  // queries: 16 kRT rows x 128 channels; per-row factor of the logits
-  __shared__ float qscale_s[16 * kRT];
-  uint2 qv[4 * kRT];                                 // all in flight at once
+  // queries: 16 rows x 128 channels; per-row factor of the logits
+  __shared__ float qscale_s[16];
+  uint2 qv[4];                                       // all in flight at once
 #pragma unroll
-  for (int k = 0; k < 4 * kRT; ++k) {
-    const int r = row0 + warp + kWarps * k;
+  for (int k = 0; k < 4; ++k) {
+    const int r = warp + kWarps * k;
     qv[k] = make_uint2(0, 0);                        // channels 4 lane .. 4 lane + 3
     if (r < p.rows) {
       const int t = r / a.groups, gh = r % a.groups;
@@ -147,68 +157,58 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
     }
   }
 #pragma unroll
-  for (int k = 0; k < 4 * kRT; ++k) {
+  for (int k = 0; k < 4; ++k) {
     const int e = warp + kWarps * k;
     const uint2 v = qv[k];
     float f = a.scale_log2;
-    if constexpr (FP8) {
-      float x[4];
-      unpack2<T>(v.x, x[0], x[1]);
-      unpack2<T>(v.y, x[2], x[3]);
-      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        float mx = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+    float x[4];
+    unpack2<T>(v.x, x[0], x[1]);
+    unpack2<T>(v.y, x[2], x[3]);
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      float mx = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        // 2^e with mx / 2^e in [1, 2): the exponent bits of mx (0 and subnormals: 2^-126)
-        const uint32_t ex = min(max(__float_as_uint(mx) >> 23, 1u), 253u);
-        const float inv = __uint_as_float((254u - ex) << 23);
+      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      // 2^e with mx / 2^e in [1, 2): the exponent bits of mx (0 and subnormals: 2^-126)
+      const uint32_t ex = min(max(__float_as_uint(mx) >> 23, 1u), 253u);
+      const float inv = __uint_as_float((254u - ex) << 23);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] *= inv;
-        f *= __uint_as_float(ex << 23);
-      }
-      // channels 4 jj .. 4 jj + 3 of a 16-channel group go to positions 2 jj, 2 jj + 1 and
-      // 2 jj + 8, 2 jj + 9 (lane = 4 * group + jj)
-      const int grp = lane >> 2, jj = lane & 3;
-      const uint32_t q0 = smem_u32(smem + L::kQ);
-      const uint32_t w0 = pack2<__half>(x[0], x[1]), w1 = pack2<__half>(x[2], x[3]);
-      asm volatile("st.shared.b32 [%0], %1;" ::"r"(q0 + at<256>(e, 2 * grp) + jj * 4), "r"(w0) : "memory");
-      asm volatile("st.shared.b32 [%0], %1;" ::"r"(q0 + at<256>(e, 2 * grp + 1) + jj * 4), "r"(w1) : "memory");
-    } else {
-      *reinterpret_cast<uint2 *>(smem + L::kQ + at<256>(e, lane >> 1) + (lane & 1) * 8) = v;
+      for (int i = 0; i < 4; ++i) x[i] *= inv;
+      f *= __uint_as_float(ex << 23);
     }
+    // channels 4 jj .. 4 jj + 3 of a 16-channel group go to positions 2 jj, 2 jj + 1 and
+    // 2 jj + 8, 2 jj + 9 (lane = 4 * group + jj)
+    const int grp = lane >> 2, jj = lane & 3;
+    const uint32_t q0 = smem_u32(smem + L::kQ);
+    const uint32_t w0 = pack2<__half>(x[0], x[1]), w1 = pack2<__half>(x[2], x[3]);
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(q0 + at<256>(e, 2 * grp) + jj * 4), "r"(w0) : "memory");
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(q0 + at<256>(e, 2 * grp + 1) + jj * 4), "r"(w1) : "memory");
     if (lane == 0) qscale_s[e] = f;
   }
   __syncthreads();
 
-  // per query row of this lane (g and g + 8 of each row tile): tokens it sees, logit factor
-  int limit[kRT][2];
-  float qf[kRT][2];
+  // per query row of this lane (g and g + 8): tokens it sees, logit factor
+  int limit[2];
+  float qf[2];
 #pragma unroll
-  for (int rt = 0; rt < kRT; ++rt)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int e = rt * 16 + g + 8 * i, r = row0 + e;
-      limit[rt][i] = r < p.rows ? len - (a.tokens - 1 - r / a.groups) : 0;
-      qf[rt][i] = qscale_s[e];
-    }
+  for (int i = 0; i < 2; ++i) {
+    const int r = g + 8 * i;
+    limit[i] = r < p.rows ? len - (a.tokens - 1 - r / a.groups) : 0;
+    qf[i] = qscale_s[r];
+  }
   const int all_see = len - (a.tokens - 1);          // every row sees tokens below this
 
-  float m[kRT][2], l[kRT][2], acc[kRT][16][4];
+  float m[2], l[2], acc[16][4];
   float vref = 0.f;
 #pragma unroll
-  for (int rt = 0; rt < kRT; ++rt) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      m[rt][i] = -INFINITY;
-      l[rt][i] = 0.f;
-    }
-#pragma unroll
-    for (int n = 0; n < 16; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[rt][n][i] = 0.f;
+  for (int i = 0; i < 2; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
   }
+#pragma unroll
+  for (int n = 0; n < 16; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
   const uint32_t q_lane = smem_u32(smem + L::kQ) + at<256>(lane & 15, lane >> 4);
-  const uint32_t k_at = at<256>((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1), v_at = at<256>(lane & 15, lane >> 4);
 
   int stage = 0;
   for (int blk = warp; blk < blocks; blk += kWarps) {
@@ -225,150 +225,116 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
     cp_async_wait_group<L::kStages - 1>();
     __syncwarp();
     const uint32_t k_addr = smem_u32(ring + stage * L::kStage), v_addr = k_addr + L::kTok * L::kRow;
-
-    if constexpr (FP8) {
-      const unsigned char *sc = ring + stage * L::kStage + L::kScales;
+    const unsigned char *sc = ring + stage * L::kStage + L::kScales;
 #pragma unroll
-      for (int n = 0; n < kNT; ++n) {
-        const float2 k2 = *reinterpret_cast<const float2 *>(sc + (n * 8 + 2 * j4) * 4);
-        const float2 v2 = *reinterpret_cast<const float2 *>(sc + 128 + (n * 8 + 2 * j4) * 4);
-        kscale[n][0] = k2.x; kscale[n][1] = k2.y;
-        vscale[n][0] = v2.x; vscale[n][1] = v2.y;
-      }
-      // the largest Value scale of the block, over the warp
-      float top = 0.f;
+    for (int n = 0; n < kNT; ++n) {
+      const float2 k2 = *reinterpret_cast<const float2 *>(sc + (n * 8 + 2 * j4) * 4);
+      const float2 v2 = *reinterpret_cast<const float2 *>(sc + 128 + (n * 8 + 2 * j4) * 4);
+      kscale[n][0] = k2.x; kscale[n][1] = k2.y;
+      vscale[n][0] = v2.x; vscale[n][1] = v2.y;
+    }
+    // the largest Value scale of the block, over the warp
+    float top = 0.f;
 #pragma unroll
-      for (int n = 0; n < kNT; ++n) top = fmaxf(top, fmaxf(vscale[n][0], vscale[n][1]));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      if (top > vref) {                              // the same in every lane
-        const float f = vref / top;
-        vref = top;
+    for (int n = 0; n < kNT; ++n) top = fmaxf(top, fmaxf(vscale[n][0], vscale[n][1]));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    if (top > vref) {                              // the same in every lane
+      const float f = vref / top;
+      vref = top;
 #pragma unroll
-        for (int rt = 0; rt < kRT; ++rt)
+      for (int n = 0; n < 16; ++n)
 #pragma unroll
-          for (int n = 0; n < 16; ++n)
+        for (int i = 0; i < 4; ++i) acc[n][i] *= f;
+    }
+    const float inv = vref > 0.f ? 1.f / vref : 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[rt][n][i] *= f;
-      }
-      const float inv = vref > 0.f ? 1.f / vref : 0.f;
+    for (int n = 0; n < kNT; ++n) {
+      vscale[n][0] *= inv;
+      vscale[n][1] *= inv;
+    }
+    float s[kNT][4];
 #pragma unroll
-      for (int n = 0; n < kNT; ++n) {
-        vscale[n][0] *= inv;
-        vscale[n][1] *= inv;
-      }
+    for (int n = 0; n < kNT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {                  // 16 channels
+      uint32_t qa[4];
+      ldmatrix_x4(even(q_lane, 2 * k), qa[0], qa[1], qa[2], qa[3]);
+      // four n-tiles of 8 tokens, the 16-byte chunk k of each
+      uint32_t r[4];
+      ldmatrix_x4(k_addr + at<128>(lane, k), r[0], r[1], r[2], r[3]);
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        mma_f16(s[n], qa, e4m3x2_f16x2((uint16_t)(r[n] & 0xffffu)), e4m3x2_f16x2((uint16_t)(r[n] >> 16)));
+    }
+    // logits but for the row's factor; unseen tokens weigh nothing
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < kNT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[n][i] *= kscale[n][i & 1];
+    if (first + L::kTok > all_see) {
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (first + n * 8 + 2 * j4 + (i & 1) >= limit[i >> 1]) s[n][i] = -INFINITY;
     }
 #pragma unroll
-    for (int rt = 0; rt < kRT; ++rt) {
-      float s[kNT][4];
+    for (int n = 0; n < kNT; ++n)
 #pragma unroll
-      for (int n = 0; n < kNT; ++n)
+      for (int i = 0; i < 4; ++i) mx[i >> 1] = fmaxf(mx[i >> 1], s[n][i]);
+    // base-2 maxima of the rows; O and l move to a new one only when it is more than 2^8
+    // above the one in use
+    bool grow[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {                  // 16 channels
-        uint32_t qa[4];
-        ldmatrix_x4(even(q_lane + rt * 4096, 2 * k), qa[0], qa[1], qa[2], qa[3]);
-        if constexpr (FP8) {
-          // four n-tiles of 8 tokens, the 16-byte chunk k of each
-          uint32_t r[4];
-          ldmatrix_x4(k_addr + at<128>(lane, k), r[0], r[1], r[2], r[3]);
-#pragma unroll
-          for (int n = 0; n < 4; ++n)
-            mma_f16(s[n], qa, e4m3x2_f16x2((uint16_t)(r[n] & 0xffffu)), e4m3x2_f16x2((uint16_t)(r[n] >> 16)));
-        } else {
-          // two n-tiles, the chunks 2k and 2k + 1
-          uint32_t r[4];
-          ldmatrix_x4(even(k_addr + k_at, 2 * k), r[0], r[1], r[2], r[3]);
-          mma_16816<T>(s[0], qa, r[0], r[1]);
-          mma_16816<T>(s[1], qa, r[2], r[3]);
-        }
-      }
-      // logits but for the row's factor; unseen tokens weigh nothing
-      float mx[2] = {-INFINITY, -INFINITY};
-      if constexpr (FP8) {
-#pragma unroll
-        for (int n = 0; n < kNT; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[n][i] *= kscale[n][i & 1];
-      }
-      if (first + L::kTok > all_see) {
-#pragma unroll
-        for (int n = 0; n < kNT; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (first + n * 8 + 2 * j4 + (i & 1) >= limit[rt][i >> 1]) s[n][i] = -INFINITY;
-      }
-#pragma unroll
-      for (int n = 0; n < kNT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx[i >> 1] = fmaxf(mx[i >> 1], s[n][i]);
-      // base-2 maxima of the rows; O and l move to a new one only when it is more than 2^8
-      // above the one in use
-      bool grow[2];
+    for (int i = 0; i < 2; ++i) {
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2)) * qf[i];      // qf > 0
+      grow[i] = mx[i] > m[i] + kLazy;          // from -inf: whenever there is a maximum
+    }
+    if (__any_sync(0xffffffffu, grow[0] || grow[1])) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2)) * qf[rt][i];      // qf > 0
-        grow[i] = mx[i] > m[rt][i] + kLazy;          // from -inf: whenever there is a maximum
-      }
-      if (__any_sync(0xffffffffu, grow[0] || grow[1])) {
+        const float f = grow[i] ? fast_exp2(m[i] - mx[i]) : 1.f;      // nothing yet: 2^-inf = 0
+        if (grow[i]) m[i] = mx[i];
+        l[i] *= f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float f = grow[i] ? fast_exp2(m[rt][i] - mx[i]) : 1.f;      // nothing yet: 2^-inf = 0
-          if (grow[i]) m[rt][i] = mx[i];
-          l[rt][i] *= f;
-#pragma unroll
-          for (int n = 0; n < 16; ++n) {
-            acc[rt][n][2 * i] *= f;
-            acc[rt][n][2 * i + 1] *= f;
-          }
+        for (int n = 0; n < 16; ++n) {
+          acc[n][2 * i] *= f;
+          acc[n][2 * i + 1] *= f;
         }
       }
-      const float base[2] = {m[rt][0] > -INFINITY ? m[rt][0] : 0.f, m[rt][1] > -INFINITY ? m[rt][1] : 0.f};
-      uint32_t pa[kNT][2];                           // weights of rows g, g + 8
+    }
+    const float base[2] = {m[0] > -INFINITY ? m[0] : 0.f, m[1] > -INFINITY ? m[1] : 0.f};
+    uint32_t pa[kNT][2];                           // weights of rows g, g + 8
 #pragma unroll
-      for (int n = 0; n < kNT; ++n)
+    for (int n = 0; n < kNT; ++n)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float w0 = fast_exp2(fmaf(s[n][2 * i], qf[rt][i], -base[i]));
-          float w1 = fast_exp2(fmaf(s[n][2 * i + 1], qf[rt][i], -base[i]));
-          if constexpr (FP8) {
-            l[rt][i] += w0 + w1;
-            w0 *= vscale[n][0];
-            w1 *= vscale[n][1];
-            pa[n][i] = pack2<M>(w0, w1);
-          } else {
-            pa[n][i] = pack2<M>(w0, w1);
-            unpack2<M>(pa[n][i], w0, w1);
-            l[rt][i] += w0 + w1;
-          }
-        }
+      for (int i = 0; i < 2; ++i) {
+        float w0 = fast_exp2(fmaf(s[n][2 * i], qf[i], -base[i]));
+        float w1 = fast_exp2(fmaf(s[n][2 * i + 1], qf[i], -base[i]));
+        l[i] += w0 + w1;
+        w0 *= vscale[n][0];
+        w1 *= vscale[n][1];
+        pa[n][i] = pack2<__half>(w0, w1);
+      }
 #pragma unroll
-      for (int kk = 0; kk < kNT / 2; ++kk) {         // 16 tokens
-        const uint32_t pf[4] = {pa[2 * kk][0], pa[2 * kk][1], pa[2 * kk + 1][0], pa[2 * kk + 1][1]};
-        if constexpr (FP8) {
+    for (int kk = 0; kk < kNT / 2; ++kk) {         // 16 tokens
+      const uint32_t pf[4] = {pa[2 * kk][0], pa[2 * kk][1], pa[2 * kk + 1][0], pa[2 * kk + 1][1]};
 #pragma unroll
-          for (int c = 0; c < 8; c += 2) {           // two 16-byte chunks of channels
-            uint32_t r[4];
-            ldmatrix_x4_trans(v_addr + at<128>(kk * 16 + (lane & 15), c + (lane >> 4)), r[0], r[1], r[2], r[3]);
+      for (int c = 0; c < 8; c += 2) {           // two 16-byte chunks of channels
+        uint32_t r[4];
+        ldmatrix_x4_trans(v_addr + at<128>(kk * 16 + (lane & 15), c + (lane >> 4)), r[0], r[1], r[2], r[3]);
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const uint32_t lo = __byte_perm(r[2 * q], 0, 0x3120), hi = __byte_perm(r[2 * q + 1], 0, 0x3120);
-              mma_f16(acc[rt][2 * (c + q)], pf, e4m3x2_f16x2((uint16_t)(lo & 0xffffu)),
-                      e4m3x2_f16x2((uint16_t)(hi & 0xffffu)));
-              mma_f16(acc[rt][2 * (c + q) + 1], pf, e4m3x2_f16x2((uint16_t)(lo >> 16)),
-                      e4m3x2_f16x2((uint16_t)(hi >> 16)));
-            }
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < 16; c += 2) {          // two chunks of 8 channels
-            uint32_t r[4];
-            ldmatrix_x4_trans(even(v_addr + v_at + kk * 4096, c), r[0], r[1], r[2], r[3]);
-            mma_16816<T>(acc[rt][c], pf, r[0], r[1]);
-            mma_16816<T>(acc[rt][c + 1], pf, r[2], r[3]);
-          }
+        for (int q = 0; q < 2; ++q) {
+          const uint32_t lo = __byte_perm(r[2 * q], 0, 0x3120), hi = __byte_perm(r[2 * q + 1], 0, 0x3120);
+          mma_f16(acc[2 * (c + q)], pf, e4m3x2_f16x2((uint16_t)(lo & 0xffffu)),
+                  e4m3x2_f16x2((uint16_t)(hi & 0xffffu)));
+          mma_f16(acc[2 * (c + q) + 1], pf, e4m3x2_f16x2((uint16_t)(lo >> 16)),
+                  e4m3x2_f16x2((uint16_t)(hi >> 16)));
         }
       }
     }
@@ -380,33 +346,24 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
 
   // join the warps, in warp order
   float *o_s = reinterpret_cast<float *>(smem + L::kRing);
-  float2 *ml_s = reinterpret_cast<float2 *>(o_s + kWarps * kRT * 16 * 128);
-  const float scale_o = FP8 ? vref : 1.f;
+  float2 *ml_s = reinterpret_cast<float2 *>(o_s + kWarps * 16 * 128);
 #pragma unroll
-  for (int rt = 0; rt < kRT; ++rt)
+  for (int i = 0; i < 2; ++i) {
+    float ll = l[i];
+    ll += __shfl_xor_sync(0xffffffffu, ll, 1);
+    ll += __shfl_xor_sync(0xffffffffu, ll, 2);
+    const int e = g + 8 * i;
+    if (j4 == 0) ml_s[warp * 16 + e] = make_float2(m[i], ll);
+    float *row = o_s + (warp * 16 + e) * 128;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float ll = l[rt][i];
-      ll += __shfl_xor_sync(0xffffffffu, ll, 1);
-      ll += __shfl_xor_sync(0xffffffffu, ll, 2);
-      const int e = rt * 16 + g + 8 * i;
-      if (j4 == 0) ml_s[warp * kRT * 16 + e] = make_float2(m[rt][i], ll);
-      float *row = o_s + (warp * kRT * 16 + e) * 128;
-      if constexpr (FP8) {
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-          *reinterpret_cast<float4 *>(row + 16 * c + 4 * j4) =
-              make_float4(acc[rt][2 * c][2 * i] * scale_o, acc[rt][2 * c + 1][2 * i] * scale_o,
-                          acc[rt][2 * c][2 * i + 1] * scale_o, acc[rt][2 * c + 1][2 * i + 1] * scale_o);
-      } else {
-#pragma unroll
-        for (int n = 0; n < 16; ++n)
-          *reinterpret_cast<float2 *>(row + 8 * n + 2 * j4) = make_float2(acc[rt][n][2 * i], acc[rt][n][2 * i + 1]);
-      }
-    }
+    for (int c = 0; c < 8; ++c)
+      *reinterpret_cast<float4 *>(row + 16 * c + 4 * j4) =
+          make_float4(acc[2 * c][2 * i] * vref, acc[2 * c + 1][2 * i] * vref,
+                      acc[2 * c][2 * i + 1] * vref, acc[2 * c + 1][2 * i + 1] * vref);
+  }
   __syncthreads();
   // the rows' factors of each warp's partial, over the warps' own (m, l)
-  const int rows = min(p.rows - row0, 16 * kRT);
+  const int rows = p.rows;                           // at most 16
   const long long slot = (long long)bh * p.chunks + chunk;
   if ((int)threadIdx.x < rows) {
     const int e = threadIdx.x;
@@ -414,27 +371,27 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
     float mm = -INFINITY, ll = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      st[w] = ml_s[w * kRT * 16 + e];
+      st[w] = ml_s[w * 16 + e];
       mm = fmaxf(mm, st[w].x);
     }
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float f = st[w].x > -INFINITY ? fast_exp2(st[w].x - mm) : 0.f;
       ll = fmaf(st[w].y, f, ll);
-      ml_s[w * kRT * 16 + e].x = f;
+      ml_s[w * 16 + e].x = f;
     }
-    reinterpret_cast<float2 *>(p.ml)[slot * p.rows + row0 + e] = make_float2(mm, ll);
+    reinterpret_cast<float2 *>(p.ml)[slot * p.rows + e] = make_float2(isnan(ll) ? ll : mm, ll);
   }
   __syncthreads();
-  float4 *out = reinterpret_cast<float4 *>(p.acc) + slot * 32 * p.rows + row0;
+  float4 *out = reinterpret_cast<float4 *>(p.acc) + slot * 32 * p.rows;
   for (int i = threadIdx.x; i < rows * 32; i += 32 * kWarps) {
     const int c4 = i / rows, e = i - c4 * rows;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = ml_s[w * kRT * 16 + e].x;
+      const float f = ml_s[w * 16 + e].x;
       if (f == 0.f) continue;
-      const float4 v = *reinterpret_cast<const float4 *>(o_s + (w * kRT * 16 + e) * 128 + c4 * 4);
+      const float4 v = *reinterpret_cast<const float4 *>(o_s + (w * 16 + e) * 128 + c4 * 4);
       o.x = fmaf(v.x, f, o.x);
       o.y = fmaf(v.y, f, o.y);
       o.z = fmaf(v.z, f, o.z);
@@ -445,10 +402,7 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
   wait_for_previous();
 }
 
-// ---- many rows (T G > 16): the warps of a CTA split the rows, 16 each, and share the
-// tokens, 32 at a time, so that 8-bit text is converted once for 64 rows (converting in
-// every warp's registers cost 3.4 times the instructions: 103 against 36 us for 64
-// questions x 8 heads of 64 rows on up to 1001 tokens).
+// ---- the warps split the rows
 template <bool FP8>
 struct RowsSmem {
   static constexpr int kTok = 32;
@@ -726,7 +680,8 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
       for (int n = 0; n < 16; ++n)
         *reinterpret_cast<float2 *>(out + 8ll * n * p.rows) =
             make_float2(acc[n][2 * i] * scale_o, acc[n][2 * i + 1] * scale_o);
-      if (j4 == 0) reinterpret_cast<float2 *>(p.ml)[slot * p.rows + r] = make_float2(m[i], ll);
+      // NaN logits: m NaN too, as no weight may drop them
+      if (j4 == 0) reinterpret_cast<float2 *>(p.ml)[slot * p.rows + r] = make_float2(isnan(ll) ? ll : m[i], ll);
     }
   }
   wait_for_previous();
@@ -743,28 +698,26 @@ cudaError_t launch_rows(const TextParams &p, cudaStream_t stream) {
   return cudaGetLastError();
 }
 
-template <typename T, bool FP8, int kRT>
-cudaError_t launch(const TextParams &p, cudaStream_t stream) {
-  const int smem = TextSmem<FP8, kRT>::kBytes;
-  cudaError_t e = allow_shared_memory<shared_text_kernel<T, FP8, kRT>>(smem);
+template <typename T>
+cudaError_t launch_few(const TextParams &p, cudaStream_t stream) {
+  cudaError_t e = allow_shared_memory<shared_text_kernel<T>>(TextSmem::kBytes);
   if (e != cudaSuccess) return e;
-  const dim3 grid(p.s.prefixes * p.s.questions * p.s.kv_heads, p.chunks, (p.rows + 16 * kRT - 1) / (16 * kRT));
-  if (p.beside) return launch_overlapping(shared_text_kernel<T, FP8, kRT>, grid, dim3(kWarps * 32), smem, stream, p);
-  shared_text_kernel<T, FP8, kRT><<<grid, kWarps * 32, smem, stream>>>(p);
+  const dim3 grid(p.s.prefixes * p.s.questions * p.s.kv_heads, p.chunks);
+  if (p.beside) return launch_overlapping(shared_text_kernel<T>, grid, dim3(kWarps * 32), TextSmem::kBytes, stream, p);
+  shared_text_kernel<T><<<grid, kWarps * 32, TextSmem::kBytes, stream>>>(p);
   return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t launch_t(const TextParams &p, cudaStream_t stream) {
-  // few rows: the warps split the tokens; more than an MMA's 16: they split the rows
-  if (p.rows <= 16) return p.s.text_fp8 ? launch<T, true, 1>(p, stream) : launch<T, false, 1>(p, stream);
-  return p.s.text_fp8 ? launch_rows<T, true>(p, stream) : launch_rows<T, false>(p, stream);
+cudaError_t launch(const TextParams &p, cudaStream_t stream) {
+  if (!p.s.text_fp8) return launch_rows<T, false>(p, stream);
+  return p.rows <= 16 ? launch_few<T>(p, stream) : launch_rows<T, true>(p, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_shared_text(const TextParams &p, cudaStream_t stream) {
-  return p.s.dtype == 1 ? launch_t<__nv_bfloat16>(p, stream) : launch_t<__half>(p, stream);
+  return p.s.dtype == 1 ? launch<__nv_bfloat16>(p, stream) : launch<__half>(p, stream);
 }
 
 }  // namespace rtk

@@ -249,53 +249,42 @@ __global__ void __launch_bounds__(256) read_any_kernel(const ReadParams p) {
   for (int d = lane; d < p.head_dim; d += 32) y[d * dst.s[3]] = from_f32<T>(e4m3_value(x[d * src.s[3]]) * sc);
 }
 
-// D = 128: 8 threads per row (16 bytes each), kRows rows per thread, 32 kRows tokens of one
-// (question, head) of either cache per CTA.
-template <typename T, int kRows>
+// D = 128: 8 threads per row (16 bytes each), 32 tokens of one (question, head) of either
+// cache per CTA.
+template <typename T>
 __global__ void __launch_bounds__(256) read_rows_kernel(const ReadParams p, int ctas) {
   const int item = blockIdx.x / ctas, part = blockIdx.x % ctas;
   const int side = item & 1, bh = item >> 1, b = bh / p.heads, h = bh % p.heads;
-  const int lane = threadIdx.x & 7, first = part * (32 * kRows) + (threadIdx.x >> 3);
+  const int lane = threadIdx.x & 7, s = part * 32 + (threadIdx.x >> 3);
   const int len = p.lens[b * p.lens_s];
   const SharedTensor &src = p.src[side], &dst = p.dst[side], &scl = p.scale[side];
   const uint8_t *x = static_cast<const uint8_t *>(src.data) + row_offset(src, b, h, 0) + lane * 16;
   const float *sc = static_cast<const float *>(scl.data) + row_offset(scl, b, h, 0);
   T *y = static_cast<T *>(const_cast<void *>(dst.data)) + row_offset(dst, b, h, 0) + lane * 16;
-  uint4 raw[kRows];
-  float scale[kRows];
+  if (s >= p.cap) return;
+  const uint4 raw = s < len ? __ldg(reinterpret_cast<const uint4 *>(x + s * src.s[2])) : make_uint4(0, 0, 0, 0);
+  const float scale = s < len ? __ldg(sc + s * scl.s[2]) : 0.f;
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  float f[16];
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    const int s = first + 32 * i;
-    const bool live = s < len && s < p.cap;
-    raw[i] = live ? __ldg(reinterpret_cast<const uint4 *>(x + s * src.s[2])) : make_uint4(0, 0, 0, 0);
-    scale[i] = live ? __ldg(sc + s * scl.s[2]) : 0.f;
+  for (int k = 0; k < 8; ++k) {
+    uint32_t hh;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hh) : "h"((uint16_t)(w[k >> 1] >> (16 * (k & 1)))));
+    unpack2<__half>(hh, f[2 * k], f[2 * k + 1]);
+    f[2 * k] *= scale;
+    f[2 * k + 1] *= scale;
   }
+  uint4 *to = reinterpret_cast<uint4 *>(y + s * dst.s[2]);
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    const int s = first + 32 * i;
-    if (s >= p.cap) break;
-    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-    float f[16];
+    for (int k = 0; k < 4; ++k)
+      to[k] = make_uint4(__float_as_uint(f[4 * k]), __float_as_uint(f[4 * k + 1]), __float_as_uint(f[4 * k + 2]),
+                         __float_as_uint(f[4 * k + 3]));
+  } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      uint32_t hh;
-      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hh) : "h"((uint16_t)(w[k >> 1] >> (16 * (k & 1)))));
-      unpack2<__half>(hh, f[2 * k], f[2 * k + 1]);
-      f[2 * k] *= scale[i];
-      f[2 * k + 1] *= scale[i];
-    }
-    uint4 *to = reinterpret_cast<uint4 *>(y + s * dst.s[2]);
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        to[k] = make_uint4(__float_as_uint(f[4 * k]), __float_as_uint(f[4 * k + 1]), __float_as_uint(f[4 * k + 2]),
-                           __float_as_uint(f[4 * k + 3]));
-    } else {
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        __stcs(to + k, make_uint4(pack2<T>(f[8 * k], f[8 * k + 1]), pack2<T>(f[8 * k + 2], f[8 * k + 3]),
-                                  pack2<T>(f[8 * k + 4], f[8 * k + 5]), pack2<T>(f[8 * k + 6], f[8 * k + 7])));
-    }
+    for (int k = 0; k < 2; ++k)
+      __stcs(to + k, make_uint4(pack2<T>(f[8 * k], f[8 * k + 1]), pack2<T>(f[8 * k + 2], f[8 * k + 3]),
+                                pack2<T>(f[8 * k + 4], f[8 * k + 5]), pack2<T>(f[8 * k + 6], f[8 * k + 7])));
   }
 }
 
@@ -305,12 +294,9 @@ cudaError_t read(const ReadParams &p, bool rows128, cudaStream_t stream) {
   const int items = 2 * p.batch * p.heads;
   if (!rows128) {
     read_any_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, stream>>>(p);
-  } else if (rows <= 32 * 1024) {                    // few rows: spread them over the SMs
-    const int ctas = (p.cap + 31) / 32;
-    read_rows_kernel<T, 1><<<items * ctas, 256, 0, stream>>>(p, ctas);
   } else {
-    const int ctas = (p.cap + 63) / 64;
-    read_rows_kernel<T, 2><<<items * ctas, 256, 0, stream>>>(p, ctas);
+    const int ctas = (p.cap + 31) / 32;
+    read_rows_kernel<T><<<items * ctas, 256, 0, stream>>>(p, ctas);
   }
   return cudaGetLastError();
 }

@@ -397,8 +397,7 @@ size_t verify_workspace_bytes(long long batch, long long drafts, long long vocab
   return (size_t)(align16(batch * 12) + batch * l.rows * l.chunks * 16);
 }
 
-cudaError_t launch_verify(const VerifyParams &p, int sms, cudaStream_t stream) {
-  (void)sms;
+cudaError_t launch_verify(const VerifyParams &p, cudaStream_t stream) {
   if (p.batch == 0) return cudaSuccess;
   if (p.dtype == 0) return verify<float>(p, stream);
   if (p.dtype == 1) return verify<__nv_bfloat16>(p, stream);

@@ -538,3 +538,43 @@ def test_verify_large_noise_and_tiny_temperature():
     top = a["target_logits"][:, 0].topk(2).values
     clear = (top[:, 0] - top[:, 1]) > 0.01          # e^100 outweighs any noise ratio here
     assert clear.any() and torch.equal(tokens[clear, 0], best[clear])
+
+
+@pytest.mark.parametrize("where", ["q", "k_full", "k_sparse", "k_text", "k_scale", "text alone", "q infinite"])
+@pytest.mark.parametrize("dtype,fp8,T,hq", [(torch.bfloat16, False, 1, 8), (torch.bfloat16, True, 1, 8), (torch.bfloat16, True, 5, 8),
+                                            (torch.float16, False, 5, 8), (torch.float32, False, 2, 8), (torch.bfloat16, False, 1, 80)])
+def test_decode_nan_that_is_seen_comes_out(where, dtype, fp8, T, hq):
+    """A NaN query row or Key makes NaN of every output that it reaches, also where it is all
+    that a row's partial result holds, and of no other."""
+    if where == "k_scale" and not fp8:
+        pytest.skip("no scales")
+    N, hk = 3, 2
+    shape = (1, N, T, hq, hk, 0, 0, 40, 32) if where == "text alone" else (1, N, T, hq, hk, 1500, 70, 40, 32)
+    a = make(*shape, dtype=dtype, fp8=fp8, seed=3, lens=[40, 33, 40])
+    G = hq // hk
+    hit = torch.zeros(N, T, hq, dtype=torch.bool)
+    if where in ("q", "text alone"):
+        a["q"][1, 0, 1, 5] = math.nan
+        hit[1, 0, 1] = True
+    elif where == "q infinite":
+        a["q"][1, 0, 1] = math.inf
+        hit[1, 0, 1] = True
+    elif where in ("k_full", "k_sparse"):
+        a[where][0, 1, 0, 3] = math.nan
+        hit[:, :, G:] = True
+    elif where == "k_scale":
+        a["k_scale"][2, 1, 0] = math.nan
+        hit[2, :, G:] = True
+    else:
+        if fp8:
+            a["k_text"][2, 1, 0, 3] = 0x7f           # e4m3's NaN
+        else:
+            a["k_text"][2, 1, 0, 3] = math.nan
+        hit[2, :, G:] = True
+    from rotatek_b200.kernels import rotatek_shared_decode
+    got = rotatek_shared_decode(**a).cpu().double()
+    assert torch.isnan(got[hit]).all()
+    assert torch.isfinite(got[~hit]).all()
+    want, mag = osh.shared_decode(**a)
+    tol = 1e-4 if dtype == torch.float32 else 2.0 ** -6
+    assert ((got - want).abs()[~hit] <= tol * (1 + mag)[~hit]).all()
