@@ -375,7 +375,7 @@ int rtk_verify_drafts(const rtk_tensor *target_logits, const rtk_tensor *draft_t
                 (draft_logits != nullptr && draft_logits->stride[2] != 1)))
     return fail(RTK_ERR_UNSUPPORTED, "logits and noise need a unit vocabulary stride");
   if (T > 64) return fail(RTK_ERR_UNSUPPORTED, "at most 64 drafted tokens (got %lld)", (long long)T);
-  if (B > 65535 || V > kMaxInt) return fail(RTK_ERR_UNSUPPORTED, "at most 65535 questions and 2^31 - 1 tokens");
+  if (B > 65535 || V > (1 << 30)) return fail(RTK_ERR_UNSUPPORTED, "at most 65535 questions and a vocabulary of 2^30");
   if (B == 0) return RTK_OK;
   for (const rtk_tensor *t : {target_logits, draft_tokens, uniforms, noise, temperature, tokens_out, accepted_out})
     if (!present(t)) return fail(RTK_ERR_INVALID, "a tensor that is not empty has no address");

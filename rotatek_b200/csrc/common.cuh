@@ -176,21 +176,48 @@ __device__ __forceinline__ void launch_dependents() {
 // Wait until the kernel before this one has finished and its writes are visible.
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// Launch that may start while the kernel before it in the stream still runs.
+// Launch that may start while the kernel before it in the stream still runs; `cluster` CTAs
+// along x form a cluster.
 template <typename... Params, typename... Args>
-cudaError_t launch_overlapping(void (*kernel)(Params...), dim3 grid, dim3 block, int smem, cudaStream_t stream,
-                               Args... args) {
+cudaError_t launch_overlapping_clusters(void (*kernel)(Params...), dim3 grid, dim3 block, unsigned cluster, int smem,
+                                        cudaStream_t stream, Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <typename... Params, typename... Args>
+cudaError_t launch_overlapping(void (*kernel)(Params...), dim3 grid, dim3 block, int smem, cudaStream_t stream,
+                               Args... args) {
+  return launch_overlapping_clusters(kernel, grid, block, 1, smem, stream, args...);
+}
+
+// ---------------------------------------------------------------- clusters
+// Arrival (with release) and wait (with acquire) at the cluster's barrier, by every thread.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// Store into the shared memory of the cluster's CTA `rank`, at this CTA's address of the object.
+__device__ __forceinline__ void st_cluster_u64(const void *smem, uint32_t rank, unsigned long long v) {
+  asm volatile(
+      "{\n"
+      ".reg .b32 addr;\n"
+      "mapa.shared::cluster.u32 addr, %0, %1;\n"
+      "st.shared::cluster.b64 [addr], %2;\n"
+      "}" ::"r"(smem_u32(smem)), "r"(rank), "l"(v)
+      : "memory");
 }
 
 // ---------------------------------------------------------------- sync

@@ -3,11 +3,20 @@
 //   out = sum_i f_i O_i / sum_i f_i l_i,   f_i = 2^(m_i - max m),
 // in slot order (the same result every time); a row that saw nothing is 0.
 //
-// Two kernels.  Where rows are many, a CTA takes 32 rows of a prefix unit: lane = row, so
-// that a warp reads four channels of a partial of its unit, or of a question's text, in
-// whole lines; it takes four such groups, so that the weights are worked out once for all
-// four, and two partials in flight; the output goes out through shared memory.  Where
-// rows are few and have many partials (few units on many SMs), a CTA takes a row.
+// Two kernels, both launched while the partials are still being made: what does not depend on
+// them (where a row's partials lie) is worked out before the wait.  Where rows are many, a CTA
+// takes 32 rows of a prefix unit: lane = row, so that a warp reads four channels of a partial
+// of its unit, or of a question's text, in whole lines; it takes four such groups, so that the
+// weights are worked out once for all four, and two partials in flight; the output goes out
+// through shared memory.  Where that would leave SMs idle, CTAs of 8 rows and 32 channels
+// whose warps split the partials.
+//
+// Measured, the whole step with tiles of 32 rows / of 8: 1024 working CTAs of 32 rows 459 /
+// 534 us, 256 of them 75.5 / 93.8, 128: 112.8 / 118.8, 64: 78.3 / 78.6, 32: 44.3 / 40.6, 8:
+// 28.8 (with its indices after the wait) / 20.6.
+//
+// What bounds it: after the last partial, latency (2 to 4 us); with the many rows of the first
+// case its bytes, 43 MB of partials and 8 of output in 19 us, mostly from L2.
 #include "common.cuh"
 #include "shared.h"
 

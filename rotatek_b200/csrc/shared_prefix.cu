@@ -33,8 +33,18 @@
 // What bounds it: with many rows the exponential unit (128 x 128 a block at 16 a cycle: 1024
 // of the 1370 cycles a block takes) and what a warp does between two blocks'
 // exponentials (waiting for S, reading it, its maximum, handing P over); with few
-// rows, HBM.  A quarter or less of the exponentials as polynomials on the FMA units made it
-// slower (373 -> 378 to 404 us).
+// rows, HBM and the latencies at a unit's ends.
+//
+// Measured: 4096 rows of each of 8 heads on 1024 + 31744 tokens 381 us (the exponential unit
+// alone 246, the tensor core 214); 560 rows, 4 prefixes of 4 heads on 640 + 15360 tokens 79;
+// 12 rows, 2 prefixes of 32 heads on 32 + 16384 tokens 63 (344 MB, 5.5 TB/s); 56 rows, 4 heads
+// on 640 + 15360 tokens 13.8; 14 rows, 4 heads on 64 + 1000 tokens 7.7.
+//
+// Taken for the first of these: one softmax group 487 us, two that take turns at the
+// exponential unit 409, P over S and one O so that a third S fits 400, the queries ahead of the
+// ring 381.  Dropped: a sixth to a half of the exponentials as polynomials on the FMA units
+// (378 to 404 where none took 373), three softmax groups (397), four that split a block's
+// columns (402), blocks of 64 visual tokens (490 to 539).
 #include <type_traits>
 
 #include "shared.h"

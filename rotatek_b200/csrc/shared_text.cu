@@ -22,9 +22,9 @@
 // takes that one.  64 rows (64 questions, 8 heads, up to 1001 tokens of 8 bits): 119 us when
 // split by tokens, 16 rows a CTA, 82 by rows.
 //
-// What bounds it: HBM where questions are many and their text 16-bit (537 MB in 84 us, 6.4
-// TB/s); with 8-bit text the conversions and their shuffling (4.1 TB/s); with few questions
-// the latency of a chunk.
+// What bounds it: HBM where questions are many and their text 16-bit (the first case: 537 MB
+// within a step of 113 us, 4.8 TB/s with all that is not text); with 8-bit text the
+// conversions (277 MB within 93 us); with few questions the latency of a chunk.
 //
 // 8-bit operands: e4m3 is exact in f16.  Queries go in as f16 scaled by a power of two per row
 // (bf16 has more range, f16 more bits: exact but for what lies 2^-24 below the row's largest).

@@ -13,8 +13,11 @@
 // it is written, so appending never touches what is already there.
 //
 // Both are bound by HBM.  Rows of 128 channels with 16-byte aligned, unit-stride
-// channels take 16-byte accesses and keep several rows of each thread in flight;
-// anything else takes the scalar kernels below them.
+// channels take 16-byte accesses; anything else takes the scalar kernels below them.
+//
+// Measured: 64 x 8 x up to 577 new bf16 tokens appended, 153 MB, in 41 us (3.7 TB/s); 64 x 8 x
+// 1024 rows read back as fp16, 90 MB in and 268 MB out, in 65 us (5.5 TB/s; a plain fill
+// writes at 3.84 TB/s, so it is the writing that bounds it).
 #include "common.cuh"
 #include "shared.h"
 
@@ -211,10 +214,12 @@ cudaError_t append(const AppendParams &p, bool rows128, cudaStream_t stream) {
   const int items = 2 * p.batch * p.heads;
   if (!rows128) {
     append_any_kernel<T, kQuantize><<<(unsigned)((rows + 7) / 8), 256, 0, stream>>>(p);
-  } else if (rows <= 32 * 1024) {                    // few rows: spread them over the SMs
+  } else if (rows <= 32 * 1024) {
+    // few rows: spread them over the SMs (one token of 8 questions: 2.2 us, 3.1 with four)
     const int ctas = (p.tokens + 31) / 32;
     append_rows_kernel<T, kQuantize, 1><<<items * ctas, 256, 0, stream>>>(p, ctas);
-  } else {                                           // many: four rows of a thread in flight
+  } else {
+    // many: four rows of a thread in flight (the 153 MB: 45 us with one, 41.7 with two, 41.1)
     const int ctas = (p.tokens + 127) / 128;
     append_rows_kernel<T, kQuantize, 4><<<items * ctas, 256, 0, stream>>>(p, ctas);
   }

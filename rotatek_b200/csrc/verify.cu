@@ -15,12 +15,20 @@
 //
 // Two kernels.  stats: a CTA per (row, chunk of the vocabulary) leaves the chunk's
 // maximum and sum of exponentials relative to it (a greedy row: its maximum and where): one
-// pass over every logits row that a decision can read, in 16-byte loads, bound by HBM.
-// pick: CTAs per (question, chunk) join a row's chunks (a warp per row, always in the
-// same tree), find k, and race over row k alone, which the first pass left in L2 or near
-// it; the chunks' winners meet in a 64-bit atomicMax on (value, ~index), whose result does
-// not depend on the order of arrival.  pick is launched while stats still runs and
-// waits for it on the device.
+// pass over every logits row that a decision can read, in 16-byte loads.
+// pick: a cluster of up to 8 CTAs per question joins the rows' chunks (a warp per row, always
+// in the same tree), finds k, and races over row k alone, which the first pass left in L2 or
+// near it; the CTAs' winners, 64-bit keys (value, ~index), meet in the shared memory of the
+// first.  (Through atomics in device memory the end took 1.2 us longer.)  pick is launched
+// while stats still runs and waits for it on the device.
+//
+// Measured, and what bounds it: 128 questions, up to 8 drafts, 131071 bf16 logits, 251 MB in
+// 62.9 us: stats 39 at 4.7 TB/s (the exponential unit alone needs half of that), then
+// 22 for the race, which reads the noise for the first time.  64 questions, up to 5 drafts,
+// 32000 fp16 logits of both models, 37 MB: 20.0 us, 10 each.  One question: 9.0 us, the
+// latency of two dependent kernels.
+#include <type_traits>
+
 #include "common.cuh"
 #include "shared.h"
 
@@ -38,7 +46,9 @@ struct VerifyLayout {
 };
 
 // Chunks of at least 2048 elements (a 16-byte load of each thread), larger where there
-// are enough rows to fill the SMs several times over.
+// are enough rows to fill the SMs several times over: what a CTA does before and after its
+// loads is paid per chunk (the 251 MB above: 199 us with 2048, 67 with 16384, 63 with 65536;
+// 37 MB: 32 and 20).
 __host__ __device__ inline VerifyLayout verify_layout(long long batch, long long drafts, long long vocab) {
   VerifyLayout l;
   l.rows = (int)(2 * drafts + 1);
@@ -46,31 +56,16 @@ __host__ __device__ inline VerifyLayout verify_layout(long long batch, long long
   l.chunk = 2048;
   while (l.chunk < 65536 && total / l.chunk > 148 * 16) l.chunk *= 2;
   l.chunks = (int)((vocab + l.chunk - 1) / l.chunk);
-  // pick: one wave of CTAs, since each of them joins and decides before it races
-  l.race = (int)((batch * vocab / (148 * 4) + 2047) / 2048 * 2048);
-  if (l.race < 2048) l.race = 2048;
-  l.races = (int)((vocab + l.race - 1) / l.race);
+  // pick: one wave of CTAs, since each of them joins and decides before it races (two waves:
+  // 67.5 against 62.9 us at 128 questions); a cluster of 1, 2, 4 or 8 per question (one
+  // question: 10.3 us with 4, 9.0 with 8)
+  l.races = 8;
+  while (l.races > 1 && (batch * l.races > 148 * 4 || vocab < 1024 * l.races)) l.races /= 2;
+  l.race = (int)((vocab + l.races * 64 - 1) / (l.races * 64) * 64);
   return l;
 }
 
-// workspace: [B] race keys, [B] tickets, then
-// float4 (max, sum, argmax bits, -) per (b, row, chunk)
-struct VerifySpace {
-  unsigned long long *key;
-  unsigned int *ticket;
-  float4 *stats;
-};
-
-__host__ __device__ inline long long align16(long long x) { return (x + 15) / 16 * 16; }
-
-__host__ __device__ inline VerifySpace verify_space(void *ws, long long batch) {
-  VerifySpace s;
-  unsigned char *p = static_cast<unsigned char *>(ws);
-  s.key = reinterpret_cast<unsigned long long *>(p);
-  s.ticket = reinterpret_cast<unsigned int *>(s.key + batch);
-  s.stats = reinterpret_cast<float4 *>(p + align16(batch * 12));
-  return s;
-}
+// The workspace holds float4 (max, sum, argmax bits, -) per (b, row, chunk).
 
 __device__ __forceinline__ int drafts_of(const VerifyParams &p, int b) {
   return p.draft_lens != nullptr ? min(max(p.draft_lens[b * p.dl_s], 0), p.drafts) : p.drafts;
@@ -140,13 +135,8 @@ __global__ void __launch_bounds__(kThreads) verify_stats_kernel(const VerifyPara
   __shared__ int i_s[kThreads / 32];
   launch_dependents();
   const VerifyLayout l = verify_layout(p.batch, p.drafts, p.vocab);
-  const VerifySpace ws = verify_space(p.workspace, p.batch);
   const int r = blockIdx.y, b = blockIdx.z, chunk = blockIdx.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (r == 0 && chunk == 0 && threadIdx.x == 0) {
-    ws.key[b] = 0ull;
-    ws.ticket[b] = 0u;
-  }
   const int n = drafts_of(p, b);
   const float heat = p.temperature[b * p.temp_s];
   const bool greedy = !(heat > 0.f);
@@ -222,26 +212,29 @@ __global__ void __launch_bounds__(kThreads) verify_stats_kernel(const VerifyPara
         join(m, z, m_s[w], z_s[w]);
       }
     }
-    ws.stats[((long long)b * l.rows + r) * l.chunks + chunk] = make_float4(m, z, __int_as_float(at), 0.f);
+    static_cast<float4 *>(p.workspace)[((long long)b * l.rows + r) * l.chunks + chunk] = make_float4(m, z, __int_as_float(at), 0.f);
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_pick_kernel(const VerifyParams p) {
+__global__ void __launch_bounds__(kThreads, 4) verify_pick_kernel(const VerifyParams p) {
   __shared__ float m_s[2 * kMaxDrafts + 1], z_s[2 * kMaxDrafts + 1];     // base-2 maximum, 1 / sum
   __shared__ int at_s[kMaxDrafts + 1];
   __shared__ int k_s;
-  __shared__ bool last_s;
   __shared__ unsigned long long key_s[kThreads / 32];
+  __shared__ unsigned long long race_s[8];       // of the cluster's first CTA: every CTA's winner
   const VerifyLayout l = verify_layout(p.batch, p.drafts, p.vocab);
-  const VerifySpace ws = verify_space(p.workspace, p.batch);
   const int b = blockIdx.y, chunk = blockIdx.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n = drafts_of(p, b), T1 = p.drafts + 1;
   const float heat = p.temperature[b * p.temp_s];
   const bool greedy = !(heat > 0.f), soft_draft = p.draft.data != nullptr;
   const float c = greedy ? 1.f : kLog2e / fmaxf(heat, 1e-30f);
-  if (greedy && chunk > 0) return;
+  if (greedy && chunk > 0) return;               // a greedy question's first CTA meets no barrier either
+  const bool clustered = l.races > 1 && !greedy;
+  if (clustered) cluster_arrive();               // this CTA has started: its shared memory is there
+  const int i0 = chunk * l.race, i1 = min(p.vocab, i0 + l.race);
+  const float *noise = p.noise + b * p.noise_s;
   // what an acceptance needs besides the sums: a draft per thread
   const int j = threadIdx.x;
   long long x = -1;
@@ -261,7 +254,7 @@ __global__ void __launch_bounds__(kThreads) verify_pick_kernel(const VerifyParam
   for (int r = warp; r < l.rows; r += kThreads / 32) {
     const bool is_draft = r > p.drafts;
     if (is_draft ? (greedy || !soft_draft || r - T1 >= n) : r > n) continue;
-    const float4 *st = ws.stats + ((long long)b * l.rows + r) * l.chunks;
+    const float4 *st = static_cast<const float4 *>(p.workspace) + ((long long)b * l.rows + r) * l.chunks;
     float m = -INFINITY, z = 0.f;
     int at = 0x7fffffff;
     for (int i = lane; i < l.chunks; i += 32) {
@@ -314,42 +307,58 @@ __global__ void __launch_bounds__(kThreads) verify_pick_kernel(const VerifyParam
   const T *dr = rejected && soft_draft ? logits_row<T>(p, b, T1 + k) : nullptr;
   const long long gone = rejected && !soft_draft ? p.tokens[b * p.tok_s[0] + k * p.tok_s[1]] : -1;
   const int drop = gone >= 0 && gone < p.vocab ? (int)gone : -1;
-  const float *noise = p.noise + b * p.noise_s;
   const float mt = m_s[k], zt = z_s[k], md = dr != nullptr ? m_s[T1 + k] : 0.f, zd = dr != nullptr ? z_s[T1 + k] : 0.f;
-  // this thread's best runner of [i0, i1)
-  auto race = [&](int i0, int i1, bool rest) {
+  // The best runner of [from, to).  About ten instructions a token: without a draft's logits
+  // 1 / z is left out (it scales every runner alike), and a runner's index is looked up only
+  // where a group of kU holds a new best.
+  constexpr int kU = 8;
+  auto race = [&](int from, int to, bool rest) {
     float top = 0.f;
     int who = 0;
     const bool minus = rest && dr != nullptr;
-    const int gone_at = rest ? drop : -1;
-    auto run = [&](int at, float t, float d, float e) {
-      float w = prob(mt, zt, t);
-      if (minus) w -= prob(md, zd, d);
-      if (at == gone_at) w -= 1.f;
-      const float v = __fdividef(w, e);
-      if (v > top) {                                // ascending indices: ties keep the lowest
-        top = v;
-        who = at;
-      }
-    };
-    constexpr int kU = 8;
-    int i = i0 + (int)threadIdx.x;
-    for (; i + (kU - 1) * kThreads < i1; i += kU * kThreads) {
-      float t[kU], d[kU], e[kU];
+    const float ct = mt > -INFINITY ? c : 0.f, cd = md > -INFINITY ? c : 0.f;      // nothing there: 2^-inf
+    const float ot = mt > -INFINITY ? -mt : -INFINITY, od = md > -INFINITY ? -md : -INFINITY;
+    auto group = [&](int i, auto whole) {
+      float t[kU], v[kU];
 #pragma unroll
       for (int q = 0; q < kU; ++q) {
-        t[q] = to_f32(tr[i + q * kThreads]);
-        e[q] = __ldg(noise + i + q * kThreads);
-        d[q] = 0.f;
+        const bool in = whole || i + q * kThreads < to;
+        t[q] = in ? to_f32(tr[i + q * kThreads]) : -INFINITY;
+        v[q] = in ? __ldg(noise + i + q * kThreads) : 1.f;
       }
       if (minus) {
+        float d[kU];
 #pragma unroll
-        for (int q = 0; q < kU; ++q) d[q] = to_f32(dr[i + q * kThreads]);
+        for (int q = 0; q < kU; ++q)
+          d[q] = whole || i + q * kThreads < to ? to_f32(dr[i + q * kThreads]) : -INFINITY;
+#pragma unroll
+        for (int q = 0; q < kU; ++q)
+          v[q] = __fdividef(__fsub_rn(__fmul_rn(fast_exp2(fmaf(t[q], ct, ot)), zt),      // not fused:
+                                      __fmul_rn(fast_exp2(fmaf(d[q], cd, od)), zd)),     // p - p is 0
+                            v[q]);
+      } else {
+#pragma unroll
+        for (int q = 0; q < kU; ++q) v[q] = __fdividef(fast_exp2(fmaf(t[q], ct, ot)), v[q]);
+        // a draft without logits is certain of its token: nothing of p is left there
+        if (rest && (unsigned)(drop - i) <= (kU - 1) * kThreads && (drop - i) % kThreads == 0) {
+#pragma unroll
+          for (int q = 0; q < kU; ++q)
+            if (i + q * kThreads == drop) v[q] = 0.f;
+        }
       }
+      float best = v[0];
 #pragma unroll
-      for (int q = 0; q < kU; ++q) run(i + q * kThreads, t[q], d[q], e[q]);
-    }
-    for (; i < i1; i += kThreads) run(i, to_f32(tr[i]), minus ? to_f32(dr[i]) : 0.f, __ldg(noise + i));
+      for (int q = 1; q < kU; ++q) best = fmaxf(best, v[q]);
+      if (best > top) {                             // groups ascend: ties keep the lowest index
+        top = best;
+#pragma unroll
+        for (int q = kU - 1; q >= 0; --q)
+          if (v[q] == best) who = i + q * kThreads;
+      }
+    };
+    int i = from + (int)threadIdx.x;
+    for (; i + (kU - 1) * kThreads < to; i += kU * kThreads) group(i, std::true_type{});
+    if (i < to) group(i, std::false_type{});
     unsigned long long best = top > 0.f ? race_key(top, (unsigned)who) : 0ull;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
@@ -361,18 +370,20 @@ __global__ void __launch_bounds__(kThreads) verify_pick_kernel(const VerifyParam
   };
   long long next = at_s[greedy ? k : 0];
   if (!greedy) {
-    const unsigned long long mine = race(chunk * l.race, min(p.vocab, (chunk + 1) * l.race), rejected);
-    if (threadIdx.x == 0) {
-      if (mine != 0ull) atomicMax(&ws.key[b], mine);
-      __threadfence();
-      last_s = atomicAdd(&ws.ticket[b], 1u) == (unsigned)l.races - 1u;
+    unsigned long long key = race(i0, i1, rejected);
+    if (clustered) {                               // the winners meet in the first CTA
+      cluster_wait();
+      if (threadIdx.x == 0) st_cluster_u64(&race_s[chunk], 0, key);
+      __syncwarp();
+      cluster_arrive();
+      cluster_wait();
+      if (chunk > 0) return;
+      for (int w = 1; w < l.races; ++w) key = max(key, race_s[w]);
     }
-    __syncthreads();
-    if (!last_s) return;
-    // the question's last CTA writes the answer
-    __threadfence();
-    unsigned long long key = __ldcg(&ws.key[b]);
-    if (key == 0ull && rejected) key = race(0, p.vocab, false);   // p - q left nothing: draw from p
+    if (key == 0ull && rejected) {                 // p - q left nothing: draw from p
+      __syncthreads();
+      key = race(0, p.vocab, false);
+    }
     next = key == 0ull ? 0 : (long long)(0xffffffffu - (unsigned)(key & 0xffffffffull));
   }
   for (int i = threadIdx.x; i < T1; i += kThreads)
@@ -387,14 +398,14 @@ cudaError_t verify(const VerifyParams &p, cudaStream_t stream) {
   verify_stats_kernel<T><<<dim3(l.chunks, rows, p.batch), kThreads, 0, stream>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  return launch_overlapping(verify_pick_kernel<T>, dim3(l.races, p.batch), dim3(kThreads), 0, stream, p);
+  return launch_overlapping_clusters(verify_pick_kernel<T>, dim3(l.races, p.batch), dim3(kThreads), l.races, 0, stream, p);
 }
 
 }  // namespace
 
 size_t verify_workspace_bytes(long long batch, long long drafts, long long vocab) {
   const VerifyLayout l = verify_layout(batch, drafts, vocab);
-  return (size_t)(align16(batch * 12) + batch * l.rows * l.chunks * 16);
+  return (size_t)(batch * l.rows * l.chunks * 16);
 }
 
 cudaError_t launch_verify(const VerifyParams &p, cudaStream_t stream) {
