@@ -15,7 +15,7 @@
 // Both are bound by HBM.  Rows of 128 channels with 16-byte aligned, unit-stride
 // channels take 16-byte accesses; anything else takes the scalar kernels below them.
 //
-// Measured: 64 x 8 x up to 577 new bf16 tokens appended, 153 MB, in 41 us (3.7 TB/s); 64 x 8 x
+// Measured: 64 x 8 x up to 577 new bf16 tokens appended, 153 MB, in 34.5 us (4.4 TB/s); 64 x 8 x
 // 1024 rows read back as fp16, 90 MB in and 268 MB out, in 65 us (5.5 TB/s; a plain fill
 // writes at 3.84 TB/s, so it is the writing that bounds it).
 #include "common.cuh"
@@ -42,11 +42,20 @@ __device__ __forceinline__ float finite_abs(float x) {
 }
 
 __device__ __forceinline__ float row_scale(float amax) {
-  return amax > 0.f ? fmaxf(__fdiv_rn(amax, kE4m3Max), 1.17549435e-38f) : 1.f;
+  // amax / 448 rounded to nearest, as the quotients below (exact remainder down to 2^-126)
+  const float r = 1.f / kE4m3Max, q = amax * r;
+  return amax > 0.f ? fmaxf(fmaf(-fmaf(q, kE4m3Max, -amax), r, q), 1.17549435e-38f) : 1.f;
 }
 
 __device__ __forceinline__ long long row_offset(const SharedTensor &x, int b, int h, int s) {
   return b * x.s[0] + h * x.s[1] + s * x.s[2];
+}
+
+// the larger, NaN if either is
+__device__ __forceinline__ float larger(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
 }
 
 // 16 channels of a row (32 or 64 bytes)
@@ -62,25 +71,25 @@ struct Sixteen {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) reinterpret_cast<uint4 *>(dst)[i] = raw[i];
   }
-  // the largest |x|, NaN passed over (16-bit types two at a time)
+  // the largest |x|, NaN if there is one (16-bit types two at a time)
   __device__ __forceinline__ float amax() const {
     if constexpr (sizeof(T) == 4) {
       float m = 0.f;
 #pragma unroll
       for (int i = 0; i < kWords; ++i)
-        m = fmaxf(m, fmaxf(fmaxf(fabsf(__uint_as_float(raw[i].x)), fabsf(__uint_as_float(raw[i].y))),
-                           fmaxf(fabsf(__uint_as_float(raw[i].z)), fabsf(__uint_as_float(raw[i].w)))));
+        m = larger(m, larger(larger(fabsf(__uint_as_float(raw[i].x)), fabsf(__uint_as_float(raw[i].y))),
+                             larger(fabsf(__uint_as_float(raw[i].z)), fabsf(__uint_as_float(raw[i].w)))));
       return m;
     } else {
       using T2 = typename std::conditional<std::is_same<T, __nv_bfloat16>::value, __nv_bfloat162, __half2>::type;
       auto h2 = [](uint32_t w) { return __habs2(*reinterpret_cast<const T2 *>(&w)); };
-      T2 m = __hmax2(h2(raw[0].x), h2(raw[1].x));
-      m = __hmax2(m, __hmax2(h2(raw[0].y), h2(raw[1].y)));
-      m = __hmax2(m, __hmax2(h2(raw[0].z), h2(raw[1].z)));
-      m = __hmax2(m, __hmax2(h2(raw[0].w), h2(raw[1].w)));
+      T2 m = __hmax2_nan(h2(raw[0].x), h2(raw[1].x));
+      m = __hmax2_nan(m, __hmax2_nan(h2(raw[0].y), h2(raw[1].y)));
+      m = __hmax2_nan(m, __hmax2_nan(h2(raw[0].z), h2(raw[1].z)));
+      m = __hmax2_nan(m, __hmax2_nan(h2(raw[0].w), h2(raw[1].w)));
       float lo, hi;
       unpack2<T>(*reinterpret_cast<const uint32_t *>(&m), lo, hi);
-      return fmaxf(fmaxf(lo, hi), 0.f);              // all NaN: 0
+      return larger(lo, hi);
     }
   }
   __device__ __forceinline__ void floats(float (&f)[16]) const {
@@ -96,22 +105,24 @@ struct Sixteen {
   }
 };
 
-// x / s rounded to nearest for finite numbers, given r = 1 / s rounded to nearest: q = x r,
-// q - (q s - x) r (Markstein 1990: correctly rounded while the remainder q s - x is
-// exact, which s >= 2^-80 grants for every quotient that e4m3 does not round to 0).
-// Written with the remainder negated, -0 stays -0.
-__device__ __forceinline__ float divide(float x, float s, float r) {
-  const float q = x * r;
-  return fmaf(-fmaf(q, s, -x), r, q);
+// -(x / s), each rounded to nearest, for two finite numbers and r = 1 / s rounded to nearest:
+// with q = x r it is -q - (x - q s) r (Markstein 1990: correctly rounded while the remainder
+// x - q s is exact, which s >= 2^-80 grants for every quotient that e4m3 does not round to 0).
+// Negated, because then every step is a fused multiply-add of what is there already, and -0
+// comes out as what it should be: the sign is put right in the packed bytes.
+__device__ __forceinline__ float2 minus_quotient(float2 x, float s, float r) {
+  const float2 q = __fmul2_rn(x, make_float2(-r, -r));
+  return __ffma2_rn(__ffma2_rn(q, make_float2(s, s), x), make_float2(-r, -r), q);
 }
 
 // D = 128: 8 threads per row of 16 channels each, kRows rows per thread.  A CTA takes
 // 32 kRows tokens of one head of one question's Keys or Values.  What it costs besides the
-// bytes is about ten instructions a channel (unpacking, the maximum, four for the
-// division, the conversion): 16 channels a thread so that the row's scale and its
-// reciprocal are worked out by 8 threads and not by 16.
+// bytes is a dozen instructions a channel (unpacking, the maximum, two to divide, the
+// conversion, the row's scale): 16 channels a thread so that the scale and its reciprocal are
+// worked out by 8 threads and not by 16, and five CTAs an SM (the 153 MB above: 41 us with one
+// quotient at a time and three CTAs, 39 with two, 37 with four CTAs, 34.5 with five).
 template <typename T, bool kQuantize, int kRows>
-__global__ void __launch_bounds__(256) append_rows_kernel(const AppendParams p, int ctas) {
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 5) append_rows_kernel(const AppendParams p, int ctas) {
   const int lane = threadIdx.x & 7;
   const int item = blockIdx.x / ctas, part = blockIdx.x % ctas;
   const int side = item & 1, bh = item >> 1, b = bh / p.heads, h = bh % p.heads;
@@ -129,8 +140,10 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const AppendParams p, 
     const int t = first + 32 * i;
     if (t < count && t + len >= 0) x[i].load(from + t * src.s[2]);
   }
+  const int last = count - ((threadIdx.x & ~31) >> 3);      // of this warp's first row
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
+    if (part * (32 * kRows) + 32 * i >= last) break;         // no row of this warp is there
     const int t = first + 32 * i;
     const bool live = t < count && t + len >= 0;
     const long long to = base + (long long)(len + t) * dst.s[2];
@@ -145,8 +158,8 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const AppendParams p, 
     float f[16];
     x[i].floats(f);
     float mx = x[i].amax();
-    const bool infinite = !(mx < INFINITY);
-    if (infinite) {
+    const bool finite = mx < INFINITY;
+    if (!finite) {
       mx = 0.f;
 #pragma unroll
       for (int k = 0; k < 16; ++k) mx = fmaxf(mx, finite_abs(f[k]));
@@ -154,10 +167,16 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const AppendParams p, 
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     const float sc = row_scale(mx);
-    if (!infinite && sc >= 8.2718061e-25f) {
+    uint32_t flip = 0u;
+    if (finite && sc >= 8.2718061e-25f) {
       const float r = __frcp_rn(sc);
+      flip = 0x80808080u;
 #pragma unroll
-      for (int k = 0; k < 16; ++k) f[k] = divide(f[k], sc, r);
+      for (int k = 0; k < 16; k += 2) {
+        const float2 y = minus_quotient(make_float2(f[k], f[k + 1]), sc, r);
+        f[k] = y.x;
+        f[k + 1] = y.y;
+      }
     } else {
 #pragma unroll
       for (int k = 0; k < 16; ++k) f[k] = __fdiv_rn(f[k], sc);
@@ -165,7 +184,7 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const AppendParams p, 
     uint32_t o[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      o[k] = (uint32_t)e4m3x2(f[4 * k], f[4 * k + 1]) | ((uint32_t)e4m3x2(f[4 * k + 2], f[4 * k + 3]) << 16);
+      o[k] = ((uint32_t)e4m3x2(f[4 * k], f[4 * k + 1]) | ((uint32_t)e4m3x2(f[4 * k + 2], f[4 * k + 3]) << 16)) ^ flip;
     if (live) {
       *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(const_cast<void *>(dst.data)) + to) =
           make_uint4(o[0], o[1], o[2], o[3]);
@@ -219,9 +238,9 @@ cudaError_t append(const AppendParams &p, bool rows128, cudaStream_t stream) {
     const int ctas = (p.tokens + 31) / 32;
     append_rows_kernel<T, kQuantize, 1><<<items * ctas, 256, 0, stream>>>(p, ctas);
   } else {
-    // many: four rows of a thread in flight (the 153 MB: 45 us with one, 41.7 with two, 41.1)
-    const int ctas = (p.tokens + 127) / 128;
-    append_rows_kernel<T, kQuantize, 4><<<items * ctas, 256, 0, stream>>>(p, ctas);
+    // many: three rows of a thread in flight (the 153 MB: 37 us with four, 39 with two)
+    const int ctas = (p.tokens + 95) / 96;
+    append_rows_kernel<T, kQuantize, 3><<<items * ctas, 256, 0, stream>>>(p, ctas);
   }
   return cudaGetLastError();
 }
