@@ -68,20 +68,20 @@ struct PrefixSplit {
   int rows;                  // N T G query rows of a (prefix, KV head)
   int row_tiles;             // ceil(rows / 128)
   int units;                 // P H_kv row_tiles
-  int blocks_full, blocks_vis, unit_weight;   // unit_weight counts kUnitStart too
+  int blocks_full, blocks_vis;
+  int unit_start;            // weight of a unit's start and end (queries, rotation, partial result)
+  int unit_weight;           // of a unit, its start included
   long long total;           // units * unit_weight
   int grid;
-
-  static constexpr int kUnitStart = 2;        // weight of starting a unit (its queries)
 
   __host__ __device__ int blocks() const { return blocks_full + blocks_vis; }
   // weight at which block j of a unit starts
   __host__ __device__ int block_start(int j) const {
-    return kUnitStart + (j < blocks_full ? j : blocks_full + 2 * (j - blocks_full));
+    return unit_start + (j < blocks_full ? j : blocks_full + 2 * (j - blocks_full));
   }
   // first block of a unit that starts at weight >= w
   __host__ __device__ int block_from(int w) const {
-    w -= kUnitStart;
+    w -= unit_start;
     if (w <= 0) return 0;
     if (w <= blocks_full) return w;
     const int j = blocks_full + (w - blocks_full + 1) / 2;
@@ -92,7 +92,7 @@ struct PrefixSplit {
   __host__ __device__ int owner(long long w) const { return (int)(((w + 1) * grid - 1) / total); }
   // CTAs that hold blocks of unit u.  Ranges are at least 2 long and block starts
   // at most 2 apart, so every CTA from the first to the last holds one.
-  __host__ __device__ int first_cta(int u) const { return owner((long long)u * unit_weight + kUnitStart); }
+  __host__ __device__ int first_cta(int u) const { return owner((long long)u * unit_weight + unit_start); }
   __host__ __device__ int last_cta(int u) const {
     return owner((long long)u * unit_weight + block_start(blocks() - 1));
   }
@@ -108,12 +108,20 @@ inline PrefixSplit prefix_split(long long prefixes, long long questions, long lo
   s.units = (int)(prefixes * kv_heads * s.row_tiles);
   s.blocks_full = (int)((seq_full + 63) / 64);
   s.blocks_vis = (int)((seq_sparse + 127) / 128);
-  s.unit_weight = PrefixSplit::kUnitStart + s.blocks_full + 2 * s.blocks_vis;
-  s.total = (long long)s.units * s.unit_weight;
+  const long long weight = s.blocks_full + 2 * s.blocks_vis, all = s.units * weight;
   // Ranges of a few blocks: a quarter of the SMs is left to the text kernel, which then runs
   // beside this one instead of after it (8 questions on 16000 tokens: 20.6 us, 23.0 on all
   // SMs; ranges of many blocks cannot spare them: 123 us against 107, 562 against 462).
-  if (text_cap > 0 && s.total < 16ll * sms) sms = sms - sms / 4;
+  if (text_cap > 0 && all < 16ll * sms) sms = sms - sms / 4;
+  // A unit's start and end take 6 to 10 thousand cycles, where a block of 128 rows (weight 2)
+  // takes 1400 and one of few rows half of that: CTAs that meet a second unit get fewer blocks,
+  // though not none.  (Weight 2 / 8 / 16: the prefix and its text in 20.6 / 18.9 / 19.2 us for
+  // 56 rows of 4 heads with ranges of 9, 107 / 106 / 104 for 80 units of up to 128 rows, 78.3 /
+  // 76.7 / 77.3 for 64 of 12; 16 units with ranges of 2 13.5 / - / 14.5.)
+  const long long range = all / sms;
+  s.unit_start = (int)(range < 2 ? 2 : range > 16 ? 16 : range);
+  s.unit_weight = (int)weight + s.unit_start;
+  s.total = (long long)s.units * s.unit_weight;
   s.grid = (int)(s.total / 2 < sms ? (s.total / 2 > 0 ? s.total / 2 : 1) : sms);
   return s;
 }
