@@ -113,7 +113,7 @@ def calls():
                 except ImportError as e:
                     raise RuntimeError("rotatek_b200/_calls.so is missing; build it with "
                                        "`python -m rotatek_b200.csrc.build`") from e
-                mod.bind(_lib._name, _DTYPES)
+                mod.bind(_lib._name, _DTYPES, torch.Tensor)
                 _calls = mod
     return _calls
 

@@ -13,6 +13,7 @@ points without ctypes.
 from __future__ import annotations
 
 import argparse
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -58,12 +59,13 @@ def build(verbose: bool = False, out_dir: str = PKG) -> str:
 
 
 def build_calls(out_dir: str = PKG) -> str:
-    """The Python module of direct calls: a C file against Python.h alone."""
+    """The Python module of direct calls: a C file against Python.h and torch's copy of dlpack.h."""
     out = os.path.join(out_dir, CALLS_NAME)
     cc = os.environ.get("CC") or shutil.which("gcc") or shutil.which("cc")
     if cc is None:
         raise RuntimeError("no C compiler found (set CC)")
     subprocess.run([cc, "-O2", "-std=c11", "-Wall", "-shared", "-fPIC", "-I", sysconfig.get_paths()["include"],
+                    "-I", os.path.join(importlib.util.find_spec("torch").submodule_search_locations[0], "include"),
                     os.path.join(CSRC, "calls.c"), "-o", out + ".tmp", "-ldl"], check=True)
     os.replace(out + ".tmp", out)
     return out

@@ -3,9 +3,9 @@
  *
  * A ctypes call spends ~1.7 us on every tensor's descriptor (a struct filled from
  * Python), 26 us for the fifteen tensors of a shared decode whose kernels take 14 us.
- * Here the descriptors are filled in C from the tensors' own attributes (get_device,
- * data_ptr, dtype, shape, stride: ~0.3 us each) and the C ABI function, found in the
- * already loaded librotatek_b200.so, is called directly.
+ * Here the descriptors are filled in C, through DLPack's C exchange API, or where a tensor
+ * has none from its attributes (get_device, data_ptr, dtype, shape, stride: ~0.3 us each),
+ * and the C ABI function, found in the already loaded librotatek_b200.so, is called directly.
  *
  * Each function takes the C ABI's tensors in its order (None for a nullable one), then
  * its integers (addresses as integers), and returns the status code, or -1 when a
@@ -14,6 +14,8 @@
 #include <Python.h>
 #include <dlfcn.h>
 #include <string.h>
+
+#include <ATen/dlpack.h>
 
 #include "../../include/rotatek_b200.h"
 
@@ -54,6 +56,45 @@ static int dims_of(PyObject *tuple, int64_t *out, int32_t *ndim) {
   for (Py_ssize_t i = 0; i < n; ++i)
     if (!as_int(PyTuple_GET_ITEM(tuple, i), &out[i])) return 0;
   *ndim = (int32_t)n;
+  return 1;
+}
+
+/* DLPack's C exchange API of torch.Tensor: a tensor's address, type, shape and strides as one
+ * C call that makes no Python object (the attributes below take seven).  NULL where this torch
+ * has none. */
+static const DLPackExchangeAPI *exchange;
+static PyTypeObject *tensor_type;
+
+static int dtype_of(DLDataType t) {
+  if (t.lanes != 1) return -1;
+  if (t.code == kDLFloat) return t.bits == 32 ? RTK_F32 : t.bits == 16 ? RTK_F16 : -1;
+  if (t.code == kDLBfloat) return t.bits == 16 ? RTK_BF16 : -1;
+  if (t.code == kDLInt) return t.bits == 32 ? RTK_I32 : t.bits == 64 ? RTK_I64 : -1;
+  if (t.code == kDLUInt) return t.bits == 8 ? RTK_U8 : -1;
+  return -1;
+}
+
+/* Descriptor by the exchange API: 1 done, 0 not possible this way (no exception is set). */
+static int describe_fast(PyObject *t, rtk_tensor *d, int64_t *device) {
+  DLTensor x;
+  if (exchange == NULL || Py_TYPE(t) != tensor_type) return 0;
+  if (exchange->dltensor_from_py_object_no_sync(t, &x) != 0) {
+    PyErr_Clear();
+    return 0;
+  }
+  if (x.ndim > 4 || (x.ndim > 0 && (x.shape == NULL || x.strides == NULL))) return 0;
+  if (x.device.device_type != kDLCUDA || (*device != -2 && x.device.device_id != *device)) {
+    *device = -1;
+    return 1;
+  }
+  *device = x.device.device_id;
+  d->data = (char *)x.data + x.byte_offset;
+  d->dtype = dtype_of(x.dtype);
+  d->ndim = x.ndim;
+  for (int i = 0; i < x.ndim; ++i) {
+    d->shape[i] = x.shape[i];
+    d->stride[i] = x.strides[i];
+  }
   return 1;
 }
 
@@ -107,7 +148,7 @@ static int parse(PyObject *const *args, Py_ssize_t nargs, int nt, int ni, rtk_te
     t[i] = NULL;
     if (args[i] == Py_None) continue;
     memset(&mem[i], 0, sizeof(mem[i]));
-    if (!describe(args[i], &mem[i], &device)) return 0;
+    if (!describe_fast(args[i], &mem[i], &device) && !describe(args[i], &mem[i], &device)) return 0;
     if (device < 0) return -1;
     t[i] = &mem[i];
   }
@@ -177,9 +218,9 @@ static int find(void *lib, const char *name, void *slot) {
 
 static PyObject *py_bind(PyObject *self, PyObject *args) {
   const char *path;
-  PyObject *codes, *key, *value;
+  PyObject *codes, *key, *value, *type;
   Py_ssize_t pos = 0;
-  if (!PyArg_ParseTuple(args, "sO!", &path, &PyDict_Type, &codes)) return NULL;
+  if (!PyArg_ParseTuple(args, "sO!O!", &path, &PyDict_Type, &codes, &PyType_Type, &type)) return NULL;
   void *lib = dlopen(path, RTLD_NOW | RTLD_LOCAL);
   if (lib == NULL) {
     PyErr_SetString(PyExc_RuntimeError, dlerror());
@@ -196,11 +237,21 @@ static PyObject *py_bind(PyObject *self, PyObject *args) {
   if (!find(lib, "rtk_shared_decode", &f_shared_decode) || !find(lib, "rtk_append_text", &f_append_text) ||
       !find(lib, "rtk_read_text", &f_read_text) || !find(lib, "rtk_verify_drafts", &f_verify_drafts))
     return NULL;
+  PyObject *capsule = PyObject_GetAttrString(type, "__dlpack_c_exchange_api__");
+  const DLPackExchangeAPI *api =
+      capsule != NULL ? (const DLPackExchangeAPI *)PyCapsule_GetPointer(capsule, "dlpack_exchange_api") : NULL;
+  Py_XDECREF(capsule);                          /* the type keeps it */
+  PyErr_Clear();
+  if (api != NULL && api->header.version.major == DLPACK_MAJOR_VERSION) {
+    Py_INCREF(type);
+    tensor_type = (PyTypeObject *)type;
+    exchange = api;
+  }
   Py_RETURN_NONE;
 }
 
 static PyMethodDef methods[] = {
-    {"bind", py_bind, METH_VARARGS, "bind(path of librotatek_b200.so, {torch dtype: rtk_dtype})"},
+    {"bind", py_bind, METH_VARARGS, "bind(path of librotatek_b200.so, {torch dtype: rtk_dtype}, torch.Tensor)"},
     {"shared_decode", (PyCFunction)(void (*)(void))py_shared_decode, METH_FASTCALL, "rtk_shared_decode"},
     {"append_text", (PyCFunction)(void (*)(void))py_append_text, METH_FASTCALL, "rtk_append_text"},
     {"read_text", (PyCFunction)(void (*)(void))py_read_text, METH_FASTCALL, "rtk_read_text"},
