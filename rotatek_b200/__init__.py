@@ -7,6 +7,13 @@ Same Python surface as the reference package ``rotatek``:
     kernels.rotatek_decode         decode over rotated-truncated visual Keys
     kernels.full_channel_decode    full-width split-K decode
 
+and, for many questions on shared images with drafted tokens (no counterpart there),
+
+    kernels.rotatek_shared_decode  attention of all questions over one prefix and their text
+    kernels.append_text, read_text text caches quantised as they are written, and read back
+    kernels.verify_drafts          which drafted tokens stand, and the token that follows
+    cache.SharedPrefixCache        the caches of such a batch
+
 backed by the hand-written CUDA kernels of ``librotatek_b200.so`` (C ABI:
 include/rotatek_b200.h).  There is no Triton and no CPU fallback.
 """

@@ -488,7 +488,7 @@ def verify_drafts(
                                  draft_lens=draft_lens)
     b, rows, vocab = target_logits.shape
     calls = _lib.calls()
-    tokens = torch.empty((b, rows), dtype=torch.int64, device=dev)
+    tokens = draft_tokens.new_empty((b, rows))
     accepted = torch.empty_like(temperature, dtype=torch.int32, memory_format=torch.contiguous_format)
     stream = _lib.raw_stream(dev)
     need = 0
