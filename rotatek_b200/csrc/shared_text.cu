@@ -38,9 +38,9 @@
 //
 // Tokens past the length are zero-filled on the way in (cp.async reads nothing there).
 //
-// The kernels may run beside the prefix kernel launched before (they need nothing of it);
-// every CTA waits for that one before it ends, so that the join, which waits for this
-// kernel, finds both done.
+// The kernels may run beside the prefix kernel launched before (they need nothing of it); one
+// CTA waits for that one before it ends, so that the join, which waits for this kernel to
+// end, finds both done.  (Where every CTA waited, the first of them held their SMs.)
 #include <type_traits>
 
 #include "common.cuh"
@@ -94,6 +94,11 @@ __device__ __forceinline__ uint32_t e4m3x2_f16x2(uint16_t v) {
   return r;
 }
 
+// The kernel ends after the one before it.
+__device__ __forceinline__ void end_after_previous() {
+  if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) wait_for_previous();
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextParams p) {
   using L = TextSmem;
@@ -107,7 +112,7 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
   const int len = min(max(a.lens[b * a.lens_s], 0), a.cap);
   const int t0 = chunk * p.chunk;
   if (t0 >= len) {
-    wait_for_previous();
+    end_after_previous();
     return;
   }
   const int t1 = min(len, t0 + p.chunk);
@@ -399,7 +404,7 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
     }
     out[(long long)c4 * p.rows + e] = o;
   }
-  wait_for_previous();
+  end_after_previous();
 }
 
 // ---- the warps split the rows
@@ -429,7 +434,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
   const int len = min(max(a.lens[b * a.lens_s], 0), a.cap);
   const int t0 = chunk * p.chunk;
   if (t0 >= len) {
-    wait_for_previous();
+    end_after_previous();
     return;
   }
   const int t1 = min(len, t0 + p.chunk);
@@ -684,7 +689,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
       if (j4 == 0) reinterpret_cast<float2 *>(p.ml)[slot * p.rows + r] = make_float2(isnan(ll) ? ll : m[i], ll);
     }
   }
-  wait_for_previous();
+  end_after_previous();
 }
 
 template <typename T, bool FP8>

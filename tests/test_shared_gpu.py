@@ -578,3 +578,19 @@ def test_decode_nan_that_is_seen_comes_out(where, dtype, fp8, T, hq):
     want, mag = osh.shared_decode(**a)
     tol = 1e-4 if dtype == torch.float32 else 2.0 ** -6
     assert ((got - want).abs()[~hit] <= tol * (1 + mag)[~hit]).all()
+
+
+def test_tensors_of_every_kind_are_taken():
+    """Parameters, tensors that require a gradient and dimensions of one entry with odd strides."""
+    from rotatek_b200.kernels import append_text, rotatek_shared_decode
+    a = make(1, 1, 1, 8, 1, 140, 20, 30, 32, seed=31)
+    want = rotatek_shared_decode(**a)
+    b = dict(a, q=torch.nn.Parameter(a["q"]), k_sparse=a["k_sparse"].clone().requires_grad_(),
+             v_full=a["v_full"].as_strided(a["v_full"].shape, (7, 3, *a["v_full"].stride()[2:])))
+    assert torch.equal(rotatek_shared_decode(**b), want)
+    k, v = torch.zeros(1, 2, 9, 128, device=DEV, dtype=torch.bfloat16), torch.zeros(1, 2, 9, 128, device=DEV, dtype=torch.bfloat16)
+    new = torch.nn.Parameter(torch.ones(1, 2, 3, 128, device=DEV, dtype=torch.bfloat16))
+    append_text(new, new, torch.tensor([4], dtype=torch.int32, device=DEV), k, v)
+    assert (k[:, :, 4:7] == 1).all() and (v[:, :, :4] == 0).all() and (v[:, :, 7:] == 0).all()
+    with pytest.raises(RuntimeError, match="CUDA"):
+        append_text(new.cpu(), new, torch.tensor([4], dtype=torch.int32, device=DEV), k, v)
