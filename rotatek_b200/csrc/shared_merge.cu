@@ -11,9 +11,9 @@
 // through shared memory.  Where that would leave SMs idle, CTAs of 8 rows and 32 channels
 // whose warps split the partials.
 //
-// Measured, the whole step with tiles of 32 rows / of 8: 1024 working CTAs of 32 rows 459 /
-// 534 us, 256 of them 75.5 / 93.8, 128: 112.8 / 118.8, 64: 78.3 / 78.6, 32: 44.3 / 40.6, 8:
-// 28.8 (with its indices after the wait) / 20.6.
+// Measured, the whole step with tiles of 32 rows / of 8: 1024 working CTAs of 32 rows 461 /
+// 536 us, 256 of them 67.4 / 85.3, 128: 109 / 114, 64: 32.6 / 31.8 and 76.9 / 76.8, 32: 40.6 /
+// 37.6, 8: 26.9 / 18.6.
 //
 // What bounds it: after the last partial, latency (2 to 4 us); with the many rows of the first
 // case its bytes, 43 MB of partials and 8 of output in 19 us, mostly from L2.

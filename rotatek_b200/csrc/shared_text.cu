@@ -16,15 +16,15 @@
 //   own (no CTA-wide barrier in the loop), convert in registers, and join at the end.
 //
 // Measured (the whole attention of a step, prefix of 1064 tokens): 8-bit, 64 questions, 8 heads
-// of 8 rows, up to 4096 tokens 93 us with split tokens, 169 with split rows; 256 questions, 8
-// heads of 4, 512 tokens 74 and 109.  16-bit, the same two 113.8 and 112.8, 80.0 and 75.5: no
-// conversion to share, and the rows' kernel ends with less to join, so 16-bit text always
-// takes that one.  64 rows (64 questions, 8 heads, up to 1001 tokens of 8 bits): 119 us when
-// split by tokens, 16 rows a CTA, 82 by rows.
+// of 8 rows, up to 4096 tokens 89.6 us with split tokens, 164 with split rows; 256 questions, 8
+// heads of 4, 512 tokens 67.7 and 103.  16-bit, the same two when both took it, 113.8 and 112.8,
+// 80.0 and 75.5: no conversion to share, and the rows' kernel ends with less to join, so 16-bit
+// text always takes that one.  64 rows (64 questions, 8 heads, up to 1001 tokens of 8 bits), the
+// kernel alone: 119 us when split by tokens, 16 rows a CTA, 82 by rows.
 //
 // What bounds it: HBM where questions are many and their text 16-bit (the first case: 537 MB
-// within a step of 113 us, 4.8 TB/s with all that is not text); with 8-bit text the
-// conversions (277 MB within 93 us); with few questions the latency of a chunk.
+// within a step of 109 us, 4.9 TB/s with all that is not text); with 8-bit text the
+// conversions (277 MB within 90 us); with few questions the latency of a chunk.
 //
 // 8-bit operands: e4m3 is exact in f16.  Queries go in as f16 scaled by a power of two per row
 // (bf16 has more range, f16 more bits: exact but for what lies 2^-24 below the row's largest).
