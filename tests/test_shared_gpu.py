@@ -594,3 +594,50 @@ def test_tensors_of_every_kind_are_taken():
     assert (k[:, :, 4:7] == 1).all() and (v[:, :, :4] == 0).all() and (v[:, :, 7:] == 0).all()
     with pytest.raises(RuntimeError, match="CUDA"):
         append_text(new.cpu(), new, torch.tensor([4], dtype=torch.int32, device=DEV), k, v)
+
+
+def far(x, stride):
+    """x with its dimension 1 moved `stride` elements apart (one allocation of that reach)."""
+    shape = x.shape
+    inner = torch.empty(shape[0:1] + shape[2:]).stride()
+    buf = torch.empty((shape[1] - 1) * stride + x[:, 0].numel(), dtype=x.dtype, device=x.device)
+    y = buf.as_strided(shape, (inner[0], stride, *inner[1:]))
+    y.copy_(x)
+    return y
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("T", [1, 9])
+def test_decode_offsets_past_32_bits(fp8, T):
+    """Heads of the spans and of the text 2^31 elements and more apart."""
+    a = make(1, 3, T, 8, 2, 140, 70, 50, 32, fp8=fp8, seed=41)
+    for name in ("k_full", "v_full", "k_sparse", "v_sparse", "k_text", "v_text"):
+        b = dict(a, **{name: far(a[name], 2 ** 31 + 1024)})
+        check(b)
+        del b
+
+
+def test_text_offsets_past_32_bits():
+    from rotatek_b200.kernels import append_text, read_text
+    B, H, C, T = 2, 2, 40, 7
+    g = torch.Generator(device=DEV).manual_seed(42)
+    new = torch.randn(2, B, H, T, 128, generator=g, device=DEV).to(torch.bfloat16)
+    lens = torch.tensor([3, 30], dtype=torch.int32, device=DEV)
+    near = [torch.zeros(B, H, C, 128, dtype=torch.uint8, device=DEV) for _ in range(2)]
+    scales = [torch.zeros(B, H, C, device=DEV) for _ in range(2)]
+    append_text(new[0], new[1], lens, *near, k_scale=scales[0], v_scale=scales[1])
+    away = [far(torch.zeros_like(near[0]), 2 ** 31 + 4096) for _ in range(2)]
+    far_scales = [far(torch.zeros_like(scales[0]), 2 ** 31 + 4096) for _ in range(2)]
+    append_text(far(new[0], 2 ** 31 + 4096), new[1], lens, *away, k_scale=far_scales[0], v_scale=far_scales[1])
+    for i in range(2):
+        assert torch.equal(away[i], near[i]) and torch.equal(far_scales[i], scales[i])
+    want = read_text(*near, lens + T, k_scale=scales[0], v_scale=scales[1])
+    got = read_text(*away, lens + T, k_scale=far_scales[0], v_scale=far_scales[1])
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+
+
+def test_verify_offsets_past_32_bits():
+    a = make_verify(3, 2, 1000, torch.float16, True, 43)
+    a["target_logits"] = far(a["target_logits"], 2 ** 31 + 8)
+    a["draft_logits"] = far(a["draft_logits"], 2 ** 31 + 8)
+    check_verify(a)
