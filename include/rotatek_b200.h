@@ -239,7 +239,8 @@ size_t rtk_shared_decode_workspace_size(int64_t prefixes, int64_t batch, int64_t
  * Query t of question b sees all of its prefix and its text rows s <
  * text_lens[b] - (T - 1 - t).  out = softmax([q.k_f ; q.R.k_s + q.delta_mu ;
  * q.k_text] / sqrt(D)) . [v_f ; v_s ; v_text], 0 for a row that sees nothing.
- * Rows of a cache past text_lens and masked prompt tokens may hold anything.
+ * Rows of a cache past text_lens and masked prompt tokens may hold anything; a
+ * NaN logit makes its row NaN.
  * `status` (device uint32, nullable) gets RTK_DEVICE_TIMEOUT if a bounded wait
  * gives up.                                                                   */
 int rtk_shared_decode(const rtk_tensor *q, const rtk_tensor *R_partial, const rtk_tensor *delta_mu,
@@ -276,7 +277,8 @@ int rtk_read_text(const rtk_tensor *k_text, const rtk_tensor *v_text, const rtk_
 size_t rtk_verify_drafts_workspace_size(int64_t batch, int64_t drafts, int64_t vocab);
 
 /* Which drafted tokens the target model accepts, and the token after them.
- *   target_logits [B, T + 1, V]  f32 | bf16 | f16; row j scores the token after draft j - 1
+ *   target_logits [B, T + 1, V]  f32 | bf16 | f16; row j scores the token after draft j - 1;
+ *                                at most 65535 questions and a vocabulary of 2^30
  *   draft_tokens  [B, T] i64     at most 64 drafts
  *   draft_logits  [B, T, V]      target's dtype, what the drafts were drawn from;
  *                                nullable: proposals without probabilities

@@ -7,7 +7,7 @@
 // block of tokens:
 //
 //   S  = Q . K^T        prompt block, 64 tokens, K = 128 channels
-//   S  = [Qhi | Qlo] . [K~ | K~]^T    visual block, 128 tokens (two sub-blocks), K = 2 D_keep: the rotated
+//   S  = [Qhi | Qlo] . [K~ | K~]^T    visual block, 128 tokens, K = 2 D_keep: the rotated
 //                       query q~ = q R is taken in fp32 and split into two 16-bit parts
 //                       (one part alone would move logits by 2^-9)
 //   x  = c (S + q . delta_mu),  c = log2(e) / sqrt(D)     (delta_mu: visual blocks)
@@ -38,10 +38,10 @@
 // Measured: 4096 rows of each of 8 heads on 1024 + 31744 tokens 381 us (the exponential unit
 // alone 246, the tensor core 214); 560 rows, 4 prefixes of 4 heads on 640 + 15360 tokens 79;
 // 12 rows, 2 prefixes of 32 heads on 32 + 16384 tokens 63 (344 MB, 5.5 TB/s); 56 rows, 4 heads
-// on 640 + 15360 tokens 13.8; 14 rows, 4 heads on 64 + 1000 tokens 7.7.
+// on 640 + 15360 tokens (111 SMs) 12.5; 14 rows, 4 heads on 64 + 1000 tokens 7.7.
 //
-// Taken for the first of these: one softmax group 487 us, two that take turns at the
-// exponential unit 409, P over S and one O so that a third S fits 400, the queries ahead of the
+// Taken for the first of these: 487 us before the two softmax groups took turns at the
+// exponential unit, 409 after, P over S and one O so that a third S fits 400, the queries ahead of the
 // ring 381.  Dropped: a sixth to a half of the exponentials as polynomials on the FMA units
 // (378 to 404 where none took 373), three softmax groups (397), four that split a block's
 // columns (402), blocks of 64 visual tokens (490 to 539).
