@@ -11,8 +11,9 @@
 //                       query q~ = q R is taken in fp32 and split into two 16-bit parts
 //                       (one part alone would move logits by 2^-9)
 //   x  = c (S + q . delta_mu),  c = log2(e) / sqrt(D)     (delta_mu: visual blocks)
-//   P  = 2^(x - m) rounded to 16 bits, the MMA's operand type; l sums it unrounded
-//   O += P . V
+//   P  = 2^(x - m) in two 16-bit parts, Phi + Plo; l sums it unrounded
+//   O += Phi . V + Plo . V     (Phi alone would move outputs by 2^-9 of sum P |v|; the
+//                       decode of one question per image splits its weights as well)
 //
 // m follows the running maximum lazily: O and l are rescaled only when a maximum
 // grows by more than 2^8 over the one in use (P stays below 2^8, O and l are fp32).
@@ -25,26 +26,27 @@
 //   warp 10     issues those of O: a single thread's instructions could not keep the
 //               tensor core fed
 // TMEM (all 512 columns): three S buffers of 128, O of 128.  The S of the next blocks is made
-// while two blocks are in the softmax; P goes over the upper half of its S as the A
-// operand of P . V.  The two softmax groups settle m in the order of the blocks, through
+// while two blocks are in the softmax; P goes over its S as the A operand of P . V, the upper
+// 64 tokens first, whose P . V then begins.  The two softmax groups settle m in the order of the blocks, through
 // shared memory; only where m moves does the group wait for the P . V before and rescale O.
 // At the end of a unit the partial result of (unit, CTA) is written for shared_merge.cu.
 //
-// What bounds it: with many rows the exponential unit (128 x 128 a block at 16 a cycle: 1024
-// of the 1370 cycles a block takes) and what a warp does between two blocks'
-// exponentials (waiting for S, reading it, its maximum, handing P over); with few
-// rows, HBM and the latencies at a unit's ends.
+// What bounds it: with many rows the tensor core (20 MMAs of 64 cycles a visual block, 16 of
+// them P . V) and the exponential unit (128 x 128 a block at 16 a cycle: 1024 cycles), at the
+// clocks that a sustained run is left with; with few rows, HBM and the latencies at a unit's ends.
 //
-// Measured: 4096 rows of each of 8 heads on 1024 + 31744 tokens 381 us (the exponential unit
-// alone 246, the tensor core 214); 560 rows, 4 prefixes of 4 heads on 640 + 15360 tokens 79;
-// 12 rows, 2 prefixes of 32 heads on 32 + 16384 tokens 63 (344 MB, 5.5 TB/s); 56 rows, 4 heads
-// on 640 + 15360 tokens (111 SMs) 12.5; 14 rows, 4 heads on 64 + 1000 tokens 7.7.
+// Measured: 4096 rows of each of 8 heads on 1024 + 31744 tokens 494 us (the tensor core alone
+// 357, 421 at its sustained rate; the exponential unit 246); 560 rows, 4 prefixes of 4 heads on
+// 640 + 15360 tokens 93; 12 rows, 2 prefixes of 32 heads on 32 + 16384 tokens 70 (344 MB); 56
+// rows, 4 heads on 640 + 15360 tokens (111 SMs) 14.2; 14 rows, 4 heads on 64 + 1000 tokens 8.2.
+// With one part of P these took 390, 82, 64, 13.4 and 8.0, with the P . V of a block begun only
+// when all of its P was there (not its upper 64 tokens) 509, 96, 73, 14.4 and 8.3.
 //
-// Taken for the first of these: 487 us before the two softmax groups took turns at the
-// exponential unit, 409 after, P over S and one O so that a third S fits 400, the queries ahead of the
-// ring 381.  Dropped: a sixth to a half of the exponentials as polynomials on the FMA units
-// (378 to 404 where none took 373), three softmax groups (397), four that split a block's
-// columns (402), blocks of 64 visual tokens (490 to 539).
+// Taken, and measured with one part of P for the first of these: 487 us before the two softmax groups
+// took turns at the exponential unit, 409 after, P over S and one O so that a third S fits 400, the
+// queries ahead of the ring 381.  Dropped: a sixth to a half of the exponentials as polynomials
+// on the FMA units (378 to 404 where none took 373), three softmax groups (397), four that split
+// a block's columns (402), blocks of 64 visual tokens (490 to 539).
 #include <type_traits>
 
 #include "shared.h"
@@ -56,7 +58,8 @@ namespace {
 constexpr int kThreads = 352;
 constexpr int kFullTok = 64, kVisTok = 128;      // tokens of a block
 constexpr uint32_t kColsS = 128;                 // TMEM columns of an S buffer
-constexpr uint32_t kColP = 64;                   // P within it
+// P over it: 64 tokens of S (64 columns) become 32 columns of Plo, then 32 of Phi
+constexpr uint32_t kColHi = 32;
 constexpr uint32_t kColO = 3 * kColsS;           // the O accumulator
 constexpr float kLazy = 8.f;
 
@@ -75,8 +78,8 @@ struct PrefixSmem {
   static constexpr int kRef = kDm + 512;                           // float[128]: m
   static constexpr int kMl = kRef + 512;                           // float2[2][128]: a group's m, l
   static constexpr int kBar = kMl + 2048;
-  // full[S], empty[S], s_ready[3], p_ready[3], pv_done[3], rot, o_done, q_here
-  static constexpr int kNumBars = 2 * kStages + 12;
+  // full[S], empty[S], s_ready[3], p_ready[3], p_upper[3], pv_done[3], rot, o_done, q_here
+  static constexpr int kNumBars = 2 * kStages + 15;
   static constexpr int kTmemSlot = kBar + kNumBars * 8;
   static constexpr int kAbort = kTmemSlot + 4;
   static constexpr int kBytes = kAbort + 4;
@@ -135,23 +138,28 @@ __device__ __forceinline__ float max_half(const uint32_t (&r)[2][32]) {
   return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
 }
 
-// Weights of 64 columns: 32 columns of P (16-bit pairs) at `p`; returns their sum.
+// Weights of the 64 columns at `p`: Plo and Phi (16-bit pairs) over them; returns their sum.
 template <typename T>
 __device__ __forceinline__ float weights_half(uint32_t p, const uint32_t (&r)[2][32], float scale, float off) {
   const float2 scale2 = make_float2(scale, scale), off2 = make_float2(off, off);
   float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    uint32_t w[16];
+    uint32_t hi[16], lo[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1])), scale2, off2);
       x.x = fast_exp2(x.x);
       x.y = fast_exp2(x.y);
       l2[i & 1] = __fadd2_rn(l2[i & 1], x);
-      w[i] = pack2<T>(x.x, x.y);
+      hi[i] = pack2<T>(x.x, x.y);
+      float2 h;
+      unpack2<T>(hi[i], h.x, h.y);
+      x = __ffma2_rn(h, make_float2(-1.f, -1.f), x);       // exact
+      lo[i] = pack2<T>(x.x, x.y);
     }
-    tmem_st16_nowait(p + 16 * c, w);
+    tmem_st16_nowait(p + kColHi + 16 * c, hi);
+    tmem_st16_nowait(p + 16 * c, lo);
   }
   return (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
 }
@@ -167,7 +175,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t *empty_bar = full_bar + L::kStages;
   uint64_t *s_bar = empty_bar + L::kStages;       // [buffer] S is in TMEM
   uint64_t *p_bar = s_bar + 3;                    // [buffer] P is in TMEM
-  uint64_t *pv_bar = p_bar + 3;                   // [buffer] its P . V is done
+  uint64_t *up_bar = p_bar + 3;                   // [buffer] P of tokens 64 .. 127 is (prompt blocks: nothing)
+  uint64_t *pv_bar = up_bar + 3;                  // [buffer] its P . V is done
   uint64_t *rot_bar = pv_bar + 3;                 // rotated queries are in TMEM
   uint64_t *o_bar = rot_bar + 1;                  // the O accumulator is complete
   uint64_t *q_bar = o_bar + 1;                    // the first unit's queries are here
@@ -195,6 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 3; ++i) {
       mbar_init(&s_bar[i], 1);
       mbar_init(&p_bar[i], 4);
+      mbar_init(&up_bar[i], 4);
       mbar_init(&pv_bar[i], 1);
     }
     mbar_init(rot_bar, 1);
@@ -343,19 +353,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else {
           for (int j = j0; j < j1; ++j) {
             mbar_wait_bounded(&full_bar[stage], stage_par, abort_flag, p.status);
-            mbar_wait_bounded(&p_bar[buf], buf_par, abort_flag, p.status);
+            mbar_wait_bounded(&up_bar[buf], buf_par, abort_flag, p.status);
             tc_fence_after();
-            const uint32_t pa = tmem + buf * kColsS + kColP, first = j > j0;
+            const uint32_t pa = tmem + buf * kColsS, first = j > j0;
             if (j >= sp.blocks_full) {
               const uint64_t vd = v_vis + stage * kStep;
 #pragma unroll
-              for (int k = 0; k < kVisTok / 16; ++k)
-                umma_f16_ts(tmem + kColO, pa + 8 * k, vd + ((k * 2048) >> 4), kIdPv, k > 0 ? 1u : first);
+              for (int k = 0; k < kVisTok / 16; ++k) {
+                const int t = k ^ 4;                 // the upper tokens first
+                if (k == 4) {
+                  mbar_wait_bounded(&p_bar[buf], buf_par, abort_flag, p.status);
+                  tc_fence_after();
+                }
+                const uint32_t pk = pa + (t >> 2) * 64 + (t & 3) * 8;
+                umma_f16_ts(tmem + kColO, pk + kColHi, vd + ((t * 2048) >> 4), kIdPv, k > 0 ? 1u : first);
+                umma_f16_ts(tmem + kColO, pk, vd + ((t * 2048) >> 4), kIdPv, 1u);
+              }
             } else {
+              mbar_wait_bounded(&p_bar[buf], buf_par, abort_flag, p.status);
+              tc_fence_after();
               const uint64_t vd = v_prompt + stage * kStep;
 #pragma unroll
-              for (int k = 0; k < kFullTok / 16; ++k)
-                umma_f16_ts(tmem + kColO, pa + 8 * k, vd + ((k * 2048) >> 4), kIdPv, k > 0 ? 1u : first);
+              for (int k = 0; k < kFullTok / 16; ++k) {
+                umma_f16_ts(tmem + kColO, pa + kColHi + 8 * k, vd + ((k * 2048) >> 4), kIdPv, k > 0 ? 1u : first);
+                umma_f16_ts(tmem + kColO, pa + 8 * k, vd + ((k * 2048) >> 4), kIdPv, 1u);
+              }
             }
             umma_commit(&pv_bar[buf]);
             umma_commit(&empty_bar[stage]);
@@ -579,15 +601,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           const float off = bi - (m > -INFINITY ? m : 0.f);
           if (!prompt) {
-            l += weights_half<T>(s + kColP + 32, r, a.scale_log2, off);
+            l += weights_half<T>(s + 64, r, a.scale_log2, off);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&up_bar[buf]);
             load_half(s, r);
           }
-          l += weights_half<T>(s + kColP, r, a.scale_log2, off);
+          l += weights_half<T>(s, r, a.scale_log2, off);
           tmem_wait_st();
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_bar[buf]);
+        if (lane == 0) {
+          if (prompt || !busy) mbar_arrive(&up_bar[buf]);
+          mbar_arrive(&p_bar[buf]);
+        }
       }
       it += blocks;
       // the partial result: each group writes 64 channels of the row

@@ -641,3 +641,36 @@ def test_verify_offsets_past_32_bits():
     a["target_logits"] = far(a["target_logits"], 2 ** 31 + 8)
     a["draft_logits"] = far(a["draft_logits"], 2 ** 31 + 8)
     check_verify(a)
+
+
+UNIT = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}       # a rounding to 16 bits, relative
+
+
+def alternating(a, name):
+    """a's Values `name` become v, -v, v, -v, ...: outputs are what the weights leave of v."""
+    v = a[name]
+    sign = 1 - 2 * (torch.arange(v.shape[2], device=DEV) % 2)
+    a[name] = (v[:, :, :1].float() * sign[:, None]).to(v.dtype).expand_as(v).contiguous()
+
+
+def check_weights(a):
+    """Weights to 16 bits and more.  The logits here are below 2 in size: products exact in fp32,
+    sums off by 128 * 2^-24 * 2, the rotated query in two 16-bit parts (2^-16 in bf16) by 2 * 2^-16;
+    the weights in two parts by 2^-16 or less.  Numerator and normaliser: 2 * (2^-15 + 2^-16) < 2^-13.
+    One 16-bit part would move a weight by up to 2^-9 (bf16) or 2^-12 (fp16)."""
+    from rotatek_b200.kernels import rotatek_shared_decode
+    got = rotatek_shared_decode(**a).cpu().double()
+    want, mag = osh.shared_decode(**a)
+    tol = UNIT[a["q"].dtype] * want.abs() + 2.0 ** -13 * mag + 2.0 ** -25
+    off = (got - want).abs()
+    assert (off <= tol).all(), f"{int((off > tol).sum())} of {off.numel()}, worst {(off / tol).max():.2f}"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("name,sv,sf", [("v_full", 0, 4), ("v_full", 0, 64), ("v_sparse", 4, 0), ("v_sparse", 128, 0),
+                                        ("v_sparse", 99, 0)])
+def test_decode_prefix_weights_hold_their_bits(name, sv, sf, dtype):
+    """Values that cancel leave the errors of the softmax weights in the output."""
+    a = make(1, 40, 1, 14, 2, sv, sf, 0, 32, dtype=dtype, seed=51, std=0.3, bias=False)
+    alternating(a, name)
+    check_weights(a)
