@@ -18,7 +18,7 @@
 // Measured (the whole attention of a step, prefix of 1064 tokens): 8-bit, 64 questions, 8 heads
 // of 8 rows, up to 4096 tokens 89.6 us with split tokens, 164 with split rows; 256 questions, 8
 // heads of 4, 512 tokens 67.7 and 103.  16-bit, the same two when both took it, 113.8 and 112.8,
-// 80.0 and 75.5: no conversion to share, and the rows' kernel ends with less to join, so 16-bit
+// 80.0 and 75.5 (with one part of P): no conversion to share, and the rows' kernel ends with less to join, so 16-bit
 // text always takes that one.  64 rows (64 questions, 8 heads, up to 1001 tokens of 8 bits), the
 // kernel alone: 119 us when split by tokens, 16 rows a CTA, 82 by rows.
 //
@@ -34,7 +34,7 @@
 // k index runs over a 16-channel group in the order 0 1 4 5 8 9 12 13 2 3 6 7 10 11 14 15, and
 // the queries are stored in that order.  ldmatrix.trans of Value bytes pairs two tokens' bytes
 // of channels (2g, 2g+1): one byte permute separates them into B fragments of an "even" and
-// an "odd" n-tile.  16-bit operands: P is rounded to 16 bits, l sums P as rounded.
+// an "odd" n-tile.  16-bit text: P in two 16-bit parts, as the prefix kernel's; l sums it unrounded.
 //
 // Tokens past the length are zero-filled on the way in (cp.async reads nothing there).
 //
@@ -642,30 +642,36 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
       }
     }
     const float base[2] = {m[0] > -INFINITY ? m[0] : 0.f, m[1] > -INFINITY ? m[1] : 0.f};
-    uint32_t pa[kNT][2];
+    uint32_t pa[kNT][2], pl[kNT][2];                 // Phi, Plo
 #pragma unroll
     for (int n = 0; n < kNT; ++n)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         float w0 = fast_exp2(fmaf(s[n][2 * i], qf[i], -base[i])), w1 = fast_exp2(fmaf(s[n][2 * i + 1], qf[i], -base[i]));
+        l[i] += w0 + w1;
         if constexpr (FP8) {
-          l[i] += w0 + w1;
           pa[n][i] = pack2<M>(w0 * vscale[n][0], w1 * vscale[n][1]);
         } else {
+          float h0, h1;
           pa[n][i] = pack2<M>(w0, w1);
-          unpack2<M>(pa[n][i], w0, w1);
-          l[i] += w0 + w1;
+          unpack2<M>(pa[n][i], h0, h1);
+          pl[n][i] = pack2<M>(w0 - h0, w1 - h1);
         }
       }
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {                 // 16 tokens
       const uint32_t pf[4] = {pa[2 * kk][0], pa[2 * kk][1], pa[2 * kk + 1][0], pa[2 * kk + 1][1]};
+      const uint32_t pg[4] = {pl[2 * kk][0], pl[2 * kk][1], pl[2 * kk + 1][0], pl[2 * kk + 1][1]};
 #pragma unroll
       for (int c = 0; c < 16; c += 2) {              // two chunks of 8 channels
         uint32_t r[4];
         ldmatrix_x4_trans(even(kk ? v_lane2 : v_lane, c), r[0], r[1], r[2], r[3]);
         mma_16816<M>(acc[c], pf, r[0], r[1]);
         mma_16816<M>(acc[c + 1], pf, r[2], r[3]);
+        if constexpr (!FP8) {
+          mma_16816<M>(acc[c], pg, r[0], r[1]);
+          mma_16816<M>(acc[c + 1], pg, r[2], r[3]);
+        }
       }
     }
   }

@@ -674,3 +674,12 @@ def test_decode_prefix_weights_hold_their_bits(name, sv, sf, dtype):
     a = make(1, 40, 1, 14, 2, sv, sf, 0, 32, dtype=dtype, seed=51, std=0.3, bias=False)
     alternating(a, name)
     check_weights(a)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,cap", [(1, 4), (1, 32), (6, 9), (6, 300)])
+def test_decode_text_weights_hold_their_bits(T, cap, dtype):
+    """16-bit text, as the prefix above."""
+    a = make(1, 20, T, 16, 2, 0, 0, cap, 32, dtype=dtype, lens=[cap] * 20, seed=52, std=0.3)
+    alternating(a, "v_text")
+    check_weights(a)
