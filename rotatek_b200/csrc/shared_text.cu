@@ -15,10 +15,10 @@
 // - 8-bit text of at most 16 rows: the warps split the tokens, blocks of 32 in rings of their
 //   own (no CTA-wide barrier in the loop), convert in registers, and join at the end.
 //
-// Measured (the whole attention of a step, prefix of 1064 tokens): 8-bit, 64 questions, 8 heads
+// Measured (the whole attention of a step, prefix of 1064 tokens; one part of P): 8-bit, 64 questions, 8 heads
 // of 8 rows, up to 4096 tokens 89.6 us with split tokens, 164 with split rows; 256 questions, 8
 // heads of 4, 512 tokens 67.7 and 103.  16-bit, the same two when both took it, 113.8 and 112.8,
-// 80.0 and 75.5 (with one part of P): no conversion to share, and the rows' kernel ends with less to join, so 16-bit
+// 80.0 and 75.5: no conversion to share, and the rows' kernel ends with less to join, so 16-bit
 // text always takes that one.  64 rows (64 questions, 8 heads, up to 1001 tokens of 8 bits), the
 // kernel alone: 119 us when split by tokens, 16 rows a CTA, 82 by rows.
 //
@@ -26,15 +26,15 @@
 // within a step of 109 us, 4.9 TB/s with all that is not text); with 8-bit text the
 // conversions (277 MB within 90 us); with few questions the latency of a chunk.
 //
-// 8-bit operands: e4m3 is exact in f16.  Queries go in as f16 scaled by a power of two per row
-// (bf16 has more range, f16 more bits: exact but for what lies 2^-24 below the row's largest).
-// A token's Key scale multiplies its logit; its Value scale multiplies its weight relative to
-// the largest Value scale met so far (`vref`), so weights stay within f16 whatever the scales.
+// 8-bit text: e4m3 is exact in f16 and in bf16.  S runs in f16: queries go in scaled by a power of
+// two per row (bf16 has more range, f16 more bits: exact but for what lies 2^-24 below the row's
+// largest), a token's Key scale multiplies its logit.  P . V runs in bf16, which has fp32's range:
+// a token's Value scale multiplies its weight, and scales of any ratio may meet in one row.
 // In registers: ldmatrix of Key bytes gives lane (g, j) bytes 4j .. 4j+3 of token g: the MMA's
 // k index runs over a 16-channel group in the order 0 1 4 5 8 9 12 13 2 3 6 7 10 11 14 15, and
 // the queries are stored in that order.  ldmatrix.trans of Value bytes pairs two tokens' bytes
 // of channels (2g, 2g+1): one byte permute separates them into B fragments of an "even" and
-// an "odd" n-tile.  16-bit text: P in two 16-bit parts, as the prefix kernel's; l sums it unrounded.
+// an "odd" n-tile.  P is taken in two 16-bit parts, as the prefix kernel's; l sums it unrounded.
 //
 // Tokens past the length are zero-filled on the way in (cp.async reads nothing there).
 //
@@ -94,13 +94,28 @@ __device__ __forceinline__ uint32_t e4m3x2_f16x2(uint16_t v) {
   return r;
 }
 
+__device__ __forceinline__ uint32_t e4m3x2_bf16x2(uint16_t v) {
+  float lo, hi;
+  unpack2<__half>(e4m3x2_f16x2(v), lo, hi);
+  return pack2<__nv_bfloat16>(lo, hi);
+}
+
+// Two weights as 16-bit parts: the nearest, and the nearest to what that leaves.
+template <typename M>
+__device__ __forceinline__ void two_parts(float w0, float w1, uint32_t &hi, uint32_t &lo) {
+  float h0, h1;
+  hi = pack2<M>(w0, w1);
+  unpack2<M>(hi, h0, h1);
+  lo = pack2<M>(w0 - h0, w1 - h1);
+}
+
 // The kernel ends after the one before it.
 __device__ __forceinline__ void end_after_previous() {
   if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) wait_for_previous();
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextParams p) {
+__global__ void __launch_bounds__(kWarps * 32, 3) shared_text_kernel(const TextParams p) {
   using L = TextSmem;
   extern __shared__ __align__(1024) unsigned char smem[];
   launch_dependents();
@@ -203,7 +218,6 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
   const int all_see = len - (a.tokens - 1);          // every row sees tokens below this
 
   float m[2], l[2], acc[16][4];
-  float vref = 0.f;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     m[i] = -INFINITY;
@@ -237,26 +251,6 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
       const float2 v2 = *reinterpret_cast<const float2 *>(sc + 128 + (n * 8 + 2 * j4) * 4);
       kscale[n][0] = k2.x; kscale[n][1] = k2.y;
       vscale[n][0] = v2.x; vscale[n][1] = v2.y;
-    }
-    // the largest Value scale of the block, over the warp
-    float top = 0.f;
-#pragma unroll
-    for (int n = 0; n < kNT; ++n) top = fmaxf(top, fmaxf(vscale[n][0], vscale[n][1]));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    if (top > vref) {                              // the same in every lane
-      const float f = vref / top;
-      vref = top;
-#pragma unroll
-      for (int n = 0; n < 16; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[n][i] *= f;
-    }
-    const float inv = vref > 0.f ? 1.f / vref : 0.f;
-#pragma unroll
-    for (int n = 0; n < kNT; ++n) {
-      vscale[n][0] *= inv;
-      vscale[n][1] *= inv;
     }
     float s[kNT][4];
 #pragma unroll
@@ -314,21 +308,20 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
       }
     }
     const float base[2] = {m[0] > -INFINITY ? m[0] : 0.f, m[1] > -INFINITY ? m[1] : 0.f};
-    uint32_t pa[kNT][2];                           // weights of rows g, g + 8
+    uint32_t pa[kNT][2], pl[kNT][2];               // weights of rows g, g + 8
 #pragma unroll
     for (int n = 0; n < kNT; ++n)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float w0 = fast_exp2(fmaf(s[n][2 * i], qf[i], -base[i]));
-        float w1 = fast_exp2(fmaf(s[n][2 * i + 1], qf[i], -base[i]));
+        const float w0 = fast_exp2(fmaf(s[n][2 * i], qf[i], -base[i]));
+        const float w1 = fast_exp2(fmaf(s[n][2 * i + 1], qf[i], -base[i]));
         l[i] += w0 + w1;
-        w0 *= vscale[n][0];
-        w1 *= vscale[n][1];
-        pa[n][i] = pack2<__half>(w0, w1);
+        two_parts<__nv_bfloat16>(w0 * vscale[n][0], w1 * vscale[n][1], pa[n][i], pl[n][i]);
       }
 #pragma unroll
     for (int kk = 0; kk < kNT / 2; ++kk) {         // 16 tokens
       const uint32_t pf[4] = {pa[2 * kk][0], pa[2 * kk][1], pa[2 * kk + 1][0], pa[2 * kk + 1][1]};
+      const uint32_t pg[4] = {pl[2 * kk][0], pl[2 * kk][1], pl[2 * kk + 1][0], pl[2 * kk + 1][1]};
 #pragma unroll
       for (int c = 0; c < 8; c += 2) {           // two 16-byte chunks of channels
         uint32_t r[4];
@@ -336,10 +329,12 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           const uint32_t lo = __byte_perm(r[2 * q], 0, 0x3120), hi = __byte_perm(r[2 * q + 1], 0, 0x3120);
-          mma_f16(acc[2 * (c + q)], pf, e4m3x2_f16x2((uint16_t)(lo & 0xffffu)),
-                  e4m3x2_f16x2((uint16_t)(hi & 0xffffu)));
-          mma_f16(acc[2 * (c + q) + 1], pf, e4m3x2_f16x2((uint16_t)(lo >> 16)),
-                  e4m3x2_f16x2((uint16_t)(hi >> 16)));
+#pragma unroll
+          for (int odd = 0; odd < 2; ++odd) {
+            const uint32_t b0 = e4m3x2_bf16x2((uint16_t)(lo >> (16 * odd))), b1 = e4m3x2_bf16x2((uint16_t)(hi >> (16 * odd)));
+            mma_16816<__nv_bfloat16>(acc[2 * (c + q) + odd], pf, b0, b1);
+            mma_16816<__nv_bfloat16>(acc[2 * (c + q) + odd], pg, b0, b1);
+          }
         }
       }
     }
@@ -363,8 +358,7 @@ __global__ void __launch_bounds__(kWarps * 32) shared_text_kernel(const TextPara
 #pragma unroll
     for (int c = 0; c < 8; ++c)
       *reinterpret_cast<float4 *>(row + 16 * c + 4 * j4) =
-          make_float4(acc[2 * c][2 * i] * vref, acc[2 * c + 1][2 * i] * vref,
-                      acc[2 * c][2 * i + 1] * vref, acc[2 * c + 1][2 * i + 1] * vref);
+          make_float4(acc[2 * c][2 * i], acc[2 * c + 1][2 * i], acc[2 * c][2 * i + 1], acc[2 * c + 1][2 * i + 1]);
   }
   __syncthreads();
   // the rows' factors of each warp's partial, over the warps' own (m, l)
@@ -415,7 +409,7 @@ struct RowsSmem {
   static constexpr int kRaw = kScales + (FP8 ? 2 * kTok * 4 : 0);
   static constexpr int kStages = 3;
   static constexpr int kQ = 0;                                    // 64 rows of 256 bytes
-  static constexpr int kTile = kQ + kWarps * 4096;                // FP8: the tile as f16
+  static constexpr int kTile = kQ + kWarps * 4096;                // FP8: the tile, Keys as f16, Values as bf16
   static constexpr int kRing = kTile + (FP8 ? 2 * kTok * 256 : 0);
   static constexpr int kBytes = kRing + kStages * kRaw;
 };
@@ -423,7 +417,8 @@ struct RowsSmem {
 template <typename T, bool FP8>
 __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const TextParams p) {
   using L = RowsSmem<FP8>;
-  using M = typename std::conditional<FP8, __half, T>::type;     // MMA operand type
+  using MK = typename std::conditional<FP8, __half, T>::type;            // operand type of S
+  using MV = typename std::conditional<FP8, __nv_bfloat16, T>::type;     // and of P . V
   extern __shared__ __align__(1024) unsigned char smem[];
   launch_dependents();
   const SharedParams &a = p.s;
@@ -513,7 +508,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
   __syncwarp();
   const bool busy = row0 < p.rows;
   int limit[2];
-  float qf[2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, acc[16][4], vref = 0.f;
+  float qf[2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, acc[16][4];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int r = row0 + g + 8 * i;
@@ -546,41 +541,26 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
         kscale[n][0] = k2.x; kscale[n][1] = k2.y;
         vscale[n][0] = v2.x; vscale[n][1] = v2.y;
       }
-      // 16 bytes of a row become 16 f16: two chunks of the row's 256 bytes
+      // 16 bytes of a row become 16 numbers of 16 bits: two chunks of the row's 256 bytes
 #pragma unroll
       for (int e = 0; e < 2 * L::kTok * 8 / (32 * kWarps); ++e) {
-        const int i = e * 32 * kWarps + threadIdx.x, r = i >> 3, c = i & 7;   // rows 0-31 Keys, 32-63 Values
+        constexpr int kStep = 32 * kWarps;
+        const int i = e * kStep + threadIdx.x, r = i >> 3, c = i & 7;         // rows 0-31 Keys, 32-63 Values
+        const bool value = e * kStep >= L::kTok * 8;
         const uint4 w = *reinterpret_cast<const uint4 *>(raw + at<128>(r, c));
-        uint4 lo, hi;
-        lo.x = e4m3x2_f16x2((uint16_t)(w.x & 0xffffu)); lo.y = e4m3x2_f16x2((uint16_t)(w.x >> 16));
-        lo.z = e4m3x2_f16x2((uint16_t)(w.y & 0xffffu)); lo.w = e4m3x2_f16x2((uint16_t)(w.y >> 16));
-        hi.x = e4m3x2_f16x2((uint16_t)(w.z & 0xffffu)); hi.y = e4m3x2_f16x2((uint16_t)(w.z >> 16));
-        hi.z = e4m3x2_f16x2((uint16_t)(w.w & 0xffffu)); hi.w = e4m3x2_f16x2((uint16_t)(w.w >> 16));
-        *reinterpret_cast<uint4 *>(smem + L::kTile + at<256>(r, 2 * c)) = lo;
-        *reinterpret_cast<uint4 *>(smem + L::kTile + at<256>(r, 2 * c + 1)) = hi;
+        const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+        uint32_t out[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint16_t two = (uint16_t)(in[k >> 1] >> (16 * (k & 1)));
+          out[k] = value ? e4m3x2_bf16x2(two) : e4m3x2_f16x2(two);
+        }
+        *reinterpret_cast<uint4 *>(smem + L::kTile + at<256>(r, 2 * c)) = make_uint4(out[0], out[1], out[2], out[3]);
+        *reinterpret_cast<uint4 *>(smem + L::kTile + at<256>(r, 2 * c + 1)) = make_uint4(out[4], out[5], out[6], out[7]);
       }
       __syncthreads();
       k_addr = smem_u32(smem + L::kTile);
       v_addr = k_addr + L::kTok * 256;
-      float top = 0.f;                               // the tile's largest Value scale
-#pragma unroll
-      for (int n = 0; n < kNT; ++n) top = fmaxf(top, fmaxf(vscale[n][0], vscale[n][1]));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      if (top > vref) {                              // the same in every lane
-        const float f = vref / top;
-        vref = top;
-#pragma unroll
-        for (int n = 0; n < 16; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[n][i] *= f;
-      }
-      const float inv = vref > 0.f ? 1.f / vref : 0.f;
-#pragma unroll
-      for (int n = 0; n < kNT; ++n) {
-        vscale[n][0] *= inv;
-        vscale[n][1] *= inv;
-      }
     } else {
       k_addr = smem_u32(raw);
       v_addr = k_addr + L::kTok * 256;
@@ -598,10 +578,10 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
       ldmatrix_x4(even(q_lane, 2 * k), qa[0], qa[1], qa[2], qa[3]);
       ldmatrix_x4(even(k_lane, 2 * k), r[0], r[1], r[2], r[3]);
       ldmatrix_x4(even(k_lane2, 2 * k), r2[0], r2[1], r2[2], r2[3]);
-      mma_16816<M>(s[0], qa, r[0], r[1]);
-      mma_16816<M>(s[1], qa, r[2], r[3]);
-      mma_16816<M>(s[2], qa, r2[0], r2[1]);
-      mma_16816<M>(s[3], qa, r2[2], r2[3]);
+      mma_16816<MK>(s[0], qa, r[0], r[1]);
+      mma_16816<MK>(s[1], qa, r[2], r[3]);
+      mma_16816<MK>(s[2], qa, r2[0], r2[1]);
+      mma_16816<MK>(s[3], qa, r2[2], r2[3]);
     }
     if constexpr (FP8) {
 #pragma unroll
@@ -650,13 +630,10 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
         float w0 = fast_exp2(fmaf(s[n][2 * i], qf[i], -base[i])), w1 = fast_exp2(fmaf(s[n][2 * i + 1], qf[i], -base[i]));
         l[i] += w0 + w1;
         if constexpr (FP8) {
-          pa[n][i] = pack2<M>(w0 * vscale[n][0], w1 * vscale[n][1]);
-        } else {
-          float h0, h1;
-          pa[n][i] = pack2<M>(w0, w1);
-          unpack2<M>(pa[n][i], h0, h1);
-          pl[n][i] = pack2<M>(w0 - h0, w1 - h1);
+          w0 *= vscale[n][0];
+          w1 *= vscale[n][1];
         }
+        two_parts<MV>(w0, w1, pa[n][i], pl[n][i]);
       }
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {                 // 16 tokens
@@ -666,17 +643,14 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
       for (int c = 0; c < 16; c += 2) {              // two chunks of 8 channels
         uint32_t r[4];
         ldmatrix_x4_trans(even(kk ? v_lane2 : v_lane, c), r[0], r[1], r[2], r[3]);
-        mma_16816<M>(acc[c], pf, r[0], r[1]);
-        mma_16816<M>(acc[c + 1], pf, r[2], r[3]);
-        if constexpr (!FP8) {
-          mma_16816<M>(acc[c], pg, r[0], r[1]);
-          mma_16816<M>(acc[c + 1], pg, r[2], r[3]);
-        }
+        mma_16816<MV>(acc[c], pf, r[0], r[1]);
+        mma_16816<MV>(acc[c + 1], pf, r[2], r[3]);
+        mma_16816<MV>(acc[c], pg, r[0], r[1]);
+        mma_16816<MV>(acc[c + 1], pg, r[2], r[3]);
       }
     }
   }
   cp_async_wait_all();
-  const float scale_o = FP8 ? vref : 1.f;
   const long long slot = (long long)bh * p.chunks + chunk;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -690,7 +664,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
 #pragma unroll
       for (int n = 0; n < 16; ++n)
         *reinterpret_cast<float2 *>(out + 8ll * n * p.rows) =
-            make_float2(acc[n][2 * i] * scale_o, acc[n][2 * i + 1] * scale_o);
+            make_float2(acc[n][2 * i], acc[n][2 * i + 1]);
       // NaN logits: m NaN too, as no weight may drop them
       if (j4 == 0) reinterpret_cast<float2 *>(p.ml)[slot * p.rows + r] = make_float2(isnan(ll) ? ll : m[i], ll);
     }

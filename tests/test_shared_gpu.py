@@ -683,3 +683,42 @@ def test_decode_text_weights_hold_their_bits(T, cap, dtype):
     a = make(1, 20, T, 16, 2, 0, 0, cap, 32, dtype=dtype, lens=[cap] * 20, seed=52, std=0.3)
     alternating(a, "v_text")
     check_weights(a)
+
+
+def quantise_text(a):
+    for side in ("k", "v"):
+        val, scale = osh.quantize_rows(a[f"{side}_text"])
+        a[f"{side}_text"] = val.float().to(torch.float8_e4m3fn).to(DEV).view(torch.uint8)
+        a[f"{side}_scale"] = scale.to(DEV)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,cap", [(1, 4), (1, 32), (6, 9), (6, 300)])
+def test_decode_text8_weights_hold_their_bits(T, cap, dtype):
+    """8-bit text, as the prefix above, for either text kernel."""
+    a = make(1, 20, T, 16, 2, 0, 0, cap, 32, dtype=dtype, lens=[cap] * 20, seed=53, std=0.3)
+    alternating(a, "v_text")
+    quantise_text(a)
+    check_weights(a)
+
+
+@pytest.mark.parametrize("T", [2, 9])
+@pytest.mark.parametrize("size", [1e-3, 1e-5, 1e-9])
+@pytest.mark.parametrize("beside", ["zeros", "weightless", "unseen"])
+def test_decode_text8_small_values_hold_the_weight(beside, size, T):
+    """Value rows of `size` that hold all the weight, beside a row of zeros (its scale is 1), a row
+    1e9 times larger whose weight is 0, or one that the earlier queries may not see."""
+    a = make(1, 2, T, 8, 2, 0, 0, 150, 32, dtype=torch.bfloat16, lens=[150, 131], seed=54)
+    a["q"][..., 0] = 4.0
+    v = a["v_text"].float() * size
+    if beside == "zeros":
+        v[:, :, [5, 40, 130]] = 0
+    elif beside == "weightless":
+        a["k_text"][:, :, 40, 0] = -1000.0            # logits near -350
+        v[:, :, 40] *= 1e9
+    else:
+        v[0, :, 149] *= 1e9
+        v[1, :, 130] *= 1e9
+    a["v_text"] = v.to(torch.bfloat16)
+    quantise_text(a)
+    check(a)
