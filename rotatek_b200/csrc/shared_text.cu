@@ -11,7 +11,7 @@
 // it).  Two kernels:
 //
 // - The warps split the rows, 16 each (64 of a CTA), and share tiles of 32 tokens through one
-//   cp.async ring; an 8-bit tile is converted to f16 in shared memory once for all of them.
+//   cp.async ring; an 8-bit tile is converted to 16 bits in shared memory once for all of them.
 // - 8-bit text of at most 16 rows: the warps split the tokens, blocks of 32 in rings of their
 //   own (no CTA-wide barrier in the loop), convert in registers, and join at the end.
 //
@@ -26,10 +26,9 @@
 // within a step of 109 us, 4.9 TB/s with all that is not text); with 8-bit text the
 // conversions (277 MB within 90 us); with few questions the latency of a chunk.
 //
-// 8-bit text: e4m3 is exact in f16 and in bf16.  S runs in f16: queries go in scaled by a power of
-// two per row (bf16 has more range, f16 more bits: exact but for what lies 2^-24 below the row's
-// largest), a token's Key scale multiplies its logit.  P . V runs in bf16, which has fp32's range:
-// a token's Value scale multiplies its weight, and scales of any ratio may meet in one row.
+// 8-bit text: e4m3 is exact in f16 and in bf16.  S runs in the queries' type, a token's Key
+// scale multiplies its logit.  P . V runs in bf16, which has fp32's range: a token's Value scale
+// multiplies its weight, and scales of any ratio may meet in one row.
 // In registers: ldmatrix of Key bytes gives lane (g, j) bytes 4j .. 4j+3 of token g: the MMA's
 // k index runs over a 16-channel group in the order 0 1 4 5 8 9 12 13 2 3 6 7 10 11 14 15, and
 // the queries are stored in that order.  ldmatrix.trans of Value bytes pairs two tokens' bytes
@@ -84,10 +83,6 @@ __device__ __forceinline__ void cp_async_4_zfill(void *dst, const void *src, boo
 // at multiples of 256 bytes).
 __device__ __forceinline__ uint32_t even(uint32_t lane_addr, int even_chunk) { return lane_addr ^ (even_chunk << 4); }
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  mma_16816<__half>(d, a, b0, b1);
-}
-
 __device__ __forceinline__ uint32_t e4m3x2_f16x2(uint16_t v) {
   uint32_t r;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
@@ -98,6 +93,12 @@ __device__ __forceinline__ uint32_t e4m3x2_bf16x2(uint16_t v) {
   float lo, hi;
   unpack2<__half>(e4m3x2_f16x2(v), lo, hi);
   return pack2<__nv_bfloat16>(lo, hi);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t e4m3x2_16(uint16_t v) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return e4m3x2_bf16x2(v);
+  else return e4m3x2_f16x2(v);
 }
 
 // Two weights as 16-bit parts: the nearest, and the nearest to what that leaves.
@@ -163,8 +164,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_kernel(const TextP
     cp_async_commit();
   }
 
-  // queries: 16 rows x 128 channels; per-row factor of the logits
-  __shared__ float qscale_s[16];
+  // queries: 16 rows x 128 channels
   uint2 qv[4];                                       // all in flight at once
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -179,41 +179,21 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_kernel(const TextP
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int e = warp + kWarps * k;
-    const uint2 v = qv[k];
-    float f = a.scale_log2;
-    float x[4];
-    unpack2<T>(v.x, x[0], x[1]);
-    unpack2<T>(v.y, x[2], x[3]);
-    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-      float mx = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      // 2^e with mx / 2^e in [1, 2): the exponent bits of mx (0 and subnormals: 2^-126)
-      const uint32_t ex = min(max(__float_as_uint(mx) >> 23, 1u), 253u);
-      const float inv = __uint_as_float((254u - ex) << 23);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] *= inv;
-      f *= __uint_as_float(ex << 23);
-    }
     // channels 4 jj .. 4 jj + 3 of a 16-channel group go to positions 2 jj, 2 jj + 1 and
     // 2 jj + 8, 2 jj + 9 (lane = 4 * group + jj)
     const int grp = lane >> 2, jj = lane & 3;
     const uint32_t q0 = smem_u32(smem + L::kQ);
-    const uint32_t w0 = pack2<__half>(x[0], x[1]), w1 = pack2<__half>(x[2], x[3]);
-    asm volatile("st.shared.b32 [%0], %1;" ::"r"(q0 + at<256>(e, 2 * grp) + jj * 4), "r"(w0) : "memory");
-    asm volatile("st.shared.b32 [%0], %1;" ::"r"(q0 + at<256>(e, 2 * grp + 1) + jj * 4), "r"(w1) : "memory");
-    if (lane == 0) qscale_s[e] = f;
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(q0 + at<256>(e, 2 * grp) + jj * 4), "r"(qv[k].x) : "memory");
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(q0 + at<256>(e, 2 * grp + 1) + jj * 4), "r"(qv[k].y) : "memory");
   }
   __syncthreads();
 
-  // per query row of this lane (g and g + 8): tokens it sees, logit factor
+  // tokens that the query rows of this lane (g and g + 8) see
   int limit[2];
-  float qf[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int r = g + 8 * i;
     limit[i] = r < p.rows ? len - (a.tokens - 1 - r / a.groups) : 0;
-    qf[i] = qscale_s[r];
   }
   const int all_see = len - (a.tokens - 1);          // every row sees tokens below this
 
@@ -266,9 +246,9 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_kernel(const TextP
       ldmatrix_x4(k_addr + at<128>(lane, k), r[0], r[1], r[2], r[3]);
 #pragma unroll
       for (int n = 0; n < 4; ++n)
-        mma_f16(s[n], qa, e4m3x2_f16x2((uint16_t)(r[n] & 0xffffu)), e4m3x2_f16x2((uint16_t)(r[n] >> 16)));
+        mma_16816<T>(s[n], qa, e4m3x2_16<T>((uint16_t)(r[n] & 0xffffu)), e4m3x2_16<T>((uint16_t)(r[n] >> 16)));
     }
-    // logits but for the row's factor; unseen tokens weigh nothing
+    // logits but for c; unseen tokens weigh nothing
     float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int n = 0; n < kNT; ++n)
@@ -291,7 +271,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_kernel(const TextP
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2)) * qf[i];      // qf > 0
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2)) * a.scale_log2;
       grow[i] = mx[i] > m[i] + kLazy;          // from -inf: whenever there is a maximum
     }
     if (__any_sync(0xffffffffu, grow[0] || grow[1])) {
@@ -313,8 +293,8 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_kernel(const TextP
     for (int n = 0; n < kNT; ++n)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float w0 = fast_exp2(fmaf(s[n][2 * i], qf[i], -base[i]));
-        const float w1 = fast_exp2(fmaf(s[n][2 * i + 1], qf[i], -base[i]));
+        const float w0 = fast_exp2(fmaf(s[n][2 * i], a.scale_log2, -base[i]));
+        const float w1 = fast_exp2(fmaf(s[n][2 * i + 1], a.scale_log2, -base[i]));
         l[i] += w0 + w1;
         two_parts<__nv_bfloat16>(w0 * vscale[n][0], w1 * vscale[n][1], pa[n][i], pl[n][i]);
       }
@@ -409,7 +389,7 @@ struct RowsSmem {
   static constexpr int kRaw = kScales + (FP8 ? 2 * kTok * 4 : 0);
   static constexpr int kStages = 3;
   static constexpr int kQ = 0;                                    // 64 rows of 256 bytes
-  static constexpr int kTile = kQ + kWarps * 4096;                // FP8: the tile, Keys as f16, Values as bf16
+  static constexpr int kTile = kQ + kWarps * 4096;                // FP8: the tile, Keys in the queries' type, Values as bf16
   static constexpr int kRing = kTile + (FP8 ? 2 * kTok * 256 : 0);
   static constexpr int kBytes = kRing + kStages * kRaw;
 };
@@ -417,8 +397,7 @@ struct RowsSmem {
 template <typename T, bool FP8>
 __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const TextParams p) {
   using L = RowsSmem<FP8>;
-  using MK = typename std::conditional<FP8, __half, T>::type;            // operand type of S
-  using MV = typename std::conditional<FP8, __nv_bfloat16, T>::type;     // and of P . V
+  using MV = typename std::conditional<FP8, __nv_bfloat16, T>::type;     // operand type of P . V (of S: T)
   extern __shared__ __align__(1024) unsigned char smem[];
   launch_dependents();
   const SharedParams &a = p.s;
@@ -472,8 +451,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
     if (i < tiles) fetch();
     cp_async_commit();
   }
-  // this warp's 16 queries, in the MMA's type (bf16 against 8-bit text: f16 scaled by a power of two)
-  __shared__ float qscale_s[kWarps * 16];
+  // this warp's 16 queries
   uint2 qv[16];                                      // all in flight at once
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
@@ -486,34 +464,16 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
     }
   }
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    uint2 v = qv[e];
-    float f = a.scale_log2;
-    if constexpr (FP8 && std::is_same<T, __nv_bfloat16>::value) {
-      float x[4];
-      unpack2<T>(v.x, x[0], x[1]);
-      unpack2<T>(v.y, x[2], x[3]);
-      float mx = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      const uint32_t ex = min(max(__float_as_uint(mx) >> 23, 1u), 253u);
-      const float inv = __uint_as_float((254u - ex) << 23);
-      v.x = pack2<__half>(x[0] * inv, x[1] * inv);
-      v.y = pack2<__half>(x[2] * inv, x[3] * inv);
-      f *= __uint_as_float(ex << 23);
-    }
-    *reinterpret_cast<uint2 *>(smem + L::kQ + at<256>(warp * 16 + e, lane >> 1) + (lane & 1) * 8) = v;
-    if (lane == 0) qscale_s[warp * 16 + e] = f;
-  }
+  for (int e = 0; e < 16; ++e)
+    *reinterpret_cast<uint2 *>(smem + L::kQ + at<256>(warp * 16 + e, lane >> 1) + (lane & 1) * 8) = qv[e];
   __syncwarp();
   const bool busy = row0 < p.rows;
   int limit[2];
-  float qf[2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, acc[16][4];
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, acc[16][4];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int r = row0 + g + 8 * i;
     limit[i] = r < p.rows ? len - (a.tokens - 1 - r / a.groups) : 0;
-    qf[i] = qscale_s[warp * 16 + g + 8 * i];
   }
 #pragma unroll
   for (int n = 0; n < 16; ++n)
@@ -553,7 +513,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const uint16_t two = (uint16_t)(in[k >> 1] >> (16 * (k & 1)));
-          out[k] = value ? e4m3x2_bf16x2(two) : e4m3x2_f16x2(two);
+          out[k] = value ? e4m3x2_bf16x2(two) : e4m3x2_16<T>(two);
         }
         *reinterpret_cast<uint4 *>(smem + L::kTile + at<256>(r, 2 * c)) = make_uint4(out[0], out[1], out[2], out[3]);
         *reinterpret_cast<uint4 *>(smem + L::kTile + at<256>(r, 2 * c + 1)) = make_uint4(out[4], out[5], out[6], out[7]);
@@ -578,10 +538,10 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
       ldmatrix_x4(even(q_lane, 2 * k), qa[0], qa[1], qa[2], qa[3]);
       ldmatrix_x4(even(k_lane, 2 * k), r[0], r[1], r[2], r[3]);
       ldmatrix_x4(even(k_lane2, 2 * k), r2[0], r2[1], r2[2], r2[3]);
-      mma_16816<MK>(s[0], qa, r[0], r[1]);
-      mma_16816<MK>(s[1], qa, r[2], r[3]);
-      mma_16816<MK>(s[2], qa, r2[0], r2[1]);
-      mma_16816<MK>(s[3], qa, r2[2], r2[3]);
+      mma_16816<T>(s[0], qa, r[0], r[1]);
+      mma_16816<T>(s[1], qa, r[2], r[3]);
+      mma_16816<T>(s[2], qa, r2[0], r2[1]);
+      mma_16816<T>(s[3], qa, r2[2], r2[3]);
     }
     if constexpr (FP8) {
 #pragma unroll
@@ -605,7 +565,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2)) * qf[i];
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2)) * a.scale_log2;
       grow[i] = mx[i] > m[i] + kLazy;
     }
     if (__any_sync(0xffffffffu, grow[0] || grow[1])) {
@@ -627,7 +587,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
     for (int n = 0; n < kNT; ++n)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float w0 = fast_exp2(fmaf(s[n][2 * i], qf[i], -base[i])), w1 = fast_exp2(fmaf(s[n][2 * i + 1], qf[i], -base[i]));
+        float w0 = fast_exp2(fmaf(s[n][2 * i], a.scale_log2, -base[i])), w1 = fast_exp2(fmaf(s[n][2 * i + 1], a.scale_log2, -base[i]));
         l[i] += w0 + w1;
         if constexpr (FP8) {
           w0 *= vscale[n][0];

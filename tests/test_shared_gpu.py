@@ -722,3 +722,14 @@ def test_decode_text8_small_values_hold_the_weight(beside, size, T):
     a["v_text"] = v.to(torch.bfloat16)
     quantise_text(a)
     check(a)
+
+
+@pytest.mark.parametrize("T", [1, 9])
+def test_decode_text8_queries_of_any_range(T):
+    """bf16 queries with one channel 2^18 times the others, where the Keys are 0: the other
+    channels alone make the logits, and keep their bits."""
+    a = make(1, 3, T, 8, 2, 0, 0, 60, 32, dtype=torch.bfloat16, lens=[60, 33, 20], seed=55, std=0.5)
+    a["q"][..., 7] = 2.0 ** 18
+    a["k_text"][..., 7] = 0
+    quantise_text(a)
+    check_weights(a)
