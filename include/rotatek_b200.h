@@ -239,8 +239,9 @@ size_t rtk_shared_decode_workspace_size(int64_t prefixes, int64_t batch, int64_t
  * Query t of question b sees all of its prefix and its text rows s <
  * text_lens[b] - (T - 1 - t).  out = softmax([q.k_f ; q.R.k_s + q.delta_mu ;
  * q.k_text] / sqrt(D)) . [v_f ; v_s ; v_text], 0 for a row that sees nothing.
- * Rows of a cache past text_lens and masked prompt tokens may hold anything; a
- * NaN logit makes its row NaN.
+ * What a query does not see -- rows past text_lens, later drafts' rows, masked
+ * prompt tokens -- may hold anything.  A NaN logit makes its row NaN, a Value
+ * that is seen and not finite leaves its channel of the row not finite.
  * `status` (device uint32, nullable) gets RTK_DEVICE_TIMEOUT if a bounded wait
  * gives up.                                                                   */
 int rtk_shared_decode(const rtk_tensor *q, const rtk_tensor *R_partial, const rtk_tensor *delta_mu,

@@ -35,7 +35,10 @@
 // of channels (2g, 2g+1): one byte permute separates them into B fragments of an "even" and
 // an "odd" n-tile.  P is taken in two 16-bit parts, as the prefix kernel's; l sums it unrounded.
 //
-// Tokens past the length are zero-filled on the way in (cp.async reads nothing there).
+// Tokens past the length are zero-filled on the way in (cp.async reads nothing there).  The last
+// T - 1 tokens within it are seen by some rows only: their weight is 0 in the others, but 0 times
+// a Value that is not finite is NaN.  Such Values are taken out of their tile, and the rows that
+// do see one (a row that sees a token sees all before it) get NaN in its channel at the end.
 //
 // The kernels may run beside the prefix kernel launched before (they need nothing of it); one
 // CTA waits for that one before it ends, so that the join, which waits for this kernel to
@@ -110,6 +113,66 @@ __device__ __forceinline__ void two_parts(float w0, float w1, uint32_t &hi, uint
   lo = pack2<M>(w0 - h0, w1 - h1);
 }
 
+// Whether a 16-byte piece holds infinities or NaN: an exponent of ones (e4m3: all of 0x7f)
+// carries into the sign's place.
+template <typename M>
+__device__ __forceinline__ bool not_finite(const uint4 &v) {
+  constexpr bool k8 = sizeof(M) == 1;
+  constexpr uint32_t kUnit = k8 ? 0x01010101u : std::is_same<M, __nv_bfloat16>::value ? 0x00800080u : 0x04000400u;
+  constexpr uint32_t kSign = k8 ? 0x80808080u : 0x80008000u;
+  auto carry = [](uint32_t w) { return (w & ~kSign) + kUnit; };
+  return ((carry(v.x) | carry(v.y) | carry(v.z) | carry(v.w)) & kSign) != 0;
+}
+
+constexpr int kNoToken = 0x7fffffff;
+
+// Values (M, or e4m3 bytes) of tokens [s0, s1) of a tile that are not finite become 0; the first such
+// token of a channel is left in apart_s.  By a whole warp; warps that share a tile may do the
+// same at once.
+template <typename M>
+__device__ __noinline__ void take_apart(unsigned char *tile, int s0, int s1, int first, int *apart_s) {
+  constexpr int kRow = 128 * sizeof(M), kPieces = kRow / 16, kEach = 16 / sizeof(M);
+  using Bits = typename std::conditional<sizeof(M) == 1, unsigned char, unsigned short>::type;
+  constexpr unsigned kTop = sizeof(M) == 1 ? 0x7fu : std::is_same<M, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+  const int lane = threadIdx.x & 31;
+  for (int s = s0; s < s1; ++s) {
+    if (lane >= kPieces) continue;
+    Bits *x = reinterpret_cast<Bits *>(tile + at<kRow>(s, lane));
+    for (int k = 0; k < kEach; ++k)
+      if ((x[k] & kTop) == kTop) {
+        atomicMin(&apart_s[lane * kEach + k], first + s);
+        x[k] = 0;
+      }
+  }
+  __syncwarp();
+}
+
+// Whether tokens [s0, s1) of a tile hold a Value that is not finite; the whole warp asks.
+template <typename M>
+__device__ __forceinline__ bool any_not_finite(const unsigned char *tile, int s0, int s1) {
+  constexpr int kRow = 128 * sizeof(M), kPieces = kRow / 16;
+  const int lane = threadIdx.x & 31;
+  bool any = false;
+  for (int s = s0 + lane / kPieces; s < s1; s += 32 / kPieces)
+    any |= not_finite<M>(*reinterpret_cast<const uint4 *>(tile + at<kRow>(s, lane % kPieces)));
+  return __any_sync(0xffffffffu, any);
+}
+
+// The same for Value scales: vscale[n][k] is that of token 8 n + 2 j4 + k, `scales` the tile's in shared memory.
+__device__ __forceinline__ bool scales_apart(const unsigned char *scales, float (&vscale)[4][2], int s0, int s1, int first,
+                                             int *apart_s) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t bad = __ballot_sync(0xffffffffu, lane >= s0 && lane < s1 && !isfinite(reinterpret_cast<const float *>(scales)[lane]));
+  if (bad == 0) return false;
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if ((bad >> (8 * n + 2 * (lane & 3) + k)) & 1u) vscale[n][k] = 0.f;
+  for (int c = lane; c < 128; c += 32) atomicMin(&apart_s[c], first + __ffs(bad) - 1);
+  return true;
+}
+
 // The kernel ends after the one before it.
 __device__ __forceinline__ void end_after_previous() {
   if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) wait_for_previous();
@@ -119,11 +182,13 @@ template <typename T>
 __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_kernel(const TextParams p) {
   using L = TextSmem;
   extern __shared__ __align__(1024) unsigned char smem[];
+  __shared__ int apart_s[128];                       // per channel: the first token taken apart
   launch_dependents();
   const SharedParams &a = p.s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, j4 = lane & 3;
   const int chunk = blockIdx.y, bh = blockIdx.x;
+  apart_s[threadIdx.x] = kNoToken;
   const int b = bh / a.kv_heads, h = bh % a.kv_heads;
   const int len = min(max(a.lens[b * a.lens_s], 0), a.cap);
   const int t0 = chunk * p.chunk;
@@ -210,6 +275,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_kernel(const TextP
   const uint32_t q_lane = smem_u32(smem + L::kQ) + at<256>(lane & 15, lane >> 4);
 
   int stage = 0;
+  bool apart = false;
   for (int blk = warp; blk < blocks; blk += kWarps) {
     const int first = t0 + blk * L::kTok;
     constexpr int kNT = L::kTok / 8;                 // n-tiles of 8 tokens
@@ -231,6 +297,15 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_kernel(const TextP
       const float2 v2 = *reinterpret_cast<const float2 *>(sc + 128 + (n * 8 + 2 * j4) * 4);
       kscale[n][0] = k2.x; kscale[n][1] = k2.y;
       vscale[n][0] = v2.x; vscale[n][1] = v2.y;
+    }
+    if (all_see < min(t1, first + L::kTok)) {      // tokens that some rows do not see
+      const int s0 = max(all_see - first, 0), s1 = min(t1 - first, L::kTok);
+      unsigned char *v = ring + stage * L::kStage + L::kTok * L::kRow;
+      if (any_not_finite<unsigned char>(v, s0, s1)) {
+        take_apart<unsigned char>(v, s0, s1, first, apart_s);
+        apart = true;
+      }
+      apart |= scales_apart(sc + 128, vscale, s0, s1, first, apart_s);
     }
     float s[kNT][4];
 #pragma unroll
@@ -322,7 +397,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_kernel(const TextP
     if (++stage == L::kStages) stage = 0;
   }
   cp_async_wait_all();
-  __syncthreads();                                   // every warp is done with its ring
+  const bool any_apart = __syncthreads_or(apart);    // every warp is done with its ring
 
   // join the warps, in warp order
   float *o_s = reinterpret_cast<float *>(smem + L::kRing);
@@ -334,6 +409,13 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_kernel(const TextP
     ll += __shfl_xor_sync(0xffffffffu, ll, 2);
     const int e = g + 8 * i;
     if (j4 == 0) ml_s[warp * 16 + e] = make_float2(m[i], ll);
+    if (any_apart) {
+#pragma unroll
+      for (int c = 0; c < 8; ++c)                    // acc[2 c + odd][2 i + k] is channel 16 c + 4 j4 + 2 k + odd
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (limit[i] > apart_s[16 * c + 4 * j4 + k]) acc[2 * c + (k & 1)][2 * i + (k >> 1)] = NAN;
+    }
     float *row = o_s + (warp * 16 + e) * 128;
 #pragma unroll
     for (int c = 0; c < 8; ++c)
@@ -399,10 +481,12 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
   using L = RowsSmem<FP8>;
   using MV = typename std::conditional<FP8, __nv_bfloat16, T>::type;     // operand type of P . V (of S: T)
   extern __shared__ __align__(1024) unsigned char smem[];
+  __shared__ int apart_s[128];                       // per channel: the first token taken apart
   launch_dependents();
   const SharedParams &a = p.s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, j4 = lane & 3;
+  apart_s[threadIdx.x] = kNoToken;
   const int chunk = blockIdx.y, bh = blockIdx.x, row0 = blockIdx.z * 64 + warp * 16;
   const int b = bh / a.kv_heads, h = bh % a.kv_heads;
   const int len = min(max(a.lens[b * a.lens_s], 0), a.cap);
@@ -483,6 +567,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
   const uint32_t q_lane = smem_u32(smem + L::kQ) + at<256>(warp * 16 + (lane & 15), lane >> 4);
   const uint32_t k_at = at<256>((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1), v_at = at<256>(lane & 15, lane >> 4);
 
+  bool apart = false;
   for (int tile = 0; tile < tiles; ++tile) {
     const int first = t0 + tile * L::kTok;
     constexpr int kNT = 4;
@@ -526,6 +611,15 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
       v_addr = k_addr + L::kTok * 256;
     }
     if (!busy) continue;
+    if (all_see < min(t1, first + L::kTok)) {        // tokens that some rows do not see
+      const int s0 = max(all_see - first, 0), s1 = min(t1 - first, L::kTok);
+      unsigned char *v = smem + (FP8 ? L::kTile : L::kRing + tile % L::kStages * L::kRaw) + L::kTok * 256;
+      if (any_not_finite<MV>(v, s0, s1)) {
+        take_apart<MV>(v, s0, s1, first, apart_s);
+        apart = true;
+      }
+      if constexpr (FP8) apart |= scales_apart(raw + L::kScales + 128, vscale, s0, s1, first, apart_s);
+    }
     float s[kNT][4];
 #pragma unroll
     for (int n = 0; n < kNT; ++n)
@@ -611,6 +705,13 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_rows_kernel(const 
     }
   }
   cp_async_wait_all();
+  if (__syncthreads_or(apart)) {
+#pragma unroll
+    for (int n = 0; n < 16; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (limit[i >> 1] > apart_s[8 * n + 2 * j4 + (i & 1)]) acc[n][i] = NAN;
+  }
   const long long slot = (long long)bh * p.chunks + chunk;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {

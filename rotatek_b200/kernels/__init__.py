@@ -337,8 +337,8 @@ def rotatek_shared_decode(
     and text logits the full query; all share one softmax.  A row that sees
     nothing gives 0.  Text caches hold q's dtype, or e4m3 rows with one scale
     each (``append_text``; uint8 or float8_e4m3fn tensors).  Inputs may be
-    strided views; rows past ``text_lens`` and masked prompt tokens may hold
-    anything.  bf16 / fp16 with D = 128, D_keep 16, 32 or 64 and 16-byte aligned
+    strided views; what a query does not see (rows past ``text_lens``, later
+    drafts' rows, masked prompt tokens) may hold anything.  bf16 / fp16 with D = 128, D_keep 16, 32 or 64 and 16-byte aligned
     channel-contiguous rows run on the tensor cores, anything else (fp32, D up to
     256) on a generic kernel.  No counterpart in the reference."""
     if q.dim() != 4:

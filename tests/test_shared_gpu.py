@@ -733,3 +733,33 @@ def test_decode_text8_queries_of_any_range(T):
     a["k_text"][..., 7] = 0
     quantise_text(a)
     check_weights(a)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("dtype,fp8", [(torch.bfloat16, False), (torch.float16, False), (torch.bfloat16, True),
+                                       (torch.float16, True), (torch.float32, True)])
+@pytest.mark.parametrize("T,lens", [(4, [33, 64, 7, 4]), (9, [33, 64, 40, 9]), (40, [45, 64, 40, 70])])
+@pytest.mark.parametrize("back", [1, 3])
+def test_decode_later_drafts_do_not_reach_earlier_queries(back, T, lens, dtype, fp8, bad):
+    """The row of the last draft but `back - 1` holds NaN or infinity in its Key, its Value and their
+    scales: the queries before it stay the same to the bit, it and those after it show it."""
+    from rotatek_b200.kernels import rotatek_shared_decode
+    a = make(1, 4, T, 8, 2, 140, 20, 70, 32, dtype=dtype, fp8=fp8, lens=lens, seed=61)
+    clean = rotatek_shared_decode(**a)
+    at = a["text_lens"].long() - back
+    rows = torch.arange(4, device=DEV)
+    variants = [("v_text", True)] + ([("v_scale", True), ("k_scale", True)] if fp8 else [("k_text", bad != bad)])
+    for name, shows in variants:
+        b = dict(a, **{name: a[name].clone()})
+        if b[name].dtype == torch.uint8:
+            b[name][rows, :, at, 64:] = 0x7F               # e4m3's NaN; the other channels stay numbers
+        elif name == "v_text":
+            b[name][rows, :, at, 64:] = bad
+        else:
+            b[name][rows, :, at] = bad
+        got = rotatek_shared_decode(**b)
+        assert torch.equal(got[:, :T - back], clean[:, :T - back])
+        if name == "v_text":
+            assert torch.isfinite(got[..., :64]).all() and not torch.isfinite(got[:, T - back:, :, 64:]).any()
+        elif shows and bad != bad:
+            assert torch.isnan(got[:, T - back:]).all()
