@@ -219,7 +219,9 @@ int rtk_spark_pack(const rtk_tensor *keep_mask, const rtk_tensor *keep_idx_out, 
 
 /* Bytes of workspace rtk_shared_decode needs for these shapes on `device`
  * (16-byte aligned, no zeroing required, free again when the call's kernels
- * have run). */
+ * have run).  A call is several launches: two host threads must not give one
+ * workspace to calls at the same time, not even on one stream.  The same holds
+ * for rtk_verify_drafts. */
 size_t rtk_shared_decode_workspace_size(int64_t prefixes, int64_t batch, int64_t tokens, int64_t q_heads,
                                         int64_t kv_heads, int64_t seq_full, int64_t seq_sparse, int64_t text_cap,
                                         int32_t device);

@@ -201,20 +201,22 @@ def workspace(device: torch.device, nbytes: int, counter_bytes: int) -> torch.Te
         return buf
 
 
-_scratch = {}        # (device index, stream address) -> uint8 buffer
+_scratch = threading.local()      # .buffers: (device index, stream address) -> uint8 buffer
 
 
 def scratch(device: torch.device, stream: int, nbytes: int = 0) -> torch.Tensor:
-    """Scratch of a stream's own, at least `nbytes` long, for kernels that need nothing
-    zeroed and nothing kept: calls on one stream follow one another on the GPU, calls on
-    several do not share it.  Grown on demand; a call that is being captured gets a
-    buffer of the capture's own."""
+    """Scratch of this thread on a stream, at least `nbytes` long, for kernels that need
+    nothing zeroed and nothing kept.  A call is several launches, and those of two threads
+    on one stream may alternate: each thread has a buffer of its own, in which its calls
+    follow one another.  Grown on demand; a call that is being captured gets a buffer of
+    the capture's own."""
     if torch._C._cuda_isCurrentStreamCapturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    buf = _scratch.get((device.index, stream))
+    buffers = _scratch.__dict__.setdefault("buffers", {})
+    buf = buffers.get((device.index, stream))
     if buf is None or buf.numel() < nbytes:
         buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-        _scratch[(device.index, stream)] = buf
+        buffers[(device.index, stream)] = buf
     return buf
 
 

@@ -157,3 +157,28 @@ def test_oracle_rows_quantise_as_torch_does():
     val, scale = osh.quantize_rows(x)
     want = (x / scale[:, None]).to(torch.float8_e4m3fn).double()
     assert torch.equal(val, want)
+
+
+def test_scratch_is_a_threads_own(monkeypatch):
+    """A call is several launches over its scratch, and the launches of two threads on one
+    stream may alternate: they share no scratch."""
+    import threading
+
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: False)
+    here, barrier, got = torch.device("cpu"), threading.Barrier(2, timeout=60), {}
+
+    def call(who):
+        mine = _lib.scratch(here, 0, 5000)
+        barrier.wait()                                   # both calls are under way
+        got[who] = (mine, _lib.scratch(here, 0, 3000), _lib.scratch(here, 1, 3000))
+        barrier.wait()
+
+    threads = [threading.Thread(target=call, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for who in range(2):
+        mine, again, elsewhere = got[who]
+        assert again.data_ptr() == mine.data_ptr() != elsewhere.data_ptr()
+    assert got[0][0].data_ptr() != got[1][0].data_ptr() and got[0][2].data_ptr() != got[1][2].data_ptr()

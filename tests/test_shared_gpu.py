@@ -763,3 +763,30 @@ def test_decode_later_drafts_do_not_reach_earlier_queries(back, T, lens, dtype, 
             assert torch.isfinite(got[..., :64]).all() and not torch.isfinite(got[:, T - back:, :, 64:]).any()
         elif shows and bad != bad:
             assert torch.isnan(got[:, T - back:]).all()
+
+
+def test_threads_on_one_stream():
+    """Threads that share the default stream, with calls of several launches each: every result is
+    that of the call alone, to the bit."""
+    import threading
+    from rotatek_b200.kernels import rotatek_shared_decode, verify_drafts
+    args = [make(2, 3, 2, 8, 2, 700, 90, 150, 32, fp8=bool(i % 2), seed=70 + i) for i in range(4)]
+    logits = [make_verify(6, 3, 9000, torch.bfloat16, True, 80 + i) for i in range(4)]
+    want = [(rotatek_shared_decode(**a), *verify_drafts(**v)) for a, v in zip(args, logits)]
+    torch.cuda.synchronize()
+    out = [[] for _ in range(4)]
+
+    def call(i):
+        for _ in range(60):
+            out[i].append((rotatek_shared_decode(**args[i]), *verify_drafts(**logits[i])))
+
+    threads = [threading.Thread(target=call, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(4):
+        assert len(out[i]) == 60
+        for got in out[i]:
+            assert all(torch.equal(g, w) for g, w in zip(got, want[i]))
