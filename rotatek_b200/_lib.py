@@ -202,15 +202,17 @@ def workspace(device: torch.device, nbytes: int, counter_bytes: int) -> torch.Te
 
 
 _scratch = threading.local()      # .buffers: (device index, stream address) -> uint8 buffer
+SCRATCH_KEPT = 64 << 20           # bytes; a longer one is the call's own
 
 
 def scratch(device: torch.device, stream: int, nbytes: int = 0) -> torch.Tensor:
     """Scratch of this thread on a stream, at least `nbytes` long, for kernels that need
     nothing zeroed and nothing kept.  A call is several launches, and those of two threads
     on one stream may alternate: each thread has a buffer of its own, in which its calls
-    follow one another.  Grown on demand; a call that is being captured gets a buffer of
-    the capture's own."""
-    if torch._C._cuda_isCurrentStreamCapturing():
+    follow one another.  Grown on demand up to SCRATCH_KEPT; beyond that, and in a call
+    that is being captured, the buffer is the call's alone (the caching allocator gives
+    it out again in the stream's order)."""
+    if nbytes > SCRATCH_KEPT or torch._C._cuda_isCurrentStreamCapturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
     buffers = _scratch.__dict__.setdefault("buffers", {})
     buf = buffers.get((device.index, stream))

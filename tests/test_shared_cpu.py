@@ -182,3 +182,11 @@ def test_scratch_is_a_threads_own(monkeypatch):
         mine, again, elsewhere = got[who]
         assert again.data_ptr() == mine.data_ptr() != elsewhere.data_ptr()
     assert got[0][0].data_ptr() != got[1][0].data_ptr() and got[0][2].data_ptr() != got[1][2].data_ptr()
+
+
+def test_long_scratch_is_not_kept(monkeypatch):
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: False)
+    here = torch.device("cpu")
+    long = _lib.scratch(here, 7, (64 << 20) + 1)
+    assert long.numel() >= (64 << 20) + 1
+    assert _lib.scratch(here, 7).numel() <= 64 << 20
