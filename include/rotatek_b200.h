@@ -244,14 +244,18 @@ size_t rtk_shared_decode_workspace_size(int64_t prefixes, int64_t batch, int64_t
  * What a query does not see -- rows past text_lens, later drafts' rows, masked
  * prompt tokens -- may hold anything.  A NaN logit makes its row NaN, a Value
  * that is seen and not finite leaves its channel of the row not finite.
- * `status` (device uint32, nullable) gets RTK_DEVICE_TIMEOUT if a bounded wait
- * gives up.                                                                   */
+ * `status` (device uint32) gets RTK_DEVICE_TIMEOUT if a bounded wait gives up;
+ * NULL: the device's own word, which rtk_read_shared_status reads.            */
 int rtk_shared_decode(const rtk_tensor *q, const rtk_tensor *R_partial, const rtk_tensor *delta_mu,
                       const rtk_tensor *k_full, const rtk_tensor *v_full, const rtk_tensor *mask_full,
                       const rtk_tensor *k_sparse, const rtk_tensor *v_sparse, const rtk_tensor *k_text,
                       const rtk_tensor *v_text, const rtk_tensor *k_scale, const rtk_tensor *v_scale,
                       const rtk_tensor *text_lens, int64_t num_kv_groups, const rtk_tensor *out, void *workspace,
                       size_t workspace_bytes, void *status, void *stream);
+
+/* rtk_read_status for the word of the current device that rtk_shared_decode
+ * calls without a `status` report to.  Synchronises `stream`.                 */
+int rtk_read_shared_status(void *stream, uint32_t *status);
 
 /* Write T new Keys and Values of each question into its text cache, at rows
  * text_lens[b] .. text_lens[b] + counts[b] - 1 (counts nullable: T).  Rows that

@@ -50,6 +50,7 @@ SIGNATURES = {
     "rtk_shared_decode_workspace_size": (ctypes.c_size_t, [ctypes.c_int64] * 8 + [ctypes.c_int32]),
     "rtk_shared_decode": (ctypes.c_int, [_P] * 13 + [ctypes.c_int64, _P, ctypes.c_void_p, ctypes.c_size_t,
                                                      ctypes.c_void_p, ctypes.c_void_p]),
+    "rtk_read_shared_status": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint32)]),
     "rtk_append_text": (ctypes.c_int, [_P] * 8 + [ctypes.c_void_p]),
     "rtk_read_text": (ctypes.c_int, [_P] * 7 + [ctypes.c_void_p]),
     "rtk_verify_drafts_workspace_size": (ctypes.c_size_t, [ctypes.c_int64] * 3),
@@ -186,17 +187,25 @@ def workspace(device: torch.device, nbytes: int, counter_bytes: int) -> torch.Te
     the last one left (a larger batch * q_heads).  Calls are ordered on the
     current stream; callers that launch on several streams at once must
     synchronise them, as for the reference's shape-keyed scratch cache
-    (rotatek/kernels/fused_decode.py:47-70)."""
+    (rotatek/kernels/fused_decode.py:47-70).  What a call that is being captured fills
+    with zeros is zero when the graph runs, not now: a buffer made there is the
+    capture's own (``read_status`` does not see it), and a prefix zeroed there is not
+    counted on."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
+    capturing = torch._C._cuda_isCurrentStreamCapturing()
     with _ws_lock:
         buf = _workspaces.get(idx)
         if buf is None or buf.numel() < nbytes:
             size = max(nbytes, 1 << 20)
             buf = torch.zeros(size, dtype=torch.uint8, device=torch.device("cuda", idx))
+            if capturing:
+                return buf
             _workspaces[idx] = buf
             _zero_prefix[idx] = size
         if _zero_prefix[idx] < counter_bytes:
             buf[:counter_bytes].zero_()
+            if capturing:
+                return buf
         _zero_prefix[idx] = counter_bytes     # what follows is scratch after the call
         return buf
 
@@ -222,28 +231,20 @@ def scratch(device: torch.device, stream: int, nbytes: int = 0) -> torch.Tensor:
     return buf
 
 
-def status_word(device: torch.device) -> int:
-    """Address of the device's status word (the head of its decode workspace), for
-    entry points that take it apart from their scratch; ``read_status`` reads it."""
-    idx = device.index if device.index is not None else torch.cuda.current_device()
-    buf = _workspaces.get(idx)
-    if buf is None:
-        buf = workspace(device, 256, 256)
-    return buf.data_ptr()
-
-
 def read_status(device: Optional[torch.device] = None) -> int:
     """Device-status bits (RTK_DEVICE_TIMEOUT) recorded since the last read; clears them."""
     dev = device or torch.device("cuda", torch.cuda.current_device())
     idx = dev.index if dev.index is not None else torch.cuda.current_device()
-    buf = _workspaces.get(idx)
-    if buf is None:
-        return 0
-    out = ctypes.c_uint32(0)
-    stream = torch.cuda.current_stream(buf.device).cuda_stream
-    check(load().rtk_read_status(ctypes.c_void_p(buf.data_ptr()), ctypes.c_void_p(stream),
-                                 ctypes.byref(out)))
-    return out.value
+    bits, out = 0, ctypes.c_uint32(0)
+    with torch.cuda.device(idx):
+        stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+        check(load().rtk_read_shared_status(stream, ctypes.byref(out)))
+        bits |= out.value
+        buf = _workspaces.get(idx)
+        if buf is not None:
+            check(load().rtk_read_status(ctypes.c_void_p(buf.data_ptr()), stream, ctypes.byref(out)))
+            bits |= out.value
+    return bits
 
 
 def read_static_status() -> int:

@@ -77,8 +77,7 @@ bool rows16(const rtk_tensor *t, int esize) {
   return true;
 }
 
-// ---- workspace of the tensor-core path: a status word for callers that give none,
-// the prefix partials, the text's
+// ---- workspace of the tensor-core path: the prefix partials, the text's
 struct SharedSpace {
   size_t prefix_ml, prefix_acc, text_ml, text_acc, bytes;
 };
@@ -88,7 +87,7 @@ size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 SharedSpace shared_space(const rtk::PrefixSplit &sp, int64_t batch, int64_t kv_heads, int64_t rows, int64_t chunks) {
   SharedSpace w;
   const size_t slots = (size_t)sp.slots() * 128, text = (size_t)(batch * kv_heads * chunks * rows);
-  w.prefix_ml = 256;
+  w.prefix_ml = 0;
   w.prefix_acc = up256(w.prefix_ml + slots * 8);
   w.text_ml = up256(w.prefix_acc + slots * 512);
   w.text_acc = up256(w.text_ml + text * 8);
@@ -245,7 +244,7 @@ int rtk_shared_decode(const rtk_tensor *q, const rtk_tensor *R_partial, const rt
     std::swap(Rt.stride[2], Rt.stride[3]);
     pp.R_layout = rows16(R_partial, 2) ? 1 : rows16(&Rt, 2) ? 2 : 0;
     pp.ml = pml; pp.acc = pacc;
-    pp.status = static_cast<unsigned int *>(status != nullptr ? status : workspace);
+    pp.status = static_cast<unsigned int *>(status);
     e = rtk::launch_shared_prefix(maps, pp, st);
     if (e != cudaSuccess) return cuda_fail(e, "shared decode (prefix kernel) launch");
   }
@@ -261,6 +260,14 @@ int rtk_shared_decode(const rtk_tensor *q, const rtk_tensor *R_partial, const rt
   e = rtk::launch_shared_merge(mp, st);
   if (e != cudaSuccess) return cuda_fail(e, "shared decode (merge kernel) launch");
   return RTK_OK;
+}
+
+int rtk_read_shared_status(void *stream, uint32_t *status) {
+  rtk::report_error(RTK_OK, "");
+  void *word = nullptr;
+  const cudaError_t e = rtk::shared_status_address(&word);
+  if (e != cudaSuccess) return cuda_fail(e, "rtk_read_shared_status");
+  return rtk_read_status(word, stream, status);
 }
 
 int rtk_append_text(const rtk_tensor *k_new, const rtk_tensor *v_new, const rtk_tensor *text_lens,

@@ -138,9 +138,11 @@ struct PrefixParams {
   PrefixSplit split;
   int R_layout;                 // R can be read 16 bytes at a time: 1 along its rows, 2 along its columns, 0 not
   float *ml, *acc;              // per slot: [128 rows][2] and [32 groups of 4 channels][128 rows][4]
-  unsigned int *status;
+  unsigned int *status;         // null: the device's own word
 };
 cudaError_t launch_shared_prefix(const PrefixMaps &maps, const PrefixParams &p, cudaStream_t stream);
+// Address of the current device's status word, which calls that give none report to.
+cudaError_t shared_status_address(void **address);
 
 // Text: CTAs per (question, KV head, chunk of tokens, 16 or 64 query rows).  Chunks of 256
 // tokens, so that few questions use many SMs; longer where that makes several waves of

@@ -63,6 +63,10 @@ constexpr uint32_t kColHi = 32;
 constexpr uint32_t kColO = 3 * kColsS;           // the O accumulator
 constexpr float kLazy = 8.f;
 
+// Where calls without a status word report a wait that gave up: zero when the library is
+// loaded, so that a call that is being captured finds it ready.
+__device__ unsigned int g_status;
+
 template <int DK>
 struct PrefixSmem {
   static constexpr int kKeyBytes = kVisTok * DK * 2;
@@ -190,6 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   launch_dependents();
   const PrefixSplit &sp = p.split;
   const SharedParams &a = p.s;
+  unsigned int *const status = p.status != nullptr ? p.status : &g_status;
   const int cta = blockIdx.x;
   const long long r0 = sp.range_begin(cta), r1 = sp.range_begin(cta + 1);
   const int u0 = (int)(r0 / sp.unit_weight), u1 = (int)((r1 - 1) / sp.unit_weight);   // r1 > r0
@@ -251,8 +256,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int stg = it % L::kStages;
           // one block ahead of the queries, the rest of the ring after them: every CTA's whole
           // ring would queue at HBM in front of them
-          if (it == 1) mbar_wait_bounded(q_bar, 0, abort_flag, p.status);
-          if (!mbar_wait_bounded(&empty_bar[stg], ((it / L::kStages) & 1) ^ 1, abort_flag, p.status)) {
+          if (it == 1) mbar_wait_bounded(q_bar, 0, abort_flag, status);
+          if (!mbar_wait_bounded(&empty_bar[stg], ((it / L::kStages) & 1) ^ 1, abort_flag, status)) {
             ok = false;
             break;
           }
@@ -275,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (*abort_flag) {                     // let the copies in flight land before the CTA exits
         int dead = 0;
         for (int k = it > L::kStages ? it - L::kStages : 0; k < it; ++k)
-          mbar_wait_bounded(&full_bar[k % L::kStages], (k / L::kStages) & 1, &dead, p.status);
+          mbar_wait_bounded(&full_bar[k % L::kStages], (k / L::kStages) & 1, &dead, status);
       }
     }
   } else if (warp >= 9) {
@@ -327,8 +332,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (for_s) {
           for (int j = j0; j < j1; ++j) {
             // the buffer's last P has been used (the first round finds its parity done)
-            mbar_wait_bounded(&pv_bar[buf], buf_par ^ 1u, abort_flag, p.status);
-            mbar_wait_bounded(&full_bar[stage], stage_par, abort_flag, p.status);
+            mbar_wait_bounded(&pv_bar[buf], buf_par ^ 1u, abort_flag, status);
+            mbar_wait_bounded(&full_bar[stage], stage_par, abort_flag, status);
             tc_fence_after();
             const uint32_t d = tmem + buf * kColsS;
             if (j >= sp.blocks_full) {
@@ -352,8 +357,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         } else {
           for (int j = j0; j < j1; ++j) {
-            mbar_wait_bounded(&full_bar[stage], stage_par, abort_flag, p.status);
-            mbar_wait_bounded(&up_bar[buf], buf_par, abort_flag, p.status);
+            mbar_wait_bounded(&full_bar[stage], stage_par, abort_flag, status);
+            mbar_wait_bounded(&up_bar[buf], buf_par, abort_flag, status);
             tc_fence_after();
             const uint32_t pa = tmem + buf * kColsS, first = j > j0;
             if (j >= sp.blocks_full) {
@@ -362,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int k = 0; k < kVisTok / 16; ++k) {
                 const int t = k ^ 4;                 // the upper tokens first
                 if (k == 4) {
-                  mbar_wait_bounded(&p_bar[buf], buf_par, abort_flag, p.status);
+                  mbar_wait_bounded(&p_bar[buf], buf_par, abort_flag, status);
                   tc_fence_after();
                 }
                 const uint32_t pk = pa + (t >> 2) * 64 + (t & 3) * 8;
@@ -370,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 umma_f16_ts(tmem + kColO, pk, vd + ((t * 2048) >> 4), kIdPv, 1u);
               }
             } else {
-              mbar_wait_bounded(&p_bar[buf], buf_par, abort_flag, p.status);
+              mbar_wait_bounded(&p_bar[buf], buf_par, abort_flag, status);
               tc_fence_after();
               const uint64_t vd = v_prompt + stage * kStep;
 #pragma unroll
@@ -480,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (vis) {
         if (x == 0) {
           // rotated queries out of TMEM, as two 16-bit parts into shared memory
-          mbar_wait_bounded(rot_bar, nrot & 1, abort_flag, p.status);
+          mbar_wait_bounded(rot_bar, nrot & 1, abort_flag, status);
           tc_fence_after();
 #pragma unroll
           for (int c = 0; c < DK; c += 16) {
@@ -547,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           v0 = __ballot_sync(0xffffffffu, lane < left && mk[tok * a.mask.s[1]] != 0);
           v1 = __ballot_sync(0xffffffffu, lane + 32 < left && mk[(tok + 32) * a.mask.s[1]] != 0);
         }
-        mbar_wait_bounded(&s_bar[buf], par, abort_flag, p.status);
+        mbar_wait_bounded(&s_bar[buf], par, abort_flag, status);
         tc_fence_after();
         const uint32_t s = tmem + lanes + buf * kColsS;
         if (masked && (v0 & v1) != ~0u) {
@@ -585,7 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (grow) now = top;
             if (k > 0) {                             // O is at rest when the P . V before is done
               const int g = it + k - 1;
-              mbar_wait_bounded(&pv_bar[g % 3], (g / 3) & 1, abort_flag, p.status);
+              mbar_wait_bounded(&pv_bar[g % 3], (g / 3) & 1, abort_flag, status);
               tc_fence_after();
               rescale_o(o_col, f);
               tc_fence_before();
@@ -621,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       it += blocks;
       // the partial result: each group writes 64 channels of the row
       ml_s[x * 128 + row] = make_float2(m, l);
-      mbar_wait_bounded(o_bar, no & 1, abort_flag, p.status);
+      mbar_wait_bounded(o_bar, no & 1, abort_flag, status);
       ++no;
       tc_fence_after();
       named_barrier_sync(2, 256);
@@ -674,6 +679,8 @@ cudaError_t launch(const PrefixMaps &maps, const PrefixParams &p, cudaStream_t s
 }
 
 }  // namespace
+
+cudaError_t shared_status_address(void **address) { return cudaGetSymbolAddress(address, g_status); }
 
 cudaError_t launch_shared_prefix(const PrefixMaps &maps, const PrefixParams &p, cudaStream_t stream) {
   const bool bf = p.s.dtype == 1;

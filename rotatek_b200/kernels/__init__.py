@@ -362,8 +362,7 @@ def rotatek_shared_decode(
     while True:
         ws = _lib.scratch(dev, stream, need)
         code = calls.shared_decode(q, R_partial, delta_mu, k_full, v_full, mask_full, k_sparse, v_sparse, k_text, v_text,
-                                   k_scale, v_scale, text_lens, out, num_kv_groups, ws.data_ptr(), ws.numel(),
-                                   _lib.status_word(dev), stream)
+                                   k_scale, v_scale, text_lens, out, num_kv_groups, ws.data_ptr(), ws.numel(), 0, stream)
         if code != _lib.RTK_ERR_WORKSPACE or need:
             break
         # the arguments are good, the stream's scratch is too small: nothing was launched

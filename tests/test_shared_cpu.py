@@ -190,3 +190,24 @@ def test_long_scratch_is_not_kept(monkeypatch):
     long = _lib.scratch(here, 7, (64 << 20) + 1)
     assert long.numel() >= (64 << 20) + 1
     assert _lib.scratch(here, 7).numel() <= 64 << 20
+
+
+def test_a_capture_leaves_no_workspace_behind(monkeypatch):
+    """What a captured call fills with zeros reads zero when the graph runs, not before: calls
+    outside the capture do not count on it."""
+    zeros, capturing = torch.zeros, [True]
+    monkeypatch.setattr(torch, "zeros", lambda n, dtype, device: zeros(n, dtype=dtype))
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: capturing[0])
+    monkeypatch.setattr(_lib, "_workspaces", {})
+    monkeypatch.setattr(_lib, "_zero_prefix", {})
+    dev = torch.device("cuda", 0)
+    assert _lib.workspace(dev, 5000, 700).numel() >= 5000 and not _lib._workspaces
+    capturing[0] = False
+    buf = _lib.workspace(dev, 5000, 700)
+    assert _lib._workspaces[0] is buf and _lib._zero_prefix[0] == 700
+    buf[700:] = 3                                        # scratch of that call
+    capturing[0] = True
+    assert _lib.workspace(dev, 5000, 4000) is buf and _lib._zero_prefix[0] == 700
+    capturing[0] = False
+    buf[700:] = 3                                        # as if the captured zeros had not been run
+    assert (_lib.workspace(dev, 5000, 4000)[:4000] == 0).all()

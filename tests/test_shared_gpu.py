@@ -790,3 +790,40 @@ def test_threads_on_one_stream():
         assert len(out[i]) == 60
         for got in out[i]:
             assert all(torch.equal(g, w) for g, w in zip(got, want[i]))
+
+
+FIRST_CALL = """
+import torch
+from rotatek_b200 import _lib, synthetic
+from rotatek_b200.kernels import rotatek_decode
+from tests.test_shared_gpu import compare, make
+from rotatek_b200.kernels import rotatek_shared_decode
+a = make(1, 4, 2, 8, 2, 500, 30, 64, 32, fp8=True, seed=19)
+d = synthetic.make_decode(2, 28, 4, 3000, 100, keep=32, seed=1, device="cuda:0", dtype=torch.bfloat16).as_kwargs()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = rotatek_shared_decode(**a)
+assert not _lib._workspaces
+h = torch.cuda.CUDAGraph()
+with torch.cuda.graph(h):
+    held, _, _ = rotatek_decode(**d)
+assert not _lib._workspaces
+eager, _, _ = rotatek_decode(**d)
+torch.cuda.synchronize()
+for _ in range(2):
+    g.replay()
+    h.replay()
+    torch.cuda.synchronize()
+    compare(out, a)
+    assert torch.equal(held, eager) and torch.equal(rotatek_decode(**d)[0], eager) and eager.abs().sum() > 0
+assert torch.equal(rotatek_shared_decode(**a), out) and _lib.read_status() == 0
+"""
+
+
+def test_first_call_of_a_process_may_be_captured():
+    import os
+    import subprocess
+    import sys
+    repo = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=repo, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
