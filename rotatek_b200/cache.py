@@ -176,15 +176,18 @@ class SharedPrefixCache:
         self.lens = torch.zeros(self.batch, dtype=torch.int32, device=dev)
         self.reach = 0                 # no row is longer than this
 
+    def need_room(self, tokens: int) -> None:
+        """Refuse ``tokens`` more per row where one may not have room for them."""
+        if self.reach + tokens > self.capacity:
+            raise ValueError(f"text caches full: {self.reach} + {tokens} tokens > capacity {self.capacity}")
+
     def append(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int,
                counts: Optional[torch.Tensor] = None, at: Optional[torch.Tensor] = None) -> None:
         """Write [B, H_kv, T, D] new Keys and Values of a layer behind the lengths
         (``at`` [B] int32: behind these instead); ``counts`` [B] int32: only the
         first counts[b] of them."""
         from rotatek_b200.kernels import append_text
-        t = key_states.shape[2]
-        if self.reach + t > self.capacity:
-            raise ValueError(f"text caches full: {self.reach} + {t} tokens > capacity {self.capacity}")
+        self.need_room(key_states.shape[2])
         k, v, ks, vs = self.text[layer_idx]
         append_text(key_states, value_states, self.lens if at is None else at, k, v, k_scale=ks, v_scale=vs,
                     counts=counts)
@@ -200,8 +203,7 @@ class SharedPrefixCache:
 
     def advance(self, tokens: torch.Tensor, most: int) -> None:
         """Lengthen every row by tokens[b] (device int32 [B], each at most ``most``)."""
-        if self.reach + most > self.capacity:
-            raise ValueError(f"text caches full: {self.reach} + {most} tokens > capacity {self.capacity}")
+        self.need_room(most)
         self.lens += tokens
         self.reach += most
 

@@ -67,14 +67,15 @@ class SharedQuestions:
 
     # ------------------------------------------------------------------ model
     @torch.no_grad()
-    def forward(self, tokens: torch.Tensor, start: torch.Tensor, layers: int, counts=None) -> torch.Tensor:
+    def forward(self, tokens: torch.Tensor, start: torch.Tensor, layers: int, counts=None, ahead: int = 0) -> torch.Tensor:
         """Logits [B, T, V] of T new tokens per question that follow ``start`` [B]
         int32 stored ones, through the first ``layers`` layers; their Keys and Values
-        are stored behind ``start``.  ``counts``: tokens[b, :counts[b]] are real, the
-        lengths end at start + counts, and the logits of real tokens alone mean
-        anything."""
+        are stored behind ``start``, which is at most ``ahead`` past the lengths.
+        ``counts``: tokens[b, :counts[b]] are real, the lengths end at start + counts,
+        and the logits of real tokens alone mean anything."""
         m, c = self.model, self.model.cfg
         b, t = tokens.shape
+        self.cache.need_room(ahead + t)          # the RoPE tables end where the caches do
         lens = start + (t if counts is None else counts)
         # query i of the T attends to rows < lens - (T - 1 - i): with ragged counts the real
         # tokens are moved to the end, so that the last one is the last query
@@ -114,6 +115,7 @@ class SharedQuestions:
     def ask(self, tokens: torch.Tensor, counts: torch.Tensor) -> torch.Tensor:
         """Put the questions in: tokens [B, T], the first counts[b] (int32, at least 1) of
         row b; returns the first answer token of each."""
+        self.cache.need_room(tokens.shape[1])
         logits = self.forward(tokens, self.cache.lens, self.model.cfg.layers, counts)
         self.cache.advance(counts, tokens.shape[1])
         self.last = self._draw(logits[:, -1].contiguous())
@@ -139,7 +141,7 @@ class SharedQuestions:
             return torch.where(drafts >= 0, drafts, self.last[:, None]), None
         token, drafts, logits = self.last, [], []
         for i in range(t):
-            out = self.forward(token[:, None], self.cache.lens + i, cfg.draft_layers)[:, 0]
+            out = self.forward(token[:, None], self.cache.lens + i, cfg.draft_layers, ahead=i)[:, 0]
             token = self._draw(out.contiguous())
             drafts.append(token)
             logits.append(out)
@@ -150,6 +152,7 @@ class SharedQuestions:
         """Draft, check and advance once: (tokens [B, T + 1] -- the new answer tokens, -1 past
         them -- and accepted [B])."""
         t = self.cfg.drafts
+        self.cache.need_room(t + 1)
         drafts, draft_logits = self._propose()
         logits = self.forward(torch.cat([self.last[:, None], drafts], 1), self.cache.lens, self.model.cfg.layers)
         tokens, accepted = verify_drafts(logits, drafts, draft_logits,

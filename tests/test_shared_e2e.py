@@ -113,3 +113,33 @@ def test_sampled_answers_run_and_stay_in_the_vocabulary():
         place = torch.arange(3, device="cuda")
         assert ((tokens >= 0) == (place <= accepted[:, None])).all() and (tokens < 300).all()
     assert all(6 <= len(a) <= 16 for a in s.answers())
+
+
+def test_a_full_cache_is_refused_before_anything_runs():
+    """Neither a step nor a question indexes the RoPE tables or drafts past the capacity."""
+    from types import SimpleNamespace
+
+    from rotatek_b200.shared_e2e import ServingConfig, SharedQuestions
+
+    class Untouched:
+        cfg = SimpleNamespace(layers=1)
+
+    def never(*args, **kwargs):
+        raise AssertionError("ran")
+
+    s = SharedQuestions.__new__(SharedQuestions)
+    s.cache, s.model, s.batch = SharedPrefixCache(_prefix(), 3, 8), Untouched(), 6
+    s.cfg = ServingConfig(questions=3, capacity=8, drafts=2, draft_layers=1)
+    s.last = torch.zeros(6, dtype=torch.int64)
+    s.cache.reach = 7
+    with pytest.raises(ValueError, match="full: 7 \\+ 2 tokens > capacity 8"):
+        s.forward(torch.zeros(6, 2, dtype=torch.int64), s.cache.lens, 1)
+    with pytest.raises(ValueError, match="full"):
+        s.forward(torch.zeros(6, 1, dtype=torch.int64), s.cache.lens + 1, 1, ahead=1)
+    s.forward = never
+    s.cache.reach = 6
+    with pytest.raises(ValueError, match="full: 6 \\+ 3 tokens > capacity 8"):
+        s.step()
+    s.cache.reach = 0
+    with pytest.raises(ValueError, match="full: 0 \\+ 9 tokens > capacity 8"):
+        s.ask(torch.zeros(6, 9, dtype=torch.int64), torch.full((6,), 9, dtype=torch.int32))
