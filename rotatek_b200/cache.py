@@ -182,12 +182,12 @@ class SharedPrefixCache:
             raise ValueError(f"text caches full: {self.reach} + {tokens} tokens > capacity {self.capacity}")
 
     def append(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int,
-               counts: Optional[torch.Tensor] = None, at: Optional[torch.Tensor] = None) -> None:
+               counts: Optional[torch.Tensor] = None, at: Optional[torch.Tensor] = None, ahead: int = 0) -> None:
         """Write [B, H_kv, T, D] new Keys and Values of a layer behind the lengths
-        (``at`` [B] int32: behind these instead); ``counts`` [B] int32: only the
-        first counts[b] of them."""
+        (``at`` [B] int32: behind these instead, which are at most ``ahead`` past the
+        lengths); ``counts`` [B] int32: only the first counts[b] of them."""
         from rotatek_b200.kernels import append_text
-        self.need_room(key_states.shape[2])
+        self.need_room(ahead + key_states.shape[2])
         k, v, ks, vs = self.text[layer_idx]
         append_text(key_states, value_states, self.lens if at is None else at, k, v, k_scale=ks, v_scale=vs,
                     counts=counts)

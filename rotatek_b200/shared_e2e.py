@@ -90,11 +90,11 @@ class SharedQuestions:
             q, k, v = m._qkv(L, x)
             q, k = m._rope(q, cos, sin), m._rope(k, cos, sin)
             if counts is None:
-                self.cache.append(k, v, li, at=start)
+                self.cache.append(k, v, li, at=start, ahead=ahead)
             else:                     # real tokens first, as they are stored
                 back = (torch.arange(t, device=self.device) + shift[:, None]).clamp_max(t - 1)
                 back = back[:, None, :, None].expand(b, c.kv_heads, t, c.head_dim).long()
-                self.cache.append(k.gather(2, back), v.gather(2, back), li, counts=counts, at=start)
+                self.cache.append(k.gather(2, back), v.gather(2, back), li, counts=counts, at=start, ahead=ahead)
             o = self.cache.attend(q.transpose(1, 2), li, lens, groups)
             x = x + F.linear(o.reshape(b, t, -1), L["wo"])
             x = x + m._mlp(L, x)

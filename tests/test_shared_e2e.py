@@ -143,3 +143,13 @@ def test_a_full_cache_is_refused_before_anything_runs():
     s.cache.reach = 0
     with pytest.raises(ValueError, match="full: 0 \\+ 9 tokens > capacity 8"):
         s.ask(torch.zeros(6, 9, dtype=torch.int64), torch.full((6,), 9, dtype=torch.int32))
+
+
+def test_rows_ahead_of_the_lengths_need_room():
+    c = SharedPrefixCache(_prefix(), 3, 8)
+    c.reach = 5
+    new = torch.zeros(6, 2, 2, 128)
+    with pytest.raises(ValueError, match="full: 5 \\+ 4 tokens > capacity 8"):
+        c.append(new, new, 0, at=c.lens + 2, ahead=2)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):       # there is room: on to the kernels
+        c.append(new, new, 0, at=c.lens + 1, ahead=1)
