@@ -325,11 +325,13 @@ cudaError_t read(const ReadParams &p, bool rows128, cudaStream_t stream) {
   return cudaGetLastError();
 }
 
-// rows of 128 elements of `esize` bytes that 16 threads (or 8) can move in
-// `align`-byte pieces
-bool aligned_rows(const SharedTensor &x, int esize, int align) {
-  return x.s[3] == 1 && reinterpret_cast<uintptr_t>(x.data) % align == 0 && x.s[0] * esize % align == 0 &&
-         x.s[1] * esize % align == 0 && x.s[2] * esize % align == 0;
+// rows of 128 elements of `esize` bytes that threads can move 16 bytes at a time: the strides of
+// dimensions with more than one entry are whole pieces
+bool aligned_rows(const SharedTensor &x, int batch, int heads, int rows, int esize) {
+  const int entries[3] = {batch, heads, rows};
+  for (int i = 0; i < 3; ++i)
+    if (entries[i] > 1 && x.s[i] * esize % 16 != 0) return false;
+  return x.s[3] == 1 && reinterpret_cast<uintptr_t>(x.data) % 16 == 0;
 }
 
 }  // namespace
@@ -339,8 +341,8 @@ cudaError_t launch_append_text(const AppendParams &p, cudaStream_t stream) {
   const int esize = p.dtype == 0 ? 4 : 2;
   bool rows128 = p.head_dim == 128;
   for (int i = 0; i < 2; ++i)
-    rows128 = rows128 && aligned_rows(p.src[i], esize, 16) &&
-              (p.quantize ? aligned_rows(p.dst[i], 1, 16) : aligned_rows(p.dst[i], esize, 16));
+    rows128 = rows128 && aligned_rows(p.src[i], p.batch, p.heads, p.tokens, esize) &&
+              aligned_rows(p.dst[i], p.batch, p.heads, p.cap, p.quantize ? 1 : esize);
   if (p.quantize) {
     if (p.dtype == 0) return append<float, true>(p, rows128, stream);
     if (p.dtype == 1) return append<__nv_bfloat16, true>(p, rows128, stream);
@@ -356,7 +358,8 @@ cudaError_t launch_read_text(const ReadParams &p, cudaStream_t stream) {
   const int esize = p.dtype == 0 ? 4 : 2;
   bool rows128 = p.head_dim == 128;
   for (int i = 0; i < 2; ++i)
-    rows128 = rows128 && aligned_rows(p.src[i], 1, 16) && aligned_rows(p.dst[i], esize, 16);
+    rows128 = rows128 && aligned_rows(p.src[i], p.batch, p.heads, p.cap, 1) &&
+              aligned_rows(p.dst[i], p.batch, p.heads, p.cap, esize);
   if (p.dtype == 0) return read<float>(p, rows128, stream);
   if (p.dtype == 1) return read<__nv_bfloat16>(p, rows128, stream);
   return read<__half>(p, rows128, stream);

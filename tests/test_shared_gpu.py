@@ -827,3 +827,24 @@ def test_first_call_of_a_process_may_be_captured():
     repo = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     done = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=repo, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_text_of_one_question_takes_the_wide_kernel_whatever_its_strides():
+    """The stride of a dimension with one entry is never used and may be anything."""
+    from torch.profiler import ProfilerActivity, profile
+
+    from rotatek_b200.kernels import append_text, read_text
+    lens = torch.tensor([3], dtype=torch.int32, device=DEV)
+    caches = [torch.zeros(1, 1, 40, 128, dtype=torch.uint8, device=DEV).as_strided((1, 1, 40, 128), (7, 5, 128, 1))
+              for _ in range(2)]
+    scales = [torch.zeros(1, 1, 40, device=DEV) for _ in range(2)]
+    new = torch.randn(1, 1, 6, 128, device=DEV).to(torch.bfloat16).as_strided((1, 1, 6, 128), (3, 1, 128, 1))
+    with profile(activities=[ProfilerActivity.CUDA]) as seen:
+        append_text(new, new, lens, *caches, k_scale=scales[0], v_scale=scales[1])
+        k, v = read_text(*caches, lens + 6, k_scale=scales[0], v_scale=scales[1])
+        torch.cuda.synchronize()
+    names = " ".join(e.name for e in seen.events())
+    assert "append_rows_kernel" in names and "read_rows_kernel" in names
+    val, scale = osh.quantize_rows(new)
+    assert torch.equal(k[:, :, 3:9].cpu().float(), (val.float() * scale[..., None]).to(torch.bfloat16).float())
+    assert torch.equal(k, v) and (k[:, :, :3] == 0).all()
