@@ -15,9 +15,20 @@
 #include <dlfcn.h>
 #include <string.h>
 
-#include <ATen/dlpack.h>
-
 #include "../../include/rotatek_b200.h"
+
+/* The exchange API came with version 1.3 of dlpack.h. */
+#if defined(__has_include)
+#if __has_include(<ATen/dlpack.h>)
+#include <ATen/dlpack.h>
+#endif
+#endif
+#if defined(DLPACK_MAJOR_VERSION) && \
+    (DLPACK_MAJOR_VERSION > 1 || (DLPACK_MAJOR_VERSION == 1 && DLPACK_MINOR_VERSION >= 3))
+#define HAVE_EXCHANGE 1
+#else
+#define HAVE_EXCHANGE 0
+#endif
 
 #define MAX_TENSORS 16
 #define MAX_DTYPES 16
@@ -59,6 +70,7 @@ static int dims_of(PyObject *tuple, int64_t *out, int32_t *ndim) {
   return 1;
 }
 
+#if HAVE_EXCHANGE
 /* DLPack's C exchange API of torch.Tensor: a tensor's address, type, shape and strides as one
  * C call that makes no Python object (the attributes below take seven).  NULL where this torch
  * has none. */
@@ -97,6 +109,23 @@ static int describe_fast(PyObject *t, rtk_tensor *d, int64_t *device) {
   }
   return 1;
 }
+
+static void find_exchange(PyObject *type) {
+  PyObject *capsule = PyObject_GetAttrString(type, "__dlpack_c_exchange_api__");
+  const DLPackExchangeAPI *api =
+      capsule != NULL ? (const DLPackExchangeAPI *)PyCapsule_GetPointer(capsule, "dlpack_exchange_api") : NULL;
+  Py_XDECREF(capsule);                          /* the type keeps it */
+  PyErr_Clear();
+  if (api != NULL && api->header.version.major == DLPACK_MAJOR_VERSION) {
+    Py_INCREF(type);
+    tensor_type = (PyTypeObject *)type;
+    exchange = api;
+  }
+}
+#else
+static int describe_fast(PyObject *t, rtk_tensor *d, int64_t *device) { return 0; }
+static void find_exchange(PyObject *type) {}
+#endif
 
 /* Descriptor of tensor t; *device is the tensors' common device so far (-2: none yet, -1:
  * not one CUDA device).  Returns 0 with an exception set on failure. */
@@ -237,16 +266,7 @@ static PyObject *py_bind(PyObject *self, PyObject *args) {
   if (!find(lib, "rtk_shared_decode", &f_shared_decode) || !find(lib, "rtk_append_text", &f_append_text) ||
       !find(lib, "rtk_read_text", &f_read_text) || !find(lib, "rtk_verify_drafts", &f_verify_drafts))
     return NULL;
-  PyObject *capsule = PyObject_GetAttrString(type, "__dlpack_c_exchange_api__");
-  const DLPackExchangeAPI *api =
-      capsule != NULL ? (const DLPackExchangeAPI *)PyCapsule_GetPointer(capsule, "dlpack_exchange_api") : NULL;
-  Py_XDECREF(capsule);                          /* the type keeps it */
-  PyErr_Clear();
-  if (api != NULL && api->header.version.major == DLPACK_MAJOR_VERSION) {
-    Py_INCREF(type);
-    tensor_type = (PyTypeObject *)type;
-    exchange = api;
-  }
+  find_exchange(type);
   Py_RETURN_NONE;
 }
 

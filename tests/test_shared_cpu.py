@@ -211,3 +211,37 @@ def test_a_capture_leaves_no_workspace_behind(monkeypatch):
     capturing[0] = False
     buf[700:] = 3                                        # as if the captured zeros had not been run
     assert (_lib.workspace(dev, 5000, 4000)[:4000] == 0).all()
+
+
+OLD_DLPACK = """#define DLPACK_MAJOR_VERSION 1
+#define DLPACK_MINOR_VERSION 0
+typedef struct { int code; } DLSomethingOlder;
+"""
+
+
+@pytest.mark.parametrize("header", [OLD_DLPACK, None])
+def test_direct_calls_build_without_the_exchange_api(header, tmp_path, lib):  # noqa: F811
+    """A torch whose dlpack.h has no exchange API, or none at all: descriptors come from attributes."""
+    import importlib.util
+    import os
+    import shutil
+    import subprocess
+    import sysconfig
+
+    from rotatek_b200.csrc import build
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    if header is not None:
+        (tmp_path / "ATen").mkdir()
+        (tmp_path / "ATen" / "dlpack.h").write_text(header)
+    out = str(tmp_path / "_calls.so")
+    subprocess.run([cc, "-std=c11", "-Wall", "-Werror", "-shared", "-fPIC", "-I", sysconfig.get_paths()["include"], "-I",
+                    str(tmp_path), os.path.join(build.CSRC, "calls.c"), "-o", out, "-ldl"], check=True)
+    spec = importlib.util.spec_from_file_location("_calls", out)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    mod.bind(_lib.LIB_PATH, _lib._DTYPES, torch.Tensor)
+    x = torch.zeros(1, 1, 1, 128)
+    assert mod.append_text(x, x, torch.zeros(1, dtype=torch.int32), None, x, x, None, None, 0) == -1     # not on a GPU
+    assert mod.append_text(*[None] * 8, 0) == 1 and "k_new must be" in lib.rtk_last_error().decode()
