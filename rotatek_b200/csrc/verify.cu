@@ -78,10 +78,15 @@ __device__ __forceinline__ const T *logits_row(const VerifyParams &p, int b, int
                        : static_cast<const T *>(p.draft.data) + b * p.draft.s[0] + (r - p.drafts - 1) * p.draft.s[1];
 }
 
-__device__ __forceinline__ void join(float &m, float &z, float m2, float z2) {
+// 2^((x - m) c): the difference is taken first, since x c and m c of a tiny temperature are too large for
+// theirs to mean anything
+__device__ __forceinline__ float weight(float x, float m, float c) { return fast_exp2((x - m) * c); }
+
+// (m, z): a maximum and the sum of weights relative to it; c = log2(e) / temperature
+__device__ __forceinline__ void join(float &m, float &z, float m2, float z2, float c) {
   const float top = fmaxf(m, m2);
   if (top == -INFINITY) return;                  // nothing on either side
-  z = z * fast_exp2(m - top) + z2 * fast_exp2(m2 - top);
+  z = z * weight(m, top, c) + z2 * weight(m2, top, c);
   m = top;
 }
 
@@ -164,23 +169,25 @@ __global__ void __launch_bounds__(kThreads) verify_stats_kernel(const VerifyPara
 #pragma unroll
         for (int e = 1; e < kVec; ++e) top = fmaxf(top, v[e]);
         if (top > m) {
-          z *= fast_exp2((m - top) * c);       // nothing yet: 0
+          z *= weight(m, top, c);              // nothing yet: 0
           m = top;
         }
         if (m > -INFINITY) {
-          const float mc = -m * c;
+          const float2 from = make_float2(-m, -m), c2 = make_float2(c, c);
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) z += fast_exp2(fmaf(v[e], c, mc));
+          for (int e = 0; e < kVec; e += 2) {
+            const float2 x = __fmul2_rn(__fadd2_rn(make_float2(v[e], v[e + 1]), from), c2);
+            z += fast_exp2(x.x) + fast_exp2(x.y);
+          }
         }
       } else {
         if (v[0] > m) {
-          z *= fast_exp2((m - v[0]) * c);
+          z *= weight(m, v[0], c);
           m = v[0];
         }
-        if (m > -INFINITY) z += fast_exp2((v[0] - m) * c);
+        if (m > -INFINITY) z += weight(v[0], m, c);
       }
     });
-    m *= c;                                    // from here on in base-2 units
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -192,7 +199,7 @@ __global__ void __launch_bounds__(kThreads) verify_stats_kernel(const VerifyPara
         at = at2;
       }
     } else {
-      join(m, z, m2, z2);
+      join(m, z, m2, z2, c);
     }
   }
   if (lane == 0) {
@@ -209,7 +216,7 @@ __global__ void __launch_bounds__(kThreads) verify_stats_kernel(const VerifyPara
           at = i_s[w];
         }
       } else {
-        join(m, z, m_s[w], z_s[w]);
+        join(m, z, m_s[w], z_s[w], c);
       }
     }
     static_cast<float4 *>(p.workspace)[((long long)b * l.rows + r) * l.chunks + chunk] = make_float4(m, z, __int_as_float(at), 0.f);
@@ -218,7 +225,7 @@ __global__ void __launch_bounds__(kThreads) verify_stats_kernel(const VerifyPara
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) verify_pick_kernel(const VerifyParams p) {
-  __shared__ float m_s[2 * kMaxDrafts + 1], z_s[2 * kMaxDrafts + 1];     // base-2 maximum, 1 / sum
+  __shared__ float m_s[2 * kMaxDrafts + 1], z_s[2 * kMaxDrafts + 1];     // maximum, 1 / sum
   __shared__ int at_s[kMaxDrafts + 1];
   __shared__ int k_s;
   __shared__ unsigned long long key_s[kThreads / 32];
@@ -265,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_pick_kernel(const VerifyPa
           at = __float_as_int(v.z);
         }
       } else {
-        join(m, z, v.x, v.y);
+        join(m, z, v.x, v.y, c);
       }
     }
 #pragma unroll
@@ -278,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_pick_kernel(const VerifyPa
           at = at2;
         }
       } else {
-        join(m, z, m2, z2);
+        join(m, z, m2, z2, c);
       }
     }
     if (lane == 0) {
@@ -290,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_pick_kernel(const VerifyPa
   __syncthreads();
   // p (or q) of a token of row r
   auto prob = [&](float m, float inv, float logit) {
-    return m > -INFINITY ? fast_exp2(fmaf(logit, c, -m)) * inv : 0.f;
+    return m > -INFINITY ? weight(logit, m, c) * inv : 0.f;
   };
   if (j < n) {
     bool ok = false;
@@ -316,8 +323,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_pick_kernel(const VerifyPa
     float top = 0.f;
     int who = 0;
     const bool minus = rest && dr != nullptr;
-    const float ct = mt > -INFINITY ? c : 0.f, cd = md > -INFINITY ? c : 0.f;      // nothing there: 2^-inf
-    const float ot = mt > -INFINITY ? -mt : -INFINITY, od = md > -INFINITY ? -md : -INFINITY;
+    const float ft = mt > -INFINITY ? mt : INFINITY, fd = md > -INFINITY ? md : INFINITY;      // nothing there: 2^-inf
     auto group = [&](int i, auto whole) {
       float t[kU], v[kU];
 #pragma unroll
@@ -333,12 +339,12 @@ __global__ void __launch_bounds__(kThreads, 4) verify_pick_kernel(const VerifyPa
           d[q] = whole || i + q * kThreads < to ? to_f32(dr[i + q * kThreads]) : -INFINITY;
 #pragma unroll
         for (int q = 0; q < kU; ++q)
-          v[q] = __fdividef(__fsub_rn(__fmul_rn(fast_exp2(fmaf(t[q], ct, ot)), zt),      // not fused:
-                                      __fmul_rn(fast_exp2(fmaf(d[q], cd, od)), zd)),     // p - p is 0
+          v[q] = __fdividef(__fsub_rn(__fmul_rn(weight(t[q], ft, c), zt),      // not fused:
+                                      __fmul_rn(weight(d[q], fd, c), zd)),     // p - p is 0
                             v[q]);
       } else {
 #pragma unroll
-        for (int q = 0; q < kU; ++q) v[q] = __fdividef(fast_exp2(fmaf(t[q], ct, ot)), v[q]);
+        for (int q = 0; q < kU; ++q) v[q] = __fdividef(weight(t[q], ft, c), v[q]);
         // a draft without logits is certain of its token: nothing of p is left there
         if (rest && (unsigned)(drop - i) <= (kU - 1) * kThreads && (drop - i) % kThreads == 0) {
 #pragma unroll

@@ -848,3 +848,18 @@ def test_text_of_one_question_takes_the_wide_kernel_whatever_its_strides():
     val, scale = osh.quantize_rows(new)
     assert torch.equal(k[:, :, 3:9].cpu().float(), (val.float() * scale[..., None]).to(torch.bfloat16).float())
     assert torch.equal(k, v) and (k[:, :, :3] == 0).all()
+
+
+@pytest.mark.parametrize("heat", [1e-6, 1e-8, 1e-9, 1e-12, 1e-30, 1e-38])
+@pytest.mark.parametrize("dtype,logits", [(torch.bfloat16, True), (torch.float32, True), (torch.float32, False)])
+def test_verify_temperatures_next_to_nothing(heat, dtype, logits):
+    """All of p is at the largest logits, whatever the temperature's size: the products of logits and
+    1 / temperature are far beyond what their difference of a bit could bear."""
+    a = make_verify(12, 3, 5000, dtype, logits, 44, near=0.2)
+    a["target_logits"] = a["target_logits"] + 30
+    a["temperature"] = torch.full((12,), heat, device=DEV)
+    if not logits:                                   # some proposals are the likeliest token
+        best = a["target_logits"][:, :3].argmax(-1)
+        a["draft_tokens"] = torch.where(torch.rand(12, 3, device=DEV) < 0.7, best, a["draft_tokens"])
+    _, accepted = check_verify(a)
+    assert accepted.sum() > 0
