@@ -153,3 +153,47 @@ def test_rows_ahead_of_the_lengths_need_room():
         c.append(new, new, 0, at=c.lens + 2, ahead=2)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):       # there is room: on to the kernels
         c.append(new, new, 0, at=c.lens + 1, ahead=1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("draft_layers,drafts,temperature", [(1, 3, 0.0), (0, 5, 0.0), (3, 2, 0.9)])
+def test_the_loop_on_the_tensor_cores(draft_layers, drafts, temperature, dtype, monkeypatch):
+    """Every attention of questions that go in, are drafted for and checked is within the tolerance of
+    tests/test_shared_gpu.py of its 64-bit value, and the emitted tokens are the verification's."""
+    from rotatek_b200.llama_e2e import RandomLlamaDecoder
+    from rotatek_b200.shared_e2e import ServingConfig, SharedQuestions
+    from tests.test_shared_gpu import UNIT, dense
+
+    cfg = DecoderConfig(layers=3, hidden=512, heads=8, kv_heads=2, ffn=512, vocab=400, prompt=40, vision=900, text=3,
+                        max_new_tokens=0, dtype=dtype, fused_key_projection=False)
+    model = RandomLlamaDecoder(cfg, "cuda", seed=4)
+    model.prefill(model.prompt_embeddings(2))
+    s = SharedQuestions(model, ServingConfig(questions=4, capacity=80, drafts=drafts, draft_layers=draft_layers,
+                                             temperature=temperature))
+    attend, seen = s.cache.attend, []
+
+    def checked(q, layer, lens, groups):
+        out = attend(q, layer, lens, groups)
+        a = s.cache.prefix.decode_args(layer)
+        k, v, ks, vs = s.cache.text[layer]
+        args = dict(q=q, R_partial=a["R_partial"], delta_mu=a["delta_mu"], k_full=a["k_full"], v_full=a["v_full"],
+                    mask_full=a["mask_full"], k_sparse=a["k_sparse"], v_sparse=a["v_sparse"], k_text=k, v_text=v,
+                    text_lens=lens, num_kv_groups=groups, k_scale=ks, v_scale=vs)
+        want, mag = dense(args)
+        off = (out.double() - want).abs()
+        assert (off <= UNIT[dtype] * want.abs() + 2.0 ** -11 * mag + 2.0 ** -25).all()
+        seen.append(q.shape[1])
+        return out
+
+    monkeypatch.setattr(s.cache, "attend", checked)
+    counts = torch.tensor([9, 3, 12, 1, 7, 12, 5, 2], dtype=torch.int32, device="cuda")
+    s.ask(torch.randint(0, 400, (8, 12), generator=torch.Generator().manual_seed(6)).cuda(), counts)
+    emitted = counts + 1
+    for _ in range(5):
+        tokens, accepted = s.step()
+        place = torch.arange(drafts + 1, device="cuda")
+        assert ((tokens >= 0) == (place <= accepted[:, None])).all() and (tokens < 400).all()
+        emitted = emitted + accepted + 1
+    assert torch.equal(s.cache.lens + 1, emitted)
+    assert {12, drafts + 1} <= set(seen) and (draft_layers == 0 or 1 in seen)

@@ -863,3 +863,123 @@ def test_verify_temperatures_next_to_nothing(heat, dtype, logits):
         a["draft_tokens"] = torch.where(torch.rand(12, 3, device=DEV) < 0.7, best, a["draft_tokens"])
     _, accepted = check_verify(a)
     assert accepted.sum() > 0
+
+
+# ------------------------------------------------------------------ long ranges, several chunks, whole questions
+def dense(a):
+    """``osh.shared_decode`` (out, A) in float64 on the GPU, a KV head of a question at a time."""
+    q = a["q"].double()
+    B, T, hq, D = q.shape
+    G, P, hk, cap = a["num_kv_groups"], a["R_partial"].shape[0], a["R_partial"].shape[1], a["k_text"].shape[2]
+    out, mag = torch.zeros_like(q), torch.zeros_like(q)
+    lens = a["text_lens"].clamp(0, cap).tolist()
+
+    def text(side, b, h, n):
+        x = a[f"{side}_text"][b, h, :n]
+        if a.get(f"{side}_scale") is None:
+            return x.double()
+        return x.view(torch.float8_e4m3fn).double() * a[f"{side}_scale"][b, h, :n, None].double()
+
+    for h in range(hk):
+        for p in range(P):
+            keys = a["k_sparse"][p, h].double() @ a["R_partial"][p, h].double().T
+            if a["delta_mu"] is not None:
+                keys = keys + a["delta_mu"][p, h].double()
+            there = slice(None) if a["mask_full"] is None else a["mask_full"][p].bool()
+            keys = torch.cat([a["k_full"][p, h].double()[there], keys])
+            values = torch.cat([a["v_full"][p, h].double()[there], a["v_sparse"][p, h].double()])
+            for b in range(p * (B // P), (p + 1) * (B // P)):
+                n = lens[b]
+                k, v = torch.cat([keys, text("k", b, h, n)]), torch.cat([values, text("v", b, h, n)])
+                if k.shape[0] == 0:
+                    continue
+                s = q[b, :, h * G:(h + 1) * G].reshape(T * G, D) @ k.T / math.sqrt(D)
+                seen = n - (T - 1) + torch.arange(T, device=DEV).repeat_interleave(G)
+                s[:, keys.shape[0]:].masked_fill_(torch.arange(n, device=DEV) >= seen[:, None], -math.inf)
+                w = torch.softmax(s, 1).nan_to_num(0.0)              # a row that sees nothing
+                out[b, :, h * G:(h + 1) * G] = (w @ v).view(T, G, D)
+                mag[b, :, h * G:(h + 1) * G] = (w @ v.abs()).view(T, G, D)
+    return out, mag
+
+
+def check_dense(a, logits=0.0):
+    """The tolerance of ``compare`` where logits stay below 50, more for larger ones: they are off by 2^-16
+    of their size (the rotated query's two parts), which moves a weight by as much, twice."""
+    from rotatek_b200.kernels import rotatek_shared_decode
+    got = rotatek_shared_decode(**a).double()
+    want, mag = dense(a)
+    tol = UNIT[a["q"].dtype] * want.abs() + (2.0 ** -11 + 2 * logits * 2.0 ** -16) * mag + 2.0 ** -25
+    off = (got - want).abs()
+    assert (off <= tol).all(), f"{int((off > tol).sum())} of {off.numel()}, worst {(off / tol).max():.2f}"
+
+
+def test_dense_is_the_oracle():
+    a = make(2, 2, 3, 8, 2, 40, 20, 30, 32, fp8=True, mask=0.6, seed=90, lens=[30, 0, 2, 17])
+    for x, y in zip(dense(a), osh.shared_decode(**a)):
+        assert (x.cpu() - y).abs().max() < 1e-12
+
+
+LONG = [
+    # P, N, T, H_q, H_kv, S_v, S_f, C, D_keep: a CTA takes a dozen blocks and more of a unit, several units
+    (2, 2, 1, 64, 64, 2900, 300, 20, 32),
+    (1, 3, 1, 160, 160, 2000, 1000, 10, 16),
+    (3, 2, 1, 128, 64, 1700, 700, 0, 64),
+    (1, 32, 1, 128, 32, 7000, 200, 30, 32),          # full tiles of 128 rows
+    (1, 21, 3, 80, 16, 9000, 64, 40, 64),            # 315 rows: two full tiles and a part
+    (1, 2, 1, 320, 160, 0, 3000, 5, 32),             # prompt alone
+]
+
+
+@pytest.mark.parametrize("shape", LONG)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("mask", [None, 0.7])
+def test_decode_long_ranges(shape, dtype, mask):
+    """Every stage and buffer of the prefix kernel is used again and again within a unit."""
+    check_dense(make(*shape, dtype=dtype, mask=mask, seed=91))
+
+
+@pytest.mark.parametrize("shape", [LONG[0], LONG[3]])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("way", ["up", "down", "there and back"])
+def test_decode_long_ranges_with_a_moving_maximum(shape, dtype, way):
+    """Logits that climb by more than 2^8 from block to block of a long range: the lazy maximum moves
+    a dozen times within a unit."""
+    a = make(*shape, dtype=dtype, seed=92, bias=False)
+    sv, groups = shape[5], a["num_kv_groups"]
+    t = torch.linspace(0, 1, sv, device=DEV)
+    t = {"up": t, "down": 1 - t, "there and back": 1 - (2 * t - 1).abs()}[way]
+    direction = a["R_partial"][0, :, :, 0].float()                       # q . R column 0 = 20 for every query
+    a["R_partial"] = a["R_partial"][:1].expand_as(a["R_partial"]).contiguous()
+    a["q"] = (a["q"].float() * 0.05 + 20.0 * direction.repeat_interleave(groups, 0)).to(dtype)
+    ramp = torch.zeros(sv, a["k_sparse"].shape[-1], device=DEV)
+    ramp[:, 0] = 250.0 * t                                                # logits up to 442
+    a["k_sparse"] = (a["k_sparse"].float() * 0.05 + ramp).to(dtype)
+    a["k_full"] = (a["k_full"].float() * 0.1).to(dtype)
+    check_dense(a, logits=442)
+
+
+@pytest.mark.parametrize("dtype,fp8", [(torch.bfloat16, False), (torch.float16, False), (torch.bfloat16, True),
+                                       (torch.float16, True)])
+@pytest.mark.parametrize("T", [1, 3, 7])
+def test_decode_several_text_chunks(T, dtype, fp8):
+    """Lengths around the edges of chunks of 256, for rows of either text kernel."""
+    lens = [0, 1, 255, 256, 257, 258, 511, 512, 513, 700, 768, 769, 800, 1023, 1024, 1025, 1099, 1100]
+    check_dense(make(1, len(lens), T, 8, 2, 200, 30, 1100, 32, dtype=dtype, fp8=fp8, lens=lens, seed=93))
+    check_dense(make(1, len(lens), T, 8, 2, 0, 0, 1100, 32, dtype=dtype, fp8=fp8, lens=lens, seed=94))
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("T", [1, 6])
+@pytest.mark.parametrize("questions,cap", [(40, 1100), (75, 2100)])
+def test_decode_longer_chunks(questions, cap, T, fp8):
+    """Enough questions for chunks of 512 and of 1024 tokens, and more than one of them each."""
+    lens = [(i * 211) % (cap + 1) for i in range(questions - 4)] + [512, 1024, 1025, cap]
+    check_dense(make(1, questions, T, 32, 8, 130, 10, cap, 32, fp8=fp8, lens=lens, seed=95))
+
+
+@pytest.mark.parametrize("dtype,fp8", [(torch.bfloat16, False), (torch.float16, True), (torch.bfloat16, True)])
+@pytest.mark.parametrize("N,T,hq,hk,cap,lens", [(3, 33, 8, 2, 40, [33, 40, 34]), (2, 100, 28, 4, 300, [300, 120]),
+                                                (2, 577, 16, 2, 700, [577, 690]), (2, 70, 4, 4, 100, [20, 100])])
+def test_decode_whole_questions(N, T, hq, hk, cap, lens, dtype, fp8):
+    """The questions themselves: T up to 577, causal among them, and one shorter than T."""
+    check_dense(make(1, N, T, hq, hk, 500, 40, cap, 32, dtype=dtype, fp8=fp8, lens=lens, seed=96))
