@@ -57,8 +57,9 @@ rtk::SharedTensor view(const rtk_tensor *t) {
   return v;
 }
 
-// a tensor that a kernel reads or writes has an address unless it is empty
+// a tensor that a kernel reads or writes has an address unless it is empty (or not given)
 bool present(const rtk_tensor *t) {
+  if (t == nullptr) return true;
   int64_t n = 1;
   for (int i = 0; i < t->ndim; ++i) n *= t->shape[i];
   return n == 0 || t->data != nullptr;
@@ -175,7 +176,8 @@ int rtk_shared_decode(const rtk_tensor *q, const rtk_tensor *R_partial, const rt
   if (B * T * Hq > kMaxInt || Sf > kMaxInt || Sv > kMaxInt || C > kMaxInt)
     return fail(RTK_ERR_UNSUPPORTED, "more than 2^31 - 1 query rows or tokens");
   if (B * T * Hq == 0) return RTK_OK;
-  for (const rtk_tensor *t : {q, R_partial, k_full, v_full, k_sparse, v_sparse, k_text, v_text, text_lens, out})
+  for (const rtk_tensor *t : {q, R_partial, delta_mu, k_full, v_full, mask_full, k_sparse, v_sparse, k_text, v_text,
+                              k_scale, v_scale, text_lens, out})
     if (!present(t)) return fail(RTK_ERR_INVALID, "a tensor that is not empty has no address");
 
   rtk::SharedParams p;
@@ -297,7 +299,7 @@ int rtk_append_text(const rtk_tensor *k_new, const rtk_tensor *v_new, const rtk_
     return fail(RTK_ERR_INVALID, "counts must be an int32 [B]");
   if (2 * B * H * T > kMaxInt || C > kMaxInt) return fail(RTK_ERR_UNSUPPORTED, "more than 2^31 - 1 rows");
   if (B * H * T * D == 0 || C == 0) return RTK_OK;
-  for (const rtk_tensor *t : {k_new, v_new, k_text, v_text, text_lens})
+  for (const rtk_tensor *t : {k_new, v_new, k_text, v_text, k_scale, v_scale, text_lens, counts})
     if (!present(t)) return fail(RTK_ERR_INVALID, "a tensor that is not empty has no address");
 
   rtk::AppendParams p;
@@ -384,7 +386,8 @@ int rtk_verify_drafts(const rtk_tensor *target_logits, const rtk_tensor *draft_t
   if (T > 64) return fail(RTK_ERR_UNSUPPORTED, "at most 64 drafted tokens (got %lld)", (long long)T);
   if (B > 65535 || V > (1 << 30)) return fail(RTK_ERR_UNSUPPORTED, "at most 65535 questions and a vocabulary of 2^30");
   if (B == 0) return RTK_OK;
-  for (const rtk_tensor *t : {target_logits, draft_tokens, uniforms, noise, temperature, tokens_out, accepted_out})
+  for (const rtk_tensor *t : {target_logits, draft_tokens, draft_logits, uniforms, noise, temperature, draft_lens,
+                              tokens_out, accepted_out})
     if (!present(t)) return fail(RTK_ERR_INVALID, "a tensor that is not empty has no address");
   const size_t need = rtk::verify_workspace_bytes(B, T, V);
   if (workspace == nullptr || workspace_bytes < need)

@@ -245,3 +245,37 @@ def test_direct_calls_build_without_the_exchange_api(header, tmp_path, lib):  # 
     x = torch.zeros(1, 1, 1, 128)
     assert mod.append_text(x, x, torch.zeros(1, dtype=torch.int32), None, x, x, None, None, 0) == -1     # not on a GPU
     assert mod.append_text(*[None] * 8, 0) == 1 and "k_new must be" in lib.rtk_last_error().decode()
+
+
+def test_given_tensors_without_an_address_are_refused(lib):  # noqa: F811
+    """Also the nullable ones: a NULL tensor is left out, a tensor with NULL data is not."""
+    bad = lambda *a: _fake(*a, data=0)  # noqa: E731
+    q, R, full = _fake((6, 2, 8, 128)), _fake((2, 2, 128, 32)), _fake((2, 2, 10, 128))
+    ks, vs, kt, k8 = _fake((2, 2, 50, 32)), _fake((2, 2, 50, 128)), _fake((6, 2, 20, 128)), _fake((6, 2, 20, 128), U8)
+    sc, lens = _fake((6, 2, 20), F32), _fake((6,), I32)
+    why = (1, "a tensor that is not empty has no address")
+
+    def attend(dm=None, mask=None, text=kt, ksc=None, vsc=None):
+        return (lib.rtk_shared_decode(q, R, dm, full, full, mask, ks, vs, text, text, ksc, vsc, lens, 4, q, None, 0, None,
+                                      None), lib.rtk_last_error().decode())
+
+    assert attend(dm=bad((2, 2, 128))) == why
+    assert attend(mask=bad((2, 10), U8)) == why
+    assert attend(text=k8, ksc=bad((6, 2, 20), F32), vsc=sc) == why
+    assert attend(text=k8, ksc=sc, vsc=bad((6, 2, 20), F32)) == why
+
+    def append(counts=None, cache=kt, ksc=None, vsc=None):
+        new = _fake((6, 2, 4, 128))
+        return lib.rtk_append_text(new, new, lens, counts, cache, cache, ksc, vsc, None), lib.rtk_last_error().decode()
+
+    assert append(counts=bad((6,), I32)) == why
+    assert append(cache=k8, ksc=bad((6, 2, 20), F32), vsc=sc) == why
+    assert append(cache=k8, ksc=sc, vsc=bad((6, 2, 20), F32)) == why
+
+    def verify(dl=None, ln=None):
+        return (lib.rtk_verify_drafts(_fake((3, 5, 100)), _fake((3, 4), I64), dl, _fake((3, 4), F32), _fake((3, 100), F32),
+                                      _fake((3,), F32), ln, _fake((3, 5), I64), _fake((3,), I32), None, 0, None),
+                lib.rtk_last_error().decode())
+
+    assert verify(dl=bad((3, 4, 100))) == why
+    assert verify(ln=bad((3,), I32)) == why
