@@ -110,17 +110,17 @@ inline PrefixSplit prefix_split(long long prefixes, long long questions, long lo
   s.blocks_vis = (int)((seq_sparse + 127) / 128);
   const long long weight = s.blocks_full + 2 * s.blocks_vis, all = s.units * weight;
   // Ranges of a few blocks: a quarter of the SMs is left to the text kernel, which then runs
-  // beside this one instead of after it (8 questions on 16000 tokens: 18.7 us, 24.1 on all
-  // SMs, 20.3 on half; ranges of many blocks cannot spare them: 123 us against 107, 562
-  // against 462); half of them where the text is the larger part, 64 tokens of the caches
-  // (half full) a weight (64 questions of 1024 tokens: 31.7, 35.1 with a quarter, 37.8 with none).
+  // beside this one instead of after it (8 questions on 16000 tokens: 20.6 us, 26.3 on all
+  // SMs, 21.9 on half; ranges of many blocks cannot spare them: 123 us against 115, 700
+  // against 600); half of them where the text is the larger part, 64 tokens of the caches
+  // (half full) a weight (64 questions of 1024 tokens: 35.3, 37.8 with a quarter, 41.0 with none).
   const long long text = prefixes * questions * kv_heads * ((tokens * groups + 63) / 64) * text_cap / 64;
   if (text > 0 && all < 16ll * sms) sms -= text >= all ? sms / 2 : sms / 4;
   // A unit's start and end take 6 to 10 thousand cycles, where a block of 128 rows (weight 2)
-  // takes 1400 and one of few rows half of that: CTAs that meet a second unit get fewer blocks,
-  // though not none.  (Weight 2 / 8 / 16: the prefix and its text in 20.6 / 18.9 / 19.2 us for
-  // 56 rows of 4 heads with ranges of 9, 107 / 106 / 104 for 80 units of up to 128 rows, 78.3 /
-  // 76.7 / 77.3 for 64 of 12; 16 units with ranges of 2 13.5 / - / 14.5.)
+  // takes 1800 and one of few rows two thirds of that: CTAs that meet a second unit get fewer blocks,
+  // though not none.  (Weight 2 / this rule / 16: the whole attention in 21.2 / 20.6 / 20.6 us for
+  // 56 rows of 4 heads with ranges of 9, 120.3 / 115.4 / 115.4 for 80 units of up to 128 rows,
+  // 83.7 / 83.4 / 83.1 for 64 of 12; with one part of P 16 units with ranges of 2 13.5 / - / 14.5.)
   const long long range = all / sms;
   s.unit_start = (int)(range < 2 ? 2 : range > 16 ? 16 : range);
   s.unit_weight = (int)weight + s.unit_start;
@@ -146,9 +146,9 @@ cudaError_t shared_status_address(void **address);
 
 // Text: CTAs per (question, KV head, chunk of tokens, 16 or 64 query rows).  Chunks of 256
 // tokens, so that few questions use many SMs; longer where that makes several waves of
-// CTAs: 64 questions, 8 heads of 64 rows, 1001 tokens take 465 us with 256 and 462 with 512,
-// and half of the partial results (34 MB, not 68).  From 128: 8 questions of 640 tokens 19.1
-// us against 18.7, of 2048 14.6 against 16.0; the many-question cases alike.
+// CTAs (the whole attention, 64 questions, 8 heads of 8 rows of 4096 tokens of 16 bits: 165 us
+// with 256, 135 with 1024; 256 questions, 8 heads of 4 rows, 512 tokens: 82 and 76).  From 128 on:
+// 8 questions of 640 tokens 20.6 us, of 2048 23.3, as from 256.
 inline int text_chunk(long long batch, long long kv_heads, long long rows, long long cap) {
   const long long tiles = rows <= 16 ? 1 : (rows + 63) / 64;
   int chunk = 256;

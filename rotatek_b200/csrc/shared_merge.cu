@@ -11,12 +11,12 @@
 // through shared memory.  Where that would leave SMs idle, CTAs of 8 rows and 32 channels
 // whose warps split the partials.
 //
-// Measured, the whole step with tiles of 32 rows / of 8: 1024 working CTAs of 32 rows 461 /
-// 536 us, 256 of them 67.4 / 85.3, 128: 109 / 114, 64: 32.6 / 31.8 and 76.9 / 76.8, 32: 40.6 /
-// 37.6, 8: 26.9 / 18.6.
+// Measured, the whole attention with tiles of 32 rows / of 8: 1024 working CTAs of 32 rows 600 /
+// 683 us, 288 of them 115 / 139, 128: 102.9 / 102.5, 64: 83.0 / 82.8 and 61.1 / 60.7, 16: 34.5 /
+// 27.5, 8: 28.7 / 20.6.
 //
 // What bounds it: after the last partial, latency (2 to 4 us); with the many rows of the first
-// case its bytes, 43 MB of partials and 8 of output in 19 us, mostly from L2.
+// case its bytes, 61 MB of partials and 8 of output, mostly from L2.
 #include "common.cuh"
 #include "shared.h"
 

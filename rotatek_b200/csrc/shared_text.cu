@@ -15,16 +15,18 @@
 // - 8-bit text of at most 16 rows: the warps split the tokens, blocks of 32 in rings of their
 //   own (no CTA-wide barrier in the loop), convert in registers, and join at the end.
 //
-// Measured (the whole attention of a step, prefix of 1064 tokens; one part of P): 8-bit, 64 questions, 8 heads
-// of 8 rows, up to 4096 tokens 89.6 us with split tokens, 164 with split rows; 256 questions, 8
-// heads of 4, 512 tokens 67.7 and 103.  16-bit, the same two when both took it, 113.8 and 112.8,
-// 80.0 and 75.5: no conversion to share, and the rows' kernel ends with less to join, so 16-bit
-// text always takes that one.  64 rows (64 questions, 8 heads, up to 1001 tokens of 8 bits), the
-// kernel alone: 119 us when split by tokens, 16 rows a CTA, 82 by rows.
+// Measured (the whole attention of a step, prefix of 1064 tokens): 8-bit, 64 questions, 8 heads
+// of 8 rows, up to 4096 tokens 105 us with split tokens, 171 with split rows; 256 questions, 8
+// heads of 4, 512 tokens 75.7 and 103; 64, 4 heads of 14, 1024 tokens 37.4 and 44.7.  16-bit text
+// always takes split rows: no conversion to share, and less to join at the end (when both took
+// it, with one part of P, 112.8 us by rows and 113.8 by tokens for the first of these, 75.5 and
+// 80.0 for the second).  The kernels alone: 64 questions, 8 heads of 64 rows, up to 1001 tokens of
+// 8 bits 72 us; 64, 4 heads of 35 rows, 512 tokens 21; 64, 8 heads of 8 rows, 4096 tokens 91 us
+// of 8 bits, 105 of 16.
 //
-// What bounds it: HBM where questions are many and their text 16-bit (the first case: 537 MB
-// within a step of 109 us, 4.9 TB/s with all that is not text); with 8-bit text the
-// conversions (277 MB within 90 us); with few questions the latency of a chunk.
+// What bounds it: with 16-bit text and many questions HBM and the second part of P (537 MB in 105
+// us, 5.1 TB/s); with 8-bit text the conversions (277 MB in 91 us) and, for many rows, the MMAs'
+// issue; with few questions the latency of a chunk.
 //
 // 8-bit text: e4m3 is exact in f16 and in bf16.  S runs in the queries' type, a token's Key
 // scale multiplies its logit.  P . V runs in bf16, which has fp32's range: a token's Value scale

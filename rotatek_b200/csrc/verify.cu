@@ -25,7 +25,7 @@
 // Measured, and what bounds it: 128 questions, up to 8 drafts, 131071 bf16 logits, 251 MB in
 // 62.9 us: stats 39 at 4.7 TB/s (the exponential unit alone needs half of that), then
 // 22 for the race, which reads the noise for the first time.  64 questions, up to 5 drafts,
-// 32000 fp16 logits of both models, 37 MB: 20.0 us, 10 each.  One question: 9.0 us, the
+// 32000 fp16 logits of both models, 37 MB: 20.0 us, 10 each.  One question: 9.6 us, the
 // latency of two dependent kernels.
 #include <type_traits>
 
