@@ -72,8 +72,8 @@ __global__ void __launch_bounds__(1024 / kQuads) shared_merge_kernel(const Merge
       }
 #pragma unroll
       for (int i = 0; i < kDepth; ++i) {
-        const float w = fast_exp2(e[i].x - ref);
-        if (w == 0.f) continue;                      // a partial that saw nothing: its O may be anything
+        if (e[i].x == -INFINITY) continue;           // a partial that saw nothing: its O may be anything
+        const float w = fast_exp2(e[i].x - ref);     // 0 times NaN stays NaN
         l = fmaf(w, e[i].y, l);
 #pragma unroll
         for (int q = 0; q < kQuads; ++q) {
@@ -201,8 +201,8 @@ __global__ void __launch_bounds__(64 * kSplitWays) shared_merge_split_kernel(con
     o.w *= f;
 #pragma unroll
     for (int k = 0; k < kSplitDepth; ++k) {
-      const float w = fast_exp2(e[k].x - ref);
-      if (w == 0.f) continue;                        // a partial that saw nothing: its O may be anything
+      if (e[k].x == -INFINITY) continue;             // a partial that saw nothing: its O may be anything
+      const float w = fast_exp2(e[k].x - ref);       // 0 times NaN stays NaN
       l = fmaf(w, e[k].y, l);
       o.x = fmaf(w, v[k].x, o.x);
       o.y = fmaf(w, v[k].y, o.y);

@@ -439,7 +439,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_kernel(const TextP
     }
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = st[w].x > -INFINITY ? fast_exp2(st[w].x - mm) : 0.f;
+      const float f = st[w].x > -INFINITY ? fast_exp2(st[w].x - mm) : -1.f;    // < 0: saw nothing (its sum is 0)
       ll = fmaf(st[w].y, f, ll);
       ml_s[w * 16 + e].x = f;
     }
@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) shared_text_kernel(const TextP
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float f = ml_s[w * 16 + e].x;
-      if (f == 0.f) continue;
+      if (f < 0.f) continue;                         // its O may be anything
       const float4 v = *reinterpret_cast<const float4 *>(o_s + (w * 16 + e) * 128 + c4 * 4);
       o.x = fmaf(v.x, f, o.x);
       o.y = fmaf(v.y, f, o.y);

@@ -983,3 +983,30 @@ def test_decode_longer_chunks(questions, cap, T, fp8):
 def test_decode_whole_questions(N, T, hq, hk, cap, lens, dtype, fp8):
     """The questions themselves: T up to 577, causal among them, and one shorter than T."""
     check_dense(make(1, N, T, hq, hk, 500, 40, cap, 32, dtype=dtype, fp8=fp8, lens=lens, seed=96))
+
+
+@pytest.mark.parametrize("where", ["v_full", "v_sparse", "v_text"])
+@pytest.mark.parametrize("dtype,fp8,N,T", [(torch.bfloat16, False, 2, 1), (torch.float16, False, 2, 1), (torch.bfloat16, True, 2, 1),
+                                           (torch.bfloat16, True, 2, 9), (torch.float32, False, 2, 1), (torch.bfloat16, False, 100, 4)])
+def test_decode_nan_values_with_next_to_no_weight_come_out(where, dtype, fp8, N, T):
+    """A NaN Value that is seen makes NaN of its channel however small its weight, wherever the weight
+    is: the other tokens' logits are hundreds larger in another partial result."""
+    from rotatek_b200.kernels import rotatek_shared_decode
+    a = make(1, N, T, 8, 2, 300, 70, 600, 32, dtype=dtype, lens=[600] * N, seed=97, bias=False)
+    a["q"][..., 0] = 40.0
+    big = 300 if where != "v_text" else 590
+    a["k_text"][:, :, :, 0] = 0
+    a["k_text"][:, :, big, 0] = 200.0                                     # a logit of 700
+    a["R_partial"] = torch.zeros_like(a["R_partial"])
+    a["R_partial"][:, :, torch.arange(32) + 1, torch.arange(32)] = 1      # channel 0 is not rotated
+    a["k_full"][..., 0] = 0
+    if fp8:
+        quantise_text(a)
+    if where == "v_text" and fp8:
+        a["v_text"][:, :, 3, 5] = 0x7F
+    else:
+        a[where][:, :, 3, 5] = math.nan
+    got = rotatek_shared_decode(**a)
+    assert torch.isnan(got[..., 5]).all()
+    rest = torch.arange(128, device=DEV) != 5
+    assert torch.isfinite(got[..., rest]).all()
